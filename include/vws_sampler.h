@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define VWS_ABI_VERSION 8
+#define VWS_ABI_VERSION 9
 
 /* status codes */
 #define VWS_OK 0
@@ -266,6 +266,123 @@ int vws_apply_penalties(float* logits, int32_t batch, int32_t vocab, int64_t row
                         const int32_t* output_lens, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ---- speculative decoding -------------------------------------------------------------------
+ *
+ * vws_verify_drafts: which of each request's drafted tokens the target accepts, and one token more
+ * (no counterpart in the reference, which decodes token by token, vllm_webgpu/v1/model_runner.py:
+ * 129-137; vLLM-v1's rejection sampler).  Request b has n_b = cu_drafts[b + 1] - cu_drafts[b]
+ * drafts and n_b + 1 consecutive rows of logits, row cu_drafts[b] + b + i holding the target's
+ * logits of the token after its first i drafts.  Row i's distribution p_i is vws_sample's for the
+ * request's temperature, top_k, top_p and min_p: the same kept tokens, p = e / (their sum).  Draft i
+ * (token d, drawn from q_i) is accepted iff q_i(d) > 0 and u_i q_i(d) < p_i(d); without draft_probs
+ * q_i is 1 at d (a looked-up or greedy draft).  After the first refusal, at row a, one token is
+ * drawn from max(p_a - q_a, 0); if none is refused, from the last row's p.  Both by vws_sample's
+ * race with the request's uniforms (lowest index on equal keys; the most probable token if the
+ * residual is empty).  The tokens so emitted are distributed as the target's own samples.
+ * Requests with temperature < 1e-5 or NaN, and rows whose maximum is not finite, have their argmax
+ * (lowest index) for sure.  A draft outside [0, vocab) is refused.  Nothing is read or written out
+ * of bounds whatever cu_drafts holds: a request whose bounds do not fit (negative, decreasing, more
+ * than max_drafts, past num_drafts) gets num_accepted -1 and no token. */
+#define VWS_MAX_DRAFTS 64
+typedef struct vws_verify_args {
+    uint32_t struct_size; /* sizeof(vws_verify_args): ABI guard */
+    int32_t batch;        /* B >= 1 requests */
+    int32_t vocab;        /* 1 <= V <= VWS_MAX_VOCAB */
+    int32_t dtype;        /* VWS_DTYPE_* of the logits */
+    int32_t num_drafts;   /* D >= 0: drafts of all requests */
+    int32_t max_drafts;   /* 0 <= K <= VWS_MAX_DRAFTS: columns of drafts in the outputs */
+    const void* logits;   /* [D + B, V], read only */
+    int64_t logits_row_stride;
+    const int32_t* draft_tokens; /* [D] (may be NULL when D = 0) */
+    const int32_t* cu_drafts;    /* [B + 1] running count of drafts, from 0 to D */
+    const void* draft_probs;     /* [D, V] probabilities the drafts were drawn from, or NULL */
+    int64_t draft_probs_row_stride;
+    int32_t draft_probs_dtype;   /* VWS_DTYPE_* */
+    /* Per request, device arrays of length B; NULL as in vws_sample_args. */
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    /* Random numbers in (0, 1): accept_uniforms [D] and uniforms [B, V] (the race of each request's
+     * one drawn token) -- or generated as in vws_sample_args (rng_seeds / rng_offsets [B], or one
+     * rng_key), draft i's acceptance from token VWS_MAX_VOCAB + i of the request's key.  One of
+     * the three is required when temperature is non-NULL. */
+    const float* accept_uniforms;
+    const float* uniforms;
+    int64_t uniforms_row_stride;
+    const uint64_t* rng_seeds;
+    const uint64_t* rng_offsets;
+    uint64_t rng_key;
+    int32_t rng_key_set;
+    /* Outputs */
+    int32_t* tokens;       /* [B, K + 1]: accepted drafts, the drawn token, then -1 */
+    int32_t* num_accepted; /* [B] accepted drafts (tokens emitted: one more) */
+    float* logprobs;       /* [B, K + 1]: log p_i of each emitted token (0 where the row is sure) */
+    /* Device scratch of vws_verify_workspace_size() bytes, 256-byte aligned; any contents past
+     * the fixed region (vws_sample_workspace_size). */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} vws_verify_args;
+
+size_t vws_verify_workspace_size(int32_t batch, int32_t num_drafts, int32_t vocab);
+int vws_verify_drafts(const vws_verify_args* args);
+
+/* vws_distill_*: the loss that keeps a draft model close to its target, from what the target's
+ * sampler returns (top-L log-probabilities), and its gradient (no counterpart in the reference,
+ * which does not train).  Row n: student logits x [V], teacher entries (id_k, l_k), k < K, weight
+ * w_n, temperature T; q = softmax(x / T).
+ *   VWS_TAIL_RENORMALIZE: p = softmax over the entries of l_k / T (l: log-probabilities or logits);
+ *     loss = w sum_k p_k (log p_k - log q(id_k)); dloss/dx_j = w / T (q_j - p_j)
+ *   VWS_TAIL_BUCKET: p_k = exp(l_k), the rest r = max(0, 1 - sum_k p_k) one more event against the
+ *     student's s = sum of q outside the entries (l: log-probabilities at temperature T);
+ *     loss = w (sum_k p_k (log p_k - log q(id_k)) + r log(r / s));
+ *     dloss/dx_j = w / T (q_j - p_j) at an entry, w / T q_j (1 - r / s) elsewhere.
+ * Ids outside [0, V) are padding; entries that share an id add up.  Rows whose weight is 0, or that
+ * have no entry (renormalize: none above -inf), have loss and gradient 0, and rows of weight 0 are
+ * not read.  A student logit of -inf at an entry of positive probability makes the loss +inf and
+ * leaves the gradient finite; a rest without a finite student logit is no event (the entries alone
+ * count then: dloss/dx_j = w / T (q_j sum_k p_k - p_j)).
+ *
+ * vws_distill_forward writes `loss` and, for the backward, `saved`; vws_distill_backward reads
+ * `saved`, the same inputs and the upstream gradient, and writes `grad`; vws_distill_step does both
+ * for an upstream gradient known beforehand.  `grad` has the logits' type and may be the logits'
+ * own memory (same pointer and stride), else must not overlap them. */
+#define VWS_TAIL_RENORMALIZE 0
+#define VWS_TAIL_BUCKET 1
+#define VWS_MAX_TEACHER 256
+typedef struct vws_distill_args {
+    uint32_t struct_size; /* sizeof(vws_distill_args): ABI guard */
+    int32_t rows;         /* N >= 1 */
+    int32_t vocab;        /* 1 <= V <= VWS_MAX_VOCAB */
+    int32_t dtype;        /* VWS_DTYPE_* of logits and grad */
+    const void* logits;   /* [N, V] */
+    int64_t logits_row_stride;
+    int32_t teacher_k;    /* 1 <= K <= VWS_MAX_TEACHER */
+    int32_t tail;         /* VWS_TAIL_* */
+    float temperature;    /* T > 0, finite */
+    const int32_t* teacher_ids;    /* [N, K] */
+    int64_t teacher_ids_row_stride;
+    const float* teacher_logprobs; /* [N, K] */
+    int64_t teacher_logprobs_row_stride;
+    const float* row_weight;       /* [N] or NULL (1) */
+    float* loss;                   /* [N] (forward, step) */
+    void* saved;                   /* vws_distill_saved_size() bytes, 16-byte aligned */
+    size_t saved_bytes;
+    const float* grad_output;      /* [N] upstream gradient of `loss`, or NULL (1) (backward, step) */
+    void* grad;                    /* [N, V] (backward, step) */
+    int64_t grad_row_stride;
+    void* workspace;               /* vws_distill_workspace_size() bytes, clean (vws_workspace_init) */
+    size_t workspace_bytes;        /* (forward, step) */
+    void* stream;
+} vws_distill_args;
+
+size_t vws_distill_saved_size(int32_t rows, int32_t teacher_k);
+size_t vws_distill_workspace_size(int32_t rows, int32_t vocab);
+int vws_distill_forward(const vws_distill_args* args);
+int vws_distill_backward(const vws_distill_args* args);
+int vws_distill_step(const vws_distill_args* args);
+
 /* Test hook (no counterpart in the reference): the bound, in polls of a few dozen cycles each,
  * of a top-p row's wait for the chunks of its shared passes that other workgroups run (default
  * 2^20; process-wide, read by each vws_sample launch).  A row that stops waiting takes the
@@ -294,7 +411,9 @@ int32_t vws_set_single_pass(int32_t enabled);
 #define VWS_KERNEL_SOFTMAX 3
 #define VWS_KERNEL_PENALTIES 4
 #define VWS_KERNEL_OTHER 5     /* workspace fill, self-test */
-#define VWS_KERNEL_KINDS 6
+#define VWS_KERNEL_VERIFY 6    /* the kernels of vws_verify_drafts */
+#define VWS_KERNEL_DISTILL 7   /* the kernels of vws_distill_* */
+#define VWS_KERNEL_KINDS 8
 int vws_profile_begin(int32_t max_launches);
 int vws_profile_end(double* ms, int32_t* count);
 

@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(_HERE, "_vws.so")
 # the same kernels built with per-workgroup phase stamps (vws_trace_set; vllm_webgpu_amd/trace.py)
 TRACE_LIB_PATH = os.path.join(_HERE, "_vws_trace.so")
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 OK = 0
 ERR_INVALID_ARGUMENT = 1
 ERR_UNSUPPORTED_DTYPE = 2
@@ -42,6 +42,10 @@ MAX_VOCAB = 1 << 19
 MAX_LOGPROBS = 64
 TOPK_MAX = 256
 NOALLOC_SCRATCH_BYTES = 16 << 20
+MAX_DRAFTS = 64
+MAX_TEACHER = 256
+TAIL_RENORMALIZE = 0
+TAIL_BUCKET = 1
 STATE_OUTPUT = 0
 STATE_PROMPT = 1
 STATE_PROMPT_FLAG = 0x80000000
@@ -60,9 +64,13 @@ EXPORTED = (
     "vws_topk", "vws_softmax", "vws_apply_penalties", "vws_math_selftest",
     "vws_profile_begin", "vws_profile_end", "vws_set_coop_wait_polls", "vws_set_single_pass",
     "vws_token_state_update", "vws_trace_set",
+    "vws_verify_workspace_size", "vws_verify_drafts",
+    "vws_distill_saved_size", "vws_distill_workspace_size", "vws_distill_forward",
+    "vws_distill_backward", "vws_distill_step",
 )
 
-KERNEL_KINDS = ("sample", "topk", "argmax", "softmax", "penalties", "other")
+KERNEL_KINDS = ("sample", "topk", "argmax", "softmax", "penalties", "other", "verify",
+                "distill")
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -91,6 +99,35 @@ class SampleArgs(ctypes.Structure):
         ("rng_key", ctypes.c_uint64), ("rng_key_set", _I32),
         ("sampled", _P), ("row_flags", _P), ("num_kept", _P),
         ("num_logprobs", _I32), ("logprob_ids", _P), ("logprob_vals", _P), ("logprob_ranks", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    """Mirror of ``vws_verify_args``."""
+
+    _fields_ = [
+        ("struct_size", _U32), ("batch", _I32), ("vocab", _I32), ("dtype", _I32),
+        ("num_drafts", _I32), ("max_drafts", _I32), ("logits", _P), ("logits_row_stride", _I64),
+        ("draft_tokens", _P), ("cu_drafts", _P), ("draft_probs", _P), ("draft_probs_row_stride", _I64),
+        ("draft_probs_dtype", _I32), ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P),
+        ("accept_uniforms", _P), ("uniforms", _P), ("uniforms_row_stride", _I64), ("rng_seeds", _P),
+        ("rng_offsets", _P), ("rng_key", ctypes.c_uint64), ("rng_key_set", _I32),
+        ("tokens", _P), ("num_accepted", _P), ("logprobs", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
+    ]
+
+
+class DistillArgs(ctypes.Structure):
+    """Mirror of ``vws_distill_args``."""
+
+    _fields_ = [
+        ("struct_size", _U32), ("rows", _I32), ("vocab", _I32), ("dtype", _I32),
+        ("logits", _P), ("logits_row_stride", _I64), ("teacher_k", _I32), ("tail", _I32),
+        ("temperature", ctypes.c_float), ("teacher_ids", _P), ("teacher_ids_row_stride", _I64),
+        ("teacher_logprobs", _P), ("teacher_logprobs_row_stride", _I64), ("row_weight", _P),
+        ("loss", _P), ("saved", _P), ("saved_bytes", _SZ), ("grad_output", _P),
+        ("grad", _P), ("grad_row_stride", _I64),
         ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
     ]
 
@@ -145,6 +182,17 @@ def _declare(L):
     L.vws_set_single_pass.argtypes = [_I32]
     L.vws_trace_set.restype = ctypes.c_int
     L.vws_trace_set.argtypes = [_P, _I32]
+    L.vws_verify_workspace_size.restype = _SZ
+    L.vws_verify_workspace_size.argtypes = [_I32, _I32, _I32]
+    L.vws_verify_drafts.restype = ctypes.c_int
+    L.vws_verify_drafts.argtypes = [ctypes.POINTER(VerifyArgs)]
+    L.vws_distill_saved_size.restype = _SZ
+    L.vws_distill_saved_size.argtypes = [_I32, _I32]
+    L.vws_distill_workspace_size.restype = _SZ
+    L.vws_distill_workspace_size.argtypes = [_I32, _I32]
+    for f in (L.vws_distill_forward, L.vws_distill_backward, L.vws_distill_step):
+        f.restype = ctypes.c_int
+        f.argtypes = [ctypes.POINTER(DistillArgs)]
     L.vws_token_state_update.restype = ctypes.c_int
     L.vws_token_state_update.argtypes = [_P, _I64, _P, _I64, _I32, _I32, _P, _I32, _P, _I32, _P]
 

@@ -10,9 +10,11 @@
 #include <mutex>
 #include <string>
 
+#include "vws_distill.h"
 #include "vws_internal.h"
 #include "vws_plain.h"
 #include "vws_sampler.h"
+#include "vws_verify.h"
 
 namespace vws {
 template <typename T> __global__ void fast_kernel(KArgs);
@@ -31,6 +33,11 @@ __global__ void selftest_kernel(int, uint32_t, uint32_t, unsigned long long*);
 __global__ void fill_u32_kernel(uint32_t*, size_t, uint32_t);
 __global__ void token_state_kernel(uint32_t*, int64_t, uint32_t*, int64_t, int, int, const int32_t*, int,
                                    const int32_t*, int);
+template <typename T> __global__ void verify_rows_kernel(VerifyArgs);
+template <typename T> __global__ void verify_cut_kernel(VerifyArgs);
+template <typename T> __global__ void verify_token_kernel(VerifyArgs);
+template <typename T, bool BUCKET> __global__ void distill_forward_kernel(DistillArgs);
+template <typename T> __global__ void distill_backward_kernel(DistillArgs);
 }  // namespace vws
 
 using namespace vws;
@@ -203,11 +210,15 @@ void prof_events(int kind, hipEvent_t* e0, hipEvent_t* e1) {
 // time is the kernel's duration, as a kernel trace reports it, with no marker packets between
 // back-to-back launches.
 template <typename F, typename... A>
-void launch(int kind, F k, dim3 g, dim3 b, hipStream_t s, A... args) {
+void launch_lds(int kind, F k, dim3 g, dim3 b, unsigned lds, hipStream_t s, A... args) {
     hipEvent_t e0, e1;
     prof_events(kind, &e0, &e1);
-    if (e0) hipExtLaunchKernelGGL(k, g, b, 0, s, e0, e1, 0u, args...);
-    else hipLaunchKernelGGL(k, g, b, 0, s, args...);
+    if (e0) hipExtLaunchKernelGGL(k, g, b, lds, s, e0, e1, 0u, args...);
+    else hipLaunchKernelGGL(k, g, b, lds, s, args...);
+}
+template <typename F, typename... A>
+void launch(int kind, F k, dim3 g, dim3 b, hipStream_t s, A... args) {
+    launch_lds(kind, k, g, b, 0, s, args...);
 }
 
 int validate_rows(const void* logits, int32_t dtype, int32_t B, int32_t V, int64_t stride) {
@@ -406,6 +417,186 @@ void softmax_launch(const T* logits, int B, int V, int64_t stride, const float* 
     launch(K, softmax_part_kernel<T>, dim3(B * n), dim3(kSmThreads), s, logits, stride, V, len, n, temperature, probs);
     launch(K, softmax_write_kernel<T>, dim3(B * n), dim3(kSmThreads), s, logits, stride, V, len, n, temperature, probs,
            row_max, log_sum);
+}
+
+// Parts of a row so that `rows` of them give about `wgs` workgroups, each of at least `min_len`
+// elements (a multiple of 64), at least `least` parts.
+void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* S, int* len) {
+    int s = wgs / rows;
+    if (s > V / min_len) s = V / min_len;
+    if (s > most) s = most;
+    if (s < least) s = least;
+    *len = ((V + s - 1) / s + 63) / 64 * 64;
+    *S = (V + *len - 1) / *len;
+}
+
+// Workgroups a launch is split into: eight of 256 threads for each of the chip's 256 compute units,
+// which is what they hold at once.
+constexpr int kSplitWgs = 2048;
+
+void verify_parts(int rows, int V, int* S, int* len) { split_row(rows, V, kSplitWgs, 4096, kVfMaxParts, 1, S, len); }
+
+// A launch takes at most kTopkRows rows (the counters of the fixed region); a part's bitmap of
+// teacher entries takes at most 32 KB.
+void distill_parts(int rows, int V, int* S, int* len) {
+    split_row(rows, V, kSplitWgs, 4096, kDsMaxParts, (V + (1 << 18) - 1) >> 18, S, len);
+}
+
+bool dtype_ok(int32_t d) { return d == VWS_DTYPE_F32 || d == VWS_DTYPE_BF16 || d == VWS_DTYPE_F16; }
+
+constexpr int kVerifyMaxRows = 1 << 24;
+
+int validate_verify(const vws_verify_args* a) {
+    if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
+    if (a->struct_size != sizeof(vws_verify_args))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(vws_verify_args));
+    if (int st = validate_rows(a->logits, a->dtype, a->batch, a->vocab, a->logits_row_stride)) return st;
+    if (a->num_drafts < 0) return fail(VWS_ERR_INVALID_ARGUMENT, "num_drafts must be >= 0 (got %d)", a->num_drafts);
+    if (a->max_drafts < 0 || a->max_drafts > VWS_MAX_DRAFTS)
+        return fail(VWS_ERR_LIMIT, "max_drafts must be in [0, %d] (got %d)", VWS_MAX_DRAFTS, a->max_drafts);
+    if (a->batch > kVerifyMaxRows || a->num_drafts > kVerifyMaxRows - a->batch)
+        return fail(VWS_ERR_LIMIT, "num_drafts + batch must be at most %d", kVerifyMaxRows);
+    if (!a->cu_drafts) return fail(VWS_ERR_INVALID_ARGUMENT, "cu_drafts is NULL");
+    if (a->num_drafts > 0 && !a->draft_tokens) return fail(VWS_ERR_INVALID_ARGUMENT, "draft_tokens is NULL");
+    if (a->draft_probs) {
+        if (!dtype_ok(a->draft_probs_dtype))
+            return fail(VWS_ERR_UNSUPPORTED_DTYPE, "unsupported draft_probs dtype %d", a->draft_probs_dtype);
+        if (a->draft_probs_row_stride < a->vocab)
+            return fail(VWS_ERR_INVALID_ARGUMENT, "draft_probs_row_stride < vocab");
+    }
+    if (a->temperature) {
+        if (!a->uniforms && !a->rng_seeds && !a->rng_key_set)
+            return fail(VWS_ERR_INVALID_ARGUMENT,
+                        "uniforms, rng_seeds or rng_key_set is required when temperature is given");
+        if (a->uniforms && a->uniforms_row_stride < a->vocab)
+            return fail(VWS_ERR_INVALID_ARGUMENT, "uniforms_row_stride < vocab");
+        if (a->uniforms && a->num_drafts > 0 && !a->accept_uniforms)
+            return fail(VWS_ERR_INVALID_ARGUMENT, "accept_uniforms is required with uniforms");
+    }
+    if (!a->tokens || !a->num_accepted || !a->logprobs) return fail(VWS_ERR_INVALID_ARGUMENT, "outputs are NULL");
+    const size_t need = vws_verify_workspace_size(a->batch, a->num_drafts, a->vocab);
+    if (!a->workspace || a->workspace_bytes < need)
+        return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu",
+                    a->workspace ? a->workspace_bytes : (size_t)0, need);
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 255u)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    return VWS_OK;
+}
+
+template <typename T>
+int verify_launch(const VerifyArgs& k, bool cuts, hipStream_t s) {
+    const int K = VWS_KERNEL_VERIFY;
+    launch(K, verify_rows_kernel<T>, dim3((unsigned)k.R * (unsigned)k.S), dim3(kVfThreads), s, k);
+    if (int st = check_launch("vws_verify_drafts (rows)")) return st;
+    if (cuts) {
+        launch(K, verify_cut_kernel<T>, dim3((unsigned)k.R), dim3(kVfCutThreads), s, k);
+        if (int st = check_launch("vws_verify_drafts (cuts)")) return st;
+    }
+    launch(K, verify_token_kernel<T>, dim3((unsigned)k.B * (unsigned)k.S2), dim3(kVfThreads), s, k);
+    return check_launch("vws_verify_drafts (tokens)");
+}
+
+enum DistillPart { kDistillForward = 1, kDistillBackward = 2 };
+
+int validate_distill(const vws_distill_args* a, int parts) {
+    if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
+    if (a->struct_size != sizeof(vws_distill_args))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(vws_distill_args));
+    if (int st = validate_rows(a->logits, a->dtype, a->rows, a->vocab, a->logits_row_stride)) return st;
+    if (a->rows > kVerifyMaxRows) return fail(VWS_ERR_LIMIT, "rows must be at most %d", kVerifyMaxRows);
+    if (a->teacher_k < 1 || a->teacher_k > VWS_MAX_TEACHER)
+        return fail(VWS_ERR_LIMIT, "teacher_k must be in [1, %d] (got %d)", VWS_MAX_TEACHER, a->teacher_k);
+    if (a->tail != VWS_TAIL_RENORMALIZE && a->tail != VWS_TAIL_BUCKET)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "tail must be VWS_TAIL_RENORMALIZE or VWS_TAIL_BUCKET (got %d)", a->tail);
+    // (the least T keeps log2(e) / T and 1 / T finite)
+    if (!(a->temperature >= 1e-5f) || a->temperature == __builtin_inff())
+        return fail(VWS_ERR_INVALID_ARGUMENT, "temperature must be finite and >= 1e-5 (got %g)", (double)a->temperature);
+    if (!a->teacher_ids || !a->teacher_logprobs) return fail(VWS_ERR_INVALID_ARGUMENT, "teacher_ids or teacher_logprobs is NULL");
+    if (a->teacher_ids_row_stride < a->teacher_k || a->teacher_logprobs_row_stride < a->teacher_k)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "a teacher row stride is less than teacher_k");
+    const size_t saved = vws_distill_saved_size(a->rows, a->teacher_k);
+    if (!a->saved || a->saved_bytes < saved)
+        return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "saved has %zu bytes, need %zu", a->saved ? a->saved_bytes : (size_t)0, saved);
+    if (reinterpret_cast<uintptr_t>(a->saved) & 15u) return fail(VWS_ERR_INVALID_ARGUMENT, "saved must be 16-byte aligned");
+    if (parts & kDistillForward) {
+        if (!a->loss) return fail(VWS_ERR_INVALID_ARGUMENT, "loss is NULL");
+        const size_t need = vws_distill_workspace_size(a->rows, a->vocab);
+        if (!a->workspace || a->workspace_bytes < need)
+            return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu",
+                        a->workspace ? a->workspace_bytes : (size_t)0, need);
+        if (reinterpret_cast<uintptr_t>(a->workspace) & 255u)
+            return fail(VWS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    }
+    if (parts & kDistillBackward) {
+        if (!a->grad) return fail(VWS_ERR_INVALID_ARGUMENT, "grad is NULL");
+        if (a->grad_row_stride < a->vocab) return fail(VWS_ERR_INVALID_ARGUMENT, "grad_row_stride < vocab");
+        const size_t es = a->dtype == VWS_DTYPE_F32 ? 4 : 2;
+        const uintptr_t x0 = reinterpret_cast<uintptr_t>(a->logits), g0 = reinterpret_cast<uintptr_t>(a->grad);
+        const uintptr_t x1 = x0 + ((size_t)(a->rows - 1) * (size_t)a->logits_row_stride + (size_t)a->vocab) * es;
+        const uintptr_t g1 = g0 + ((size_t)(a->rows - 1) * (size_t)a->grad_row_stride + (size_t)a->vocab) * es;
+        const bool same = x0 == g0 && (a->rows == 1 || a->logits_row_stride == a->grad_row_stride);
+        if (!same && x0 < g1 && g0 < x1)
+            return fail(VWS_ERR_INVALID_ARGUMENT, "grad overlaps the logits without being their memory");
+    }
+    return VWS_OK;
+}
+
+template <typename T>
+int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
+    DistillArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.x = static_cast<const T*>(a->logits) + (size_t)r0 * a->logits_row_stride;
+    k.xstride = a->logits_row_stride;
+    k.N = rows;
+    k.V = a->vocab;
+    k.K = a->teacher_k;
+    k.ids = a->teacher_ids + (size_t)r0 * a->teacher_ids_row_stride;
+    k.ids_stride = a->teacher_ids_row_stride;
+    k.lp = a->teacher_logprobs + (size_t)r0 * a->teacher_logprobs_row_stride;
+    k.lp_stride = a->teacher_logprobs_row_stride;
+    k.weight = a->row_weight ? a->row_weight + r0 : nullptr;
+    k.c = (float)(1.4426950408889634 / (double)a->temperature);
+    k.inv_T = 1.0f / a->temperature;
+    k.gout = a->grad_output ? a->grad_output + r0 : nullptr;
+    k.grad = a->grad ? static_cast<T*>(a->grad) + (size_t)r0 * a->grad_row_stride : nullptr;
+    k.gstride = a->grad_row_stride;
+    k.loss = a->loss ? a->loss + r0 : nullptr;
+    k.stats = static_cast<float*>(a->saved) + (size_t)r0 * kDsRowStats;
+    k.entry_p = static_cast<float*>(a->saved) + (size_t)a->rows * kDsRowStats + (size_t)r0 * k.K;
+    const int K = VWS_KERNEL_DISTILL;
+    hipStream_t s = (hipStream_t)a->stream;
+    distill_parts(rows, k.V, &k.S, &k.part_len);
+    const dim3 grid((unsigned)rows * (unsigned)k.S), block(kDsThreads);
+    if (parts & kDistillForward) {
+        k.ctr = static_cast<CoopState*>(a->workspace)->topk_ctr;
+        k.rec = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + align256(sizeof(CoopState)));
+        if (a->tail == VWS_TAIL_BUCKET) {
+            const unsigned lds = (unsigned)((k.part_len + 31) / 32) * 4u;
+            launch_lds(K, distill_forward_kernel<T, true>, grid, block, lds, s, k);
+        } else {
+            launch(K, distill_forward_kernel<T, false>, grid, block, s, k);
+        }
+        if (int st = check_launch("vws_distill (forward)")) return st;
+    }
+    if (parts & kDistillBackward) {
+        launch(K, distill_backward_kernel<T>, grid, block, s, k);
+        if (int st = check_launch("vws_distill (backward)")) return st;
+    }
+    return VWS_OK;
+}
+
+template <typename T>
+int distill_launch(const vws_distill_args* a, int parts) {
+    for (int r0 = 0; r0 < a->rows; r0 += kTopkRows)
+        if (int st = distill_rows<T>(a, parts, r0, a->rows - r0 < kTopkRows ? a->rows - r0 : kTopkRows)) return st;
+    return ok();
+}
+
+int distill(const vws_distill_args* a, int parts) {
+    if (int st = validate_distill(a, parts)) return st;
+    if (a->dtype == VWS_DTYPE_F32) return distill_launch<float>(a, parts);
+    if (a->dtype == VWS_DTYPE_BF16) return distill_launch<uint16_t>(a, parts);
+    return distill_launch<_Float16>(a, parts);
 }
 
 }  // namespace
@@ -714,6 +905,84 @@ int vws_apply_penalties(float* logits, int32_t batch, int32_t vocab, int64_t row
     if ((st = check_launch("vws_apply_penalties"))) return st;
     return ok();
 }
+
+size_t vws_verify_workspace_size(int32_t batch, int32_t num_drafts, int32_t vocab) {
+    if (batch < 1 || num_drafts < 0 || vocab < 1 || vocab > VWS_MAX_VOCAB || batch > kVerifyMaxRows ||
+        num_drafts > kVerifyMaxRows - batch)
+        return 0;
+    int S, S2, len;
+    verify_parts(batch + num_drafts, vocab, &S, &len);
+    verify_parts(batch, vocab, &S2, &len);
+    return vf_layout(batch + num_drafts, batch, S, S2).total;
+}
+
+int vws_verify_drafts(const vws_verify_args* a) {
+    if (int st = validate_verify(a)) return st;
+    VerifyArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.x = a->logits;
+    k.xstride = a->logits_row_stride;
+    k.B = a->batch;
+    k.D = a->num_drafts;
+    k.R = a->batch + a->num_drafts;
+    k.V = a->vocab;
+    k.K = a->max_drafts;
+    k.drafts = a->draft_tokens;
+    k.cu = a->cu_drafts;
+    k.q = a->draft_probs;
+    k.qstride = a->draft_probs_row_stride;
+    k.qdtype = a->draft_probs_dtype;
+    k.temperature = a->temperature;
+    k.top_k = a->top_k;
+    k.top_p = a->top_p;
+    k.min_p = a->min_p;
+    k.au = a->accept_uniforms;
+    k.u = a->uniforms;
+    k.ustride = a->uniforms_row_stride;
+    k.rng_seed = a->rng_seeds;
+    k.rng_offset = a->rng_offsets;
+    k.rng_key = a->rng_key;
+    k.tokens = a->tokens;
+    k.accepted = a->num_accepted;
+    k.logprobs = a->logprobs;
+    verify_parts(k.R, k.V, &k.S, &k.part_len);
+    verify_parts(k.B, k.V, &k.S2, &k.part2_len);
+    const VfLayout w = vf_layout(k.R, k.B, k.S, k.S2);
+    char* base = static_cast<char*>(a->workspace);
+    k.rec = reinterpret_cast<VfRec*>(base + w.rec);
+    k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
+    k.best = reinterpret_cast<uint64_t*>(base + w.best);
+    k.ctr = reinterpret_cast<uint32_t*>(base + w.ctr);
+    const bool cuts = a->temperature && (a->top_k || a->top_p || a->min_p);
+    hipStream_t s = (hipStream_t)a->stream;
+    const int st = a->dtype == VWS_DTYPE_F32    ? verify_launch<float>(k, cuts, s)
+                   : a->dtype == VWS_DTYPE_BF16 ? verify_launch<uint16_t>(k, cuts, s)
+                                                : verify_launch<_Float16>(k, cuts, s);
+    return st ? st : ok();
+}
+
+size_t vws_distill_saved_size(int32_t rows, int32_t teacher_k) {
+    if (rows < 1 || teacher_k < 1) return 0;
+    return sizeof(float) * (size_t)rows * (size_t)(kDsRowStats + teacher_k);
+}
+
+size_t vws_distill_workspace_size(int32_t rows, int32_t vocab) {
+    if (rows < 1 || vocab < 1 || vocab > VWS_MAX_VOCAB) return 0;
+    int S, len;
+    // (of the launches of at most kTopkRows rows, the last may be split further than the others)
+    const int most = rows < kTopkRows ? rows : kTopkRows, tail = rows % kTopkRows;
+    distill_parts(most, vocab, &S, &len);
+    size_t recs = (size_t)most * S;
+    if (tail) {
+        distill_parts(tail, vocab, &S, &len);
+        if ((size_t)tail * S > recs) recs = (size_t)tail * S;
+    }
+    return align256(sizeof(CoopState)) + align256(sizeof(uint64_t) * recs);
+}
+
+int vws_distill_forward(const vws_distill_args* args) { return distill(args, kDistillForward); }
+int vws_distill_backward(const vws_distill_args* args) { return distill(args, kDistillBackward); }
+int vws_distill_step(const vws_distill_args* args) { return distill(args, kDistillForward | kDistillBackward); }
 
 int vws_math_selftest(int32_t fn, uint32_t key_lo, uint32_t key_hi, uint64_t* out2, void* stream) {
     if (fn < 0 || fn > 3) return fail(VWS_ERR_INVALID_ARGUMENT, "fn must be 0 (exp), 1 (log), 2 (soft cap) or 3 (f16 rounding)");

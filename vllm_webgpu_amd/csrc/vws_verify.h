@@ -1,0 +1,71 @@
+// vws_verify.h -- argument block, shape constants and workspace layout of draft verification
+// (vws_verify.hip), shared with its launcher (vws_capi.hip).
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "vws_internal.h"
+
+namespace vws {
+
+constexpr int kVfThreads = 256;      // threads of a part (row statistics, race)
+constexpr int kVfCutThreads = 1024;  // threads of a cut row
+constexpr int kVfMaxParts = 64;      // parts of a row: one lane each in the join
+constexpr int kVfMaxDrafts = 64;     // VWS_MAX_DRAFTS: one lane each in the decision
+constexpr uint32_t kVfAcceptBase = 1u << 19;  // VWS_MAX_VOCAB: generated acceptance uniforms' tokens
+
+// A row's statistics.  One per part for rows that nothing cuts (sum: of exp2(x log2(e) / T - m2)
+// over the part), or the row's own (part 0) where its request cuts it (sum: the kept exponentials).
+struct VfRec {
+    uint64_t top;  // key of the largest logit << 32 | 0x7FFFFFFF - its lowest index; 0: all NaN
+    float m2;      // the maximum that `sum` is relative to
+    float sum;
+};
+
+struct VerifyArgs {
+    const void* x;               // [R, V] target logits, n_b + 1 rows per request
+    int64_t xstride;
+    int R, V, B, D, K;           // K: columns of drafts in the outputs
+    const int32_t* drafts;       // [D]
+    const int32_t* cu;           // [B + 1]
+    const void* q;               // [D, V] draft probabilities or null
+    int64_t qstride;
+    int qdtype;
+    const float* temperature;    // [B]; null: greedy
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* au;             // [D] acceptance uniforms (when u is given)
+    const float* u;              // [B, V] race uniforms or null
+    int64_t ustride;
+    const uint64_t* rng_seed;    // [B]
+    const uint64_t* rng_offset;  // [B] or null
+    uint64_t rng_key;
+    int32_t* tokens;             // [B, K + 1]
+    int32_t* accepted;           // [B]
+    float* logprobs;             // [B, K + 1]
+    int S, part_len;             // parts of a row in the statistics
+    int S2, part2_len;           // parts of a row in the race
+    VfRec* rec;                  // [R, S]
+    uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
+    uint64_t* best;              // [B, S2] race: key bits << 32 | 0x7FFFFFFF - index
+    uint32_t* ctr;               // [B] race parts arrived; cleared by the statistics' launch
+};
+
+struct VfLayout {
+    size_t rec, cut, best, ctr, total;
+};
+
+inline VfLayout vf_layout(int R, int B, int S, int S2) {
+    VfLayout w{};
+    size_t off = align256(sizeof(CoopState));  // every workspace starts with the fixed region
+    w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
+    w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
+    w.best = off;  off = align256(off + sizeof(uint64_t) * (size_t)B * S2);
+    w.ctr = off;   off = align256(off + sizeof(uint32_t) * (size_t)B);
+    w.total = off;
+    return w;
+}
+
+}  // namespace vws

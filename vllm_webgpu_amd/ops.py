@@ -436,6 +436,228 @@ def apply_penalties(logits: torch.Tensor, repetition_penalty=None, presence_pena
     return logits
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with contiguous rows that do not overlap (a broadcast tensor is copied)."""
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    # (a single row's stride says nothing)
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
+
+
+@dataclass
+class VerifyResult:
+    tokens: torch.Tensor        # [B, max_drafts + 1] int32: accepted drafts, the drawn token, then -1
+    num_accepted: torch.Tensor  # [B] int32
+    logprobs: torch.Tensor      # [B, max_drafts + 1] float32 of the emitted tokens
+
+
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor, max_drafts: int,
+                  draft_probs: torch.Tensor | None = None, temperature=None, top_k=None, top_p=None, min_p=None,
+                  accept_uniforms: torch.Tensor | None = None, uniforms: torch.Tensor | None = None,
+                  rng_seeds: torch.Tensor | None = None, rng_offsets: torch.Tensor | None = None,
+                  rng_key: int | None = None) -> VerifyResult:
+    """Verifies each request's drafted tokens against the target's logits and draws one token more,
+    so that the emitted tokens are distributed as ``sample``'s.
+
+    ``cu_drafts`` [B + 1] int32 is the running count of drafts (0 first, D last); request b's
+    drafts are ``draft_tokens[cu_drafts[b]:cu_drafts[b + 1]]`` (int32, at most ``max_drafts`` <= 64)
+    and its rows of ``logits`` [D + B, V] are ``cu_drafts[b] + b`` and the next n_b: row i holds the
+    target's logits after its first i drafts.  ``draft_probs`` [D, V] (float32, bfloat16 or
+    float16) are the distributions that the drafts were drawn from; None: looked-up or greedy
+    drafts (all mass on the draft).  ``temperature`` (None = every request greedy), ``top_k``,
+    ``top_p`` and ``min_p`` are scalars or [B] tensors, with ``sample``'s rules.
+
+    Draft i is accepted iff ``q(d) > 0 and u q(d) < p(d)``; after the first refusal a token is drawn
+    from ``max(p - q, 0)`` (None: p without the draft), after the last accepted draft from the last
+    row's p.  The random numbers are ``accept_uniforms`` [D] and ``uniforms`` [B, V] float32 in
+    (0, 1), or generated from ``rng_seeds`` / ``rng_offsets`` [B] int64 or one ``rng_key`` as for
+    ``sample`` (draft i's acceptance: token 2**19 + i of the request's key).
+
+    Returns tokens [B, max_drafts + 1] (-1 past the drawn token), the number of accepted drafts [B]
+    (-1 and no token for a request whose bounds do not fit) and the emitted tokens' log
+    probabilities under p (0 where it is a sure token)."""
+    _check_device(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [num_drafts + batch, V]")
+    logits = _rows(logits)
+    dev, (R, V) = logits.device, logits.shape
+    cu = cu_drafts.to(device=dev, dtype=torch.int32).contiguous()
+    drafts = draft_tokens.to(device=dev, dtype=torch.int32).contiguous()
+    if cu.dim() != 1 or cu.numel() < 1 or drafts.dim() != 1:
+        raise ValueError("cu_drafts must be [batch + 1] and draft_tokens [num_drafts]")
+    B, D, K = cu.numel() - 1, drafts.numel(), int(max_drafts)
+    if R != D + B:
+        raise ValueError(f"logits must have a row per draft and one more per request: {D} + {B}, got {R}")
+    if not 0 <= K <= _lib.MAX_DRAFTS:
+        raise ValueError(f"max_drafts must be in [0, {_lib.MAX_DRAFTS}] (got {max_drafts})")
+    T = _row_param(temperature, B, torch.float32, dev, "temperature")
+    TK = _row_param(top_k, B, torch.int32, dev, "top_k")
+    TP = _row_param(top_p, B, torch.float32, dev, "top_p")
+    MP = _row_param(min_p, B, torch.float32, dev, "min_p")
+    if draft_probs is not None:
+        _check_device(draft_probs, "draft_probs")
+        if draft_probs.shape != (D, V):
+            raise ValueError(f"draft_probs must be [{D}, {V}] (got {tuple(draft_probs.shape)})")
+        draft_probs = _rows(draft_probs)
+    U = AU = SEED = OFF = None
+    if uniforms is not None:
+        _check_device(uniforms, "uniforms")
+        if uniforms.shape != (B, V):
+            raise ValueError(f"uniforms must be [{B}, {V}]")
+        U = _rows(uniforms if uniforms.dtype == torch.float32 else uniforms.float())
+        if accept_uniforms is None:
+            raise ValueError("accept_uniforms is required with uniforms")
+        AU = accept_uniforms.to(device=dev, dtype=torch.float32).contiguous()
+        if AU.shape != (D,):
+            raise ValueError(f"accept_uniforms must have shape ({D},), got {tuple(AU.shape)}")
+    elif rng_seeds is not None:
+        SEED = _row_param(rng_seeds, B, torch.int64, dev, "rng_seeds")
+        OFF = _row_param(rng_offsets, B, torch.int64, dev, "rng_offsets")
+    elif T is not None and rng_key is None:
+        raise ValueError("uniforms, rng_seeds or rng_key is required when temperature is given")
+    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    logprobs = torch.empty((B, K + 1), dtype=torch.float32, device=dev)
+    if B == 0:
+        return VerifyResult(tokens, accepted, logprobs)
+    L = _lib.lib()
+    stream = _stream_ptr()
+    ws = _workspace(L.vws_verify_workspace_size(B, D, V), dev.index, stream, _capturing(stream))
+    a = _lib.VerifyArgs()
+    a.struct_size = ctypes.sizeof(_lib.VerifyArgs)
+    a.batch, a.vocab, a.dtype = B, V, _dtype_code(logits)
+    a.num_drafts, a.max_drafts = D, K
+    a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
+    a.draft_tokens, a.cu_drafts = drafts.data_ptr() if D else None, cu.data_ptr()
+    if draft_probs is not None and D:
+        a.draft_probs, a.draft_probs_row_stride = draft_probs.data_ptr(), _row_stride(draft_probs)
+        a.draft_probs_dtype = _dtype_code(draft_probs)
+    a.temperature, a.top_k, a.top_p, a.min_p = _ptr(T), _ptr(TK), _ptr(TP), _ptr(MP)
+    a.accept_uniforms, a.uniforms = AU.data_ptr() if AU is not None and D else None, _ptr(U)
+    a.uniforms_row_stride = _row_stride(U) if U is not None else 0
+    a.rng_seeds, a.rng_offsets = _ptr(SEED), _ptr(OFF)
+    if U is None and SEED is None and rng_key is not None:
+        a.rng_key, a.rng_key_set = int(rng_key) & 0xFFFFFFFFFFFFFFFF, 1
+    a.tokens, a.num_accepted, a.logprobs = tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr()
+    a.workspace, a.workspace_bytes, a.stream = ws.data_ptr(), ws.numel(), stream
+    _lib.check(L.vws_verify_drafts(ctypes.byref(a)))
+    return VerifyResult(tokens, accepted, logprobs)
+
+
+_TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "bucket": _lib.TAIL_BUCKET}
+
+
+def _distill_args(logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail):
+    """(argument block, the tensors it points at): the checks and inputs the distillation calls share."""
+    _check_device(logits, "logits")
+    _check_device(teacher_ids, "teacher_ids")
+    _check_device(teacher_logprobs, "teacher_logprobs")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, V]")
+    if tail not in _TAILS:
+        raise ValueError(f"tail must be one of {sorted(_TAILS)} (got {tail!r})")
+    (N, V), dev = logits.shape, logits.device
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != N or teacher_logprobs.shape != teacher_ids.shape:
+        raise ValueError(f"teacher_ids and teacher_logprobs must be [{N}, K] (got {tuple(teacher_ids.shape)} and "
+                         f"{tuple(teacher_logprobs.shape)})")
+    K = teacher_ids.shape[1]
+    if not 1 <= K <= _lib.MAX_TEACHER:
+        raise ValueError(f"teacher entries per row must be in [1, {_lib.MAX_TEACHER}] (got {K})")
+    if teacher_ids.dtype != torch.int32:
+        teacher_ids = teacher_ids.to(torch.int32)
+    if teacher_logprobs.dtype != torch.float32:
+        teacher_logprobs = teacher_logprobs.float()
+    logits, ids, lp = _rows(logits), _rows(teacher_ids), _rows(teacher_logprobs)
+    W = _row_param(row_weight, N, torch.float32, dev, "row_weight")
+    a = _lib.DistillArgs()
+    a.struct_size = ctypes.sizeof(_lib.DistillArgs)
+    a.rows, a.vocab, a.dtype, a.teacher_k, a.tail = N, V, _dtype_code(logits), K, _TAILS[tail]
+    a.temperature = float(temperature)
+    a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
+    a.teacher_ids, a.teacher_ids_row_stride = ids.data_ptr(), _row_stride(ids)
+    a.teacher_logprobs, a.teacher_logprobs_row_stride = lp.data_ptr(), _row_stride(lp)
+    a.row_weight = _ptr(W)
+    return a, (logits, ids, lp, W)
+
+
+def _distill_run(a, dev, forward: bool, fn) -> None:
+    L = _lib.lib()
+    a.stream = stream = _stream_ptr()
+    if forward:
+        ws = _workspace(L.vws_distill_workspace_size(a.rows, a.vocab), dev.index, stream, _capturing(stream))
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _lib.check(fn(ctypes.byref(a)))
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail):
+        a, keep = _distill_args(logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail)
+        N, dev = a.rows, logits.device
+        loss = torch.empty(N, dtype=torch.float32, device=dev)
+        saved = torch.empty(N * (8 + a.teacher_k), dtype=torch.float32, device=dev)
+        if N:
+            a.loss, a.saved, a.saved_bytes = loss.data_ptr(), saved.data_ptr(), 4 * saved.numel()
+            _distill_run(a, dev, True, _lib.lib().vws_distill_forward)
+        ctx.save_for_backward(keep[0], keep[1], keep[2], *([] if keep[3] is None else [keep[3]]), saved)
+        ctx.options = temperature, tail
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        logits, ids, lp, *weight, saved = ctx.saved_tensors
+        a, keep = _distill_args(logits, ids, lp, weight[0] if weight else None, *ctx.options)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if a.rows:
+            g = grad_output.to(torch.float32).contiguous()
+            a.saved, a.saved_bytes, a.grad_output = saved.data_ptr(), 4 * saved.numel(), g.data_ptr()
+            a.grad, a.grad_row_stride = grad.data_ptr(), grad.shape[1]
+            _distill_run(a, logits.device, False, _lib.lib().vws_distill_backward)
+        return grad, None, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, row_weight=None,
+                 temperature: float = 1.0, tail: str = "renormalize") -> torch.Tensor:
+    """Per-row distillation loss [N] float32 of student ``logits`` [N, V] against the teacher's top
+    entries ``teacher_ids`` [N, K] int32 and ``teacher_logprobs`` [N, K] float32, K <= 256 (the
+    columns that ``sample`` returns as ``logprob_ids`` / ``logprob_vals``), differentiable in
+    ``logits`` (whose gradient has their type).
+
+    q = softmax(x / T).  ``tail="renormalize"``: the teacher's entries are a distribution of their
+    own, p = softmax(l / T); the loss is sum p (log p - log q).  ``tail="bucket"``: p = exp(l) (log
+    probabilities at temperature T) and the rest of the vocabulary is one more event, 1 - sum p
+    against the student's probability of everything outside the entries.  Ids outside [0, V) are
+    padding, entries that share an id add up.  ``row_weight`` (scalar or [N]) multiplies a row's
+    loss and gradient; rows of weight 0 are not read.  Rows without an entry have loss 0."""
+    return _DistillLoss.apply(logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail)
+
+
+def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor,
+                          row_weight=None, temperature: float = 1.0, tail: str = "renormalize", grad_output=None,
+                          out: torch.Tensor | None = None):
+    """``distill_loss`` [N] and its gradient [N, V] in one call, for an upstream gradient known
+    beforehand: ``grad_output``, a scalar or [N] (None = 1).  The gradient is written to ``out``
+    if given: a tensor of the logits' shape and type, ``logits`` itself among them."""
+    a, keep = _distill_args(logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail)
+    (N, V), dev = logits.shape, logits.device
+    g = _row_param(grad_output, N, torch.float32, dev, "grad_output")
+    if out is None:
+        out = torch.empty((N, V), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or out.stride(1) != 1:
+        raise ValueError("out must have the logits' shape, type and device, with contiguous rows")
+    loss = torch.empty(N, dtype=torch.float32, device=dev)
+    if N:
+        saved = torch.empty(N * (8 + a.teacher_k), dtype=torch.float32, device=dev)
+        a.loss, a.saved, a.saved_bytes = loss.data_ptr(), saved.data_ptr(), 4 * saved.numel()
+        a.grad_output, a.grad = _ptr(g), out.data_ptr()
+        a.grad_row_stride = _row_stride(out)
+        _distill_run(a, dev, True, _lib.lib().vws_distill_step)
+    return loss, out
+
+
 def math_selftest(fn: int, key_lo: int, key_hi: int) -> tuple[int, int]:
     """Device hash of exp_det (fn=0), log_det (fn=1) or the soft cap's tanh (fn=2, cap 1) over
     an order-key range; synchronises."""
