@@ -950,6 +950,7 @@ int vws_verify_drafts(const vws_verify_args* a) {
     const VfLayout w = vf_layout(k.R, k.B, k.S, k.S2);
     char* base = static_cast<char*>(a->workspace);
     k.rec = reinterpret_cast<VfRec*>(base + w.rec);
+    k.peaks = reinterpret_cast<float*>(base + w.peaks);
     k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
     k.best = reinterpret_cast<uint64_t*>(base + w.best);
     k.ctr = reinterpret_cast<uint32_t*>(base + w.ctr);

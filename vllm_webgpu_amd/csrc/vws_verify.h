@@ -16,7 +16,8 @@ constexpr int kVfMaxDrafts = 64;     // VWS_MAX_DRAFTS: one lane each in the dec
 constexpr uint32_t kVfAcceptBase = 1u << 19;  // VWS_MAX_VOCAB: generated acceptance uniforms' tokens
 
 // A row's statistics.  One per part for rows that nothing cuts (sum: of exp2(x log2(e) / T - m2)
-// over the part), or the row's own (part 0) where its request cuts it (sum: the kept exponentials).
+// over the part), or the row's own (part 0) once verify_cut_kernel has cut it (m2: the maximum of
+// y, sum: the kept exponentials).
 struct VfRec {
     uint64_t top;  // key of the largest logit << 32 | 0x7FFFFFFF - its lowest index; 0: all NaN
     float m2;      // the maximum that `sum` is relative to
@@ -48,19 +49,31 @@ struct VerifyArgs {
     int S, part_len;             // parts of a row in the statistics
     int S2, part2_len;           // parts of a row in the race
     VfRec* rec;                  // [R, S]
+    float* peaks;                // [R, vf_peaks(S)] maxima of groups of threads, rows that are cut
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
     uint64_t* best;              // [B, S2] race: key bits << 32 | 0x7FFFFFFF - index
     uint32_t* ctr;               // [B] race parts arrived; cleared by the statistics' launch
 };
 
+constexpr int kVfPeaks = 1024;       // most maxima kept of a row
+
+// Threads of a part that share one maximum, and the maxima of a row.
+inline __host__ __device__ int vf_peak_group(int S) {
+    int g = 1;
+    while (kVfThreads * S / g > kVfPeaks) g *= 2;
+    return g;
+}
+inline __host__ __device__ int vf_peaks(int S) { return S * (kVfThreads / vf_peak_group(S)); }
+
 struct VfLayout {
-    size_t rec, cut, best, ctr, total;
+    size_t rec, peaks, cut, best, ctr, total;
 };
 
 inline VfLayout vf_layout(int R, int B, int S, int S2) {
     VfLayout w{};
     size_t off = align256(sizeof(CoopState));  // every workspace starts with the fixed region
     w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
+    w.peaks = off; off = align256(off + sizeof(float) * (size_t)R * vf_peaks(S));
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
     w.best = off;  off = align256(off + sizeof(uint64_t) * (size_t)B * S2);
     w.ctr = off;   off = align256(off + sizeof(uint32_t) * (size_t)B);

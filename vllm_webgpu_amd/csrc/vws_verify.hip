@@ -78,6 +78,7 @@ struct VfParams {
     float T, top_p, min_p;
     int k;
     bool greedy, cuts;
+    bool sums;  // the row's sum of exponentials over all its tokens is used
 };
 __device__ __forceinline__ VfParams vf_params(const VerifyArgs& a, int b) {
     VfParams p;
@@ -88,6 +89,7 @@ __device__ __forceinline__ VfParams vf_params(const VerifyArgs& a, int b) {
     p.top_p = a.top_p ? a.top_p[b] : 1.0f;
     p.min_p = a.min_p ? a.min_p[b] : 0.0f;
     p.cuts = !p.greedy && (p.k > 0 || 1.0f - p.top_p > 0.0f || p.min_p > 0.0f);
+    p.sums = !p.greedy && p.k == 0 && !(p.min_p > 0.0f);
     return p;
 }
 
@@ -125,7 +127,6 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, wave = tid >> 6;
     if (p == 0 && tid == 0 && r < a.B) a.ctr[r] = 0u;  // (R >= B)
     const VfParams prm = vf_params(a, vf_request(a, r));
-    if (prm.cuts) return;
     const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) g = __builtin_fmaxf(g, v[u][j]);
         if (g == g && !(g <= best)) { best = g; group = b; }
-        if (!prm.greedy) {
+        if (prm.sums) {
             const float n = __builtin_fmaxf(t.m, g * c), ref = n == -kVfInf ? 0.0f : n;
             float acc[4] = {t.s * vf_exp2(t.m - ref), 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -179,7 +180,13 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     if (i < len) {
         const float x = Elem<T>::load1(row + i);
         top = vws_max64(top, vf_pack(key_of(x), lo + i));
-        if (!prm.greedy && x == x) t.merge(x * c, x > -kVfInf ? 1.0f : 0.0f);
+        if (prm.sums && x == x) t.merge(x * c, x > -kVfInf ? 1.0f : 0.0f);
+    }
+    if (prm.cuts) {
+        float v = best == best ? best : -kVfInf;  // (the tail's elements are not among the maxima)
+        const int g = vf_peak_group(S);
+        for (int o = 1; o < g; o <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, kWave));
+        if ((tid & (g - 1)) == 0) a.peaks[(size_t)r * vf_peaks(S) + (p * kVfThreads + tid) / g] = v;
     }
     top = wave_max_u64(top);
     t.wave_merge();
@@ -201,33 +208,72 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 }
 
 // ---- rows that their request cuts ---------------------------------------------------------
+//
+// The kept set is that of vws_sample, decided on the integer masses w = floor(exp_det(y - m) 2^44):
+// their sums do not depend on the order, so the set does not depend on how it is found.  Three ways,
+// by what bounds the row's survivors:
+//   * top-k or min-p: a bound on the logit below which nothing survives (the k-th largest of the
+//     thread maxima that the first pass left, or m + log(min_p)); the few logits above it go into
+//     a list, which decides everything (one read of the row, a compare per logit);
+//   * top-p alone: the list of the logits above the thread maxima's bound, if it holds the cut for
+//     any total within the error of the first pass's sum (a peaked row);
+//   * else the masses of all logits, summed in bins by the distance from the maximum;
+//     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).
+// A list that overflows (many equal logits) leaves the row to passes over its keys' bits.
 
 constexpr int kVfBins = 2048;
 constexpr int kVfCutWaves = kVfCutThreads / 64;
+constexpr int kVfList = 2048;     // list entries (a row's candidates)
+constexpr int kVfSmall = 512;     // entries that are compared with each other, all pairs
 
 struct VfCutShared {
     uint64_t hist[kVfBins];
+    uint64_t list[kVfList];       // key(y) << 32 | index
     uint64_t red[kVfCutWaves];
     uint64_t out[4];
+    uint32_t count;
 };
 
-// Calls f(index, y) for every element of a row (each thread its vectors, then one tail element).
+__device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
+
+// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element).
 template <typename T, typename F>
-__device__ __forceinline__ void vf_each(const T* row, int V, float Tt, F f) {
+__device__ __forceinline__ void vf_each(const T* row, int V, F f) {
     constexpr int VEC = Elem<T>::kVec;
     const int nvec = V / VEC;
     for (int vi = threadIdx.x; vi < nvec; vi += kVfCutThreads) {
         float v[VEC];
         vf_load<T>(row, vi, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f(vi * VEC + j, Tt == 1.0f ? v[j] : v[j] / Tt);
+        for (int j = 0; j < VEC; ++j) f(vi * VEC + j, v[j]);
     }
     const int i = nvec * VEC + threadIdx.x;
-    if (i < V) {
-        const float x = Elem<T>::load1(row + i);
-        f(i, Tt == 1.0f ? x : x / Tt);
-    }
+    if (i < V) f(i, Elem<T>::load1(row + i));
 }
+
+// What the selection below runs over: a row's elements, or the list's.  each(f): f(index, key, y).
+template <typename T> struct VfRowIter {
+    const T* row;
+    int V;
+    float Tt;
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        const float t = Tt;
+        vf_each<T>(row, V, [&](int i, float x) {
+            const float y = vf_scaled(x, t);
+            f(i, key_of(y), y);
+        });
+    }
+};
+struct VfListIter {
+    const uint64_t* list;
+    int n;
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        for (int j = threadIdx.x; j < n; j += kVfCutThreads) {
+            const uint64_t v = list[j];
+            f((int)(uint32_t)v, (uint32_t)(v >> 32), val_of((uint32_t)(v >> 32)));
+        }
+    }
+};
 
 __device__ __forceinline__ uint64_t vf_block_max(uint64_t v, VfCutShared& sh) {
     v = wave_max_u64(v);
@@ -248,6 +294,15 @@ __device__ __forceinline__ uint64_t vf_block_sum(uint64_t v, VfCutShared& sh) {
 #pragma unroll
     for (int i = 0; i < kVfCutWaves; ++i) t += sh.red[i];
     return t;
+}
+
+__device__ __forceinline__ void vf_clear(VfCutShared& sh) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) sh.hist[i] = 0ull;
+    __syncthreads();
+}
+__device__ __forceinline__ void vf_count(VfCutShared& sh, int bin, uint64_t w) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin]), (unsigned long long)w);
 }
 
 // The bin of sh.hist (bins [0, n), n a multiple of 64, up to kVfBins) where the running sum from
@@ -279,22 +334,18 @@ __device__ __forceinline__ void vf_find(VfCutShared& sh, int n, uint64_t thr, in
 }
 
 // The key at which the running sum of weight(key, y) over ascending keys first exceeds thr, with the
-// sum of all smaller keys: three passes over the row, 11, 11 and 10 bits of the key.
-template <typename T, typename W>
-__device__ __forceinline__ uint32_t vf_select(const T* row, int V, float Tt, VfCutShared& sh, uint64_t thr,
-                                              uint64_t* below, W weight) {
+// sum of all smaller keys: three passes, 11, 11 and 10 bits of the key.
+template <typename I, typename W>
+__device__ __forceinline__ uint32_t vf_select(const I& it, VfCutShared& sh, uint64_t thr, uint64_t* below, W weight) {
     uint32_t prefix = 0u;
     uint64_t under = 0ull;
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-        for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) sh.hist[i] = 0ull;
-        __syncthreads();
-        vf_each<T>(row, V, Tt, [&](int, float y) {
-            const uint32_t k = key_of(y);
+        vf_clear(sh);
+        it.each([&](int, uint32_t k, float y) {
             if (pass > 0 && (k >> (shift + bits)) != prefix) return;
             const uint64_t w = weight(k, y);
-            if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[(k >> shift) & ((1u << bits) - 1u)]),
-                             (unsigned long long)w);
+            if (w) vf_count(sh, (int)((k >> shift) & ((1u << bits) - 1u)), w);
         });
         int bin;
         uint64_t c;
@@ -306,22 +357,187 @@ __device__ __forceinline__ uint32_t vf_select(const T* row, int V, float Tt, VfC
     return prefix;
 }
 
-// The n-th (from 0) lowest index among the row's elements whose key is `key`: two passes over the row.
-template <typename T>
-__device__ __forceinline__ int vf_nth_index(const T* row, int V, float Tt, VfCutShared& sh, uint32_t key, uint64_t n) {
+// The n-th (from 0) lowest index among the elements whose key is `key`: two passes.
+template <typename I>
+__device__ __forceinline__ int vf_nth_index(const I& it, VfCutShared& sh, uint32_t key, uint64_t n) {
     int hi = 0, lo = 0;
     uint64_t under;
     for (int pass = 0; pass < 2; ++pass) {
-        for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) sh.hist[i] = 0ull;
-        __syncthreads();
-        vf_each<T>(row, V, Tt, [&](int i, float y) {
-            if (key_of(y) != key || (pass && (i >> 8) != hi)) return;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[pass ? (i & 255) : (i >> 8)]), 1ull);
+        vf_clear(sh);
+        it.each([&](int i, uint32_t k, float) {
+            if (k != key || (pass && (i >> 8) != hi)) return;
+            vf_count(sh, pass ? (i & 255) : (i >> 8), 1ull);
         });
         vf_find(sh, pass ? 256 : kVfBins, n, pass ? &lo : &hi, &under);
         n -= under;
     }
     return hi * 256 + lo;
+}
+
+struct VfCut {
+    uint64_t cut, kept;  // the smallest (key << 32 | index) kept, the kept masses' sum
+};
+
+// What a row keeps, and the rest of what the selection needs to know.
+struct VfRule {
+    float m, lp_min, q32;
+    int k;
+    __device__ __forceinline__ bool above(float y) const { return y - m >= lp_min; }
+    __device__ __forceinline__ uint64_t mass(float y) const { return mass_of(exp_det(y - m)); }
+};
+
+// The kept set by passes over the elements, which hold everything that may survive (`n`: those that
+// are not NaN).
+template <typename I>
+__device__ __forceinline__ VfCut vf_solve(const I& it, VfCutShared& sh, const VfRule& u, uint64_t n) {
+    uint32_t kth = 1u;  // every key but a NaN's
+    if (u.k > 0 && (uint64_t)u.k <= n) {
+        uint64_t under;
+        kth = vf_select(it, sh, n - (uint64_t)u.k, &under, [](uint32_t k, float) { return (uint64_t)(k ? 1u : 0u); });
+    }
+    uint64_t W = 0ull, kmin = ~0ull;
+    it.each([&](int, uint32_t k, float y) {
+        if (k >= kth && u.above(y)) {
+            W += u.mass(y);
+            kmin = vws_min64(kmin, k);
+        }
+    });
+    VfCut o;
+    W = vf_block_sum(W, sh);
+    kmin = ~vf_block_max(~kmin, sh);
+    o.cut = kmin << 32;
+    o.kept = W;
+    if (u.q32 > 0.0f && u.q32 < 1.0f) {
+        const uint64_t thr = scale_floor(u.q32, W);
+        uint64_t under;
+        const uint32_t key = vf_select(it, sh, thr, &under, [&](uint32_t k, float y) -> uint64_t {
+            return k >= kth && u.above(y) ? u.mass(y) : 0ull;
+        });
+        const uint64_t w = u.mass(val_of(key));
+        const uint64_t gone = (thr - under) / w;  // of the elements with that key, the lowest indices
+        o.cut = (uint64_t)key << 32;
+        if (gone) o.cut |= (uint32_t)vf_nth_index(it, sh, key, gone);
+        o.kept = W - under - gone * w;
+    }
+    return o;
+}
+
+// The same for at most kVfSmall listed elements, one per thread, each against all others.
+__device__ __forceinline__ VfCut vf_solve_small(VfCutShared& sh, const VfRule& u, int n) {
+    const int j = threadIdx.x;
+    const uint64_t mine = j < n ? sh.list[j] : 0ull;
+    const uint32_t key = (uint32_t)(mine >> 32);
+    const float y = val_of(key);
+    bool on = j < n && u.above(y);
+    if (u.k > 0 && j < n) {
+        int more = 0;
+        for (int i = 0; i < n; ++i) more += (uint32_t)(sh.list[i] >> 32) > key ? 1 : 0;
+        on = on && more < u.k;
+    }
+    const uint64_t w = on ? u.mass(y) : 0ull;
+    if (j < n) sh.hist[j] = w;
+    const uint64_t W = vf_block_sum(w, sh);
+    if (on && u.q32 > 0.0f && u.q32 < 1.0f) {
+        const uint64_t thr = scale_floor(u.q32, W);
+        uint64_t C = 0ull;
+        for (int i = 0; i < n; ++i) C += sh.list[i] <= mine ? sh.hist[i] : 0ull;
+        on = C > thr;  // (the last, whose C is W, stays)
+    }
+    VfCut o;
+    o.cut = ~vf_block_max(on ? ~mine : 0ull, sh);
+    o.kept = vf_block_sum(on ? w : 0ull, sh);
+    return o;
+}
+
+// The elements listed are the row's largest.  Whether top-p's cut lies among them for every total
+// in [lo, hi]: then the smallest kept (the lowest element whose sum of larger ones is below p W) is
+// found from above.
+__device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, int n, double lo, double hi, VfCut* o) {
+    const int j = threadIdx.x;
+    const uint64_t mine = j < n ? sh.list[j] : 0ull;
+    const uint64_t w = j < n ? u.mass(val_of((uint32_t)(mine >> 32))) : 0ull;
+    if (j < n) sh.hist[j] = w;
+    __syncthreads();
+    // kept iff the sum C from below up to it exceeds floor(q W): C = W - A, A the sum above it;
+    // W is an integer in [lo, hi]: with f(W) = W - floor(q W), which never falls, A < f(W)
+    uint64_t A = 0ull;
+    if (j < n)
+        for (int i = 0; i < n; ++i) A += sh.list[i] > mine ? sh.hist[i] : 0ull;
+    const uint64_t Wl = (uint64_t)lo, Wh = (uint64_t)hi + 1ull;
+    const uint64_t fl = Wl - scale_floor(u.q32, Wl), fh = Wh - scale_floor(u.q32, Wh);
+    const bool sure = j < n && A < fl, maybe = j < n && A < fh;
+    const uint64_t unsure = vf_block_max(maybe && !sure ? 1ull : 0ull, sh);
+    const uint64_t total = vf_block_sum(w, sh);
+    // the list ends below the cut: the elements past it would be refused too
+    if (unsure || total < fh) return false;
+    o->cut = ~vf_block_max(sure ? ~mine : 0ull, sh);
+    o->kept = vf_block_sum(sure ? w : 0ull, sh);
+    return true;
+}
+
+// Lists the row's elements with x >= t and, of those, y in [ylo, yhi] by `in`; false when they are
+// more than the list holds.
+template <typename T, typename F>
+__device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutShared& sh, float lo, float hi, F in) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0u;
+    __syncthreads();
+    vf_each<T>(row, V, [&](int i, float x) {
+        if (x >= lo && x <= hi) {
+            const float y = vf_scaled(x, Tt);
+            if (in(y)) {
+                const uint32_t at = agg_reserve(&sh.count);
+                if (at < (uint32_t)kVfList) sh.list[at] = ((uint64_t)key_of(y) << 32) | (uint32_t)i;
+            }
+        }
+    });
+    __syncthreads();
+    return sh.count <= (uint32_t)kVfList;
+}
+
+// The n-th largest (from 1) of the row's maxima, with its low 16 bits cleared (a bound below it):
+// found bit by bit by every wave for itself.  -inf when there are fewer.
+__device__ __forceinline__ float vf_peak(const float* peaks, int G, int n) {
+    uint32_t k[kVfPeaks / kWave];
+#pragma unroll
+    for (int i = 0; i < kVfPeaks / kWave; ++i) {
+        const int at = i * kWave + lane_id();
+        k[i] = at < G ? key_of(peaks[at]) : 0u;
+    }
+    uint32_t ans = 0u;
+    for (int b = 31; b >= 16; --b) {
+        const uint32_t cand = ans | (1u << b);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kVfPeaks / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
+        if (c >= n) ans = cand;
+    }
+    return ans >= 0x00800000u ? val_of(ans) : -kVfInf;  // (below: -inf or none)
+}
+
+struct VfRow {
+    uint64_t top, cut;
+    float m, sum;
+    bool sure;  // greedy, or the maximum is not finite: the row's distribution is its argmax
+};
+
+// Row r's statistics from its parts, in every lane of the calling wave.
+__device__ __forceinline__ VfRow vf_join(const VerifyArgs& a, const VfParams& prm, int r) {
+    VfRec v{0ull, -kVfInf, 0.0f};
+    if (lane_id() < a.S) v = a.rec[(size_t)r * a.S + lane_id()];
+    VfSum t;
+    t.m = v.m2;
+    t.s = v.sum;
+    VfRow o;
+    o.top = wave_max_u64(v.top);
+    o.cut = 0ull;
+    const float x = vf_value(o.top);
+    o.m = prm.greedy ? x : x / prm.T;
+    o.sure = prm.greedy || !(__builtin_fabsf(o.m) < kVfInf);
+    t.wave_merge();
+    // relative to x c - maximum, whose rounding leaves the largest element's own term off 1
+    o.sum = t.s * vf_exp2(-__builtin_fmaf(x, prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T, -t.m));
+    return o;
 }
 
 // One workgroup per row: the kept set of a row that its request cuts, as the smallest
@@ -335,107 +551,128 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const float Tt = prm.T;
     const int V = a.V;
-    uint64_t top = 0ull, nvalid = 0ull;
-    vf_each<T>(row, V, 1.0f, [&](int i, float x) {
-        const uint32_t k = key_of(x);
-        top = vws_max64(top, vf_pack(k, i));
-        nvalid += k ? 1u : 0u;
-    });
-    top = vf_block_max(top, sh);
-    nvalid = vf_block_sum(nvalid, sh);
-    const float m = vf_value(top) / Tt;
-    VfRec o;
-    o.top = top;
-    o.m2 = m;
-    o.sum = 0.0f;
-    uint64_t cut = 0ull;
-    if (__builtin_fabsf(m) < kVfInf) {
-        const float lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
-        uint32_t kth = 1u;  // every key but a NaN's
-        if (prm.k > 0 && (uint64_t)prm.k <= nvalid) {
-            uint64_t under;
-            kth = vf_select<T>(row, V, Tt, sh, nvalid - (uint64_t)prm.k, &under,
-                               [](uint32_t k, float) { return (uint64_t)(k ? 1u : 0u); });
-        }
-        auto weight = [=](uint32_t k, float y) -> uint64_t {
-            const float d = y - m;
-            return k >= kth && d >= lp_min ? mass_of(exp_det(d)) : 0ull;
-        };
-        // (the kept set without top-p, as one bound on the key)
-        uint64_t W = 0ull, kmin = ~0ull;
-        vf_each<T>(row, V, Tt, [&](int, float y) {
-            const uint32_t k = key_of(y);
-            if (k >= kth && y - m >= lp_min) {
-                W += mass_of(exp_det(y - m));
-                kmin = vws_min64(kmin, k);
-            }
-        });
-        W = vf_block_sum(W, sh);
-        kmin = ~vf_block_max(~kmin, sh);
-        cut = kmin << 32;
-        uint64_t kept = W;
-        const float q32 = 1.0f - prm.top_p;
-        if (q32 >= 1.0f) {
+    const VfRow w = vf_join(a, prm, r);
+    VfRule u;
+    u.m = w.m;
+    u.q32 = 1.0f - prm.top_p;
+    u.k = prm.k;
+    u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
+    VfCut o{0ull, 0ull};
+    if (!w.sure) {
+        const int G = vf_peaks(a.S);
+        const float* peaks = a.peaks + (size_t)r * G;
+        // y = fl(x / T) and y - m round, and a maximum's group may hold the k-th largest itself:
+        // a margin of some ulps below the bound keeps every element that could survive
+        // (T 2^-120: where y is subnormal)
+        const float tiny = Tt * 0x1p-120f;
+        auto below = [tiny](float x) { return x - __builtin_fabsf(x) * 0x1p-20f - tiny; };
+        bool done = false;
+        if (u.q32 >= 1.0f) {
             // only the last of (key, index)
-            uint64_t lastk = 0ull;
-            const uint32_t mk = key_of(m);
-            vf_each<T>(row, V, Tt, [&](int i, float y) {
-                if (key_of(y) == mk) lastk = vws_max64(lastk, ((uint64_t)mk << 32) | (uint32_t)i);
+            const uint32_t mk = key_of(u.m);
+            uint64_t last = 0ull;
+            vf_each<T>(row, V, [&](int i, float x) {
+                if (key_of(vf_scaled(x, Tt)) == mk) last = vws_max64(last, ((uint64_t)mk << 32) | (uint32_t)i);
             });
-            cut = vf_block_max(lastk, sh);
-            kept = 1ull << 44;
-        } else if (q32 > 0.0f) {
-            const uint64_t thr = scale_floor(q32, W);
-            uint64_t under;
-            const uint32_t key = vf_select<T>(row, V, Tt, sh, thr, &under, weight);
-            const uint64_t w = mass_of(exp_det(val_of(key) - m));
-            const uint64_t gone = (thr - under) / w;  // of the elements with that key, the lowest indices
-            cut = (uint64_t)key << 32;
-            if (gone) cut |= (uint32_t)vf_nth_index<T>(row, V, Tt, sh, key, gone);
-            kept = W - under - gone * w;
+            o.cut = vf_block_max(last, sh);
+            o.kept = 1ull << 44;
+            done = true;
+        } else if (u.k > 0 || u.lp_min > -kVfInf) {
+            float t = -kVfInf;
+            if (u.k > 0 && u.k <= G) t = below(vf_peak(peaks, G, u.k));
+            if (u.lp_min > -kVfInf) {
+                const float y = u.m + u.lp_min;
+                t = __builtin_fmaxf(t, Tt * (y - (__builtin_fabsf(u.m) - u.lp_min) * 0x1p-20f) - tiny);
+            }
+            const bool k_listed = u.k == 0 || t > -kVfInf;
+            if (k_listed && vf_collect<T>(row, V, Tt, sh, t, kVfInf, [](float) { return true; })) {
+                const int n = (int)sh.count;
+                o = n <= kVfSmall ? vf_solve_small(sh, u, n) : vf_solve(VfListIter{sh.list, n}, sh, u, (uint64_t)n);
+                done = true;
+            }
+        } else {
+            // top-p alone.  The first pass's sum is off by at most 2^-22 (2 |m| + 64) of itself: y and
+            // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
+            // its constant likewise, the exponential and the sums by a few 2^-24
+            const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
+            // (so many of G maxima that about 350 logits lie above the last of them)
+            const float t = below(vf_peak(peaks, G, (int)((float)G * (1.0f - __expf(-350.0f / (float)G)))));
+            if (t > -kVfInf && vf_collect<T>(row, V, Tt, sh, t, kVfInf, [](float) { return true; }) && sh.count <= (uint32_t)kVfSmall)
+                done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
+            if (!done) {
+                // every mass, by distance from the maximum; what lies further than `far` holds less
+                // than q W (W is at least the maximum's own mass) and is only summed
+                const float far = fminf(logf((float)V / u.q32) + 0.01f, 31.0f), scale = (float)(kVfBins - 1) / far;
+                vf_clear(sh);
+                uint64_t s = 0ull;
+                vf_each<T>(row, V, [&](int, float x) {
+                    const float d = u.m - vf_scaled(x, Tt);
+                    const uint64_t q = mass_of(exp_det(-d));
+                    if (d < far) vf_count(sh, (int)(d * scale), q);
+                    else s += q;
+                });
+                uint64_t in = 0ull;
+                __syncthreads();
+                for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) in += sh.hist[i];
+                in = vf_block_sum(in, sh);
+                const uint64_t total = in + vf_block_sum(s, sh), thr = scale_floor(u.q32, total);
+                // from the maximum down: the cut lies where the running sum reaches total - thr
+                if (total - thr <= in) {
+                    int bin;
+                    uint64_t over;
+                    vf_find(sh, kVfBins, total - thr - 1ull, &bin, &over);
+                    const uint64_t under = total - over - sh.hist[bin];
+                    const float yhi = u.m - (float)bin / scale, ylo = u.m - (float)(bin + 1) / scale;
+                    const float slack = (__builtin_fabsf(u.m) + 32.0f) * 0x1p-20f;
+                    if (vf_collect<T>(row, V, Tt, sh, Tt * (ylo - slack), Tt * (yhi + slack), [&](float y) {
+                            const float d = u.m - y;
+                            return d < far && (int)(d * scale) == bin;
+                        })) {
+                        const int n = (int)sh.count;
+                        // among the bin's elements: kept iff under + their sum up to it exceeds thr
+                        const VfListIter it{sh.list, n};
+                        uint64_t c;
+                        const uint32_t key = vf_select(it, sh, thr - under, &c, [&](uint32_t, float y) { return u.mass(y); });
+                        const uint64_t q = u.mass(val_of(key));
+                        const uint64_t gone = (thr - under - c) / q;
+                        o.cut = (uint64_t)key << 32;
+                        if (gone) o.cut |= (uint32_t)vf_nth_index(it, sh, key, gone);
+                        o.kept = total - under - c - gone * q;
+                        done = true;
+                    }
+                }
+            }
         }
-        o.sum = (float)kept * 0x1p-44f;
+        if (!done) {
+            uint64_t n = 0ull;
+            vf_each<T>(row, V, [&](int, float x) { n += x == x ? 1u : 0u; });
+            n = vf_block_sum(n, sh);
+            o = vf_solve(VfRowIter<T>{row, V, Tt}, sh, u, n);
+        }
     }
+    __syncthreads();  // every wave has read the row's parts
     if (threadIdx.x == 0) {
-        a.rec[(size_t)r * a.S] = o;
-        a.cut[r] = cut;
+        VfRec c;
+        c.top = w.top;
+        c.m2 = w.m;
+        c.sum = (float)o.kept * 0x1p-44f;
+        a.rec[(size_t)r * a.S] = c;
+        a.cut[r] = o.cut;
     }
 }
 
 // ---- decision and race ----------------------------------------------------------------------
 
-struct VfRow {
-    uint64_t top, cut;
-    float m, sum;
-    bool sure;  // greedy, or the maximum is not finite: the row's distribution is its argmax
-};
-
-// Row r's statistics from its parts, in every lane of the calling wave.
+// Row r's statistics for the decision, in every lane of the calling wave.
 __device__ __forceinline__ VfRow vf_row(const VerifyArgs& a, const VfParams& prm, int r) {
+    if (!prm.cuts) return vf_join(a, prm, r);
+    const VfRec v = a.rec[(size_t)r * a.S];
     VfRow o;
-    VfRec v{0ull, -kVfInf, 0.0f};
-    const int lane = lane_id();
-    if (prm.cuts) {
-        v = a.rec[(size_t)r * a.S];
-        o.top = v.top;
-        o.cut = a.cut[r];
-        o.m = v.m2;
-        o.sum = v.sum;
-        o.sure = !(__builtin_fabsf(v.m2) < kVfInf);
-        return o;
-    }
-    if (lane < a.S) v = a.rec[(size_t)r * a.S + lane];
-    VfSum t;
-    t.m = v.m2;
-    t.s = v.sum;
-    o.top = wave_max_u64(v.top);
-    o.cut = 0ull;
-    const float x = vf_value(o.top);
-    o.m = prm.greedy ? x : x / prm.T;
-    o.sure = prm.greedy || !(__builtin_fabsf(o.m) < kVfInf);
-    t.wave_merge();
-    // relative to x c - maximum, whose rounding leaves the largest element's own term off 1
-    o.sum = t.s * vf_exp2(-__builtin_fmaf(x, prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T, -t.m));
+    o.top = v.top;
+    o.cut = a.cut[r];
+    o.m = v.m2;
+    o.sum = v.sum;
+    o.sure = !(__builtin_fabsf(v.m2) < kVfInf);
     return o;
 }
 
