@@ -910,10 +910,11 @@ size_t vws_verify_workspace_size(int32_t batch, int32_t num_drafts, int32_t voca
     if (batch < 1 || num_drafts < 0 || vocab < 1 || vocab > VWS_MAX_VOCAB || batch > kVerifyMaxRows ||
         num_drafts > kVerifyMaxRows - batch)
         return 0;
-    int S, S2, len;
+    int S, S2, len, len2;
     verify_parts(batch + num_drafts, vocab, &S, &len);
-    verify_parts(batch, vocab, &S2, &len);
-    return vf_layout(batch + num_drafts, batch, S, S2).total;
+    verify_parts(batch, vocab, &S2, &len2);
+    // (vectors of 4: the most groups)
+    return vf_layout(batch + num_drafts, batch, S, S2, vf_groups(S, len, 4)).total;
 }
 
 int vws_verify_drafts(const vws_verify_args* a) {
@@ -947,14 +948,15 @@ int vws_verify_drafts(const vws_verify_args* a) {
     k.logprobs = a->logprobs;
     verify_parts(k.R, k.V, &k.S, &k.part_len);
     verify_parts(k.B, k.V, &k.S2, &k.part2_len);
-    const VfLayout w = vf_layout(k.R, k.B, k.S, k.S2);
+    const bool cuts = a->temperature && (a->top_k || a->top_p || a->min_p);
+    k.groups = vf_groups(k.S, k.part_len, a->dtype == VWS_DTYPE_F32 ? 4 : 8);
+    const VfLayout w = vf_layout(k.R, k.B, k.S, k.S2, k.groups);
     char* base = static_cast<char*>(a->workspace);
     k.rec = reinterpret_cast<VfRec*>(base + w.rec);
-    k.peaks = reinterpret_cast<float*>(base + w.peaks);
+    k.gmax = reinterpret_cast<float*>(base + w.gmax);
     k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
     k.best = reinterpret_cast<uint64_t*>(base + w.best);
     k.ctr = reinterpret_cast<uint32_t*>(base + w.ctr);
-    const bool cuts = a->temperature && (a->top_k || a->top_p || a->min_p);
     hipStream_t s = (hipStream_t)a->stream;
     const int st = a->dtype == VWS_DTYPE_F32    ? verify_launch<float>(k, cuts, s)
                    : a->dtype == VWS_DTYPE_BF16 ? verify_launch<uint16_t>(k, cuts, s)

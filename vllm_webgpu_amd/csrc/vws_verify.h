@@ -49,31 +49,30 @@ struct VerifyArgs {
     int S, part_len;             // parts of a row in the statistics
     int S2, part2_len;           // parts of a row in the race
     VfRec* rec;                  // [R, S]
-    float* peaks;                // [R, vf_peaks(S)] maxima of groups of threads, rows that are cut
+    float* gmax;                 // [R, groups] maxima of groups of vectors, of rows that are cut; or null
+    int groups;                  // of a row
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
     uint64_t* best;              // [B, S2] race: key bits << 32 | 0x7FFFFFFF - index
     uint32_t* ctr;               // [B] race parts arrived; cleared by the statistics' launch
 };
 
-constexpr int kVfPeaks = 1024;       // most maxima kept of a row
+constexpr int kVfGroup = 4;          // vectors whose maximum the first pass leaves together
 
-// Threads of a part that share one maximum, and the maxima of a row.
-inline __host__ __device__ int vf_peak_group(int S) {
-    int g = 1;
-    while (kVfThreads * S / g > kVfPeaks) g *= 2;
-    return g;
+// Groups of a row (their maxima's places): those of its parts, kVfThreads an iteration.
+inline int vf_groups(int S, int part_len, int vec) {
+    const int per = kVfGroup * kVfThreads * vec;
+    return S * ((part_len + per - 1) / per) * kVfThreads;
 }
-inline __host__ __device__ int vf_peaks(int S) { return S * (kVfThreads / vf_peak_group(S)); }
 
 struct VfLayout {
-    size_t rec, peaks, cut, best, ctr, total;
+    size_t rec, gmax, cut, best, ctr, total;
 };
 
-inline VfLayout vf_layout(int R, int B, int S, int S2) {
+inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
     VfLayout w{};
     size_t off = align256(sizeof(CoopState));  // every workspace starts with the fixed region
     w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
-    w.peaks = off; off = align256(off + sizeof(float) * (size_t)R * vf_peaks(S));
+    w.gmax = off;  off = align256(off + sizeof(float) * (size_t)R * groups);
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
     w.best = off;  off = align256(off + sizeof(uint64_t) * (size_t)B * S2);
     w.ctr = off;   off = align256(off + sizeof(uint32_t) * (size_t)B);

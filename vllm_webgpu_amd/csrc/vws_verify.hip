@@ -26,9 +26,15 @@ template <typename T> struct VfVec { typedef uint32_t U4 __attribute__((ext_vect
 template <> struct VfVec<float> { typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(4))); };
 
 template <typename T>
-__device__ __forceinline__ void vf_load(const T* row, int vi, float (&v)[Elem<T>::kVec]) {
+__device__ __forceinline__ void vf_load_raw(const T* row, int vi, uint32_t (&w)[4]) {
     const auto u = *reinterpret_cast<const typename VfVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec);
-    Elem<T>::from_words(u[0], u[1], u[2], u[3], v);
+    w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
+}
+template <typename T>
+__device__ __forceinline__ void vf_load(const T* row, int vi, float (&v)[Elem<T>::kVec]) {
+    uint32_t w[4];
+    vf_load_raw<T>(row, vi, w);
+    Elem<T>::from_words(w[0], w[1], w[2], w[3], v);
 }
 
 // N floats from element i of a row of any supported type.
@@ -63,15 +69,19 @@ __device__ __forceinline__ float vf_load_any1(const void* row, int dtype, int i)
 }
 __device__ __forceinline__ size_t vf_esize(int dtype) { return dtype == VWS_DTYPE_F32 ? 4 : 2; }
 
-// The request of row r: the number of requests whose first row lies at or before it, less one.
-// Every lane of the calling wave returns it.
+// The request of row r: the last whose first row (cu[b] + b) lies at or before it.  64 bounds at a
+// time, so two loads for up to 4096 requests; every lane of the calling wave returns it.
 __device__ __forceinline__ int vf_request(const VerifyArgs& a, int r) {
-    int n = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kWave) {
-        const int b = b0 + lane_id();
-        n += __popcll(wave_ballot(b < a.B && a.cu[min(b, a.B)] + b <= r));
+    int lo = 0, n = a.B;
+    while (n > 1) {
+        const int step = (n + kWave - 1) / kWave, at = lane_id() * step;
+        const int b = lo + min(at, n - 1);
+        const int c = __popcll(wave_ballot(at < n && a.cu[b] + b <= r));
+        const int skip = c > 0 ? (c - 1) * step : 0;
+        lo += skip;
+        n = min(step, n - skip);
     }
-    return n > 0 ? n - 1 : 0;
+    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 struct VfParams {
@@ -118,35 +128,49 @@ __device__ __forceinline__ float vf_value(uint64_t top) {
 }
 
 // Part p of row r: its largest logit, the lowest index that has it, and the sum of exponentials.
-// NaN logits are never the largest and add nothing.
+// NaN logits are never the largest and add nothing.  Of rows that are cut it leaves the maximum of
+// every group (the kVfGroup vectors of a thread's iteration), with which verify_cut_kernel finds the
+// few logits that matter without a second read of the row.
+//
+// Bound: HBM.  The next iteration's loads are issued before this one's are used, and the first
+// before the request's parameters are known.
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
-    constexpr int VEC = Elem<T>::kVec, U = 4;
+    constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
     __shared__ uint64_t red_top[kVfThreads / 64];
     __shared__ float red_m[kVfThreads / 64], red_s[kVfThreads / 64];
     const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, wave = tid >> 6;
-    if (p == 0 && tid == 0 && r < a.B) a.ctr[r] = 0u;  // (R >= B)
-    const VfParams prm = vf_params(a, vf_request(a, r));
-    const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
     row += lo;
+    uint32_t next[U][4];
+    auto fetch = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int vi = b + u * kVfThreads;
+            if (nvec > 0) vf_load_raw<T>(row, vi < nvec ? vi : nvec - 1, next[u]);
+        }
+    };
+    fetch(tid);
+    if (p == 0 && tid == 0 && r < a.B) a.ctr[r] = 0u;  // (R >= B)
+    const VfParams prm = vf_params(a, vf_request(a, r));
+    const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
+    float* gmax = a.gmax + (size_t)r * a.groups + (size_t)p * (a.groups / S);
     VfSum t;
-    float best = __builtin_nanf("");  // the largest logit so far, and the first group of U vectors that holds it
+    float best = __builtin_nanf("");  // the largest logit so far, and the first group that holds it
     int group = tid;
     for (int b = tid; b < nvec; b += U * kVfThreads) {
         float v[U][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vi = b + u * kVfThreads;
-            vf_load<T>(row, vi < nvec ? vi : b, v[u]);
-        }
+        for (int u = 0; u < U; ++u) Elem<T>::from_words(next[u][0], next[u][1], next[u][2], next[u][3], v[u]);
+        if (b + U * kVfThreads < nvec) fetch(b + U * kVfThreads);
         float g = v[0][0];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) g = __builtin_fmaxf(g, v[u][j]);
+            for (int j = 0; j < VEC; ++j) g = b + u * kVfThreads < nvec ? __builtin_fmaxf(g, v[u][j]) : g;
         if (g == g && !(g <= best)) { best = g; group = b; }
+        if (prm.cuts) gmax[(b / (U * kVfThreads)) * kVfThreads + tid] = g;
         if (prm.sums) {
             const float n = __builtin_fmaxf(t.m, g * c), ref = n == -kVfInf ? 0.0f : n;
             float acc[4] = {t.s * vf_exp2(t.m - ref), 0.0f, 0.0f, 0.0f};
@@ -182,12 +206,6 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
         top = vws_max64(top, vf_pack(key_of(x), lo + i));
         if (prm.sums && x == x) t.merge(x * c, x > -kVfInf ? 1.0f : 0.0f);
     }
-    if (prm.cuts) {
-        float v = best == best ? best : -kVfInf;  // (the tail's elements are not among the maxima)
-        const int g = vf_peak_group(S);
-        for (int o = 1; o < g; o <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, kWave));
-        if ((tid & (g - 1)) == 0) a.peaks[(size_t)r * vf_peaks(S) + (p * kVfThreads + tid) / g] = v;
-    }
     top = wave_max_u64(top);
     t.wave_merge();
     if ((tid & 63) == 0) { red_top[wave] = top; red_m[wave] = t.m; red_s[wave] = t.s; }
@@ -212,11 +230,11 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 // The kept set is that of vws_sample, decided on the integer masses w = floor(exp_det(y - m) 2^44):
 // their sums do not depend on the order, so the set does not depend on how it is found.  Three ways,
 // by what bounds the row's survivors:
-//   * top-k or min-p: a bound on the logit below which nothing survives (the k-th largest of the
-//     thread maxima that the first pass left, or m + log(min_p)); the few logits above it go into
-//     a list, which decides everything (one read of the row, a compare per logit);
-//   * top-p alone: the list of the logits above the thread maxima's bound, if it holds the cut for
-//     any total within the error of the first pass's sum (a peaked row);
+//   * top-k or min-p: a bound on the logit below which nothing survives (the k-th largest of 1024
+//     maxima, joined from the groups' that the first pass left, or m + log(min_p)); the few logits
+//     above it, read where a group's maximum reaches it, go into a list, which decides everything;
+//   * top-p alone: the list of the logits above such a bound, if it holds the cut for any total
+//     within the error of the first pass's sum (a peaked row);
 //   * else the masses of all logits, summed in bins by the distance from the maximum;
 //     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).
 // A list that overflows (many equal logits) leaves the row to passes over its keys' bits.
@@ -225,13 +243,16 @@ constexpr int kVfBins = 2048;
 constexpr int kVfCutWaves = kVfCutThreads / 64;
 constexpr int kVfList = 2048;     // list entries (a row's candidates)
 constexpr int kVfSmall = 512;     // entries that are compared with each other, all pairs
+constexpr int kVfGroups = 1024;   // groups that are read for the list
 
 struct VfCutShared {
     uint64_t hist[kVfBins];
     uint64_t list[kVfList];       // key(y) << 32 | index
+    float peaks[kVfCutThreads];
+    uint32_t groups[kVfGroups];
     uint64_t red[kVfCutWaves];
     uint64_t out[4];
-    uint32_t count;
+    uint32_t count, ngroups;
 };
 
 __device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
@@ -303,6 +324,12 @@ __device__ __forceinline__ void vf_clear(VfCutShared& sh) {
 }
 __device__ __forceinline__ void vf_count(VfCutShared& sh, int bin, uint64_t w) {
     atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[bin]), (unsigned long long)w);
+}
+
+// Vectors of part p of a row.
+template <typename T>
+__device__ __forceinline__ int vf_part_vecs(const VerifyArgs& a, int p) {
+    return (min(a.V, (p + 1) * a.part_len) - p * a.part_len) / Elem<T>::kVec;
 }
 
 // The bin of sh.hist (bins [0, n), n a multiple of 64, up to kVfBins) where the running sum from
@@ -475,8 +502,8 @@ __device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, i
     return true;
 }
 
-// Lists the row's elements with x >= t and, of those, y in [ylo, yhi] by `in`; false when they are
-// more than the list holds.
+// Lists the row's elements with lo <= x <= hi whose y passes `in`; false when they are more than the
+// list holds.
 template <typename T, typename F>
 __device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutShared& sh, float lo, float hi, F in) {
     __syncthreads();
@@ -495,21 +522,74 @@ __device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutS
     return sh.count <= (uint32_t)kVfList;
 }
 
+// Lists the row's elements with x >= t by the groups' maxima (and the few elements past the parts'
+// last vectors); false when groups or elements are too many.
+template <typename T>
+__device__ __forceinline__ bool vf_gather(const VerifyArgs& a, int r, const T* row, float Tt, VfCutShared& sh, float t) {
+    constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
+    const int per = a.groups / a.S, tid = threadIdx.x;  // groups of a part
+    const float* gmax = a.gmax + (size_t)r * a.groups;
+    __syncthreads();
+    if (tid == 0) sh.count = sh.ngroups = 0u;
+    __syncthreads();
+    for (int g = tid; g < a.groups; g += kVfCutThreads) {
+        const int p = g / per, b = ((g - p * per) / kVfThreads) * U * kVfThreads + (g % kVfThreads);
+        if (b < vf_part_vecs<T>(a, p) && gmax[g] >= t) {
+            const uint32_t at = agg_reserve(&sh.ngroups);
+            if (at < (uint32_t)kVfGroups) sh.groups[at] = (uint32_t)g;
+        }
+    }
+    __syncthreads();
+    const int n = (int)sh.ngroups;
+    if (n > kVfGroups) return false;
+    auto add = [&](float x, int i) {
+        if (x >= t) {
+            const uint32_t at = agg_reserve(&sh.count);
+            if (at < (uint32_t)kVfList) sh.list[at] = ((uint64_t)key_of(vf_scaled(x, Tt)) << 32) | (uint32_t)i;
+        }
+    };
+    for (int k = tid; k < n * U; k += kVfCutThreads) {
+        const int g = (int)sh.groups[k / U], p = g / per;
+        const int vi = ((g - p * per) / kVfThreads) * U * kVfThreads + (g % kVfThreads) + (k % U) * kVfThreads;
+        if (vi >= vf_part_vecs<T>(a, p)) continue;
+        float v[VEC];
+        vf_load<T>(row + p * a.part_len, vi, v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) add(v[j], p * a.part_len + vi * VEC + j);
+    }
+    // (a part but the last is whole vectors)
+    const int i = a.V / VEC * VEC + tid;
+    if (i < a.V) add(Elem<T>::load1(row + i), i);
+    __syncthreads();
+    return sh.count <= (uint32_t)kVfList;
+}
+
+// The groups' maxima of a row, joined into at most 1024 (thread j: those of j, j + 1024, ...).
+template <typename T>
+__device__ __forceinline__ void vf_join_peaks(const VerifyArgs& a, int r, VfCutShared& sh) {
+    const int per = a.groups / a.S;
+    const float* gmax = a.gmax + (size_t)r * a.groups;
+    float m = -kVfInf;
+    for (int g = threadIdx.x; g < a.groups; g += kVfCutThreads) {
+        const int p = g / per, b = ((g - p * per) / kVfThreads) * kVfGroup * kVfThreads + (g % kVfThreads);
+        if (b < vf_part_vecs<T>(a, p)) m = __builtin_fmaxf(m, gmax[g]);
+    }
+    sh.peaks[threadIdx.x] = m;
+    __syncthreads();
+}
+
 // The n-th largest (from 1) of the row's maxima, with its low 16 bits cleared (a bound below it):
 // found bit by bit by every wave for itself.  -inf when there are fewer.
-__device__ __forceinline__ float vf_peak(const float* peaks, int G, int n) {
-    uint32_t k[kVfPeaks / kWave];
+__device__ __forceinline__ float vf_peak(const VfCutShared& sh, int n) {
+    uint32_t k[kVfCutThreads / kWave];
 #pragma unroll
-    for (int i = 0; i < kVfPeaks / kWave; ++i) {
-        const int at = i * kWave + lane_id();
-        k[i] = at < G ? key_of(peaks[at]) : 0u;
-    }
+    for (int i = 0; i < kVfCutThreads / kWave; ++i) k[i] = key_of(sh.peaks[i * kWave + lane_id()]);
     uint32_t ans = 0u;
     for (int b = 31; b >= 16; --b) {
         const uint32_t cand = ans | (1u << b);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < kVfPeaks / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
+        for (int i = 0; i < kVfCutThreads / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
         if (c >= n) ans = cand;
     }
     return ans >= 0x00800000u ? val_of(ans) : -kVfInf;  // (below: -inf or none)
@@ -559,8 +639,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
     u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
     VfCut o{0ull, 0ull};
     if (!w.sure) {
-        const int G = vf_peaks(a.S);
-        const float* peaks = a.peaks + (size_t)r * G;
+        vf_join_peaks<T>(a, r, sh);
         // y = fl(x / T) and y - m round, and a maximum's group may hold the k-th largest itself:
         // a margin of some ulps below the bound keeps every element that could survive
         // (T 2^-120: where y is subnormal)
@@ -579,13 +658,13 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             done = true;
         } else if (u.k > 0 || u.lp_min > -kVfInf) {
             float t = -kVfInf;
-            if (u.k > 0 && u.k <= G) t = below(vf_peak(peaks, G, u.k));
+            if (u.k > 0 && u.k <= kVfCutThreads) t = below(vf_peak(sh, u.k));
             if (u.lp_min > -kVfInf) {
                 const float y = u.m + u.lp_min;
                 t = __builtin_fmaxf(t, Tt * (y - (__builtin_fabsf(u.m) - u.lp_min) * 0x1p-20f) - tiny);
             }
             const bool k_listed = u.k == 0 || t > -kVfInf;
-            if (k_listed && vf_collect<T>(row, V, Tt, sh, t, kVfInf, [](float) { return true; })) {
+            if (k_listed && vf_gather<T>(a, r, row, Tt, sh, t)) {
                 const int n = (int)sh.count;
                 o = n <= kVfSmall ? vf_solve_small(sh, u, n) : vf_solve(VfListIter{sh.list, n}, sh, u, (uint64_t)n);
                 done = true;
@@ -595,9 +674,9 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
             // its constant likewise, the exponential and the sums by a few 2^-24
             const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
-            // (so many of G maxima that about 350 logits lie above the last of them)
-            const float t = below(vf_peak(peaks, G, (int)((float)G * (1.0f - __expf(-350.0f / (float)G)))));
-            if (t > -kVfInf && vf_collect<T>(row, V, Tt, sh, t, kVfInf, [](float) { return true; }) && sh.count <= (uint32_t)kVfSmall)
+            // (about 360 logits lie above the 300th of 1024 maxima)
+            const float t = below(vf_peak(sh, 300));
+            if (t > -kVfInf && vf_gather<T>(a, r, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
                 done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
             if (!done) {
                 // every mass, by distance from the maximum; what lies further than `far` holds less
@@ -687,7 +766,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     constexpr int VEC = Elem<T>::kVec;
     __shared__ VfRow rows[kVfMaxDrafts + 1];
     __shared__ uint64_t red[kVfThreads / 64];
-    __shared__ uint32_t last;
+    __shared__ uint32_t last, shared_bound;
     const int S2 = a.S2, b = blockIdx.x / S2, p = blockIdx.x - b * S2, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const VfParams prm = vf_params(a, b);
     const int first = a.cu[b], n = a.cu[b + 1] - first, K1 = a.K + 1;
@@ -741,6 +820,14 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
         const char* q = a.q && acc < n ? q0 + (size_t)acc * qbytes : nullptr;
         const float inv = 1.0f / w.sum;
         const float* u = a.u ? a.u + (size_t)b * a.ustride : nullptr;
+        // The largest key so far, of the workgroup, is a bound: a key is w / E with E = -ln u >= 1 - u
+        // >= 2^-24, so an element whose w (from the hardware's exp2, with its error on top) stays
+        // below bound (1 - u) cannot win, and a logit below tl cannot whatever its uniform.
+        const float c = 0x1.715476p+0f / prm.T, x_top = vf_value(w.top), m2 = x_top * c;
+        const float eps = 1.0f + 0x1p-22f * (2.0f * __builtin_fabsf(w.m) + 64.0f), scale = (q ? inv : 1.0f) * eps;
+        const float y_cut = w.cut ? val_of((uint32_t)(w.cut >> 32)) : -kVfInf;
+        const float x_cut = w.cut ? prm.T * (y_cut - __builtin_fabsf(y_cut) * 0x1p-20f) - prm.T * 0x1p-120f : -kVfInf;
+        float bound = 0.0f;
         auto add = [&](int i, float x, float qi, float ui) {
             const float y = x / prm.T;
             if (!vf_kept(w, y, i) || i == drop) return;
@@ -748,18 +835,67 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
             const float wt = q ? __builtin_fmaxf(e * inv - qi, 0.0f) : e;
             if (!(wt > 0.0f)) return;
             const float key = wt / (0.0f - log_det(ui));
-            if (key >= 0.0f) best = vws_max64(best, vf_pack(f2u(key) + 1u, i));
+            if (key >= 0.0f) {
+                best = vws_max64(best, vf_pack(f2u(key) + 1u, i));
+                if (key < kVfInf) bound = __builtin_fmaxf(bound, key * 0.9999f);
+            }
+        };
+        auto can_win = [&](float x, float qi, float ui) {
+            const float e = vf_exp2(__builtin_fmaf(x, c, -m2)) * scale;
+            return !((q ? e - qi : e) < bound * (1.0f - ui)) || !(ui < 1.0f);  // (true for NaN)
         };
         const int lo = p * a.part2_len, len = min(a.V, lo + a.part2_len) - lo, nvec = len / VEC;
-        for (int vi = tid; vi < nvec; vi += kVfThreads) {
-            float v[VEC], qv[VEC] = {}, uv[VEC];
-            const int i0 = lo + vi * VEC;
-            vf_load<T>(row + lo, vi, v);
-            if (q) vf_load_any<VEC>(q, a.qdtype, i0, qv);
-            if (u) vf_load_any<VEC>(u, VWS_DTYPE_F32, i0, uv);
-            else philox_uniforms_aligned<VEC>(seed, offset, (uint32_t)i0, uv);
+        // the most probable token's key first (each thread for itself): a good bound
+        {
+            const int i = vf_index(w.top);
+            add(i, x_top, q ? vf_load_any1(q, a.qdtype, i) : 0.0f, u ? u[i] : philox_uniform(seed, offset, (uint32_t)i));
+        }
+        if (tid == 0) shared_bound = f2u(bound);
+        __syncthreads();
+        const bool dense = w.cut == 0ull && (u || q);  // read q and u with the logits
+        constexpr int U = 2;
+        for (int b0 = tid; b0 < nvec; b0 += U * kVfThreads) {
+            float v[U][VEC], qv[U][VEC], uv[U][VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) add(i0 + j, v[j], qv[j], uv[j]);
+            for (int k = 0; k < U; ++k) {
+                const int vi = min(b0 + k * kVfThreads, nvec - 1), i0 = lo + vi * VEC;
+                vf_load<T>(row + lo, vi, v[k]);
+                if (dense && q) vf_load_any<VEC>(q, a.qdtype, i0, qv[k]);
+                if (dense && u) vf_load_any<VEC>(u, VWS_DTYPE_F32, i0, uv[k]);
+            }
+            bound = __builtin_fmaxf(bound, u2f(__hip_atomic_load(&shared_bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)));
+            const float had = bound;
+            // (1 / c = T ln 2; the slack covers the roundings)
+            const float lg = m2 + __builtin_amdgcn_logf(bound / scale) - 24.01f;
+            const float tl = __builtin_fmaxf(x_cut, (lg - __builtin_fabsf(lg) * 0x1p-20f - __builtin_fabsf(m2) * 0x1p-20f) * (prm.T * 0x1.62e43p-1f));
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int vi = b0 + k * kVfThreads, i0 = lo + vi * VEC;
+#pragma unroll
+                for (int g = 0; g < VEC; g += 4) {
+                    const float top4 = __builtin_fmaxf(__builtin_fmaxf(v[k][g], v[k][g + 1]), __builtin_fmaxf(v[k][g + 2], v[k][g + 3]));
+                    if (!(vi < nvec && top4 >= tl)) continue;
+                    float q4[4] = {}, u4[4];
+                    if (dense && q) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) q4[j] = qv[k][g + j];
+                    } else if (q) {
+                        vf_load_any<4>(q, a.qdtype, i0 + g, q4);
+                    }
+                    if (dense && u) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) u4[j] = uv[k][g + j];
+                    } else if (u) {
+                        vf_load_any<4>(u, VWS_DTYPE_F32, i0 + g, u4);
+                    } else {
+                        philox_uniforms_aligned<4>(seed, offset, (uint32_t)(i0 + g), u4);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (can_win(v[k][g + j], q4[j], u4[j])) add(i0 + g + j, v[k][g + j], q4[j], u4[j]);
+                }
+            }
+            if (bound > had) atomicMax(&shared_bound, f2u(bound));  // (positive floats order as their bits)
         }
         const int i = lo + nvec * VEC + tid;
         if (i < lo + len)
