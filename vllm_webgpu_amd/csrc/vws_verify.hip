@@ -248,7 +248,7 @@ constexpr int kVfGroups = 1024;   // groups that are read for the list
 struct VfCutShared {
     uint64_t hist[kVfBins];
     uint64_t list[kVfList];       // key(y) << 32 | index
-    float peaks[kVfCutThreads];
+    uint32_t above[kVfSmall];     // of each listed element: the elements with larger keys
     uint32_t groups[kVfGroups];
     uint64_t red[kVfCutWaves];
     uint64_t out[4];
@@ -257,18 +257,38 @@ struct VfCutShared {
 
 __device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
 
-// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element).
+// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element); the
+// next four vectors are on their way while these are used.
 template <typename T, typename F>
 __device__ __forceinline__ void vf_each(const T* row, int V, F f) {
-    constexpr int VEC = Elem<T>::kVec;
-    const int nvec = V / VEC;
-    for (int vi = threadIdx.x; vi < nvec; vi += kVfCutThreads) {
-        float v[VEC];
-        vf_load<T>(row, vi, v);
+    constexpr int VEC = Elem<T>::kVec, U = 4;
+    const int nvec = V / VEC, tid = threadIdx.x;
+    if (nvec > 0) {
+        uint32_t next[U][4];
+        auto fetch = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f(vi * VEC + j, v[j]);
+            for (int u = 0; u < U; ++u) vf_load_raw<T>(row, min(b + u * kVfCutThreads, nvec - 1), next[u]);
+        };
+        fetch(tid);
+        for (int b = tid; b < nvec; b += U * kVfCutThreads) {
+            uint32_t w[U][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[u][k] = next[u][k];
+            fetch(b + U * kVfCutThreads);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int vi = b + u * kVfCutThreads;
+                if (vi >= nvec) break;
+                float v[VEC];
+                Elem<T>::from_words(w[u][0], w[u][1], w[u][2], w[u][3], v);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f(vi * VEC + j, v[j]);
+            }
+        }
     }
-    const int i = nvec * VEC + threadIdx.x;
+    const int i = nvec * VEC + tid;
     if (i < V) f(i, Elem<T>::load1(row + i));
 }
 
@@ -332,27 +352,26 @@ __device__ __forceinline__ int vf_part_vecs(const VerifyArgs& a, int p) {
     return (min(a.V, (p + 1) * a.part_len) - p * a.part_len) / Elem<T>::kVec;
 }
 
-// The bin of sh.hist (bins [0, n), n a multiple of 64, up to kVfBins) where the running sum from
-// bin 0 up first exceeds `thr`, and the sum below it.  All threads call; the total exceeds thr.
+// The bin of sh.hist (bins [0, n), n <= kVfBins, even) where the running sum from bin 0 up first
+// exceeds `thr`, and the sum below it.  All threads call, two bins each; the total exceeds thr.
 __device__ __forceinline__ void vf_find(VfCutShared& sh, int n, uint64_t thr, int* bin, uint64_t* below) {
     __syncthreads();
-    if (threadIdx.x < kWave) {
-        const int per = n / kWave, lane = lane_id();
-        uint64_t s = 0;
-        for (int i = 0; i < per; ++i) s += sh.hist[lane * per + i];
-        uint64_t incl = s;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, at = 2 * (int)threadIdx.x;
+    const uint64_t h0 = at < n ? sh.hist[at] : 0ull, h1 = at < n ? sh.hist[at + 1] : 0ull;
+    uint64_t incl = h0 + h1;
 #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const uint64_t t = __shfl_up(incl, o, kWave);
-            if (lane >= o) incl += t;
-        }
-        uint64_t c = incl - s;
-        if (c <= thr && thr < incl) {
-            int i = 0;
-            while (c + sh.hist[lane * per + i] <= thr) { c += sh.hist[lane * per + i]; ++i; }
-            sh.out[0] = (uint64_t)(lane * per + i);
-            sh.out[1] = c;
-        }
+    for (int o = 1; o < kWave; o <<= 1) {
+        const uint64_t t = __shfl_up(incl, o, kWave);
+        if (lane >= o) incl += t;
+    }
+    if (lane == kWave - 1) sh.red[wave] = incl;
+    __syncthreads();
+    uint64_t c = incl - h0 - h1;
+    for (int w = 0; w < wave; ++w) c += sh.red[w];
+    if (c <= thr && thr < c + h0 + h1) {
+        const bool second = c + h0 <= thr;
+        sh.out[0] = (uint64_t)(at + (second ? 1 : 0));
+        sh.out[1] = second ? c + h0 : c;
     }
     __syncthreads();
     *bin = (int)sh.out[0];
@@ -449,57 +468,139 @@ __device__ __forceinline__ VfCut vf_solve(const I& it, VfCutShared& sh, const Vf
     return o;
 }
 
-// The same for at most kVfSmall listed elements, one per thread, each against all others.
-__device__ __forceinline__ VfCut vf_solve_small(VfCutShared& sh, const VfRule& u, int n) {
-    const int j = threadIdx.x;
-    const uint64_t mine = j < n ? sh.list[j] : 0ull;
-    const uint32_t key = (uint32_t)(mine >> 32);
-    const float y = val_of(key);
-    bool on = j < n && u.above(y);
-    if (u.k > 0 && j < n) {
-        int more = 0;
-        for (int i = 0; i < n; ++i) more += (uint32_t)(sh.list[i] >> 32) > key ? 1 : 0;
-        on = on && more < u.k;
+// At most kVfSmall listed elements, thread j < n the j-th: its mass w, how many have a larger key, and
+// the sum A of the masses above it in (key, index).  All pairs, spread over the workgroup.
+struct VfRank {
+    uint64_t mine, w, A;
+    float y;
+    int more;
+};
+__device__ __forceinline__ VfRank vf_rank(VfCutShared& sh, const VfRule& u, int n) {
+    const int tid = threadIdx.x;
+    VfRank o{0ull, 0ull, 0ull, 0.0f, 0};
+    uint64_t* mass = sh.hist;
+    uint64_t* A = sh.hist + kVfSmall;
+    if (tid < n) {
+        o.mine = sh.list[tid];
+        o.y = val_of((uint32_t)(o.mine >> 32));
+        o.w = u.mass(o.y);
+        mass[tid] = o.w;
+        A[tid] = 0ull;
+        sh.above[tid] = 0u;
     }
-    const uint64_t w = on ? u.mass(y) : 0ull;
-    if (j < n) sh.hist[j] = w;
-    const uint64_t W = vf_block_sum(w, sh);
-    if (on && u.q32 > 0.0f && u.q32 < 1.0f) {
-        const uint64_t thr = scale_floor(u.q32, W);
-        uint64_t C = 0ull;
-        for (int i = 0; i < n; ++i) C += sh.list[i] <= mine ? sh.hist[i] : 0ull;
-        on = C > thr;  // (the last, whose C is W, stays)
+    __syncthreads();
+    int width = kWave;
+    while (width < n) width *= 2;
+    const int j = tid & (width - 1), parts = kVfCutThreads / width, len = (n + parts - 1) / parts;
+    const int i0 = (tid / width) * len, i1 = min(n, i0 + len);
+    if (j < n) {
+        const uint64_t mine = sh.list[j];
+        uint64_t sum = 0ull;
+        uint32_t more = 0u;
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) {
+            const uint64_t v = sh.list[i];
+            sum += v > mine ? mass[i] : 0ull;
+            more += (uint32_t)(v >> 32) > (uint32_t)(mine >> 32) ? 1u : 0u;
+        }
+        if (more) atomicAdd(&sh.above[j], more);
+        if (sum) atomicAdd(reinterpret_cast<unsigned long long*>(&A[j]), (unsigned long long)sum);
     }
-    VfCut o;
-    o.cut = ~vf_block_max(on ? ~mine : 0ull, sh);
-    o.kept = vf_block_sum(on ? w : 0ull, sh);
+    __syncthreads();
+    if (tid < n) {
+        o.A = A[tid];
+        o.more = (int)sh.above[tid];
+    }
     return o;
 }
 
-// The elements listed are the row's largest.  Whether top-p's cut lies among them for every total
-// in [lo, hi]: then the smallest kept (the lowest element whose sum of larger ones is below p W) is
-// found from above.
-__device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, int n, double lo, double hi, VfCut* o) {
-    const int j = threadIdx.x;
-    const uint64_t mine = j < n ? sh.list[j] : 0ull;
-    const uint64_t w = j < n ? u.mass(val_of((uint32_t)(mine >> 32))) : 0ull;
-    if (j < n) sh.hist[j] = w;
+// Sum of v over threads 0 .. kVfSmall - 1 (those past it pass 0), in every thread.
+__device__ __forceinline__ uint64_t vf_small_sum(uint64_t v, VfCutShared& sh) {
+    const int wave = threadIdx.x >> 6;
     __syncthreads();
-    // kept iff the sum C from below up to it exceeds floor(q W): C = W - A, A the sum above it;
-    // W is an integer in [lo, hi]: with f(W) = W - floor(q W), which never falls, A < f(W)
-    uint64_t A = 0ull;
-    if (j < n)
-        for (int i = 0; i < n; ++i) A += sh.list[i] > mine ? sh.hist[i] : 0ull;
+    if (wave < kVfSmall / kWave) {
+        v = wave_sum_u64(v);
+        if (lane_id() == 0) sh.red[wave] = v;
+    }
+    __syncthreads();
+    uint64_t t = 0ull;
+#pragma unroll
+    for (int i = 0; i < kVfSmall / kWave; ++i) t += sh.red[i];
+    return t;
+}
+// The kept elements' smallest (key, index) and the sum of their masses.
+__device__ __forceinline__ VfCut vf_small_cut(bool on, const VfRank& e, VfCutShared& sh) {
+    VfCut o;
+    o.kept = vf_small_sum(on ? e.w : 0ull, sh);
+    uint64_t v = on ? ~e.mine : 0ull;
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (wave < kVfSmall / kWave) {
+        v = wave_max_u64(v);
+        if (lane_id() == 0) sh.red[wave] = v;
+    }
+    __syncthreads();
+    uint64_t t = 0ull;
+#pragma unroll
+    for (int i = 0; i < kVfSmall / kWave; ++i) t = vws_max64(t, sh.red[i]);
+    o.cut = ~t;
+    return o;
+}
+
+// vf_solve for at most kVfSmall listed elements.  Those above a survivor survive too, so its A is
+// the sum of survivors above it, and it is kept iff what lies up to it, W - A, exceeds floor(q W).
+__device__ __forceinline__ VfCut vf_solve_small(VfCutShared& sh, const VfRule& u, int n) {
+    const VfRank e = vf_rank(sh, u, n);
+    bool on = (int)threadIdx.x < n && u.above(e.y) && (u.k <= 0 || e.more < u.k);
+    if (u.q32 > 0.0f && u.q32 < 1.0f) {
+        const uint64_t W = vf_small_sum(on ? e.w : 0ull, sh);
+        on = on && W - e.A > scale_floor(u.q32, W);
+    }
+    return vf_small_cut(on, e, sh);
+}
+
+// The elements listed are the row's largest.  Whether top-p's cut lies among them, and is the same, for
+// every total W in [lo, hi]: kept iff A < f(W) = W - floor(q W), which never falls.  If not, the part of
+// what is kept that they hold (0 where W is what leaves it open).
+__device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, int n, double lo, double hi, VfCut* o,
+                                             double* held) {
+    const VfRank e = vf_rank(sh, u, n);
+    const bool in = (int)threadIdx.x < n;
     const uint64_t Wl = (uint64_t)lo, Wh = (uint64_t)hi + 1ull;
     const uint64_t fl = Wl - scale_floor(u.q32, Wl), fh = Wh - scale_floor(u.q32, Wh);
-    const bool sure = j < n && A < fl, maybe = j < n && A < fh;
-    const uint64_t unsure = vf_block_max(maybe && !sure ? 1ull : 0ull, sh);
-    const uint64_t total = vf_block_sum(w, sh);
-    // the list ends below the cut: the elements past it would be refused too
-    if (unsure || total < fh) return false;
-    o->cut = ~vf_block_max(sure ? ~mine : 0ull, sh);
-    o->kept = vf_block_sum(sure ? w : 0ull, sh);
+    const bool sure = in && e.A < fl, open = in && e.A < fh && !sure;
+    // (the sum of all masses listed is below 2^53: the count of open ones goes on top)
+    const uint64_t total = vf_small_sum((in ? e.w : 0ull) + (open ? 1ull << 54 : 0ull), sh);
+    // elements past the list have A >= total: refused for every W if total >= f(hi)
+    if (total >= 1ull << 54 || total < fh) {
+        *held = total >= 1ull << 54 ? 0.0 : (double)total / (double)fh;
+        return false;
+    }
+    *o = vf_small_cut(sure, e, sh);
     return true;
+}
+
+// The listed elements are those of one bin, with `under` below them: kept iff under and what lies
+// up to it in the bin exceed thr.  `total`: the sum of all masses.
+__device__ __forceinline__ VfCut vf_solve_bin(VfCutShared& sh, const VfRule& u, int n, uint64_t total, uint64_t under,
+                                              uint64_t thr) {
+    VfCut o;
+    if (n <= kVfSmall) {
+        const VfRank e = vf_rank(sh, u, n);
+        const uint64_t in = vf_small_sum((int)threadIdx.x < n ? e.w : 0ull, sh);
+        o = vf_small_cut((int)threadIdx.x < n && under + (in - e.A) > thr, e, sh);
+        o.kept += total - under - in;
+        return o;
+    }
+    const VfListIter it{sh.list, n};
+    uint64_t c;
+    const uint32_t key = vf_select(it, sh, thr - under, &c, [&](uint32_t, float y) { return u.mass(y); });
+    const uint64_t q = u.mass(val_of(key));
+    const uint64_t gone = (thr - under - c) / q;
+    o.cut = (uint64_t)key << 32;
+    if (gone) o.cut |= (uint32_t)vf_nth_index(it, sh, key, gone);
+    o.kept = total - under - c - gone * q;
+    return o;
 }
 
 // Lists the row's elements with lo <= x <= hi whose y passes `in`; false when they are more than the
@@ -522,23 +623,36 @@ __device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutS
     return sh.count <= (uint32_t)kVfList;
 }
 
+// Calls f(g, part, first vector) for the groups of a row that exist: kVfThreads of them to a quarter
+// of the workgroup at a time.
+template <typename T, typename F>
+__device__ __forceinline__ void vf_each_group(const VerifyArgs& a, F f) {
+    const int its = a.groups / a.S / kVfThreads, t = threadIdx.x & (kVfThreads - 1);
+    int p = 0, it = threadIdx.x / kVfThreads;
+    for (int g = threadIdx.x; g < a.groups; g += kVfCutThreads, it += kVfCutThreads / kVfThreads) {
+        while (it >= its) { it -= its; ++p; }
+        const int b = it * kVfGroup * kVfThreads + t;
+        if (b < vf_part_vecs<T>(a, p)) f(g, p, b);
+    }
+}
+
 // Lists the row's elements with x >= t by the groups' maxima (and the few elements past the parts'
 // last vectors); false when groups or elements are too many.
 template <typename T>
-__device__ __forceinline__ bool vf_gather(const VerifyArgs& a, int r, const T* row, float Tt, VfCutShared& sh, float t) {
+__device__ __forceinline__ bool vf_gather(const VerifyArgs& a, const float* gmax, const T* row, float Tt, VfCutShared& sh,
+                                          float t) {
     constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
-    const int per = a.groups / a.S, tid = threadIdx.x;  // groups of a part
-    const float* gmax = a.gmax + (size_t)r * a.groups;
+    const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.count = sh.ngroups = 0u;
     __syncthreads();
-    for (int g = tid; g < a.groups; g += kVfCutThreads) {
-        const int p = g / per, b = ((g - p * per) / kVfThreads) * U * kVfThreads + (g % kVfThreads);
-        if (b < vf_part_vecs<T>(a, p) && gmax[g] >= t) {
+    vf_each_group<T>(a, [&](int g, int p, int b) {
+        if (gmax[g] >= t) {
             const uint32_t at = agg_reserve(&sh.ngroups);
-            if (at < (uint32_t)kVfGroups) sh.groups[at] = (uint32_t)g;
+            // (parts are whole vectors but for the last: a part's place in vectors of the row)
+            if (at < (uint32_t)kVfGroups) sh.groups[at] = (uint32_t)(p * (a.part_len / VEC) + b);
         }
-    }
+    });
     __syncthreads();
     const int n = (int)sh.ngroups;
     if (n > kVfGroups) return false;
@@ -549,50 +663,61 @@ __device__ __forceinline__ bool vf_gather(const VerifyArgs& a, int r, const T* r
         }
     };
     for (int k = tid; k < n * U; k += kVfCutThreads) {
-        const int g = (int)sh.groups[k / U], p = g / per;
-        const int vi = ((g - p * per) / kVfThreads) * U * kVfThreads + (g % kVfThreads) + (k % U) * kVfThreads;
-        if (vi >= vf_part_vecs<T>(a, p)) continue;
+        const int b = (int)sh.groups[k / U], p = b / (a.part_len / VEC), vi = b + (k % U) * kVfThreads;
+        if (vi >= p * (a.part_len / VEC) + vf_part_vecs<T>(a, p)) continue;
         float v[VEC];
-        vf_load<T>(row + p * a.part_len, vi, v);
+        vf_load<T>(row, vi, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) add(v[j], p * a.part_len + vi * VEC + j);
+        for (int j = 0; j < VEC; ++j) add(v[j], vi * VEC + j);
     }
-    // (a part but the last is whole vectors)
     const int i = a.V / VEC * VEC + tid;
     if (i < a.V) add(Elem<T>::load1(row + i), i);
     __syncthreads();
     return sh.count <= (uint32_t)kVfList;
 }
 
-// The groups' maxima of a row, joined into at most 1024 (thread j: those of j, j + 1024, ...).
+// The maxima of a row's groups, joined into one for each thread.
 template <typename T>
-__device__ __forceinline__ void vf_join_peaks(const VerifyArgs& a, int r, VfCutShared& sh) {
-    const int per = a.groups / a.S;
-    const float* gmax = a.gmax + (size_t)r * a.groups;
+__device__ __forceinline__ float vf_join_peaks(const VerifyArgs& a, const float* gmax) {
     float m = -kVfInf;
-    for (int g = threadIdx.x; g < a.groups; g += kVfCutThreads) {
-        const int p = g / per, b = ((g - p * per) / kVfThreads) * kVfGroup * kVfThreads + (g % kVfThreads);
-        if (b < vf_part_vecs<T>(a, p)) m = __builtin_fmaxf(m, gmax[g]);
-    }
-    sh.peaks[threadIdx.x] = m;
-    __syncthreads();
+    vf_each_group<T>(a, [&](int g, int, int) { m = __builtin_fmaxf(m, gmax[g]); });
+    return m;
 }
 
-// The n-th largest (from 1) of the row's maxima, with its low 16 bits cleared (a bound below it):
-// found bit by bit by every wave for itself.  -inf when there are fewer.
-__device__ __forceinline__ float vf_peak(const VfCutShared& sh, int n) {
-    uint32_t k[kVfCutThreads / kWave];
-#pragma unroll
-    for (int i = 0; i < kVfCutThreads / kWave; ++i) k[i] = key_of(sh.peaks[i * kWave + lane_id()]);
-    uint32_t ans = 0u;
-    for (int b = 31; b >= 16; --b) {
-        const uint32_t cand = ans | (1u << b);
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < kVfCutThreads / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
-        if (c >= n) ans = cand;
+// A bound that at least n (from 1) of the threads' maxima reach, and few more: the lower edge of the
+// bin that holds the n-th of them, in bins over their range, again within a bin that holds too many.
+// -inf when fewer than n are finite.
+__device__ __forceinline__ float vf_peak(VfCutShared& sh, float peak, int n) {
+    const bool fin = peak > -kVfInf;
+    if (__syncthreads_count(fin) < n) return -kVfInf;
+    float hi = val_of((uint32_t)vf_block_max(key_of(peak), sh));
+    float lo = -val_of((uint32_t)vf_block_max(fin ? key_of(-peak) : 0ull, sh));
+    uint64_t rank = (uint64_t)n - 1ull;  // in what is left, from the top
+    float t = -kVfInf;
+    for (int round = 0; round < 5; ++round) {
+        // (halves: the difference may overflow)
+        const float scale = (float)(kVfBins - 1) / (0.5f * hi - 0.5f * lo);
+        if (!(scale < kVfInf && scale > 0.0f)) return lo;
+        vf_clear(sh);
+        int at = -1;
+        if (fin && peak <= hi && peak >= lo) {
+            at = min((int)((0.5f * hi - 0.5f * peak) * scale), kVfBins - 1);
+            vf_count(sh, at, 1ull);
+        }
+        int bin;
+        uint64_t over;
+        vf_find(sh, kVfBins, rank, &bin, &over);
+        const uint64_t in = sh.hist[bin];
+        // the bin's own smallest: at least n reach it
+        t = -val_of((uint32_t)vf_block_max(at == bin ? key_of(-peak) : 0ull, sh));
+        if (over + in - rank <= 1ull + (uint64_t)n / 16ull) return t;
+        const float top = val_of((uint32_t)vf_block_max(at == bin ? key_of(peak) : 0ull, sh));
+        if (!(top > t)) return t;
+        rank -= over;
+        hi = top;
+        lo = t;
     }
-    return ans >= 0x00800000u ? val_of(ans) : -kVfInf;  // (below: -inf or none)
+    return t;
 }
 
 struct VfRow {
@@ -639,7 +764,8 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
     u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
     VfCut o{0ull, 0ull};
     if (!w.sure) {
-        vf_join_peaks<T>(a, r, sh);
+        const float* gmax = a.gmax + (size_t)r * a.groups;
+        const float peak = vf_join_peaks<T>(a, gmax);
         // y = fl(x / T) and y - m round, and a maximum's group may hold the k-th largest itself:
         // a margin of some ulps below the bound keeps every element that could survive
         // (T 2^-120: where y is subnormal)
@@ -658,13 +784,13 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             done = true;
         } else if (u.k > 0 || u.lp_min > -kVfInf) {
             float t = -kVfInf;
-            if (u.k > 0 && u.k <= kVfCutThreads) t = below(vf_peak(sh, u.k));
+            if (u.k > 0 && u.k <= kVfCutThreads) t = below(vf_peak(sh, peak, u.k));
             if (u.lp_min > -kVfInf) {
                 const float y = u.m + u.lp_min;
                 t = __builtin_fmaxf(t, Tt * (y - (__builtin_fabsf(u.m) - u.lp_min) * 0x1p-20f) - tiny);
             }
             const bool k_listed = u.k == 0 || t > -kVfInf;
-            if (k_listed && vf_gather<T>(a, r, row, Tt, sh, t)) {
+            if (k_listed && vf_gather<T>(a, gmax, row, Tt, sh, t)) {
                 const int n = (int)sh.count;
                 o = n <= kVfSmall ? vf_solve_small(sh, u, n) : vf_solve(VfListIter{sh.list, n}, sh, u, (uint64_t)n);
                 done = true;
@@ -674,10 +800,14 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
             // its constant likewise, the exponential and the sums by a few 2^-24
             const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
-            // (about 360 logits lie above the 300th of 1024 maxima)
-            const float t = below(vf_peak(sh, 300));
-            if (t > -kVfInf && vf_gather<T>(a, r, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
-                done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
+            // the 105 or so logits above the 100th of 1024 maxima, or, where they hold a good part of
+            // what is kept, the 355 or so above the 300th
+            double held = 1.0;
+            for (int n = 100; !done && n <= 300 && held > 0.5; n += 200) {
+                const float t = below(vf_peak(sh, peak, n));
+                if (!(t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)) break;
+                done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
+            }
             if (!done) {
                 // every mass, by distance from the maximum; what lies further than `far` holds less
                 // than q W (W is at least the maximum's own mass) and is only summed
@@ -707,16 +837,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
                             const float d = u.m - y;
                             return d < far && (int)(d * scale) == bin;
                         })) {
-                        const int n = (int)sh.count;
-                        // among the bin's elements: kept iff under + their sum up to it exceeds thr
-                        const VfListIter it{sh.list, n};
-                        uint64_t c;
-                        const uint32_t key = vf_select(it, sh, thr - under, &c, [&](uint32_t, float y) { return u.mass(y); });
-                        const uint64_t q = u.mass(val_of(key));
-                        const uint64_t gone = (thr - under - c) / q;
-                        o.cut = (uint64_t)key << 32;
-                        if (gone) o.cut |= (uint32_t)vf_nth_index(it, sh, key, gone);
-                        o.kept = total - under - c - gone * q;
+                        o = vf_solve_bin(sh, u, (int)sh.count, total, under, thr);
                         done = true;
                     }
                 }
