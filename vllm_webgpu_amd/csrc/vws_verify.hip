@@ -230,7 +230,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 // The kept set is that of vws_sample, decided on the integer masses w = floor(exp_det(y - m) 2^44):
 // their sums do not depend on the order, so the set does not depend on how it is found.  Three ways,
 // by what bounds the row's survivors:
-//   * top-k or min-p: a bound on the logit below which nothing survives (the k-th largest of 1024
+//   * top-k or min-p: a bound on the logit below which nothing survives (the k-th largest of 256
 //     maxima, joined from the groups' that the first pass left, or m + log(min_p)); the few logits
 //     above it, read where a group's maximum reaches it, go into a list, which decides everything;
 //   * top-p alone: the list of the logits above such a bound, if it holds the cut for any total
@@ -244,6 +244,8 @@ constexpr int kVfCutWaves = kVfCutThreads / 64;
 constexpr int kVfList = 2048;     // list entries (a row's candidates)
 constexpr int kVfSmall = 512;     // entries that are compared with each other, all pairs
 constexpr int kVfGroups = 1024;   // groups that are read for the list
+constexpr int kVfPeaks = 256;     // maxima that bound the list
+constexpr int kVfPeakMost = 232;  // of them, the last whose rank is used (the next are few and far between)
 
 struct VfCutShared {
     uint64_t hist[kVfBins];
@@ -252,7 +254,9 @@ struct VfCutShared {
     uint32_t groups[kVfGroups];
     uint64_t red[kVfCutWaves];
     uint64_t out[4];
+    float peaks[kVfPeaks];        // maxima, each of the groups of four threads
     uint32_t count, ngroups;
+    float bound;
 };
 
 __device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
@@ -530,20 +534,22 @@ __device__ __forceinline__ uint64_t vf_small_sum(uint64_t v, VfCutShared& sh) {
 }
 // The kept elements' smallest (key, index) and the sum of their masses.
 __device__ __forceinline__ VfCut vf_small_cut(bool on, const VfRank& e, VfCutShared& sh) {
-    VfCut o;
-    o.kept = vf_small_sum(on ? e.w : 0ull, sh);
-    uint64_t v = on ? ~e.mine : 0ull;
+    constexpr int W = kVfSmall / kWave;
+    static_assert(2 * W <= kVfCutWaves, "two words a wave");
     const int wave = threadIdx.x >> 6;
     __syncthreads();
-    if (wave < kVfSmall / kWave) {
-        v = wave_max_u64(v);
-        if (lane_id() == 0) sh.red[wave] = v;
+    if (wave < W) {
+        const uint64_t s = wave_sum_u64(on ? e.w : 0ull), v = wave_max_u64(on ? ~e.mine : 0ull);
+        if (lane_id() == 0) { sh.red[wave] = s; sh.red[W + wave] = v; }
     }
     __syncthreads();
-    uint64_t t = 0ull;
+    VfCut o{0ull, 0ull};
 #pragma unroll
-    for (int i = 0; i < kVfSmall / kWave; ++i) t = vws_max64(t, sh.red[i]);
-    o.cut = ~t;
+    for (int i = 0; i < W; ++i) {
+        o.kept += sh.red[i];
+        o.cut = vws_max64(o.cut, sh.red[W + i]);
+    }
+    o.cut = ~o.cut;
     return o;
 }
 
@@ -623,16 +629,24 @@ __device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutS
     return sh.count <= (uint32_t)kVfList;
 }
 
-// Calls f(g, part, first vector) for the groups of a row that exist: kVfThreads of them to a quarter
-// of the workgroup at a time.
+// Calls f(maximum, part, first vector) for the groups of a row that exist: kVfThreads of them to a
+// quarter of the workgroup at a time, four loads in flight.
 template <typename T, typename F>
-__device__ __forceinline__ void vf_each_group(const VerifyArgs& a, F f) {
+__device__ __forceinline__ void vf_each_group(const VerifyArgs& a, const float* gmax, F f) {
+    constexpr int U = 4, kStep = kVfCutThreads / kVfThreads;
     const int its = a.groups / a.S / kVfThreads, t = threadIdx.x & (kVfThreads - 1);
-    int p = 0, it = threadIdx.x / kVfThreads;
-    for (int g = threadIdx.x; g < a.groups; g += kVfCutThreads, it += kVfCutThreads / kVfThreads) {
-        while (it >= its) { it -= its; ++p; }
-        const int b = it * kVfGroup * kVfThreads + t;
-        if (b < vf_part_vecs<T>(a, p)) f(g, p, b);
+    int p = 0, it = __builtin_amdgcn_readfirstlane(threadIdx.x / kVfThreads);
+    for (int g = threadIdx.x; g < a.groups; g += U * kVfCutThreads) {
+        float m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) m[u] = gmax[min(g + u * kVfCutThreads, a.groups - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            while (it >= its) { it -= its; ++p; }
+            const int b = it * kVfGroup * kVfThreads + t;
+            if (p < a.S && b < vf_part_vecs<T>(a, p)) f(m[u], p, b);
+            it += kStep;
+        }
     }
 }
 
@@ -646,8 +660,8 @@ __device__ __forceinline__ bool vf_gather(const VerifyArgs& a, const float* gmax
     __syncthreads();
     if (tid == 0) sh.count = sh.ngroups = 0u;
     __syncthreads();
-    vf_each_group<T>(a, [&](int g, int p, int b) {
-        if (gmax[g] >= t) {
+    vf_each_group<T>(a, gmax, [&](float m, int p, int b) {
+        if (m >= t) {
             const uint32_t at = agg_reserve(&sh.ngroups);
             // (parts are whole vectors but for the last: a part's place in vectors of the row)
             if (at < (uint32_t)kVfGroups) sh.groups[at] = (uint32_t)(p * (a.part_len / VEC) + b);
@@ -676,48 +690,38 @@ __device__ __forceinline__ bool vf_gather(const VerifyArgs& a, const float* gmax
     return sh.count <= (uint32_t)kVfList;
 }
 
-// The maxima of a row's groups, joined into one for each thread.
+// The maxima of a row's groups, joined into kVfPeaks.
 template <typename T>
-__device__ __forceinline__ float vf_join_peaks(const VerifyArgs& a, const float* gmax) {
+__device__ __forceinline__ void vf_join_peaks(const VerifyArgs& a, const float* gmax, VfCutShared& sh) {
     float m = -kVfInf;
-    vf_each_group<T>(a, [&](int g, int, int) { m = __builtin_fmaxf(m, gmax[g]); });
-    return m;
+    vf_each_group<T>(a, gmax, [&](float g, int, int) { m = __builtin_fmaxf(m, g); });
+    m = __builtin_fmaxf(m, vf_lane_xor(m, 1));
+    m = __builtin_fmaxf(m, vf_lane_xor(m, 2));
+    static_assert(kVfCutThreads / kVfPeaks == 4, "a maximum for every four threads");
+    if ((threadIdx.x & 3) == 0) sh.peaks[threadIdx.x / 4] = m;
+    __syncthreads();
 }
 
-// A bound that at least n (from 1) of the threads' maxima reach, and few more: the lower edge of the
-// bin that holds the n-th of them, in bins over their range, again within a bin that holds too many.
-// -inf when fewer than n are finite.
-__device__ __forceinline__ float vf_peak(VfCutShared& sh, float peak, int n) {
-    const bool fin = peak > -kVfInf;
-    if (__syncthreads_count(fin) < n) return -kVfInf;
-    float hi = val_of((uint32_t)vf_block_max(key_of(peak), sh));
-    float lo = -val_of((uint32_t)vf_block_max(fin ? key_of(-peak) : 0ull, sh));
-    uint64_t rank = (uint64_t)n - 1ull;  // in what is left, from the top
-    float t = -kVfInf;
-    for (int round = 0; round < 5; ++round) {
-        // (halves: the difference may overflow)
-        const float scale = (float)(kVfBins - 1) / (0.5f * hi - 0.5f * lo);
-        if (!(scale < kVfInf && scale > 0.0f)) return lo;
-        vf_clear(sh);
-        int at = -1;
-        if (fin && peak <= hi && peak >= lo) {
-            at = min((int)((0.5f * hi - 0.5f * peak) * scale), kVfBins - 1);
-            vf_count(sh, at, 1ull);
+// The n-th largest (from 1) of the row's peaks, with its low 16 bits cleared (a bound below it): found
+// bit by bit by one wave.  -inf when fewer are finite.
+__device__ __forceinline__ float vf_peak(VfCutShared& sh, int n) {
+    if (threadIdx.x < kWave) {
+        uint32_t k[kVfPeaks / kWave];
+#pragma unroll
+        for (int i = 0; i < kVfPeaks / kWave; ++i) k[i] = key_of(sh.peaks[i * kWave + lane_id()]);
+        uint32_t ans = 0u;
+#pragma unroll
+        for (int b = 31; b >= 16; --b) {
+            const uint32_t cand = ans | (1u << b);
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < kVfPeaks / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
+            if (c >= n) ans = cand;
         }
-        int bin;
-        uint64_t over;
-        vf_find(sh, kVfBins, rank, &bin, &over);
-        const uint64_t in = sh.hist[bin];
-        // the bin's own smallest: at least n reach it
-        t = -val_of((uint32_t)vf_block_max(at == bin ? key_of(-peak) : 0ull, sh));
-        if (over + in - rank <= 1ull + (uint64_t)n / 16ull) return t;
-        const float top = val_of((uint32_t)vf_block_max(at == bin ? key_of(peak) : 0ull, sh));
-        if (!(top > t)) return t;
-        rank -= over;
-        hi = top;
-        lo = t;
+        if (threadIdx.x == 0) sh.bound = ans >= 0x00800000u ? val_of(ans) : -kVfInf;  // (below: -inf or none)
     }
-    return t;
+    __syncthreads();
+    return sh.bound;
 }
 
 struct VfRow {
@@ -765,7 +769,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
     VfCut o{0ull, 0ull};
     if (!w.sure) {
         const float* gmax = a.gmax + (size_t)r * a.groups;
-        const float peak = vf_join_peaks<T>(a, gmax);
+        vf_join_peaks<T>(a, gmax, sh);
         // y = fl(x / T) and y - m round, and a maximum's group may hold the k-th largest itself:
         // a margin of some ulps below the bound keeps every element that could survive
         // (T 2^-120: where y is subnormal)
@@ -784,7 +788,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             done = true;
         } else if (u.k > 0 || u.lp_min > -kVfInf) {
             float t = -kVfInf;
-            if (u.k > 0 && u.k <= kVfCutThreads) t = below(vf_peak(sh, peak, u.k));
+            if (u.k > 0 && u.k <= kVfPeakMost) t = below(vf_peak(sh, u.k));
             if (u.lp_min > -kVfInf) {
                 const float y = u.m + u.lp_min;
                 t = __builtin_fmaxf(t, Tt * (y - (__builtin_fabsf(u.m) - u.lp_min) * 0x1p-20f) - tiny);
@@ -800,11 +804,11 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
             // its constant likewise, the exponential and the sums by a few 2^-24
             const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
-            // the 105 or so logits above the 100th of 1024 maxima, or, where they hold a good part of
-            // what is kept, the 355 or so above the 300th
+            // the 100 or so logits above the 84th of 256 maxima, or, where they hold a good part of
+            // what is kept, the 350 or so above the 192nd
             double held = 1.0;
-            for (int n = 100; !done && n <= 300 && held > 0.5; n += 200) {
-                const float t = below(vf_peak(sh, peak, n));
+            for (int n = 84; !done && n <= 192 && held > 0.5; n += 108) {
+                const float t = below(vf_peak(sh, n));
                 if (!(t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)) break;
                 done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
             }
