@@ -38,6 +38,7 @@ template <typename T> __global__ void verify_cut_kernel(VerifyArgs);
 template <typename T> __global__ void verify_token_kernel(VerifyArgs);
 template <typename T, bool BUCKET> __global__ void distill_forward_kernel(DistillArgs);
 template <typename T> __global__ void distill_backward_kernel(DistillArgs);
+template <typename T, bool BUCKET, int NV> __global__ void distill_step_kernel(DistillArgs);
 }  // namespace vws
 
 using namespace vws;
@@ -541,6 +542,18 @@ int validate_distill(const vws_distill_args* a, int parts) {
     return VWS_OK;
 }
 
+// The kernel that holds a row in one workgroup's registers, or null: rows that fit (40 vectors of 16
+// bytes for each of 512 threads), and enough of them to keep half of the compute units at work.
+template <typename T>
+auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
+    const int per = (V / (16 / (int)sizeof(T)) + kDsStepThreads - 1) / kDsStepThreads;
+    if (rows < device_info().cus / 2 || per < 1) return nullptr;
+    if (per <= 16) return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
+    if (per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
+    if (per <= 40) return bucket ? distill_step_kernel<T, true, 40> : distill_step_kernel<T, false, 40>;
+    return nullptr;
+}
+
 template <typename T>
 int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
     DistillArgs k;
@@ -565,6 +578,14 @@ int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
     k.entry_p = static_cast<float*>(a->saved) + (size_t)a->rows * kDsRowStats + (size_t)r0 * k.K;
     const int K = VWS_KERNEL_DISTILL;
     hipStream_t s = (hipStream_t)a->stream;
+    if (parts == (kDistillForward | kDistillBackward)) {
+        if (const auto f = distill_step<T>(rows, k.V, a->tail == VWS_TAIL_BUCKET)) {
+            const int cus = device_info().cus;
+            const unsigned lds = a->tail == VWS_TAIL_BUCKET ? (unsigned)((k.V + 31) / 32) * 4u : 0u;
+            launch_lds(K, f, dim3(rows < cus ? rows : cus), dim3(kDsStepThreads), lds, s, k);
+            return check_launch("vws_distill (step)");
+        }
+    }
     distill_parts(rows, k.V, &k.S, &k.part_len);
     const dim3 grid((unsigned)rows * (unsigned)k.S), block(kDsThreads);
     if (parts & kDistillForward) {

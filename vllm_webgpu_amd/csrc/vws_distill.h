@@ -8,7 +8,7 @@
 namespace vws {
 
 constexpr int kDsThreads = 256;     // threads of a part (forward and backward)
-constexpr int kDsStepThreads = 1024;  // threads of a row (step)
+constexpr int kDsStepThreads = 512;   // threads of a row (step)
 constexpr int kDsMaxK = 256;        // teacher entries of a row, one per thread of a part
 constexpr int kDsMaxParts = 64;     // parts of a row: one lane each in the join
 constexpr int kDsRowStats = 8;      // floats of a row's statistics (DistillStat)

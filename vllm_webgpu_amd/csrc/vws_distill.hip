@@ -38,6 +38,7 @@ template <> struct DsVec<float> {
 };
 template <> struct DsVec<uint16_t> {
     typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2)));
+    static constexpr uint32_t kNegInf = 0xFF80FF80u;
     static __device__ __forceinline__ void set_neg_inf(uint32_t (&w)[4], int j) {
         w[j >> 1] = (j & 1) ? (w[j >> 1] & 0xFFFFu) | 0xFF800000u : (w[j >> 1] & 0xFFFF0000u) | 0xFF80u;
     }
@@ -49,6 +50,7 @@ template <> struct DsVec<uint16_t> {
 };
 template <> struct DsVec<_Float16> {
     typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2)));
+    static constexpr uint32_t kNegInf = 0xFC00FC00u;
     static __device__ __forceinline__ void set_neg_inf(uint32_t (&w)[4], int j) {
         w[j >> 1] = (j & 1) ? (w[j >> 1] & 0xFFFFu) | 0xFC000000u : (w[j >> 1] & 0xFFFF0000u) | 0xFC00u;
     }
@@ -61,16 +63,17 @@ template <> struct DsVec<_Float16> {
     }
 };
 
+// (vi: a 32-bit offset, at most 2 MB, on the row's pointer)
 template <typename T>
 __device__ __forceinline__ void ds_load(const T* row, int vi, uint32_t (&w)[4]) {
-    const auto u = *reinterpret_cast<const typename DsVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec);
+    const auto u = *reinterpret_cast<const typename DsVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi);
     w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
 }
 template <typename T>
 __device__ __forceinline__ void ds_store(T* row, int vi, const uint32_t (&w)[4]) {
     typename DsVec<T>::U4 u;
     u[0] = w[0]; u[1] = w[1]; u[2] = w[2]; u[3] = w[3];
-    __builtin_nontemporal_store(u, reinterpret_cast<typename DsVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec));
+    __builtin_nontemporal_store(u, reinterpret_cast<typename DsVec<T>::U4*>(reinterpret_cast<char*>(row) + 16u * (uint32_t)vi));
 }
 
 __device__ __forceinline__ float ds_lane_xor(float v, int s) { return u2f(lane_xor(f2u(v), s)); }
@@ -123,6 +126,10 @@ __device__ __forceinline__ void ds_add(DsSum& t, const uint32_t (&w)[U][4], floa
     t.m = n;
 }
 
+__device__ __forceinline__ void ds_add1(DsSum& t, float z) {
+    t.merge(z, z == z && z < kDsInf ? (z == -kDsInf ? 0.0f : 1.0f) : __builtin_nanf(""));
+}
+
 // The bits of a part's elements that are teacher entries, from its first element on.
 __device__ __forceinline__ void ds_bitmap(uint32_t* bm, int len, const int32_t* ids, int K, int lo, int threads) {
     for (int i = threadIdx.x; i < (len + 31) / 32; i += threads) bm[i] = 0u;
@@ -146,19 +153,27 @@ __device__ __forceinline__ void ds_drop(const uint32_t* bm, int vi, uint32_t (&w
     }
 }
 
-// A part's running sum: elements [0, len) of `row`, without those whose bit is set (BUCKET).
-template <typename T, bool BUCKET>
-__device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const uint32_t* bm) {
+// A part's running sum: elements [0, len) of `row`, without those whose bit is set (BUCKET).  The next
+// four vectors' loads are issued before these are used; the first before `ready` (the bitmap).
+template <typename T, bool BUCKET, typename F>
+__device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const uint32_t* bm, F ready) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
     const int nvec = len / VEC, tid = threadIdx.x;
+    uint32_t next[U][4];
+    auto fetch = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) ds_load<T>(row, min(b + u * kDsThreads, nvec - 1), next[u]);
+    };
+    if (nvec > 0) fetch(tid);
+    ready();
     DsSum t;
     for (int b = tid; b < nvec; b += U * kDsThreads) {
         uint32_t w[U][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vi = b + u * kDsThreads;
-            ds_load<T>(row, vi < nvec ? vi : b, w[u]);
-        }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[u][k] = next[u][k];
+        if (b + U * kDsThreads < nvec) fetch(b + U * kDsThreads);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int vi = b + u * kDsThreads;
@@ -172,10 +187,7 @@ __device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const
         ds_add<T, U>(t, w, c);
     }
     const int i = nvec * VEC + tid;
-    if (i < len && !(BUCKET && ((bm[i >> 5] >> (i & 31)) & 1u))) {
-        const float z = Elem<T>::load1(row + i) * c;
-        t.merge(z, z == z && z < kDsInf ? (z == -kDsInf ? 0.0f : 1.0f) : __builtin_nanf(""));
-    }
+    if (i < len && !(BUCKET && ((bm[i >> 5] >> (i & 31)) & 1u))) ds_add1(t, Elem<T>::load1(row + i) * c);
     return t;
 }
 
@@ -209,13 +221,25 @@ struct DsRow {
 };
 
 // A row's loss and statistics from the running sum of its rest (BUCKET) or of all of it.  Called by
-// every thread of a workgroup of at least 256; thread k < K has entry k.  `lid`, `lpr`: K words of
-// LDS each, `red`: 16.
+// every thread of a workgroup of at least 256; thread k < K has entry k.
+struct DsShared {
+    float red[16];
+    float lpr[kDsMaxK];
+    int32_t lid[kDsMaxK];
+    // the entries' ids, hashed: an id, its first entry, its entries
+    int32_t hid[2 * kDsMaxK];
+    uint32_t hfirst[2 * kDsMaxK], hcount[2 * kDsMaxK];
+};
+
 template <typename T, bool BUCKET>
-__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T* row, DsSum rest, float w,
-                                           int32_t* lid, float* lpr, float* red) {
+__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T* row, DsSum rest, float w, DsShared& sh) {
     const int k = threadIdx.x, K = a.K;
-    DsBlock blk{red};
+    DsBlock blk{sh.red};
+    for (int i = k; i < 2 * kDsMaxK; i += blockDim.x) {
+        sh.hid[i] = -1;
+        sh.hfirst[i] = ~0u;
+        sh.hcount[i] = 0u;
+    }
     int id = -1;
     float l = -kDsInf, x = 0.0f;
     if (k < K) {
@@ -225,10 +249,10 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T*
             l = a.lp[(size_t)r * a.lp_stride + k];
             x = Elem<T>::load1(row + id);
         }
-        lid[k] = id;
+        sh.lid[k] = id;
     }
     const bool valid = id >= 0;
-    // the teacher's probabilities
+    // the teacher's probabilities (the reductions' barriers order the table's clearing before its use)
     float p, logp;
     bool live;
     if (BUCKET) {
@@ -244,23 +268,26 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T*
         p = e / tot;
         logp = logp - top - logf(tot);
     }
-    if (k < K) lpr[k] = p;
-    __syncthreads();
     // entries that share an id: the first takes their probability together
-    bool first = valid;
+    if (k < K) sh.lpr[k] = p;
+    int slot = 0;
+    if (valid) {  // (at most 256 of 512 places are taken)
+        slot = (int)(((uint32_t)id * 2654435761u) >> 23);
+        for (;;) {
+            const int had = atomicCAS(&sh.hid[slot], -1, id);
+            if (had == -1 || had == id) break;
+            slot = (slot + 1) & (2 * kDsMaxK - 1);
+        }
+        atomicMin(&sh.hfirst[slot], (uint32_t)k);
+        atomicAdd(&sh.hcount[slot], 1u);
+    }
+    __syncthreads();
+    const bool first = valid && sh.hfirst[slot] == (uint32_t)k;
     float P = p;
-    if (valid) {
-        bool more = false;
-        for (int j = 0; j < K; ++j) {
-            const bool same = lid[j] == id && j != k;
-            first = first && !(same && j < k);
-            more = more || same;
-        }
-        if (more) {
-            P = 0.0f;
-            for (int j = 0; j < K; ++j)
-                if (lid[j] == id) P += lpr[j];
-        }
+    if (first && sh.hcount[slot] > 1u) {
+        P = 0.0f;
+        for (int j = 0; j < K; ++j)
+            if (sh.lid[j] == id) P += sh.lpr[j];
     }
     // the student's total
     float M = rest.m, Z = rest.s;
@@ -317,9 +344,7 @@ __device__ __forceinline__ void ds_save(const DistillArgs& a, int r, const DsRow
 template <typename T, bool BUCKET>
 __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs a) {
     extern __shared__ uint32_t bm[];
-    __shared__ int32_t lid[kDsMaxK];
-    __shared__ float lpr[kDsMaxK];
-    __shared__ float red[16];
+    __shared__ DsShared sh;
     __shared__ float wm[kDsThreads / 64], ws[kDsThreads / 64];
     __shared__ uint32_t last;
     const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, wave = tid >> 6;
@@ -333,8 +358,9 @@ __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs
     }
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo;
-    if (BUCKET) ds_bitmap(bm, len, a.ids + (size_t)r * a.ids_stride, a.K, lo, kDsThreads);
-    DsSum t = ds_stream<T, BUCKET>(row + lo, len, a.c, bm);
+    DsSum t = ds_stream<T, BUCKET>(row + lo, len, a.c, bm, [&] {
+        if (BUCKET) ds_bitmap(bm, len, a.ids + (size_t)r * a.ids_stride, a.K, lo, kDsThreads);
+    });
     t.wave_merge();
     if ((tid & 63) == 0) { wm[wave] = t.m; ws[wave] = t.s; }
     __syncthreads();
@@ -360,15 +386,16 @@ __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs
         }
         t.wave_merge();
     }
-    const DsRow o = ds_finish<T, BUCKET>(a, r, row, t, w, lid, lpr, red);
+    const DsRow o = ds_finish<T, BUCKET>(a, r, row, t, w, sh);
     ds_save(a, r, o);
 }
 
-// The gradient of part p of row r.
+// The gradient of part p of row r.  Rows from the last to the first: those that the forward read last
+// are still in the last-level cache.
 template <typename T>
 __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
-    const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x;
+    const int S = a.S, block = gridDim.x - 1 - blockIdx.x, r = block / S, p = block - r * S, tid = threadIdx.x;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     T* out = static_cast<T*>(a.grad) + (size_t)r * a.gstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
@@ -421,7 +448,123 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
     if (at >= 0) out[at] = DsVec<T>::narrow(fix);
 }
 
+// Loss and gradient of rows that one workgroup holds in its registers (NV vectors a thread): every
+// logit is read once and its gradient written once.  One workgroup for each compute unit, a row at a
+// time; as a row's gradients are written, the next row's logits are loaded into the registers they
+// leave.
+template <typename T, bool BUCKET, int NV>
+__global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArgs a) {
+    constexpr int VEC = Elem<T>::kVec, U = 2, W = kDsStepThreads / 64;
+    extern __shared__ uint32_t bm[];
+    __shared__ DsShared sh;
+    __shared__ float wm[W], ws[W];
+    const int tid = threadIdx.x, wave = tid >> 6, V = a.V, nvec = V / VEC, edge = nvec * VEC + tid;
+    const T* x = static_cast<const T*>(a.x);
+    T* grad = static_cast<T*>(a.grad);
+    auto live = [&](int r) { return !a.weight || a.weight[r] != 0.0f; };
+    uint32_t w[NV][4];
+    float xe = 0.0f;  // the thread's logit past the last vector
+    // What follows is for registers: the scheduler must not work on many vectors at once, nor the
+    // compiler keep every vector's offsets, bounds or widened logits from one use to the next.
+    auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    auto fresh = [](int v) __attribute__((always_inline)) {
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    // vectors past `end` repeat it: every load is unconditional
+    auto fetch = [&](const T* row, int q, int end) __attribute__((always_inline)) {
+        ds_load<T>(row, min(fresh(tid) + q * kDsStepThreads, end), w[q]);
+    };
+    int r = blockIdx.x;
+    auto skip = [&]() {  // rows that do not count: zeros
+        for (; r < a.N && !live(r); r += gridDim.x) {
+            const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+            T* out = grad + (size_t)r * a.gstride;
+            for (int vi = tid; vi < nvec; vi += kDsStepThreads) ds_store<T>(out, vi, zero);
+            if (edge < V) out[edge] = DsVec<T>::narrow(0.0f);
+            if (tid == 0) a.loss[r] = 0.0f;
+        }
+    };
+    skip();
+    if (r >= a.N) return;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) fetch(x + (size_t)r * a.xstride, q, nvec - 1);
+    if (edge < V) xe = Elem<T>::load1(x + (size_t)r * a.xstride + edge);
+    for (;;) {
+        const T* row = x + (size_t)r * a.xstride;
+        T* out = grad + (size_t)r * a.gstride;
+        const float wt = a.weight ? a.weight[r] : 1.0f;
+        if (BUCKET) ds_bitmap(bm, V, a.ids + (size_t)r * a.ids_stride, a.K, 0, kDsStepThreads);
+        DsSum t;
+#pragma unroll
+        for (int q0 = 0; q0 < NV; q0 += U) {
+            uint32_t g[U][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int vi = fresh(tid) + (q0 + u) * kDsStepThreads;
+                if (BUCKET) ds_drop<T>(bm, min(vi, nvec - 1), w[q0 + u]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // (in place: what lies past the row is never written)
+                    w[q0 + u][k] = vi < nvec ? w[q0 + u][k] : DsVec<T>::kNegInf;
+                    asm volatile("" : "+v"(w[q0 + u][k]));
+                    g[u][k] = w[q0 + u][k];
+                }
+            }
+            ds_add<T, U>(t, g, a.c);
+            fence();
+        }
+        const bool drop = BUCKET && edge < V && ((bm[edge >> 5] >> (edge & 31)) & 1u);
+        if (edge < V && !drop) ds_add1(t, xe * a.c);
+        t.wave_merge();
+        if ((tid & 63) == 0) { wm[wave] = t.m; ws[wave] = t.s; }
+        __syncthreads();
+        t = DsSum();
+#pragma unroll
+        for (int i = 0; i < W; ++i) t.merge(wm[i], ws[i]);
+        const DsRow o = ds_finish<T, BUCKET>(a, r, row, t, wt, sh);
+        const float gs = wt * (a.gout ? a.gout[r] : 1.0f) * a.inv_T;
+        const bool on = o.live && gs != 0.0f;
+        const float ref = o.ref, coef = o.coef * gs;
+        const int id = tid < a.K && !(o.p < 0.0f) ? sh.lid[tid] : -1;
+        const float fix = gs * (ds_exp2(__builtin_fmaf(o.x, a.c, -o.max)) * o.inv_total - o.p);
+        r += gridDim.x;
+        skip();
+        const bool more = r < a.N;
+        const T* after = more ? x + (size_t)r * a.xstride : row;
+        const int end = more ? nvec - 1 : 0;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            const int vi = fresh(tid) + q * kDsStepThreads;
+            float v[VEC];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(w[q][k]));
+            Elem<T>::from_words(w[q][0], w[q][1], w[q][2], w[q][3], v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = on ? ds_exp2(__builtin_fmaf(v[j], a.c, -ref)) * coef : 0.0f;
+            uint32_t g[4];
+            DsVec<T>::pack(v, g);
+            if (vi < nvec) ds_store<T>(out + (size_t)q * kDsStepThreads * VEC, fresh(tid), g);
+            fetch(after, q, end);
+            fence();
+        }
+        if (edge < V) out[edge] = DsVec<T>::narrow(on ? ds_exp2(__builtin_fmaf(xe, a.c, -ref)) * coef : 0.0f);
+        if (more && edge < V) xe = Elem<T>::load1(after + edge);
+        // the teacher's entries over what was written there, once that has arrived
+        stores_complete();
+        __syncthreads();
+        if (on && id >= 0) out[id] = DsVec<T>::narrow(fix);
+        if (!more) return;
+    }
+}
+
+#define VWS_DISTILL_STEP(T, NV)                                                      \
+    template __global__ void distill_step_kernel<T, false, NV>(DistillArgs);         \
+    template __global__ void distill_step_kernel<T, true, NV>(DistillArgs);
 #define VWS_DISTILL_INST(T)                                                   \
+    VWS_DISTILL_STEP(T, 16)                                                   \
+    VWS_DISTILL_STEP(T, 32)                                                   \
+    VWS_DISTILL_STEP(T, 40)                                                   \
     template __global__ void distill_forward_kernel<T, false>(DistillArgs);   \
     template __global__ void distill_forward_kernel<T, true>(DistillArgs);    \
     template __global__ void distill_backward_kernel<T>(DistillArgs);
