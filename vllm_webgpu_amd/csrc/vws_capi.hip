@@ -542,7 +542,7 @@ int validate_distill(const vws_distill_args* a, int parts) {
     return VWS_OK;
 }
 
-// The kernel that holds a row in one workgroup's registers, or null: rows that fit (40 vectors of 16
+// The kernel that holds a row in one workgroup's registers, or null: rows that fit (38 vectors of 16
 // bytes for each of 512 threads), and enough of them to keep half of the compute units at work.
 template <typename T>
 auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
@@ -550,7 +550,7 @@ auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
     if (rows < device_info().cus / 2 || per < 1) return nullptr;
     if (per <= 16) return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
     if (per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
-    if (per <= 40) return bucket ? distill_step_kernel<T, true, 40> : distill_step_kernel<T, false, 40>;
+    if (per <= 38) return bucket ? distill_step_kernel<T, true, 38> : distill_step_kernel<T, false, 38>;
     return nullptr;
 }
 
@@ -581,7 +581,7 @@ int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
     if (parts == (kDistillForward | kDistillBackward)) {
         if (const auto f = distill_step<T>(rows, k.V, a->tail == VWS_TAIL_BUCKET)) {
             const int cus = device_info().cus;
-            const unsigned lds = a->tail == VWS_TAIL_BUCKET ? (unsigned)((k.V + 31) / 32) * 4u : 0u;
+            const unsigned lds = 2u * (unsigned)((k.V + 31) / 32) * 4u;  // two bitmaps
             launch_lds(K, f, dim3(rows < cus ? rows : cus), dim3(kDsStepThreads), lds, s, k);
             return check_launch("vws_distill (step)");
         }

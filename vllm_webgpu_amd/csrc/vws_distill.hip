@@ -130,22 +130,24 @@ __device__ __forceinline__ void ds_add1(DsSum& t, float z) {
     t.merge(z, z == z && z < kDsInf ? (z == -kDsInf ? 0.0f : 1.0f) : __builtin_nanf(""));
 }
 
-// The bits of a part's elements that are teacher entries, from its first element on.
-__device__ __forceinline__ void ds_bitmap(uint32_t* bm, int len, const int32_t* ids, int K, int lo, int threads) {
-    for (int i = threadIdx.x; i < (len + 31) / 32; i += threads) bm[i] = 0u;
-    __syncthreads();
-    for (int k = threadIdx.x; k < K; k += threads) {
-        const int d = ids[k] - lo;
-        if (ids[k] >= 0 && d >= 0 && d < len) atomicOr(&bm[d >> 5], 1u << (d & 31));
-    }
-    __syncthreads();
+// Bitmap of a part's elements that are teacher entries, from its first element on.
+__device__ __forceinline__ void ds_clear_bits(uint32_t* bm, int len) {
+    for (int i = threadIdx.x; i < (len + 31) / 32; i += blockDim.x) bm[i] = 0u;
+}
+__device__ __forceinline__ void ds_set_bit(uint32_t* bm, int len, int d) {
+    if (d >= 0 && d < len) atomicOr(&bm[d >> 5], 1u << (d & 31));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t ds_bits(const uint32_t* bm, int vi) {
+    constexpr int VEC = Elem<T>::kVec;
+    return (bm[(vi * VEC) >> 5] >> ((vi * VEC) & 31)) & ((1u << VEC) - 1u);
 }
 
 // Sets the elements of vector vi whose bit is set to -inf.
 template <typename T>
 __device__ __forceinline__ void ds_drop(const uint32_t* bm, int vi, uint32_t (&w)[4]) {
     constexpr int VEC = Elem<T>::kVec;
-    const uint32_t b = (bm[(vi * VEC) >> 5] >> ((vi * VEC) & 31)) & ((1u << VEC) - 1u);
+    const uint32_t b = ds_bits<T>(bm, vi);
     if (b) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
@@ -191,123 +193,136 @@ __device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const
     return t;
 }
 
-// Sums and maxima over the first four waves of a workgroup (the teacher's entries), returned to
-// every thread.  `red`: 16 floats of LDS.  All threads call.
-struct DsBlock {
-    float* red;
-    template <typename F>
-    __device__ __forceinline__ float reduce(float v, float none, F op) {
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if (wave < 4 && (threadIdx.x & 63) == 0) red[wave] = v;
-        __syncthreads();
-        float t = none;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t = op(t, red[i]);
-        return t;
+// A row's teacher entry k, one for each of a workgroup's first K threads (id -1: none).
+struct DsEntry {
+    int id;
+    float l, x;  // its log-probability, the student's logit
+};
+__device__ __forceinline__ DsEntry ds_entry(const DistillArgs& a, int r) {
+    const int k = threadIdx.x;
+    DsEntry e{-1, -kDsInf, 0.0f};
+    if (k < a.K) {
+        e.id = a.ids[(size_t)r * a.ids_stride + k];
+        e.l = a.lp[(size_t)r * a.lp_stride + k];
+        if (e.id < 0 || e.id >= a.V) e.id = -1;
     }
-    __device__ __forceinline__ float max(float v) {
-        return reduce(ds_wave_max(v), -kDsInf, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    return e;
+}
+
+// The entries' ids, hashed: at most 256 of 512 places are taken.
+struct DsHash {
+    int32_t id[2 * kDsMaxK];
+    uint32_t first[2 * kDsMaxK], count[2 * kDsMaxK];  // its first entry, its entries
+    float value[2 * kDsMaxK];                         // its gradient (step)
+    __device__ __forceinline__ void clear() {
+        for (int i = threadIdx.x; i < 2 * kDsMaxK; i += blockDim.x) {
+            id[i] = -1;
+            first[i] = ~0u;
+            count[i] = 0u;
+        }
     }
-    __device__ __forceinline__ float sum(float v) {
-        return reduce(ds_wave_sum(v), 0.0f, [](float a, float b) { return a + b; });
+    __device__ __forceinline__ int insert(int t) {
+        int slot = (int)(((uint32_t)t * 2654435761u) >> 23);
+        for (;;) {
+            const int had = atomicCAS(&id[slot], -1, t);
+            if (had == -1 || had == t) break;
+            slot = (slot + 1) & (2 * kDsMaxK - 1);
+        }
+        atomicMin(&first[slot], threadIdx.x);
+        atomicAdd(&count[slot], 1u);
+        return slot;
     }
+    __device__ __forceinline__ float of(int t) const {  // (t has been inserted)
+        int slot = (int)(((uint32_t)t * 2654435761u) >> 23);
+        while (id[slot] != t) slot = (slot + 1) & (2 * kDsMaxK - 1);
+        return value[slot];
+    }
+};
+
+struct DsShared {
+    float wm[kDsStepThreads / 64], ws[kDsStepThreads / 64];  // the waves' sums
+    float top[kDsMaxK / 64], sums[kDsMaxK / 64][5];          // the entries' maxima and sums, of four waves
+    float p[kDsMaxK];
+    int32_t id[kDsMaxK];
 };
 
 struct DsRow {
     float ref, coef, max, inv_total;  // DistillStat
     bool live;
-    float x, p;                       // this thread's entry: its logit, its P (-1: none)
+    float p;                          // P of this thread's entry (-1: none)
 };
 
-// A row's loss and statistics from the running sum of its rest (BUCKET) or of all of it.  Called by
-// every thread of a workgroup of at least 256; thread k < K has entry k.
-struct DsShared {
-    float red[16];
-    float lpr[kDsMaxK];
-    int32_t lid[kDsMaxK];
-    // the entries' ids, hashed: an id, its first entry, its entries
-    int32_t hid[2 * kDsMaxK];
-    uint32_t hfirst[2 * kDsMaxK], hcount[2 * kDsMaxK];
-};
-
-template <typename T, bool BUCKET>
-__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T* row, DsSum rest, float w, DsShared& sh) {
-    const int k = threadIdx.x, K = a.K;
-    DsBlock blk{sh.red};
-    for (int i = k; i < 2 * kDsMaxK; i += blockDim.x) {
-        sh.hid[i] = -1;
-        sh.hfirst[i] = ~0u;
-        sh.hcount[i] = 0u;
+// A row's loss and statistics, from each wave's merged sum over its rest (BUCKET) or all of it.  Every
+// thread of a workgroup of NW waves calls; `slot`: where this thread's entry was inserted, since
+// the last barrier or before.  Two barriers.
+template <typename T, bool BUCKET, int NW>
+__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, DsSum t, float w, DsEntry e, int slot,
+                                           const DsHash& hash, DsShared& sh) {
+    constexpr int EW = kDsMaxK / 64;
+    const int k = threadIdx.x, K = a.K, wave = k >> 6;
+    const bool valid = e.id >= 0, lead = (k & 63) == 0;
+    // first the maxima: of the student over its entries, or of the teacher
+    const float z = e.x * a.c, logp = BUCKET ? e.l : e.l * a.inv_T;
+    // (a NaN makes the row NaN by way of the sums)
+    const float mine = valid ? (BUCKET ? z : (logp != logp ? kDsInf : logp)) : -kDsInf;
+    if (lead) { sh.wm[wave] = t.m; sh.ws[wave] = t.s; }
+    if (wave < EW) {
+        const float m = ds_wave_max(mine);
+        if (lead) sh.top[wave] = m;
     }
-    int id = -1;
-    float l = -kDsInf, x = 0.0f;
-    if (k < K) {
-        id = a.ids[(size_t)r * a.ids_stride + k];
-        if (id < 0 || id >= a.V) id = -1;
-        if (id >= 0) {
-            l = a.lp[(size_t)r * a.lp_stride + k];
-            x = Elem<T>::load1(row + id);
-        }
-        sh.lid[k] = id;
-    }
-    const bool valid = id >= 0;
-    // the teacher's probabilities (the reductions' barriers order the table's clearing before its use)
-    float p, logp;
-    bool live;
-    if (BUCKET) {
-        logp = l;
-        p = valid ? expf(l) : 0.0f;
-        live = blk.max(valid ? 1.0f : 0.0f) > 0.0f;
-    } else {
-        logp = valid ? l * a.inv_T : -kDsInf;
-        const float top = blk.max(valid && logp != logp ? kDsInf : logp);  // (a NaN makes the row NaN)
-        live = top > -kDsInf;
-        const float e = valid && live ? expf(logp - top) : 0.0f;
-        const float tot = blk.sum(e);
-        p = e / tot;
-        logp = logp - top - logf(tot);
-    }
+    if (k < K) sh.id[k] = e.id;
+    __syncthreads();
+    DsSum rest;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) rest.m = __builtin_fmaxf(rest.m, sh.wm[i]);
+    const float ref = rest.m == -kDsInf ? 0.0f : rest.m;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) rest.s += sh.ws[i] * ds_exp2(sh.wm[i] - ref);
+    float top = -kDsInf;
+#pragma unroll
+    for (int i = 0; i < EW; ++i) top = __builtin_fmaxf(top, sh.top[i]);
+    const float M = BUCKET ? __builtin_fmaxf(rest.m, top) : rest.m, mref = M == -kDsInf ? 0.0f : M;
     // entries that share an id: the first takes their probability together
-    if (k < K) sh.lpr[k] = p;
-    int slot = 0;
-    if (valid) {  // (at most 256 of 512 places are taken)
-        slot = (int)(((uint32_t)id * 2654435761u) >> 23);
-        for (;;) {
-            const int had = atomicCAS(&sh.hid[slot], -1, id);
-            if (had == -1 || had == id) break;
-            slot = (slot + 1) & (2 * kDsMaxK - 1);
+    const bool first = valid && hash.first[slot] == (uint32_t)k, several = first && hash.count[slot] > 1u;
+    // then the sums: p, p log p, p log2 q + log2(total), the student's at the entries, the entries
+    float p = 0.0f;
+    if (valid) p = BUCKET ? expf(logp) : (top > -kDsInf ? expf(logp - top) : 0.0f);
+    const float rel = __builtin_fmaf(e.x, a.c, -mref);
+    const bool on = valid && !(p <= 0.0f);
+    float v[5] = {p, on ? p * (BUCKET ? logp : logp - top) : 0.0f, on ? p * rel : 0.0f,
+                  BUCKET && first ? ds_exp2(rel) : 0.0f, valid ? 1.0f : 0.0f};
+    if (k < K) sh.p[k] = p;
+    if (wave < EW) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            v[i] = ds_wave_sum(v[i]);
+            if (lead) sh.sums[wave][i] = v[i];
         }
-        atomicMin(&sh.hfirst[slot], (uint32_t)k);
-        atomicAdd(&sh.hcount[slot], 1u);
     }
     __syncthreads();
-    const bool first = valid && sh.hfirst[slot] == (uint32_t)k;
-    float P = p;
-    if (first && sh.hcount[slot] > 1u) {
-        P = 0.0f;
-        for (int j = 0; j < K; ++j)
-            if (sh.lid[j] == id) P += sh.lpr[j];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        v[i] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < EW; ++q) v[i] += sh.sums[q][i];
     }
-    // the student's total
-    float M = rest.m, Z = rest.s;
-    if (BUCKET) {
-        M = __builtin_fmaxf(M, blk.max(first ? x * a.c : -kDsInf));
-        const float mref = M == -kDsInf ? 0.0f : M;
-        const float zk = blk.sum(first ? ds_exp2(__builtin_fmaf(x, a.c, -mref)) : 0.0f);
-        Z = (rest.s != 0.0f ? rest.s * ds_exp2(rest.m - mref) : 0.0f) + zk;
+    if (several) {
+        p = 0.0f;
+        for (int i = 0; i < K; ++i)
+            if (sh.id[i] == e.id) p += sh.p[i];
     }
-    const float mref = M == -kDsInf ? 0.0f : M;
-    const float lz = log2f(Z);  // (-inf when no logit is finite: every log q is then -inf)
-    const float logq = Z > 0.0f || Z != Z ? (__builtin_fmaf(x, a.c, -mref) - lz) * kLn2 : -kDsInf;
-    float L = blk.sum(valid && !(p <= 0.0f) ? p * (logp - logq) : 0.0f);
     DsRow o;
     o.max = mref;
-    o.inv_total = Z > 0.0f || Z != Z ? 1.0f / Z : 0.0f;
-    o.ref = rest.m == -kDsInf ? 0.0f : rest.m;
+    o.ref = ref;
+    const float Z = BUCKET ? (rest.s != 0.0f ? rest.s * ds_exp2(ref - mref) : 0.0f) + v[3] : rest.s;
+    const bool some = Z > 0.0f || Z != Z;  // (no finite logit: every log q is -inf)
+    const float lz = some ? log2f(Z) : 0.0f;
+    o.inv_total = some ? 1.0f / Z : 0.0f;
+    float L;
     if (BUCKET) {
-        const float sp = blk.sum(p);
-        const float rr = 1.0f - sp;
+        o.live = v[4] > 0.0f;
+        const float sp = v[0], rr = 1.0f - sp;
+        L = v[1] - (v[2] - lz * sp) * kLn2;
         // a rest without a finite logit is no event
         const bool have = rest.s > 0.0f || rest.s != rest.s;
         const float rem = have && !(rr < 0.0f) ? rr : 0.0f;
@@ -315,15 +330,17 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const T*
         // the teacher's events add up to tot, 1 but where the rest is no event or sp exceeds 1:
         // an entry's gradient is tot q - p, the rest's tot q - rem q / s
         const float tot = sp + rem;
-        o.coef = have ? (tot * (rest.s * ds_exp2(rest.m - mref) * o.inv_total) - rem) / rest.s : 0.0f;
+        o.coef = have ? (tot * (rest.s * ds_exp2(ref - mref) * o.inv_total) - rem) / rest.s : 0.0f;
         o.inv_total *= tot;
     } else {
+        o.live = top > -kDsInf;
+        const float inv = 1.0f / v[0];
+        L = (v[1] - v[2] * kLn2) * inv - logf(v[0]) + lz * kLn2;
         o.coef = o.inv_total;
+        p *= inv;
     }
-    o.live = live;
-    o.x = x;
-    o.p = first ? P : -1.0f;
-    if (threadIdx.x == 0) a.loss[r] = live ? w * L : 0.0f;
+    o.p = first ? p : -1.0f;
+    if (k == 0) a.loss[r] = o.live ? w * L : 0.0f;
     return o;
 }
 
@@ -345,48 +362,60 @@ template <typename T, bool BUCKET>
 __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs a) {
     extern __shared__ uint32_t bm[];
     __shared__ DsShared sh;
-    __shared__ float wm[kDsThreads / 64], ws[kDsThreads / 64];
+    __shared__ DsHash hash;
     __shared__ uint32_t last;
-    const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, wave = tid >> 6;
+    constexpr int NW = kDsThreads / 64;
+    const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x;
     const float w = a.weight ? a.weight[r] : 1.0f;
     if (w == 0.0f) {  // the row does not count: not read
-        if (p == 0) {
-            if (tid == 0) a.loss[r] = 0.0f;
-            if (tid == 0) a.stats[(size_t)r * kDsRowStats + kDsLive] = 0.0f;
+        if (p == 0 && tid == 0) {
+            a.loss[r] = 0.0f;
+            a.stats[(size_t)r * kDsRowStats + kDsLive] = 0.0f;
         }
         return;
     }
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo;
+    DsEntry e = ds_entry(a, r);
     DsSum t = ds_stream<T, BUCKET>(row + lo, len, a.c, bm, [&] {
-        if (BUCKET) ds_bitmap(bm, len, a.ids + (size_t)r * a.ids_stride, a.K, lo, kDsThreads);
+        hash.clear();
+        if (BUCKET) {
+            ds_clear_bits(bm, len);
+            __syncthreads();
+            if (e.id >= 0) ds_set_bit(bm, len, e.id - lo);
+        }
+        __syncthreads();
     });
     t.wave_merge();
-    if ((tid & 63) == 0) { wm[wave] = t.m; ws[wave] = t.s; }
-    __syncthreads();
-    t = DsSum();
-#pragma unroll
-    for (int i = 0; i < kDsThreads / 64; ++i) t.merge(wm[i], ws[i]);
     if (S > 1) {
         // the part that arrives last joins them, in their order
+        if ((tid & 63) == 0) { sh.wm[tid >> 6] = t.m; sh.ws[tid >> 6] = t.s; }
+        __syncthreads();
         if (tid == 0) {
-            ag_store64(&a.rec[(size_t)r * S + p], ((uint64_t)f2u(t.m) << 32) | f2u(t.s));
+            DsSum s;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) s.merge(sh.wm[i], sh.ws[i]);
+            ag_store64(&a.rec[(size_t)r * S + p], ((uint64_t)f2u(s.m) << 32) | f2u(s.s));
             stores_complete();
             last = ag_add32(&a.ctr[r], 1u) == (uint32_t)S - 1u ? 1u : 0u;
         }
         __syncthreads();
         if (!last) return;
         if (tid == 0) ag_store32(&a.ctr[r], 0u);
-        const int lane = tid & 63;
         t = DsSum();
-        if (lane < S) {
-            const uint64_t v = ag_load64(&a.rec[(size_t)r * S + lane]);
+        if (tid < S) {  // (S <= 64: the first wave holds them)
+            const uint64_t v = ag_load64(&a.rec[(size_t)r * S + tid]);
             t.m = u2f((uint32_t)(v >> 32));
             t.s = u2f((uint32_t)v);
         }
         t.wave_merge();
     }
-    const DsRow o = ds_finish<T, BUCKET>(a, r, row, t, w, sh);
+    int slot = 0;
+    if (e.id >= 0) {
+        slot = hash.insert(e.id);
+        e.x = Elem<T>::load1(row + e.id);
+    }
+    const DsRow o = ds_finish<T, BUCKET, NW>(a, r, t, w, e, slot, hash, sh);
     ds_save(a, r, o);
 }
 
@@ -450,15 +479,16 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
 
 // Loss and gradient of rows that one workgroup holds in its registers (NV vectors a thread): every
 // logit is read once and its gradient written once.  One workgroup for each compute unit, a row at a
-// time; as a row's gradients are written, the next row's logits are loaded into the registers they
-// leave.
+// time; as a row's gradients are written, the next row's logits and entries are loaded into the
+// registers they leave.  No barrier waits for memory: a vector that holds teacher entries (by the
+// bitmap) takes their gradients from the hash, so nothing is written twice.
 template <typename T, bool BUCKET, int NV>
 __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArgs a) {
-    constexpr int VEC = Elem<T>::kVec, U = 2, W = kDsStepThreads / 64;
-    extern __shared__ uint32_t bm[];
+    constexpr int VEC = Elem<T>::kVec, U = 2, NW = kDsStepThreads / 64;
+    extern __shared__ uint32_t bms[];  // two bitmaps: this row's and the next one's
     __shared__ DsShared sh;
-    __shared__ float wm[W], ws[W];
-    const int tid = threadIdx.x, wave = tid >> 6, V = a.V, nvec = V / VEC, edge = nvec * VEC + tid;
+    __shared__ DsHash hashes[2];
+    const int tid = threadIdx.x, V = a.V, nvec = V / VEC, edge = nvec * VEC + tid, words = (V + 31) / 32;
     const T* x = static_cast<const T*>(a.x);
     T* grad = static_cast<T*>(a.grad);
     auto live = [&](int r) { return !a.weight || a.weight[r] != 0.0f; };
@@ -487,14 +517,26 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
     };
     skip();
     if (r >= a.N) return;
+    DsEntry e = ds_entry(a, r);
 #pragma unroll
     for (int q = 0; q < NV; ++q) fetch(x + (size_t)r * a.xstride, q, nvec - 1);
     if (edge < V) xe = Elem<T>::load1(x + (size_t)r * a.xstride + edge);
-    for (;;) {
+    if (e.id >= 0) e.x = Elem<T>::load1(x + (size_t)r * a.xstride + e.id);
+    hashes[0].clear();
+    ds_clear_bits(bms, V);
+    __syncthreads();
+    for (int parity = 0;; parity ^= 1) {
         const T* row = x + (size_t)r * a.xstride;
         T* out = grad + (size_t)r * a.gstride;
         const float wt = a.weight ? a.weight[r] : 1.0f;
-        if (BUCKET) ds_bitmap(bm, V, a.ids + (size_t)r * a.ids_stride, a.K, 0, kDsStepThreads);
+        DsHash& hash = hashes[parity];
+        uint32_t* bm = bms + parity * words;
+        int slot = 0;
+        if (e.id >= 0) {
+            slot = hash.insert(e.id);
+            ds_set_bit(bm, V, e.id);
+        }
+        __syncthreads();
         DsSum t;
 #pragma unroll
         for (int q0 = 0; q0 < NV; q0 += U) {
@@ -514,25 +556,27 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
             ds_add<T, U>(t, g, a.c);
             fence();
         }
-        const bool drop = BUCKET && edge < V && ((bm[edge >> 5] >> (edge & 31)) & 1u);
-        if (edge < V && !drop) ds_add1(t, xe * a.c);
+        const bool edge_entry = edge < V && ((bm[edge >> 5] >> (edge & 31)) & 1u);
+        if (edge < V && !(BUCKET && edge_entry)) ds_add1(t, xe * a.c);
         t.wave_merge();
-        if ((tid & 63) == 0) { wm[wave] = t.m; ws[wave] = t.s; }
-        __syncthreads();
-        t = DsSum();
-#pragma unroll
-        for (int i = 0; i < W; ++i) t.merge(wm[i], ws[i]);
-        const DsRow o = ds_finish<T, BUCKET>(a, r, row, t, wt, sh);
+        const DsRow o = ds_finish<T, BUCKET, NW>(a, r, t, wt, e, slot, hash, sh);
         const float gs = wt * (a.gout ? a.gout[r] : 1.0f) * a.inv_T;
         const bool on = o.live && gs != 0.0f;
         const float ref = o.ref, coef = o.coef * gs;
-        const int id = tid < a.K && !(o.p < 0.0f) ? sh.lid[tid] : -1;
-        const float fix = gs * (ds_exp2(__builtin_fmaf(o.x, a.c, -o.max)) * o.inv_total - o.p);
+        if (!(o.p < 0.0f)) {  // (the first of its id)
+            const float q = ds_exp2(__builtin_fmaf(e.x, a.c, -o.max)) * o.inv_total;
+            hash.value[slot] = on ? gs * (q - o.p) : 0.0f;
+        }
         r += gridDim.x;
         skip();
         const bool more = r < a.N;
         const T* after = more ? x + (size_t)r * a.xstride : row;
         const int end = more ? nvec - 1 : 0;
+        e = more ? ds_entry(a, r) : DsEntry{-1, 0.0f, 0.0f};
+        hashes[parity ^ 1].clear();
+        ds_clear_bits(bms + (parity ^ 1) * words, V);
+        __syncthreads();
+        auto value = [&](float v) { return on ? ds_exp2(__builtin_fmaf(v, a.c, -ref)) * coef : 0.0f; };
 #pragma unroll
         for (int q = 0; q < NV; ++q) {
             const int vi = fresh(tid) + q * kDsStepThreads;
@@ -541,20 +585,24 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
             for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(w[q][k]));
             Elem<T>::from_words(w[q][0], w[q][1], w[q][2], w[q][3], v);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = on ? ds_exp2(__builtin_fmaf(v[j], a.c, -ref)) * coef : 0.0f;
+            for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
+            const uint32_t bits = ds_bits<T>(bm, min(vi, nvec - 1));
+            if (bits) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if ((bits >> j) & 1u) v[j] = hash.of(min(vi, nvec - 1) * VEC + j);
+            }
             uint32_t g[4];
             DsVec<T>::pack(v, g);
             if (vi < nvec) ds_store<T>(out + (size_t)q * kDsStepThreads * VEC, fresh(tid), g);
             fetch(after, q, end);
             fence();
         }
-        if (edge < V) out[edge] = DsVec<T>::narrow(on ? ds_exp2(__builtin_fmaf(xe, a.c, -ref)) * coef : 0.0f);
+        if (edge < V) out[edge] = DsVec<T>::narrow(edge_entry ? hash.of(edge) : value(xe));
         if (more && edge < V) xe = Elem<T>::load1(after + edge);
-        // the teacher's entries over what was written there, once that has arrived
-        stores_complete();
-        __syncthreads();
-        if (on && id >= 0) out[id] = DsVec<T>::narrow(fix);
+        if (e.id >= 0) e.x = Elem<T>::load1(after + e.id);
         if (!more) return;
+        __syncthreads();
     }
 }
 
@@ -564,7 +612,7 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
 #define VWS_DISTILL_INST(T)                                                   \
     VWS_DISTILL_STEP(T, 16)                                                   \
     VWS_DISTILL_STEP(T, 32)                                                   \
-    VWS_DISTILL_STEP(T, 40)                                                   \
+    VWS_DISTILL_STEP(T, 38)                                                   \
     template __global__ void distill_forward_kernel<T, false>(DistillArgs);   \
     template __global__ void distill_forward_kernel<T, true>(DistillArgs);    \
     template __global__ void distill_backward_kernel<T>(DistillArgs);
