@@ -976,6 +976,7 @@ int vws_verify_drafts(const vws_verify_args* a) {
     k.rec = reinterpret_cast<VfRec*>(base + w.rec);
     k.gmax = reinterpret_cast<float*>(base + w.gmax);
     k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
+    k.kept = reinterpret_cast<int32_t*>(base + w.kept);
     k.best = reinterpret_cast<uint64_t*>(base + w.best);
     k.ctr = reinterpret_cast<uint32_t*>(base + w.ctr);
     hipStream_t s = (hipStream_t)a->stream;

@@ -52,6 +52,7 @@ struct VerifyArgs {
     float* gmax;                 // [R, groups] maxima of groups of vectors, of rows that are cut; or null
     int groups;                  // of a row
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
+    int32_t* kept;               // [R, 1 + kVfKept] of cut rows: how many are kept (-1: not listed), and they
     uint64_t* best;              // [B, S2] race: key bits << 32 | 0x7FFFFFFF - index
     uint32_t* ctr;               // [B] race parts arrived; cleared by the statistics' launch
 };
@@ -64,8 +65,10 @@ inline int vf_groups(int S, int part_len, int vec) {
     return S * ((part_len + per - 1) / per) * kVfThreads;
 }
 
+constexpr int kVfKept = 511;         // tokens of a cut row that the race takes from a list
+
 struct VfLayout {
-    size_t rec, gmax, cut, best, ctr, total;
+    size_t rec, gmax, cut, kept, best, ctr, total;
 };
 
 inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
@@ -74,6 +77,7 @@ inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
     w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
     w.gmax = off;  off = align256(off + sizeof(float) * (size_t)R * groups);
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
+    w.kept = off;  off = align256(off + sizeof(int32_t) * (size_t)R * (1 + kVfKept));
     w.best = off;  off = align256(off + sizeof(uint64_t) * (size_t)B * S2);
     w.ctr = off;   off = align256(off + sizeof(uint32_t) * (size_t)B);
     w.total = off;

@@ -776,6 +776,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
         const float tiny = Tt * 0x1p-120f;
         auto below = [tiny](float x) { return x - __builtin_fabsf(x) * 0x1p-20f - tiny; };
         bool done = false;
+        bool listed = false;  // the list holds everything kept
         if (u.q32 >= 1.0f) {
             // only the last of (key, index)
             const uint32_t mk = key_of(u.m);
@@ -797,7 +798,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             if (k_listed && vf_gather<T>(a, gmax, row, Tt, sh, t)) {
                 const int n = (int)sh.count;
                 o = n <= kVfSmall ? vf_solve_small(sh, u, n) : vf_solve(VfListIter{sh.list, n}, sh, u, (uint64_t)n);
-                done = true;
+                done = listed = true;
             }
         } else {
             // top-p alone.  The first pass's sum is off by at most 2^-22 (2 |m| + 64) of itself: y and
@@ -810,7 +811,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             for (int n = 84; !done && n <= 192 && held > 0.5; n += 108) {
                 const float t = below(vf_peak(sh, n));
                 if (!(t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)) break;
-                done = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
+                done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
             }
             if (!done) {
                 // every mass, by distance from the maximum; what lies further than `far` holds less
@@ -853,6 +854,19 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             n = vf_block_sum(n, sh);
             o = vf_solve(VfRowIter<T>{row, V, Tt}, sh, u, n);
         }
+        // the kept tokens for the race, where the list holds them and they are few
+        int32_t* kept = a.kept + (size_t)r * (1 + kVfKept);
+        const int n = listed ? (int)sh.count : 0;
+        __syncthreads();
+        if (threadIdx.x == 0) sh.ngroups = 0u;
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += kVfCutThreads)
+            if (sh.list[j] >= o.cut) {
+                const uint32_t at = agg_reserve(&sh.ngroups);
+                if (at < (uint32_t)kVfKept) kept[1 + at] = (int32_t)(uint32_t)sh.list[j];
+            }
+        __syncthreads();
+        if (threadIdx.x == 0) kept[0] = listed && sh.ngroups <= (uint32_t)kVfKept ? (int32_t)sh.ngroups : -1;
     }
     __syncthreads();  // every wave has read the row's parts
     if (threadIdx.x == 0) {
@@ -969,9 +983,18 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
             const float e = vf_exp2(__builtin_fmaf(x, c, -m2)) * scale;
             return !((q ? e - qi : e) < bound * (1.0f - ui)) || !(ui < 1.0f);  // (true for NaN)
         };
-        const int lo = p * a.part2_len, len = min(a.V, lo + a.part2_len) - lo, nvec = len / VEC;
+        // a cut row whose kept tokens are listed: they alone, by the first part
+        const int32_t* kept = a.kept + (size_t)(first + b + acc) * (1 + kVfKept);
+        const int nkept = prm.cuts ? kept[0] : -1;
+        if (nkept >= 0 && p > 0) return;
+        for (int k = tid; k < nkept; k += kVfThreads) {
+            const int i = kept[1 + k];
+            add(i, Elem<T>::load1(row + i), q ? vf_load_any1(q, a.qdtype, i) : 0.0f,
+                u ? u[i] : philox_uniform(seed, offset, (uint32_t)i));
+        }
+        const int lo = p * a.part2_len, len = nkept >= 0 ? 0 : min(a.V, lo + a.part2_len) - lo, nvec = len / VEC;
         // the most probable token's key first (each thread for itself): a good bound
-        {
+        if (nkept < 0) {
             const int i = vf_index(w.top);
             add(i, x_top, q ? vf_load_any1(q, a.qdtype, i) : 0.0f, u ? u[i] : philox_uniform(seed, offset, (uint32_t)i));
         }
@@ -1033,7 +1056,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
         best = 0ull;
 #pragma unroll
         for (int k = 0; k < kVfThreads / 64; ++k) best = vws_max64(best, red[k]);
-        if (S2 > 1) {
+        if (S2 > 1 && nkept < 0) {
             if (tid == 0) {
                 ag_store64(&a.best[(size_t)b * S2 + p], best);
                 stores_complete();

@@ -525,23 +525,16 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: t
     L = _lib.lib()
     stream = _stream_ptr()
     ws = _workspace(L.vws_verify_workspace_size(B, D, V), dev.index, stream, _capturing(stream))
-    a = _lib.VerifyArgs()
-    a.struct_size = ctypes.sizeof(_lib.VerifyArgs)
-    a.batch, a.vocab, a.dtype = B, V, _dtype_code(logits)
-    a.num_drafts, a.max_drafts = D, K
-    a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
-    a.draft_tokens, a.cu_drafts = drafts.data_ptr() if D else None, cu.data_ptr()
-    if draft_probs is not None and D:
-        a.draft_probs, a.draft_probs_row_stride = draft_probs.data_ptr(), _row_stride(draft_probs)
-        a.draft_probs_dtype = _dtype_code(draft_probs)
-    a.temperature, a.top_k, a.top_p, a.min_p = _ptr(T), _ptr(TK), _ptr(TP), _ptr(MP)
-    a.accept_uniforms, a.uniforms = AU.data_ptr() if AU is not None and D else None, _ptr(U)
-    a.uniforms_row_stride = _row_stride(U) if U is not None else 0
-    a.rng_seeds, a.rng_offsets = _ptr(SEED), _ptr(OFF)
-    if U is None and SEED is None and rng_key is not None:
-        a.rng_key, a.rng_key_set = int(rng_key) & 0xFFFFFFFFFFFFFFFF, 1
-    a.tokens, a.num_accepted, a.logprobs = tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr()
-    a.workspace, a.workspace_bytes, a.stream = ws.data_ptr(), ws.numel(), stream
+    Q = draft_probs if D else None
+    key = U is None and SEED is None and rng_key is not None
+    # (in the block's order: one call in place of an assignment per field)
+    a = _lib.VerifyArgs(
+        ctypes.sizeof(_lib.VerifyArgs), B, V, _dtype_code(logits), D, K, logits.data_ptr(), _row_stride(logits),
+        drafts.data_ptr() if D else None, cu.data_ptr(), _ptr(Q), 0 if Q is None else _row_stride(Q),
+        0 if Q is None else _dtype_code(Q), _ptr(T), _ptr(TK), _ptr(TP), _ptr(MP),
+        AU.data_ptr() if AU is not None and D else None, _ptr(U), 0 if U is None else _row_stride(U), _ptr(SEED), _ptr(OFF),
+        int(rng_key) & 0xFFFFFFFFFFFFFFFF if key else 0, 1 if key else 0, tokens.data_ptr(), accepted.data_ptr(),
+        logprobs.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     _lib.check(L.vws_verify_drafts(ctypes.byref(a)))
     return VerifyResult(tokens, accepted, logprobs)
 
@@ -571,14 +564,9 @@ def _distill_args(logits, teacher_ids, teacher_logprobs, row_weight, temperature
         teacher_logprobs = teacher_logprobs.float()
     logits, ids, lp = _rows(logits), _rows(teacher_ids), _rows(teacher_logprobs)
     W = _row_param(row_weight, N, torch.float32, dev, "row_weight")
-    a = _lib.DistillArgs()
-    a.struct_size = ctypes.sizeof(_lib.DistillArgs)
-    a.rows, a.vocab, a.dtype, a.teacher_k, a.tail = N, V, _dtype_code(logits), K, _TAILS[tail]
-    a.temperature = float(temperature)
-    a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
-    a.teacher_ids, a.teacher_ids_row_stride = ids.data_ptr(), _row_stride(ids)
-    a.teacher_logprobs, a.teacher_logprobs_row_stride = lp.data_ptr(), _row_stride(lp)
-    a.row_weight = _ptr(W)
+    a = _lib.DistillArgs(
+        ctypes.sizeof(_lib.DistillArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), K, _TAILS[tail],
+        float(temperature), ids.data_ptr(), _row_stride(ids), lp.data_ptr(), _row_stride(lp), _ptr(W))
     return a, (logits, ids, lp, W)
 
 
