@@ -431,16 +431,21 @@ void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* 
     *S = (V + *len - 1) / *len;
 }
 
-// Workgroups a launch is split into: eight of 256 threads for each of the chip's 256 compute units,
-// which is what they hold at once.
-constexpr int kSplitWgs = 2048;
+constexpr int kRowsWgs = 768;
+constexpr int kRaceWgs = 1024;
+constexpr int kRaceCutWgs = 2048;
+constexpr int kDistillWgs = 768;
+constexpr int kGradWgs = 16384;
 
-void verify_parts(int rows, int V, int* S, int* len) { split_row(rows, V, kSplitWgs, 4096, kVfMaxParts, 1, S, len); }
+void verify_parts(int rows, int V, int* S, int* len) { split_row(rows, V, kRowsWgs, 4096, kVfMaxParts, 1, S, len); }
+void race_parts(int rows, int V, bool cuts, int* S, int* len) {
+    split_row(rows, V, cuts ? kRaceCutWgs : kRaceWgs, 4096, kVfMaxParts, 1, S, len);
+}
 
 // A launch takes at most kTopkRows rows (the counters of the fixed region); a part's bitmap of
 // teacher entries takes at most 32 KB.
 void distill_parts(int rows, int V, int* S, int* len) {
-    split_row(rows, V, kSplitWgs, 4096, kDsMaxParts, (V + (1 << 18) - 1) >> 18, S, len);
+    split_row(rows, V, kDistillWgs, 4096, kDsMaxParts, (V + (1 << 18) - 1) >> 18, S, len);
 }
 
 bool dtype_ok(int32_t d) { return d == VWS_DTYPE_F32 || d == VWS_DTYPE_BF16 || d == VWS_DTYPE_F16; }
@@ -586,9 +591,10 @@ int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
             return check_launch("vws_distill (step)");
         }
     }
-    distill_parts(rows, k.V, &k.S, &k.part_len);
-    const dim3 grid((unsigned)rows * (unsigned)k.S), block(kDsThreads);
+    const dim3 block(kDsThreads);
     if (parts & kDistillForward) {
+        distill_parts(rows, k.V, &k.S, &k.part_len);
+        const dim3 grid((unsigned)rows * (unsigned)k.S);
         k.ctr = static_cast<CoopState*>(a->workspace)->topk_ctr;
         k.rec = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + align256(sizeof(CoopState)));
         if (a->tail == VWS_TAIL_BUCKET) {
@@ -600,7 +606,8 @@ int distill_rows(const vws_distill_args* a, int parts, int r0, int rows) {
         if (int st = check_launch("vws_distill (forward)")) return st;
     }
     if (parts & kDistillBackward) {
-        launch(K, distill_backward_kernel<T>, grid, block, s, k);
+        split_row(rows, k.V, kGradWgs, 4096, 1 << 10, 1, &k.S, &k.part_len);
+        launch(K, distill_backward_kernel<T>, dim3((unsigned)rows * (unsigned)k.S), block, s, k);
         if (int st = check_launch("vws_distill (backward)")) return st;
     }
     return VWS_OK;
@@ -933,7 +940,7 @@ size_t vws_verify_workspace_size(int32_t batch, int32_t num_drafts, int32_t voca
         return 0;
     int S, S2, len, len2;
     verify_parts(batch + num_drafts, vocab, &S, &len);
-    verify_parts(batch, vocab, &S2, &len2);
+    race_parts(batch, vocab, true, &S2, &len2);
     // (vectors of 4: the most groups)
     return vf_layout(batch + num_drafts, batch, S, S2, vf_groups(S, len, 4)).total;
 }
@@ -967,9 +974,9 @@ int vws_verify_drafts(const vws_verify_args* a) {
     k.tokens = a->tokens;
     k.accepted = a->num_accepted;
     k.logprobs = a->logprobs;
-    verify_parts(k.R, k.V, &k.S, &k.part_len);
-    verify_parts(k.B, k.V, &k.S2, &k.part2_len);
     const bool cuts = a->temperature && (a->top_k || a->top_p || a->min_p);
+    verify_parts(k.R, k.V, &k.S, &k.part_len);
+    race_parts(k.B, k.V, cuts, &k.S2, &k.part2_len);
     k.groups = vf_groups(k.S, k.part_len, a->dtype == VWS_DTYPE_F32 ? 4 : 8);
     const VfLayout w = vf_layout(k.R, k.B, k.S, k.S2, k.groups);
     char* base = static_cast<char*>(a->workspace);
