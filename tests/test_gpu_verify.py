@@ -390,3 +390,12 @@ def test_refusals(cuda):
         big = torch.zeros((5, (1 << 19) + 8), device=cuda)
         ops.verify_drafts(big, t["draft_tokens"], t["cu_drafts"], 2)
     assert e.value.status == _lib.ERR_LIMIT
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("requests", [1, 12, 70])
+def test_flat_rows(cuda, dtype, requests):
+    """Rows whose nucleus is most of the vocabulary, few and more than the launch sets aside."""
+    t = make(cuda, [2] * requests, 9001 if requests > 12 else 33001, dtype, "f32", seed=requests, spread=0.5, spikes=1)
+    check(t, 2, T=1.3, p=0.9, max_near=0.5)
+    check(t, 2, T=0.9, p=0.5, max_near=0.5)

@@ -35,6 +35,7 @@ __global__ void token_state_kernel(uint32_t*, int64_t, uint32_t*, int64_t, int, 
                                    const int32_t*, int);
 template <typename T> __global__ void verify_rows_kernel(VerifyArgs);
 template <typename T> __global__ void verify_cut_kernel(VerifyArgs);
+template <typename T> __global__ void verify_mass_kernel(VerifyArgs);
 template <typename T> __global__ void verify_token_kernel(VerifyArgs);
 template <typename T, bool BUCKET> __global__ void distill_forward_kernel(DistillArgs);
 template <typename T> __global__ void distill_backward_kernel(DistillArgs);
@@ -490,13 +491,17 @@ int validate_verify(const vws_verify_args* a) {
 }
 
 template <typename T>
-int verify_launch(const VerifyArgs& k, bool cuts, hipStream_t s) {
+int verify_launch(const VerifyArgs& k, bool cuts, bool top_p, hipStream_t s) {
     const int K = VWS_KERNEL_VERIFY;
     launch(K, verify_rows_kernel<T>, dim3((unsigned)k.R * (unsigned)k.S), dim3(kVfThreads), s, k);
     if (int st = check_launch("vws_verify_drafts (rows)")) return st;
     if (cuts) {
         launch(K, verify_cut_kernel<T>, dim3((unsigned)k.R), dim3(kVfCutThreads), s, k);
         if (int st = check_launch("vws_verify_drafts (cuts)")) return st;
+        if (top_p) {
+            launch(K, verify_mass_kernel<T>, dim3(kVfMassWgs), dim3(kVfCutThreads), s, k);
+            if (int st = check_launch("vws_verify_drafts (masses)")) return st;
+        }
     }
     launch(K, verify_token_kernel<T>, dim3((unsigned)k.B * (unsigned)k.S2), dim3(kVfThreads), s, k);
     return check_launch("vws_verify_drafts (tokens)");
@@ -984,12 +989,15 @@ int vws_verify_drafts(const vws_verify_args* a) {
     k.gmax = reinterpret_cast<float*>(base + w.gmax);
     k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
     k.kept = reinterpret_cast<int32_t*>(base + w.kept);
+    k.flat_n = reinterpret_cast<uint32_t*>(base + w.flat_n);
+    k.flat = reinterpret_cast<VfFlat*>(base + w.flat);
     k.best = reinterpret_cast<uint64_t*>(base + w.best);
     k.ctr = reinterpret_cast<uint32_t*>(base + w.ctr);
     hipStream_t s = (hipStream_t)a->stream;
-    const int st = a->dtype == VWS_DTYPE_F32    ? verify_launch<float>(k, cuts, s)
-                   : a->dtype == VWS_DTYPE_BF16 ? verify_launch<uint16_t>(k, cuts, s)
-                                                : verify_launch<_Float16>(k, cuts, s);
+    const bool top_p = a->top_p != nullptr;
+    const int st = a->dtype == VWS_DTYPE_F32    ? verify_launch<float>(k, cuts, top_p, s)
+                   : a->dtype == VWS_DTYPE_BF16 ? verify_launch<uint16_t>(k, cuts, top_p, s)
+                                                : verify_launch<_Float16>(k, cuts, top_p, s);
     return st ? st : ok();
 }
 

@@ -24,6 +24,17 @@ struct VfRec {
     float sum;
 };
 
+constexpr int kVfBins = 2048;      // bins of a row's masses
+constexpr int kVfFlat = 128;       // rows of a launch that verify_mass_kernel takes
+constexpr int kVfMassWgs = 512;    // its workgroups: two of 1024 threads for each compute unit
+
+struct VfFlat {
+    int32_t row;
+    uint32_t ctr;                  // parts arrived
+    uint64_t rest;                 // the masses beyond the bins
+    uint64_t hist[kVfBins];
+};
+
 struct VerifyArgs {
     const void* x;               // [R, V] target logits, n_b + 1 rows per request
     int64_t xstride;
@@ -53,6 +64,8 @@ struct VerifyArgs {
     int groups;                  // of a row
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
     int32_t* kept;               // [R, 1 + kVfKept] of cut rows: how many are kept (-1: not listed), and they
+    uint32_t* flat_n;            // rows whose masses verify_mass_kernel adds up; cleared by the statistics' launch
+    VfFlat* flat;                // [kVfFlat]
     uint64_t* best;              // [B, S2] race: key bits << 32 | 0x7FFFFFFF - index
     uint32_t* ctr;               // [B] race parts arrived; cleared by the statistics' launch
 };
@@ -68,7 +81,7 @@ inline int vf_groups(int S, int part_len, int vec) {
 constexpr int kVfKept = 511;         // tokens of a cut row that the race takes from a list
 
 struct VfLayout {
-    size_t rec, gmax, cut, kept, best, ctr, total;
+    size_t rec, gmax, cut, kept, flat_n, flat, best, ctr, total;
 };
 
 inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
@@ -78,6 +91,8 @@ inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
     w.gmax = off;  off = align256(off + sizeof(float) * (size_t)R * groups);
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
     w.kept = off;  off = align256(off + sizeof(int32_t) * (size_t)R * (1 + kVfKept));
+    w.flat_n = off; off = align256(off + sizeof(uint32_t));
+    w.flat = off;  off = align256(off + sizeof(VfFlat) * (size_t)(R < kVfFlat ? R : kVfFlat));
     w.best = off;  off = align256(off + sizeof(uint64_t) * (size_t)B * S2);
     w.ctr = off;   off = align256(off + sizeof(uint32_t) * (size_t)B);
     w.total = off;

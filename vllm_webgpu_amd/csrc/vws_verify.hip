@@ -8,9 +8,10 @@
 // accepted draft from p_n, both by the sampler's exponential race.  The emitted tokens are then
 // distributed as if the target had sampled them one by one.
 //
-// Three kernels: verify_rows_kernel reads every row once, split over workgroups, for its maximum and
-// sum; verify_cut_kernel finds the kept set of the rows that their request cuts; verify_token_kernel
-// decides each request and races one of its rows, split over workgroups.
+// verify_rows_kernel reads every row once, split over workgroups, for its maximum and sum;
+// verify_cut_kernel finds the kept set of the rows that their request cuts, of most from a short list;
+// verify_mass_kernel (launches with a top-p) adds up the masses of the others, each split over
+// workgroups; verify_token_kernel decides each request and races one of its rows.
 #include "vws_device.h"
 #include "vws_sampler.h"
 #include "vws_verify.h"
@@ -152,7 +153,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
         }
     };
     fetch(tid);
-    if (p == 0 && tid == 0 && r < a.B) a.ctr[r] = 0u;  // (R >= B)
+    if (p == 0 && tid == 0) {
+        if (r < a.B) a.ctr[r] = 0u;  // (R >= B)
+        if (r == 0) *a.flat_n = 0u;
+    }
     const VfParams prm = vf_params(a, vf_request(a, r));
     const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
     float* gmax = a.gmax + (size_t)r * a.groups + (size_t)p * (a.groups / S);
@@ -237,9 +241,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 //     within the error of the first pass's sum (a peaked row);
 //   * else the masses of all logits, summed in bins by the distance from the maximum;
 //     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).
+//     verify_mass_kernel does that for the first kVfFlat such rows, all compute units at it
+//     however few the rows, and verify_cut_kernel itself for further ones.
 // A list that overflows (many equal logits) leaves the row to passes over its keys' bits.
 
-constexpr int kVfBins = 2048;
 constexpr int kVfCutWaves = kVfCutThreads / 64;
 constexpr int kVfList = 2048;     // list entries (a row's candidates)
 constexpr int kVfSmall = 512;     // entries that are compared with each other, all pairs
@@ -261,20 +266,20 @@ struct VfCutShared {
 
 __device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
 
-// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element); the
-// next four vectors are on their way while these are used.
+// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element), or for
+// its vectors [v0, v1) and, with `tail`, that element; the next four vectors are on their way while these are used.
 template <typename T, typename F>
-__device__ __forceinline__ void vf_each(const T* row, int V, F f) {
+__device__ __forceinline__ void vf_each(const T* row, int V, F f, int v0 = 0, int v1 = 1 << 30, bool tail = true) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
-    const int nvec = V / VEC, tid = threadIdx.x;
-    if (nvec > 0) {
+    const int tid = threadIdx.x, last = V / VEC, nvec = min(v1, last);
+    if (nvec > v0) {
         uint32_t next[U][4];
         auto fetch = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < U; ++u) vf_load_raw<T>(row, min(b + u * kVfCutThreads, nvec - 1), next[u]);
         };
-        fetch(tid);
-        for (int b = tid; b < nvec; b += U * kVfCutThreads) {
+        fetch(v0 + tid);
+        for (int b = v0 + tid; b < nvec; b += U * kVfCutThreads) {
             uint32_t w[U][4];
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -292,8 +297,8 @@ __device__ __forceinline__ void vf_each(const T* row, int V, F f) {
             }
         }
     }
-    const int i = nvec * VEC + tid;
-    if (i < V) f(i, Elem<T>::load1(row + i));
+    const int i = last * VEC + tid;
+    if (tail && i < V) f(i, Elem<T>::load1(row + i));
 }
 
 // What the selection below runs over: a row's elements, or the list's.  each(f): f(index, key, y).
@@ -749,6 +754,114 @@ __device__ __forceinline__ VfRow vf_join(const VerifyArgs& a, const VfParams& pr
     return o;
 }
 
+// Bins of a row's masses, by distance from the maximum: what lies further than `far` holds less than
+// q W (W is at least the maximum's own mass), so the cut does not lie there.
+struct VfFar {
+    float far, scale;
+    __device__ __forceinline__ VfFar(const VfRule& u, int V) {
+        far = __builtin_fminf(logf((float)V / u.q32) + 0.01f, 31.0f);
+        scale = (float)(kVfBins - 1) / far;
+    }
+    __device__ __forceinline__ int bin(float d) const { return (int)(d * scale); }
+};
+
+// Adds the masses of a row's vectors [v0, v1) to the bins; returns those further away (this thread's).
+//
+// Bound: VALU, so the arithmetic is cut to what a mass needs, to the same bits: y = fl(x / T) from the
+// reciprocal by two exact remainders (correctly rounded: the first makes the quotient faithful;
+// for temperatures whose reciprocal is far from subnormal), exp_det without the cases that
+// d <= 0 excludes, its scaling and the mass's in one ldexp.
+template <typename T>
+__device__ __forceinline__ uint64_t vf_masses(const T* row, int V, float Tt, VfCutShared& sh, const VfRule& u, int v0, int v1,
+                                              bool tail) {
+    const VfFar fr(u, V);
+    const float inv = 1.0f / Tt;
+    const bool quick = Tt < 0x1p60f;
+    uint64_t rest = 0ull;
+    vf_each<T>(row, V, [&](int, float x) {
+        float y;
+        if (quick) {
+            y = x * inv;
+            y = __builtin_fmaf(__builtin_fmaf(-y, Tt, x), inv, y);
+            y = __builtin_fmaf(__builtin_fmaf(-y, Tt, x), inv, y);
+        } else {
+            y = x / Tt;
+        }
+        const float d = y - u.m;  // (NaN where y overflows: no mass, as its exp_det is 0)
+        const float n = __builtin_rintf(d * 0x1.715476p+0f);
+        float e = __builtin_fmaf(-n, 0x1.62e4p-1f, d);
+        e = __builtin_fmaf(-n, 0x1.7f7d1cp-20f, e);
+        float p = __builtin_fmaf(0x1.6d7532p-10f, e, 0x1.120b66p-7f);
+        p = __builtin_fmaf(p, e, 0x1.5554b8p-5f);
+        p = __builtin_fmaf(p, e, 0x1.5554dcp-3f);
+        p = __builtin_fmaf(p, e, 0.5f);
+        p = __builtin_fmaf(p, e, 1.0f);
+        p = __builtin_fmaf(p, e, 1.0f);
+        // 2^44 exp(d), 0 from where a mass is 0 (d < -31: below 2^-44)
+        const float f = d >= -31.0f ? __builtin_ldexpf(p, (int)n + 44) : 0.0f;
+        const float hf = __builtin_truncf(f * 0x1p-32f);
+        const uint64_t q = ((uint64_t)(uint32_t)hf << 32) | (uint32_t)__builtin_fmaf(-hf, 0x1p32f, f);
+        if (-d < fr.far) vf_count(sh, fr.bin(-d), q);
+        else rest += q;
+    }, v0, v1, tail);
+    return rest;
+}
+
+// The kept set of a row from its bins in sh.hist and the masses beyond; false when the cut's bin does
+// not fit the list.
+template <typename T>
+__device__ __forceinline__ bool vf_flat(const T* row, int V, float Tt, VfCutShared& sh, const VfRule& u, uint64_t rest, VfCut* o) {
+    const VfFar fr(u, V);
+    uint64_t in = 0ull;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) in += sh.hist[i];
+    in = vf_block_sum(in, sh);
+    const uint64_t total = in + rest, thr = scale_floor(u.q32, total);
+    if (total - thr > in) return false;
+    // from the maximum down: the cut lies where the running sum reaches total - thr
+    int bin;
+    uint64_t over;
+    vf_find(sh, kVfBins, total - thr - 1ull, &bin, &over);
+    const uint64_t under = total - over - sh.hist[bin];
+    const float yhi = u.m - (float)bin / fr.scale, ylo = u.m - (float)(bin + 1) / fr.scale;
+    const float slack = (__builtin_fabsf(u.m) + 32.0f) * 0x1p-20f;
+    if (!vf_collect<T>(row, V, Tt, sh, Tt * (ylo - slack), Tt * (yhi + slack), [&](float y) {
+            const float d = u.m - y;
+            return d < fr.far && fr.bin(d) == bin;
+        }))
+        return false;
+    *o = vf_solve_bin(sh, u, (int)sh.count, total, under, thr);
+    return true;
+}
+
+__device__ __forceinline__ VfRule vf_rule(const VfParams& prm, const VfRow& w) {
+    VfRule u;
+    u.m = w.m;
+    u.q32 = 1.0f - prm.top_p;
+    u.k = prm.k;
+    u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
+    return u;
+}
+
+// The kept set by passes over the whole row.
+template <typename T>
+__device__ __forceinline__ VfCut vf_solve_row(const T* row, int V, float Tt, VfCutShared& sh, const VfRule& u) {
+    uint64_t n = 0ull;
+    vf_each<T>(row, V, [&](int, float x) { n += x == x ? 1u : 0u; });
+    n = vf_block_sum(n, sh);
+    return vf_solve(VfRowIter<T>{row, V, Tt}, sh, u, n);
+}
+
+// Thread 0: row r's own statistics in place of its parts' (which every wave has read).
+__device__ __forceinline__ void vf_write(const VerifyArgs& a, int r, const VfRow& w, const VfCut& o) {
+    VfRec c;
+    c.top = w.top;
+    c.m2 = w.m;
+    c.sum = (float)o.kept * 0x1p-44f;
+    a.rec[(size_t)r * a.S] = c;
+    a.cut[r] = o.cut;
+}
+
 // One workgroup per row: the kept set of a row that its request cuts, as the smallest
 // (key(y) << 32 | index) kept, and the sum of its exponentials.
 template <typename T>
@@ -761,11 +874,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
     const float Tt = prm.T;
     const int V = a.V;
     const VfRow w = vf_join(a, prm, r);
-    VfRule u;
-    u.m = w.m;
-    u.q32 = 1.0f - prm.top_p;
-    u.k = prm.k;
-    u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
+    const VfRule u = vf_rule(prm, w);
     VfCut o{0ull, 0ull};
     if (!w.sure) {
         const float* gmax = a.gmax + (size_t)r * a.groups;
@@ -814,46 +923,26 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
                 done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
             }
             if (!done) {
-                // every mass, by distance from the maximum; what lies further than `far` holds less
-                // than q W (W is at least the maximum's own mass) and is only summed
-                const float far = fminf(logf((float)V / u.q32) + 0.01f, 31.0f), scale = (float)(kVfBins - 1) / far;
-                vf_clear(sh);
-                uint64_t s = 0ull;
-                vf_each<T>(row, V, [&](int, float x) {
-                    const float d = u.m - vf_scaled(x, Tt);
-                    const uint64_t q = mass_of(exp_det(-d));
-                    if (d < far) vf_count(sh, (int)(d * scale), q);
-                    else s += q;
-                });
-                uint64_t in = 0ull;
+                // for verify_mass_kernel, or (the launch has many such rows) here
+                if (threadIdx.x == 0) sh.ngroups = ag_add32(a.flat_n, 1u);
                 __syncthreads();
-                for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) in += sh.hist[i];
-                in = vf_block_sum(in, sh);
-                const uint64_t total = in + vf_block_sum(s, sh), thr = scale_floor(u.q32, total);
-                // from the maximum down: the cut lies where the running sum reaches total - thr
-                if (total - thr <= in) {
-                    int bin;
-                    uint64_t over;
-                    vf_find(sh, kVfBins, total - thr - 1ull, &bin, &over);
-                    const uint64_t under = total - over - sh.hist[bin];
-                    const float yhi = u.m - (float)bin / scale, ylo = u.m - (float)(bin + 1) / scale;
-                    const float slack = (__builtin_fabsf(u.m) + 32.0f) * 0x1p-20f;
-                    if (vf_collect<T>(row, V, Tt, sh, Tt * (ylo - slack), Tt * (yhi + slack), [&](float y) {
-                            const float d = u.m - y;
-                            return d < far && (int)(d * scale) == bin;
-                        })) {
-                        o = vf_solve_bin(sh, u, (int)sh.count, total, under, thr);
-                        done = true;
+                const uint32_t at = sh.ngroups;
+                if (at < (uint32_t)min(a.R, kVfFlat)) {
+                    VfFlat& f = a.flat[at];
+                    for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) f.hist[i] = 0ull;
+                    if (threadIdx.x == 0) {
+                        f.row = r;
+                        f.ctr = 0u;
+                        f.rest = 0ull;
                     }
+                    return;
                 }
+                vf_clear(sh);
+                const uint64_t rest = vf_block_sum(vf_masses<T>(row, V, Tt, sh, u, 0, V, true), sh);
+                done = vf_flat<T>(row, V, Tt, sh, u, rest, &o);
             }
         }
-        if (!done) {
-            uint64_t n = 0ull;
-            vf_each<T>(row, V, [&](int, float x) { n += x == x ? 1u : 0u; });
-            n = vf_block_sum(n, sh);
-            o = vf_solve(VfRowIter<T>{row, V, Tt}, sh, u, n);
-        }
+        if (!done) o = vf_solve_row<T>(row, V, Tt, sh, u);
         // the kept tokens for the race, where the list holds them and they are few
         int32_t* kept = a.kept + (size_t)r * (1 + kVfKept);
         const int n = listed ? (int)sh.count : 0;
@@ -869,13 +958,44 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
         if (threadIdx.x == 0) kept[0] = listed && sh.ngroups <= (uint32_t)kVfKept ? (int32_t)sh.ngroups : -1;
     }
     __syncthreads();  // every wave has read the row's parts
+    if (threadIdx.x == 0) vf_write(a, r, w, o);
+}
+
+// The rows that verify_cut_kernel has left, each split over as many workgroups as there are for it; the
+// part that arrives last finishes the row.
+template <typename T>
+__global__ __launch_bounds__(kVfCutThreads) void verify_mass_kernel(VerifyArgs a) {
+    __shared__ VfCutShared sh;
+    const int rows = min((int)min(*a.flat_n, (uint32_t)kVfFlat), a.R);
+    if (rows == 0) return;
+    const int parts = min((int)gridDim.x / rows, 64), at = blockIdx.x / parts, p = blockIdx.x - at * parts;
+    if (at >= rows) return;
+    VfFlat& f = a.flat[at];
+    const int r = f.row;
+    const VfParams prm = vf_params(a, vf_request(a, r));
+    const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
+    const VfRow w = vf_join(a, prm, r);
+    const VfRule u = vf_rule(prm, w);
+    const int V = a.V, nvec = V / Elem<T>::kVec, len = (nvec + parts - 1) / parts;
+    vf_clear(sh);
+    // (a part past the row's end only arrives; the last takes the elements past the vectors)
+    const uint64_t mine = vf_masses<T>(row, V, prm.T, sh, u, min(p * len, nvec), min((p + 1) * len, nvec), p == parts - 1);
+    uint64_t rest = vf_block_sum(mine, sh);
+    for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads)
+        if (const uint64_t h = sh.hist[i]) ag_add64(&f.hist[i], h);
+    if (threadIdx.x == 0 && rest) ag_add64(&f.rest, rest);
+    stores_complete();
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = ag_add32(&f.ctr, 1u);
+    __syncthreads();
+    if (sh.count != (uint32_t)parts - 1u) return;
+    for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) sh.hist[i] = ag_load64(&f.hist[i]);
+    rest = ag_load64(&f.rest);
+    VfCut o;
+    if (!vf_flat<T>(row, V, prm.T, sh, u, rest, &o)) o = vf_solve_row<T>(row, V, prm.T, sh, u);
     if (threadIdx.x == 0) {
-        VfRec c;
-        c.top = w.top;
-        c.m2 = w.m;
-        c.sum = (float)o.kept * 0x1p-44f;
-        a.rec[(size_t)r * a.S] = c;
-        a.cut[r] = o.cut;
+        vf_write(a, r, w, o);
+        a.kept[(size_t)r * (1 + kVfKept)] = -1;
     }
 }
 
@@ -1087,6 +1207,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
 #define VWS_VERIFY_INST(T)                                       \
     template __global__ void verify_rows_kernel<T>(VerifyArgs);  \
     template __global__ void verify_cut_kernel<T>(VerifyArgs);   \
+    template __global__ void verify_mass_kernel<T>(VerifyArgs);  \
     template __global__ void verify_token_kernel<T>(VerifyArgs);
 VWS_VERIFY_INST(float)
 VWS_VERIFY_INST(uint16_t)
