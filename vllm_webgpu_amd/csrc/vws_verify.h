@@ -26,7 +26,7 @@ struct VfRec {
 
 constexpr int kVfBins = 2048;      // bins of a row's masses
 constexpr int kVfFlat = 128;       // rows of a launch that verify_mass_kernel takes
-constexpr int kVfMassWgs = 512;    // its workgroups: two of 1024 threads for each compute unit
+constexpr int kVfMassWgs = 256;    // its workgroups: one of 1024 threads for each compute unit
 
 struct VfFlat {
     int32_t row;

@@ -248,6 +248,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 constexpr int kVfCutWaves = kVfCutThreads / 64;
 constexpr int kVfList = 2048;     // list entries (a row's candidates)
 constexpr int kVfSmall = 512;     // entries that are compared with each other, all pairs
+constexpr int kVfPairs = 128;     // (of one bin: more of them are mostly equal)
 constexpr int kVfGroups = 1024;   // groups that are read for the list
 constexpr int kVfPeaks = 256;     // maxima that bound the list
 constexpr int kVfPeakMost = 232;  // of them, the last whose rank is used (the next are few and far between)
@@ -571,10 +572,8 @@ __device__ __forceinline__ VfCut vf_solve_small(VfCutShared& sh, const VfRule& u
 }
 
 // The elements listed are the row's largest.  Whether top-p's cut lies among them, and is the same, for
-// every total W in [lo, hi]: kept iff A < f(W) = W - floor(q W), which never falls.  If not, the part of
-// what is kept that they hold (0 where W is what leaves it open).
-__device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, int n, double lo, double hi, VfCut* o,
-                                             double* held) {
+// every total W in [lo, hi]: kept iff A < f(W) = W - floor(q W), which never falls.
+__device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, int n, double lo, double hi, VfCut* o) {
     const VfRank e = vf_rank(sh, u, n);
     const bool in = (int)threadIdx.x < n;
     const uint64_t Wl = (uint64_t)lo, Wh = (uint64_t)hi + 1ull;
@@ -583,10 +582,7 @@ __device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, i
     // (the sum of all masses listed is below 2^53: the count of open ones goes on top)
     const uint64_t total = vf_small_sum((in ? e.w : 0ull) + (open ? 1ull << 54 : 0ull), sh);
     // elements past the list have A >= total: refused for every W if total >= f(hi)
-    if (total >= 1ull << 54 || total < fh) {
-        *held = total >= 1ull << 54 ? 0.0 : (double)total / (double)fh;
-        return false;
-    }
+    if (total >= 1ull << 54 || total < fh) return false;
     *o = vf_small_cut(sure, e, sh);
     return true;
 }
@@ -596,16 +592,25 @@ __device__ __forceinline__ bool vf_solve_top(VfCutShared& sh, const VfRule& u, i
 __device__ __forceinline__ VfCut vf_solve_bin(VfCutShared& sh, const VfRule& u, int n, uint64_t total, uint64_t under,
                                               uint64_t thr) {
     VfCut o;
-    if (n <= kVfSmall) {
+    if (n <= kVfPairs) {
         const VfRank e = vf_rank(sh, u, n);
         const uint64_t in = vf_small_sum((int)threadIdx.x < n ? e.w : 0ull, sh);
         o = vf_small_cut((int)threadIdx.x < n && under + (in - e.A) > thr, e, sh);
         o.kept += total - under - in;
         return o;
     }
+    // (in 16-bit logits a bin is mostly one value)
     const VfListIter it{sh.list, n};
-    uint64_t c;
-    const uint32_t key = vf_select(it, sh, thr - under, &c, [&](uint32_t, float y) { return u.mass(y); });
+    uint64_t hi = 0ull, lo = 0ull;
+    it.each([&](int, uint32_t k, float) {
+        hi = vws_max64(hi, k);
+        lo = vws_max64(lo, (uint32_t)~k);
+    });
+    hi = vf_block_max(hi, sh);
+    lo = vf_block_max(lo, sh);
+    uint64_t c = 0ull;
+    uint32_t key = (uint32_t)hi;
+    if (key != ~(uint32_t)lo) key = vf_select(it, sh, thr - under, &c, [&](uint32_t, float y) { return u.mass(y); });
     const uint64_t q = u.mass(val_of(key));
     const uint64_t gone = (thr - under - c) / q;
     o.cut = (uint64_t)key << 32;
@@ -914,14 +919,10 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
             // its constant likewise, the exponential and the sums by a few 2^-24
             const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
-            // the 100 or so logits above the 84th of 256 maxima, or, where they hold a good part of
-            // what is kept, the 350 or so above the 192nd
-            double held = 1.0;
-            for (int n = 84; !done && n <= 192 && held > 0.5; n += 108) {
-                const float t = below(vf_peak(sh, n));
-                if (!(t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)) break;
-                done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o, &held);
-            }
+            // the 130 or so logits above the 100th of 256 maxima
+            const float t = below(vf_peak(sh, 100));
+            if (t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
+                done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
             if (!done) {
                 // for verify_mass_kernel, or (the launch has many such rows) here
                 if (threadIdx.x == 0) sh.ngroups = ag_add32(a.flat_n, 1u);
