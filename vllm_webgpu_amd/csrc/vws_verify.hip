@@ -919,8 +919,8 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
             // its constant likewise, the exponential and the sums by a few 2^-24
             const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
-            // the 130 or so logits above the 100th of 256 maxima
-            const float t = below(vf_peak(sh, 100));
+            // the 100 or so logits above the 84th of 256 maxima
+            const float t = below(vf_peak(sh, 84));
             if (t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
                 done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
             if (!done) {
