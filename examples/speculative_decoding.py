@@ -1,6 +1,6 @@
 """Speculative decoding with a draft that learns from its target, on synthetic models.
 
-    python examples/speculative_decoding.py [--vocab 32000] [--rounds 4] [--batch 64] [--drafts 4]
+    python examples/speculative_decoding.py [--vocab 4000] [--rounds 5] [--batch 64] [--drafts 4]
 
 The target is a fixed random next-token model (an embedding of the last token, one hidden layer, an
 output matrix); the draft a smaller one that starts with random weights.  Each round the requests
@@ -60,7 +60,7 @@ def draft_tokens(draft, last: torch.Tensor, count: int, temperature: float):
     return torch.stack(tokens, 1), torch.stack(probs, 1)
 
 
-def run(vocab=32000, rounds=4, batch=64, drafts=4, steps=8, temperature=0.8, top_p=0.95, top=32, train_steps=40, seed=0):
+def run(vocab=4000, rounds=5, batch=64, drafts=4, steps=8, temperature=0.8, top_p=0.95, top=32, train_steps=100, seed=0):
     """Accepted drafts per request and step, of each round."""
     dev = torch.device("cuda")
     torch.manual_seed(seed)
@@ -100,7 +100,7 @@ def run(vocab=32000, rounds=4, batch=64, drafts=4, steps=8, temperature=0.8, top
 
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    for name, default in (("vocab", 32000), ("rounds", 4), ("batch", 64), ("drafts", 4)):
+    for name, default in (("vocab", 4000), ("rounds", 5), ("batch", 64), ("drafts", 4)):
         ap.add_argument(f"--{name}", type=int, default=default)
     a = ap.parse_args()
     for i, rate in enumerate(run(a.vocab, a.rounds, a.batch, a.drafts)):
