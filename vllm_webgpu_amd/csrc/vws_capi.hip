@@ -434,7 +434,7 @@ void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* 
 
 constexpr int kRowsWgs = 768;
 constexpr int kRaceWgs = 1024;
-constexpr int kRaceCutWgs = 2048;
+constexpr int kRaceCutWgs = 4096;
 constexpr int kDistillWgs = 768;
 constexpr int kGradWgs = 16384;
 
