@@ -110,6 +110,30 @@ def test_long_rows_with_many_of_them(cuda, V, dtype, tail):
     assert torch.equal(one, loss) and torch.equal(inplace, grad)
 
 
+@pytest.mark.parametrize("V,dtype,N", [(49160, "bf16", 4200), (65529, "f16", 3100), (128257, "bf16", 1600), (25001, "f32", 4100),
+                                       (65533, "f32", 1600), (155000, "f16", 1310), (77000, "f32", 1400)])
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+def test_large_steps(cuda, V, dtype, N, tail):
+    """Calls beyond the last-level cache, whose rows one workgroup holds: against the two kernels (forward
+    and backward by autograd) on some rows, rows that do not count among them, and in place."""
+    x, ids, lp = make(cuda, 1, V, 40, dtype, seed=V)
+    w = (torch.arange(N, device=cuda) % 5 != 2).float() * 1.5
+    x = x.expand(N, -1).contiguous()
+    x[:, ::7] += torch.linspace(-2, 2, N, device=cuda).to(x.dtype).unsqueeze(1)
+    x[2] = float("nan")          # (weight 0: not read)
+    ids, lp = ids.expand(N, -1).contiguous(), lp.expand(N, -1).contiguous()
+    ids[4, 3], ids[5, 1], ids[N - 1, 6:] = -1, ids[5, 0], V + 3
+    g = torch.linspace(0.5, 1.5, N, device=cuda)
+    loss, grad = ops.distill_loss_and_grad(x, ids, lp, w, 1.0, tail, grad_output=g)
+    for part in (slice(0, 24), slice(N - 24, N)):
+        live = [i for i in range(*part.indices(N)) if w[i] != 0]
+        want, want_grad = reference(x[live], ids[live], lp[live], w[live], 1.0, tail, g[live])
+        close(loss[live], grad[live], want, want_grad, w[live], g[live], 1.0, x.dtype)
+    assert not loss[2::5].any() and not grad[2::5].any()
+    again = ops.distill_loss_and_grad(x, ids, lp, w, 1.0, tail, grad_output=g, out=x)
+    assert torch.equal(again[0], loss) and torch.equal(x, grad)
+
+
 @pytest.mark.parametrize("T", [0.5, 1.0, 2.0, 3.7])
 @pytest.mark.parametrize("tail", ["renormalize", "bucket"])
 def test_temperature_and_weights(cuda, T, tail):

@@ -552,15 +552,21 @@ int validate_distill(const vws_distill_args* a, int parts) {
     return VWS_OK;
 }
 
-// The kernel that holds a row in one workgroup's registers, or null: rows that fit (38 vectors of 16
-// bytes for each of 512 threads), and enough of them to keep half of the compute units at work.
+// The step's kernel that holds a row in one workgroup's registers and reads it once, or null: the
+// forward, then the backward, which read it twice.  Those split every row over the chip and find
+// in the last-level cache (256 MB) what they read first, so the one kernel is for calls well beyond
+// it, whose rows fill at least three quarters of its registers (16, 32 or 38 vectors of 16 bytes
+// for each of 512 threads).  Measured, one kernel against two, us: 1024 x 128256 bf16 (263 MB) 141
+// and 145, 2048 x (525 MB) 253 and 295, 4096 x 464 and 594; 300 x 128256 68 and 47; 1024 x 151936 177
+// and 170, 2048 x 310 and 354; 4096 x 64000 271 and 295, 2048 x 150 and 144; half-filled registers:
+// 4096 x 66000 401 and 315, 4096 x 80000 398 and 375 (of fp32 at 40000 322 and 372).
 template <typename T>
 auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
+    if ((size_t)rows * (size_t)V * sizeof(T) < ((size_t)384 << 20)) return nullptr;
     const int per = (V / (16 / (int)sizeof(T)) + kDsStepThreads - 1) / kDsStepThreads;
-    if (rows < device_info().cus / 2 || per < 1) return nullptr;
-    if (per <= 16) return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
-    if (per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
-    if (per <= 38) return bucket ? distill_step_kernel<T, true, 38> : distill_step_kernel<T, false, 38>;
+    if (per > 12 && per <= 16) return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
+    if (per > 24 && per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
+    if (per > 32 && per <= 38) return bucket ? distill_step_kernel<T, true, 38> : distill_step_kernel<T, false, 38>;
     return nullptr;
 }
 
