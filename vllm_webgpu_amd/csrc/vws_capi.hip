@@ -432,10 +432,21 @@ void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* 
     *S = (V + *len - 1) / *len;
 }
 
+// Workgroups (of 256 threads) that a launch's rows are split over, at most; parts of at least 4096
+// logits.  A pass that keeps a maximum and a sum pays for every part (its reduction, its record, the
+// join), so three a compute unit read fastest: 276 rows x 128256 fp32, the whole verification, with
+// 512, 768, 1024, 2048, 4096: 61, 60, 63, 74, 76 us; 512 x 151936 bf16, a loss: 31.7, 31.5, 36.7, 40, 42;
+// 48 x 262144 f16, loss and gradient: 25.1, 24.4, 26.2, 35.5, 45.
 constexpr int kRowsWgs = 768;
+constexpr int kDistillWgs = 768;
+// The race reads one row a request.  Uncut rows are all read (64 x 128256 fp32 with 1024, 2048: 60.3,
+// 67.9 us).  Of cut rows most are raced from their list, by one part while the others leave at once, so
+// many short parts spread the few that are read (256 x 262144 bf16 with 1024, 2048, 4096, 8192, 16384:
+// 284, 260, 252, 259, 277 us; 48 requests with a top-k have lists only: 35.5, -, 37.4, 37.3).
 constexpr int kRaceWgs = 1024;
 constexpr int kRaceCutWgs = 4096;
-constexpr int kDistillWgs = 768;
+// A gradient has no sums to join: short parts keep reads and writes of a row close to each other (2048 x
+// 128256 bf16, loss and gradient, with 1024, 4096, 8192, 16384: 246, 238, 234.5, 231 us).
 constexpr int kGradWgs = 16384;
 
 void verify_parts(int rows, int V, int* S, int* len) { split_row(rows, V, kRowsWgs, 4096, kVfMaxParts, 1, S, len); }
@@ -554,20 +565,26 @@ int validate_distill(const vws_distill_args* a, int parts) {
 
 // The step's kernel that holds a row in one workgroup's registers and reads it once, or null: the
 // forward, then the backward, which read it twice.  Those split every row over the chip and find
-// in the last-level cache (256 MB) what they read first, so the one kernel is for calls well beyond
-// it, whose rows fill at least three quarters of its registers (16, 32 or 38 vectors of 16 bytes
-// for each of 512 threads).  Measured, one kernel against two, us: 1024 x 128256 bf16 (263 MB) 141
-// and 145, 2048 x (525 MB) 253 and 295, 4096 x 464 and 594; 300 x 128256 68 and 47; 1024 x 151936 177
-// and 170, 2048 x 310 and 354; 4096 x 64000 271 and 295, 2048 x 150 and 144; half-filled registers:
-// 4096 x 66000 401 and 315, 4096 x 80000 398 and 375 (of fp32 at 40000 322 and 372).
+// in the last-level cache (256 MB) what they read first, so the one kernel is for calls beyond it
+// (long rows, of which a workgroup gets few and the last ones leave units idle: well beyond), whose
+// rows fill at least three quarters or so of its registers (16, 32 or 38 vectors of 16 bytes for each of 512
+// threads).  Measured, one kernel against two, us, bf16: 1024 x 128256 (263 MB) 143 and 145, 1200 x 165 and
+// 159, 1450 x (372 MB) 192 and 195, 2048 x 251 and 295, 4096 x 462 and 594, 300 x 68 and 47; 1200 x 151936
+// (365 MB) 209 and 192, 2048 x 310 and 354; 2300 x 64000 (294 MB) 153 and 156, 2100 x (269 MB) 149 and
+// 146, 1800 x 127 and 120, 4096 x 271 and 295.  By the registers' filling: 4096 x 53248 (13 vectors) 247 and
+// 247, 50264 250 and 240, 57344 252 and 263; 2048 x 102400 (25) 226 and 235; 2048 x 136000 (33.2) 313 and
+// 311; 4096 x 66000 (16.1 of 32) 401 and 315.
 template <typename T>
 auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
-    if ((size_t)rows * (size_t)V * sizeof(T) < ((size_t)384 << 20)) return nullptr;
+    const size_t bytes = (size_t)rows * (size_t)V * sizeof(T);
     const int per = (V / (16 / (int)sizeof(T)) + kDsStepThreads - 1) / kDsStepThreads;
-    if (per > 12 && per <= 16) return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
-    if (per > 24 && per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
-    if (per > 32 && per <= 38) return bucket ? distill_step_kernel<T, true, 38> : distill_step_kernel<T, false, 38>;
-    return nullptr;
+    if (per <= 16) {
+        if (per <= 13 || bytes < ((size_t)256 << 20)) return nullptr;
+        return bucket ? distill_step_kernel<T, true, 16> : distill_step_kernel<T, false, 16>;
+    }
+    if (per <= 24 || per > 38 || bytes < ((size_t)384 << 20)) return nullptr;
+    if (per <= 32) return bucket ? distill_step_kernel<T, true, 32> : distill_step_kernel<T, false, 32>;
+    return bucket ? distill_step_kernel<T, true, 38> : distill_step_kernel<T, false, 38>;
 }
 
 template <typename T>

@@ -366,6 +366,11 @@ __device__ __forceinline__ void ds_save(const DistillArgs& a, int r, const DsRow
     }
 }
 
+// Loss of rows split over workgroups: each part's running maximum and sum in one read, entries kept out of
+// the rest's sum by a bitmap; the part that arrives last joins them and takes the entries' logits.
+// Bound: HBM: 512 x 151936 bf16 (156 MB) 30.8 us, 5.05 TB/s, a copy's rate; before a gradient it leaves what it reads
+// to the caches (2048 x 128256 bf16, three rows in ten weightless, 353 MB fetched: 80 us, 4.4 TB/s).  4 x 32000
+// fp32 6.6 us, 301 x 50257 17 (starts and ends of the launch, unaligned rows).
 template <typename T, bool BUCKET>
 __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs a) {
     extern __shared__ uint32_t bm[];
@@ -428,7 +433,9 @@ __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs
 }
 
 // The gradient of part p of row r.  Rows from the last to the first: those that the forward read last
-// are still in the last-level cache.
+// are still in the last-level cache.  Gradients are stored past the caches, which keeps the logits there
+// (forward and backward of 2048 x 128256 bf16: 244 us, 287 with plain stores).
+// Bound: HBM: of those rows 149 us, 353 MB fetched and 502 written, 5.7 TB/s; 301 x 50257 fp32 (121 MB) 22 us.
 template <typename T>
 __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
@@ -490,6 +497,9 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
 // time; as a row's gradients are written, the next row's logits and entries are loaded into the
 // registers they leave.  No barrier waits for memory: a vector that holds teacher entries (by the
 // bitmap) takes their gradients from the hash, so nothing is written twice.
+// Bound: HBM: 4096 x 128256 bf16 (1.05 GB read and as much written) 462 us, 4.5 TB/s of a copy's 5.07; forward and
+// backward kernels take 594.  What is left is each row's two reductions, in which its workgroup moves nothing but
+// the next row's loads.
 template <typename T, bool BUCKET, int NV>
 __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = 2, NW = kDsStepThreads / 64;
@@ -533,12 +543,12 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
     hashes[0].clear();
     ds_clear_bits(bms, V);
     __syncthreads();
-    // Every row takes a workgroup some 13 us of sums and then some 15 of reading and writing.  Started
-    // together the workgroups would keep time, and the memory idle while all sum: they start up
-    // to 20 us apart, where there are rows enough to make up for that (4096 rows of 128256 bf16
-    // 491 -> 463 us).
-    if (a.N >= 8 * (int)gridDim.x)
-        for (int k = (int)((blockIdx.x >> 3) & 7u); k > 0; --k) __builtin_amdgcn_s_sleep(115);
+    // A row of 128256 bf16 takes a workgroup some 13 us of sums and then some 15 of reading and writing.
+    // Started together the workgroups would keep time, and the memory idle while all sum: they start
+    // up to most of a row's time apart.  Against a common start, us: bf16 1600 x 128256 231 -> 216, 4096 x
+    // 487 -> 462, 3328 x 64000 219 -> 212, 1400 x 151936 249 -> 231; fp32 4000 x 32000 220 -> 213, but 2048 x
+    // 64000 226 -> 231 (twice the sleep for rows of 64000 bf16 would lose: 224).
+    for (int k = (int)((blockIdx.x >> 3) & 7u); k > 0; --k) __builtin_amdgcn_s_sleep(NV * 7 / 2);
     for (int parity = 0;; parity ^= 1) {
         const T* row = x + (size_t)r * a.xstride;
         T* out = grad + (size_t)r * a.gstride;

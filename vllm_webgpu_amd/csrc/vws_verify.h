@@ -25,8 +25,8 @@ struct VfRec {
 };
 
 constexpr int kVfBins = 2048;      // bins of a row's masses
-constexpr int kVfFlat = 128;       // rows of a launch that verify_mass_kernel takes
-constexpr int kVfMassWgs = 256;    // its workgroups: one of 1024 threads for each compute unit
+constexpr int kVfFlat = 256;       // rows of a launch that verify_mass_kernel takes: a workgroup each, at least
+constexpr int kVfMassWgs = 256;    // its workgroups, one of 1024 threads for each compute unit
 
 struct VfFlat {
     int32_t row;

@@ -134,7 +134,9 @@ __device__ __forceinline__ float vf_value(uint64_t top) {
 // few logits that matter without a second read of the row.
 //
 // Bound: HBM.  The next iteration's loads are issued before this one's are used, and the first
-// before the request's parameters are known.
+// before the request's parameters are known.  274 rows x 128256 fp32 (141 MB): 34.5 us, 4.1 TB/s, most of a
+// copy's rate (5.07); 745 x 262144 bf16 (391 MB), most of them cut: 92 us, 4.2 TB/s read, and 19 MB of groups' maxima
+// written; small batches are one latency chain (6 x 128256 bf16 6.2 us, 4 x 32000 fp32 5.4).
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
@@ -242,7 +244,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 //   * else the masses of all logits, summed in bins by the distance from the maximum;
 //     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).
 //     verify_mass_kernel does that for the first kVfFlat such rows, all compute units at it
-//     however few the rows, and verify_cut_kernel itself for further ones.
+//     however few the rows, and verify_cut_kernel itself for further ones (rows of 128256 bf16 in
+//     whole calls, with 64, 128, 256 rows taken: 80 such rows 128, 87, 87 us, 200 147, 154, 118, 320 217,
+//     222, 190).
 // A list that overflows (many equal logits) leaves the row to passes over its keys' bits.
 
 constexpr int kVfCutWaves = kVfCutThreads / 64;
@@ -868,7 +872,15 @@ __device__ __forceinline__ void vf_write(const VerifyArgs& a, int r, const VfRow
 }
 
 // One workgroup per row: the kept set of a row that its request cuts, as the smallest
-// (key(y) << 32 | index) kept, and the sum of its exponentials.
+// (key(y) << 32 | index) kept, and the sum of its exponentials.  The n-th largest of 256 peaks (maxima
+// of groups, each from its own logits) is a lower bound of the n-th largest logit, so the logits above it
+// are a list of n or a few more, read by way of the groups' maxima alone (a number for 16 or 32 logits).
+// Top-k is decided in the list if k <= kVfPeakMost; top-p if the list's masses reach p of the row's sum even at the
+// edge of that sum's error.
+//
+// Bound: latency, a chain of about ten barriers for one row (6 rows x 128256 17 us, 150 x 151936
+// with a top-k 13.5), then rows a compute unit: 745 x 262144 42 us, of which 31 MB fetched.  Reading
+// the row again in its place took 120 us of one request's 155, and of the 745 rows 1.1 ms.
 template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
@@ -963,7 +975,13 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
 }
 
 // The rows that verify_cut_kernel has left, each split over as many workgroups as there are for it; the
-// part that arrives last finishes the row.
+// part that arrives last finishes the row.  Exact masses fall into bins by distance from the maximum
+// (integers: no order of the atomics changes them); the bin where the sum passes p is then read
+// and decided.
+//
+// Bound: the last part's chain (for a row of 262144 about 20 us of masses, 20 of the deciding bin's read by one
+// compute unit, 7 of its order).  70 such rows of 745: 62 us, against 165 by verify_cut_kernel alone,
+// where they held up the launch; with no such row 2 to 4 us, the price of a launch with a top-p.
 template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_mass_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
@@ -1021,6 +1039,12 @@ __device__ __forceinline__ bool vf_kept(const VfRow& w, float y, int i) {
 }
 
 // Part p of request b's race; every part decides the request for itself.
+//
+// A draw is argmax w / E, E = -ln u; as E >= 1 - u, a token whose w / (1 - u) is below the best so far needs
+// no logarithm.  Rows whose kept tokens are listed race those alone.
+// Bound: for uncut rows the reads (64 x 128256 fp32 logits, draft's probabilities and uniforms, 82 MB fetched:
+// 24 us, 3.4 TB/s); for listed ones the latency of decision and race (48 requests, top-k 50: 8.3 us, 22.6 reading
+// the row; one request 6.4); 256 mixed requests of 262144 bf16 45 us, Philox for the tokens near the best.
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec;
