@@ -193,9 +193,13 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
             t.m = n;
         }
     }
-    // the largest logit's first place in its group
+    // the largest logit's first place in its group, where it is the wave's (every lane's group read
+    // again was a third of the part)
+    float most = best;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, vf_lane_xor(most, o));
     uint64_t top = 0ull;
-    if (tid < nvec) {
+    if (best == most) {  // (not of a thread without vectors: NaN)
         for (int u = U - 1; u >= 0; --u) {
             const int vi = group + u * kVfThreads;
             if (vi >= nvec) continue;
