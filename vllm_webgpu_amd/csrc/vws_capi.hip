@@ -434,8 +434,8 @@ void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* 
 
 // Workgroups (of 256 threads) that a launch's rows are split over, at most; parts of at least 4096
 // logits.  A pass that keeps a maximum and a sum pays for every part (its reduction, its record, the
-// join), so three a compute unit read fastest: 276 rows x 128256 fp32, the whole verification, with
-// 512, 768, 1024, 2048, 4096: 61, 60, 63, 74, 76 us; 512 x 151936 bf16, a loss: 31.7, 31.5, 36.7, 40, 42;
+// join), and too few leave loads out: 276 rows x 128256 fp32, the whole verification, with
+// 512, 768, 1024, 1536: 57.1, 55.8, 56.8, 56.1 us; 512 x 151936 bf16, a loss: 31.7, 31.5, 36.7, 40, 42;
 // 48 x 262144 f16, loss and gradient: 25.1, 24.4, 26.2, 35.5, 45.
 constexpr int kRowsWgs = 768;
 constexpr int kDistillWgs = 768;

@@ -275,10 +275,11 @@ struct VfCutShared {
 
 __device__ __forceinline__ float vf_scaled(float x, float Tt) { return Tt == 1.0f ? x : x / Tt; }
 
-// Calls f(index, x) for every logit of a row (each thread its vectors, then one tail element), or for
-// its vectors [v0, v1) and, with `tail`, that element; the next four vectors are on their way while these are used.
-template <typename T, typename F>
-__device__ __forceinline__ void vf_each(const T* row, int V, F f, int v0 = 0, int v1 = 1 << 30, bool tail = true) {
+// Calls fv(first index, logits) for every vector of a row and f(index, x) for the logits past them (each thread its
+// vectors, then one element), or for its vectors [v0, v1) and, with `tail`, that element; the next four
+// vectors are on their way while these are used.
+template <typename T, typename FV, typename F>
+__device__ __forceinline__ void vf_vectors(const T* row, int V, FV fv, F f, int v0 = 0, int v1 = 1 << 30, bool tail = true) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
     const int tid = threadIdx.x, last = V / VEC, nvec = min(v1, last);
     if (nvec > v0) {
@@ -301,13 +302,22 @@ __device__ __forceinline__ void vf_each(const T* row, int V, F f, int v0 = 0, in
                 if (vi >= nvec) break;
                 float v[VEC];
                 Elem<T>::from_words(w[u][0], w[u][1], w[u][2], w[u][3], v);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) f(vi * VEC + j, v[j]);
+                fv(vi * VEC, v);
             }
         }
     }
     const int i = last * VEC + tid;
     if (tail && i < V) f(i, Elem<T>::load1(row + i));
+}
+
+// The same with f(index, x) for every logit.
+template <typename T, typename F>
+__device__ __forceinline__ void vf_each(const T* row, int V, F f, int v0 = 0, int v1 = 1 << 30, bool tail = true) {
+    constexpr int VEC = Elem<T>::kVec;
+    vf_vectors<T>(row, V, [&](int i, const float (&v)[VEC]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f(i + j, v[j]);
+    }, f, v0, v1, tail);
 }
 
 // What the selection below runs over: a row's elements, or the list's.  each(f): f(index, key, y).
@@ -627,24 +637,46 @@ __device__ __forceinline__ VfCut vf_solve_bin(VfCutShared& sh, const VfRule& u, 
     return o;
 }
 
-// Lists the row's elements with lo <= x <= hi whose y passes `in`; false when they are more than the
-// list holds.
+// Lists the row's elements with lo <= x <= hi whose y passes `in`; false when those with lo <= x <= hi are
+// more than the list holds.  One compute unit goes over the whole row, so a vector takes two compares
+// an element and a branch; places are listed first, values looked up from there.
 template <typename T, typename F>
 __device__ __forceinline__ bool vf_collect(const T* row, int V, float Tt, VfCutShared& sh, float lo, float hi, F in) {
+    constexpr int VEC = Elem<T>::kVec, kMine = kVfList / kVfCutThreads;
     __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0u;
+    if (threadIdx.x == 0) sh.count = sh.ngroups = 0u;
     __syncthreads();
-    vf_each<T>(row, V, [&](int i, float x) {
-        if (x >= lo && x <= hi) {
-            const float y = vf_scaled(x, Tt);
-            if (in(y)) {
-                const uint32_t at = agg_reserve(&sh.count);
-                if (at < (uint32_t)kVfList) sh.list[at] = ((uint64_t)key_of(y) << 32) | (uint32_t)i;
-            }
+    auto add = [&](int i) {
+        const uint32_t at = agg_reserve(&sh.ngroups);
+        if (at < (uint32_t)kVfList) sh.list[at] = (uint32_t)i;
+    };
+    vf_vectors<T>(row, V, [&](int i, const float (&v)[VEC]) __attribute__((always_inline)) {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m |= v[j] >= lo && v[j] <= hi ? 1u << j : 0u;
+        while (m) {
+            add(i + (int)__builtin_ctz(m));
+            m &= m - 1u;
         }
-    });
+    }, [&](int i, float x) { if (x >= lo && x <= hi) add(i); });
     __syncthreads();
-    return sh.count <= (uint32_t)kVfList;
+    const int n = (int)sh.ngroups;
+    if (n > kVfList) return false;
+    int at[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+        const int e = (int)threadIdx.x + k * kVfCutThreads;
+        at[k] = e < n ? (int)sh.list[e] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+        if (at[k] < 0) continue;
+        const float y = vf_scaled(Elem<T>::load1(row + at[k]), Tt);
+        if (in(y)) sh.list[agg_reserve(&sh.count)] = ((uint64_t)key_of(y) << 32) | (uint32_t)at[k];
+    }
+    __syncthreads();
+    return true;
 }
 
 // Calls f(maximum, part, first vector) for the groups of a row that exist: kVfThreads of them to a
