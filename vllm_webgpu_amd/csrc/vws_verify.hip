@@ -134,9 +134,8 @@ __device__ __forceinline__ float vf_value(uint64_t top) {
 // few logits that matter without a second read of the row.
 //
 // Bound: HBM.  The next iteration's loads are issued before this one's are used, and the first
-// before the request's parameters are known.  274 rows x 128256 fp32 (141 MB): 34.5 us, 4.1 TB/s, most of a
-// copy's rate (5.07); 745 x 262144 bf16 (391 MB), most of them cut: 92 us, 4.2 TB/s read, and 19 MB of groups' maxima
-// written; small batches are one latency chain (6 x 128256 bf16 6.2 us, 4 x 32000 fp32 5.4).
+// before the request's parameters are known.  274 rows x 128256 fp32 (141 MB): 30.6 us, 4.6 TB/s of a copy's
+// 5.07; 745 x 262144 bf16 (391 MB), most of them cut: 87 us, 4.5 TB/s, and 19 MB of groups' maxima written; small batches are one latency chain (6 x 128256 bf16 5.6 us, 4 x 32000 fp32 4.6).
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
@@ -1015,9 +1014,10 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
 // (integers: no order of the atomics changes them); the bin where the sum passes p is then read
 // and decided.
 //
-// Bound: the last part's chain (for a row of 262144 about 20 us of masses, 20 of the deciding bin's read by one
-// compute unit, 7 of its order).  70 such rows of 745: 62 us, against 165 by verify_cut_kernel alone,
-// where they held up the launch; with no such row 2 to 4 us, the price of a launch with a top-p.
+// Bound: the last part's chain (for a row of 262144 about 18 us of masses and 5 of waiting in its own sum, 16
+// of the deciding bin's read by one compute unit, 8 of its order; 27 in all for one row of 128256).  70 such
+// rows of 745: 54 us, against 165 by verify_cut_kernel alone, where they held up the launch; with no such row 1
+// to 4 us, the price of a launch with a top-p.
 template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_mass_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
@@ -1079,8 +1079,8 @@ __device__ __forceinline__ bool vf_kept(const VfRow& w, float y, int i) {
 // A draw is argmax w / E, E = -ln u; as E >= 1 - u, a token whose w / (1 - u) is below the best so far needs
 // no logarithm.  Rows whose kept tokens are listed race those alone.
 // Bound: for uncut rows the reads (64 x 128256 fp32 logits, draft's probabilities and uniforms, 82 MB fetched:
-// 24 us, 3.4 TB/s); for listed ones the latency of decision and race (48 requests, top-k 50: 8.3 us, 22.6 reading
-// the row; one request 6.4); 256 mixed requests of 262144 bf16 45 us, Philox for the tokens near the best.
+// 24 us, 4.1 TB/s of the 98 they hold); for listed ones the latency of decision and race (48 requests, top-k 50: 8.3 us, 22.6 reading
+// the row; one request 6.1); 256 mixed requests of 262144 bf16 44 us, Philox for the tokens near the best.
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec;
