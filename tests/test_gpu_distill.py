@@ -111,7 +111,8 @@ def test_long_rows_with_many_of_them(cuda, V, dtype, tail):
 
 
 @pytest.mark.parametrize("V,dtype,N", [(49160, "bf16", 4200), (65529, "f16", 3100), (128257, "bf16", 1600), (25001, "f32", 4100),
-                                       (65533, "f32", 1600), (155000, "f16", 1310), (77000, "f32", 1400)])
+                                       (65533, "f32", 1600), (155000, "f16", 1310), (77000, "f32", 1400), (57347, "bf16", 2400),
+                                       (29001, "f32", 2350)])
 @pytest.mark.parametrize("tail", ["renormalize", "bucket"])
 def test_large_steps(cuda, V, dtype, N, tail):
     """Calls beyond the last-level cache, whose rows one workgroup holds: against the two kernels (forward
