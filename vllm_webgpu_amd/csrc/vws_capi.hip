@@ -443,15 +443,22 @@ constexpr int kDistillWgs = 768;
 // 67.9 us).  Of cut rows most are raced from their list, by one part while the others leave at once, so
 // many short parts spread the few that are read (256 x 262144 bf16 with 1024, 2048, 4096, 8192, 16384:
 // 284, 260, 252, 259, 277 us; 48 requests with a top-k have lists only: 35.5, -, 37.4, 37.3).
+// Up to two workgroups a compute unit the parts are shorter, as a thread's generated uniforms and their
+// logarithms are a chain (parts of at least 4096, 1024: one request of 32000 bf16 25.0, 19.3 us, of 128256 with a flat
+// nucleus 61.4, 58.6; 6 of 48621 62.8, 55.7); without that limit 48 requests with a top-k lose (34.9, 37.0).
 constexpr int kRaceWgs = 1024;
 constexpr int kRaceCutWgs = 4096;
+constexpr int kRaceFewWgs = 512;
 // A gradient has no sums to join: short parts keep reads and writes of a row close to each other (2048 x
 // 128256 bf16, loss and gradient, with 1024, 4096, 8192, 16384: 246, 238, 234.5, 231 us).
 constexpr int kGradWgs = 16384;
 
 void verify_parts(int rows, int V, int* S, int* len) { split_row(rows, V, kRowsWgs, 4096, kVfMaxParts, 1, S, len); }
 void race_parts(int rows, int V, bool cuts, int* S, int* len) {
+    int s, l;
     split_row(rows, V, cuts ? kRaceCutWgs : kRaceWgs, 4096, kVfMaxParts, 1, S, len);
+    split_row(rows, V, kRaceFewWgs, 1024, kVfMaxParts, 1, &s, &l);
+    if (s > *S) *S = s, *len = l;
 }
 
 // A launch takes at most kTopkRows rows (the counters of the fixed region); a part's bitmap of
