@@ -393,7 +393,7 @@ def test_refusals(cuda):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("requests", [1, 12, 70])
+@pytest.mark.parametrize("requests", [1, 12, 70, 110])
 def test_flat_rows(cuda, dtype, requests):
     """Rows whose nucleus is most of the vocabulary, few and more than the launch sets aside."""
     t = make(cuda, [2] * requests, 9001 if requests > 12 else 33001, dtype, "f32", seed=requests, spread=0.5, spikes=1)
