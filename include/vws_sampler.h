@@ -282,7 +282,8 @@ int vws_apply_penalties(float* logits, int32_t batch, int32_t vocab, int64_t row
  * Requests with temperature < 1e-5 or NaN, and rows whose maximum is not finite, have their argmax
  * (lowest index) for sure.  A draft outside [0, vocab) is refused.  Nothing is read or written out
  * of bounds whatever cu_drafts holds: a request whose bounds do not fit (negative, decreasing, more
- * than max_drafts, past num_drafts) gets num_accepted -1 and no token. */
+ * than max_drafts, past num_drafts) gets num_accepted -1 and no token, and so does one with a row that
+ * the bounds give to another as well (a row is the last request's that starts at or before it). */
 #define VWS_MAX_DRAFTS 64
 typedef struct vws_verify_args {
     uint32_t struct_size; /* sizeof(vws_verify_args): ABI guard */

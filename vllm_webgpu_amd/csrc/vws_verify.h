@@ -62,6 +62,7 @@ struct VerifyArgs {
     VfRec* rec;                  // [R, S]
     float* gmax;                 // [R, groups] maxima of groups of vectors, of rows that are cut; or null
     int groups;                  // of a row
+    int32_t* owner;              // [R] the request whose parameters cut the row
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
     int32_t* kept;               // [R, 1 + kVfKept] of cut rows: how many are kept (-1: not listed), and they
     uint32_t* flat_n;            // rows whose masses verify_mass_kernel adds up; cleared by the statistics' launch
@@ -81,7 +82,7 @@ inline int vf_groups(int S, int part_len, int vec) {
 constexpr int kVfKept = 511;         // tokens of a cut row that the race takes from a list
 
 struct VfLayout {
-    size_t rec, gmax, cut, kept, flat_n, flat, best, ctr, total;
+    size_t rec, gmax, owner, cut, kept, flat_n, flat, best, ctr, total;
 };
 
 inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
@@ -89,6 +90,7 @@ inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
     size_t off = align256(sizeof(CoopState));  // every workspace starts with the fixed region
     w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
     w.gmax = off;  off = align256(off + sizeof(float) * (size_t)R * groups);
+    w.owner = off; off = align256(off + sizeof(int32_t) * (size_t)R);
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
     w.kept = off;  off = align256(off + sizeof(int32_t) * (size_t)R * (1 + kVfKept));
     w.flat_n = off; off = align256(off + sizeof(uint32_t));

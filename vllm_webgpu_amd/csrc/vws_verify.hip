@@ -71,14 +71,15 @@ __device__ __forceinline__ float vf_load_any1(const void* row, int dtype, int i)
 __device__ __forceinline__ size_t vf_esize(int dtype) { return dtype == VWS_DTYPE_F32 ? 4 : 2; }
 
 // The request of row r: the last whose first row (cu[b] + b) lies at or before it.  64 bounds at a
-// time, so two loads for up to 4096 requests; every lane of the calling wave returns it.
+// time, so two loads for up to 4096 requests; every lane of the calling wave returns it.  Bounds that
+// decrease can name a row twice: this is the one request that it is taken for, VerifyArgs::owner.
 __device__ __forceinline__ int vf_request(const VerifyArgs& a, int r) {
     int lo = 0, n = a.B;
     while (n > 1) {
         const int step = (n + kWave - 1) / kWave, at = lane_id() * step;
         const int b = lo + min(at, n - 1);
-        const int c = __popcll(wave_ballot(at < n && a.cu[b] + b <= r));
-        const int skip = c > 0 ? (c - 1) * step : 0;
+        const uint64_t before = wave_ballot(at < n && a.cu[b] <= r - b);  // (r - b: any bound goes)
+        const int skip = before ? (kWave - 1 - (int)__builtin_clzll(before)) * step : 0;
         lo += skip;
         n = min(step, n - skip);
     }
@@ -158,7 +159,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
         if (r < a.B) a.ctr[r] = 0u;  // (R >= B)
         if (r == 0) *a.flat_n = 0u;
     }
-    const VfParams prm = vf_params(a, vf_request(a, r));
+    const int req = vf_request(a, r);
+    if (p == 0 && tid == 0) a.owner[r] = req;
+    const VfParams prm = vf_params(a, req);
     const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
     float* gmax = a.gmax + (size_t)r * a.groups + (size_t)p * (a.groups / S);
     VfSum t;
@@ -920,7 +923,7 @@ template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
     const int r = blockIdx.x;
-    const VfParams prm = vf_params(a, vf_request(a, r));
+    const VfParams prm = vf_params(a, a.owner[r]);
     if (!prm.cuts) return;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const float Tt = prm.T;
@@ -1027,7 +1030,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_mass_kernel(VerifyArgs a
     if (at >= rows) return;
     VfFlat& f = a.flat[at];
     const int r = f.row;
-    const VfParams prm = vf_params(a, vf_request(a, r));
+    const VfParams prm = vf_params(a, a.owner[r]);
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const VfRow w = vf_join(a, prm, r);
     const VfRule u = vf_rule(prm, w);
@@ -1089,21 +1092,25 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     __shared__ uint32_t last, shared_bound;
     const int S2 = a.S2, b = blockIdx.x / S2, p = blockIdx.x - b * S2, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const VfParams prm = vf_params(a, b);
-    const int first = a.cu[b], n = a.cu[b + 1] - first, K1 = a.K + 1;
-    if (first < 0 || n < 0 || n > a.K || first > a.D - n) {  // bounds that do not fit: no token
-        if (p == 0) {
-            for (int i = tid; i < K1; i += kVfThreads) {
-                a.tokens[(size_t)b * K1 + i] = -1;
-                a.logprobs[(size_t)b * K1 + i] = 0.0f;
-            }
-            if (tid == 0) a.accepted[b] = -1;
+    const int first = a.cu[b], end = a.cu[b + 1], n = (int)((uint32_t)end - (uint32_t)first), K1 = a.K + 1;
+    auto misfit = [&] {  // bounds that do not fit: no token
+        if (p > 0) return;
+        for (int i = tid; i < K1; i += kVfThreads) {
+            a.tokens[(size_t)b * K1 + i] = -1;
+            a.logprobs[(size_t)b * K1 + i] = 0.0f;
         }
-        return;
-    }
+        if (tid == 0) a.accepted[b] = -1;
+    };
+    if (first < 0 || end < first || n > a.K || end > a.D) return misfit();
+    // Rows that decreasing bounds make another request's have its statistics, and its cut or none: what
+    // this request would read of them need not have been written.
+    const int32_t* owner = a.owner + first + b;
+    const bool mine = (lane > n || owner[lane] == b) && owner[n] == b;  // (n <= 64)
     for (int i = wave; i <= n; i += kVfThreads / 64) {
         const VfRow w = vf_row(a, prm, first + b + i);
         if (lane == 0) rows[i] = w;
     }
+    if (wave_ballot(!mine)) return misfit();  // (every wave alike)
     __syncthreads();
     const T* x0 = static_cast<const T*>(a.x) + (size_t)(first + b) * a.xstride;
     const char* q0 = static_cast<const char*>(a.q) + (a.q ? (size_t)first * a.qstride * vf_esize(a.qdtype) : 0);
