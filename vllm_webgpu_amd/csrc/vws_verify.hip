@@ -272,6 +272,7 @@ struct VfCutShared {
     uint64_t out[4];
     float peaks[kVfPeaks];        // maxima, each of the groups of four threads
     uint32_t count, ngroups;
+    uint32_t slot;                // the row's place in VerifyArgs::flat
     float bound;
 };
 
@@ -975,9 +976,10 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
                 done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
             if (!done) {
                 // for verify_mass_kernel, or (the launch has many such rows) here
-                if (threadIdx.x == 0) sh.ngroups = ag_add32(a.flat_n, 1u);
+                // (a word of its own: others may still be reading the count on which vf_gather gave up)
+                if (threadIdx.x == 0) sh.slot = ag_add32(a.flat_n, 1u);
                 __syncthreads();
-                const uint32_t at = sh.ngroups;
+                const uint32_t at = sh.slot;
                 if (at < (uint32_t)min(a.R, kVfFlat)) {
                     VfFlat& f = a.flat[at];
                     for (int i = threadIdx.x; i < kVfBins; i += kVfCutThreads) f.hist[i] = 0ull;
