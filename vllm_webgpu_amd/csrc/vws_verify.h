@@ -15,12 +15,12 @@ constexpr int kVfMaxParts = 64;      // parts of a row: one lane each in the joi
 constexpr int kVfMaxDrafts = 64;     // VWS_MAX_DRAFTS: one lane each in the decision
 constexpr uint32_t kVfAcceptBase = 1u << 19;  // VWS_MAX_VOCAB: generated acceptance uniforms' tokens
 
-// A row's statistics.  One per part for rows that nothing cuts (sum: of exp2(x log2(e) / T - m2)
-// over the part), or the row's own (part 0) once verify_cut_kernel has cut it (m2: the maximum of
-// y, sum: the kept exponentials).
+// A row's statistics.  One per part for rows that nothing cuts (sum: of the part's exponentials relative to
+// its own largest logit), or the row's own (part 0) once verify_cut_kernel has cut it (m: the
+// maximum of y, sum: the kept exponentials).
 struct VfRec {
     uint64_t top;  // key of the largest logit << 32 | 0x7FFFFFFF - its lowest index; 0: all NaN
-    float m2;      // the maximum that `sum` is relative to
+    float m;
     float sum;
 };
 

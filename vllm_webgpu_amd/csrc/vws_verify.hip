@@ -13,22 +13,15 @@
 // verify_mass_kernel (launches with a top-p) adds up the masses of the others, each split over
 // workgroups; verify_token_kernel decides each request and races one of its rows.
 #include "vws_device.h"
+#include "vws_expsum.h"
 #include "vws_sampler.h"
 #include "vws_verify.h"
 
 namespace vws {
 
-constexpr float kVfInf = __builtin_inff();
-
-__device__ __forceinline__ float vf_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// 16 bytes at any element's address: rows of an odd vocabulary start unaligned.
-template <typename T> struct VfVec { typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2))); };
-template <> struct VfVec<float> { typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(4))); };
-
 template <typename T>
 __device__ __forceinline__ void vf_load_raw(const T* row, int vi, uint32_t (&w)[4]) {
-    const auto u = *reinterpret_cast<const typename VfVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec);
+    const auto u = *reinterpret_cast<const typename RowVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec);
     w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
 }
 template <typename T>
@@ -45,7 +38,7 @@ __device__ __forceinline__ void vf_load_any(const void* row, int dtype, int i, f
         const float* p = static_cast<const float*>(row) + i;
 #pragma unroll
         for (int g = 0; g < N / 4; ++g) {
-            const auto u = *reinterpret_cast<const VfVec<float>::U4*>(p + 4 * g);
+            const auto u = *reinterpret_cast<const RowVec<float>::U4*>(p + 4 * g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[4 * g + j] = u2f(u[j]);
         }
@@ -105,21 +98,11 @@ __device__ __forceinline__ VfParams vf_params(const VerifyArgs& a, int b) {
     return p;
 }
 
-__device__ __forceinline__ float vf_lane_xor(float v, int s) { return u2f(lane_xor(f2u(v), s)); }
-
-// A running (maximum, sum of exp2(x c - maximum)).
-struct VfSum {
-    float m = -kVfInf, s = 0.0f;
-    __device__ __forceinline__ void merge(float om, float os) {
-        const float n = __builtin_fmaxf(m, om), ref = n == -kVfInf ? 0.0f : n;
-        s = s * vf_exp2(m - ref) + os * vf_exp2(om - ref);
-        m = n;
-    }
-    __device__ __forceinline__ void wave_merge() {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) merge(vf_lane_xor(m, o), vf_lane_xor(s, o));
-    }
-};
+// log2(e) / T of a row that is not greedy (T may be infinite: the least number above 0, by which -inf
+// stays what it is).
+__device__ __forceinline__ float vf_c(const VfParams& p) {
+    return p.greedy ? 0.0f : __builtin_fmaxf(kExpLog2e / p.T, 0x1p-149f);
+}
 
 __device__ __forceinline__ uint64_t vf_pack(uint32_t key, int i) {
     return key ? ((uint64_t)key << 32) | (uint32_t)(0x7FFFFFFF - i) : 0ull;
@@ -162,9 +145,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     const int req = vf_request(a, r);
     if (p == 0 && tid == 0) a.owner[r] = req;
     const VfParams prm = vf_params(a, req);
-    const float c = prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T;
+    const float c = vf_c(prm);
     float* gmax = a.gmax + (size_t)r * a.groups + (size_t)p * (a.groups / S);
-    VfSum t;
+    ExpRun run(c);
     float best = __builtin_nanf("");  // the largest logit so far, and the first group that holds it
     int group = tid;
     for (int b = tid; b < nvec; b += U * kVfThreads) {
@@ -180,26 +163,24 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
         if (g == g && !(g <= best)) { best = g; group = b; }
         if (prm.cuts) gmax[(b / (U * kVfThreads)) * kVfThreads + tid] = g;
         if (prm.sums) {
-            const float n = __builtin_fmaxf(t.m, g * c), ref = n == -kVfInf ? 0.0f : n;
-            float acc[4] = {t.s * vf_exp2(t.m - ref), 0.0f, 0.0f, 0.0f};
+            float acc[4] = {run.raise(g, c), 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const bool in = b + u * kVfThreads < nvec;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float e = vf_exp2(__builtin_fmaf(v[u][j], c, -ref));
+                    const float e = es_exp2(__builtin_fmaf(v[u][j], c, -run.ref));
                     acc[j & 3] += in && e == e ? e : 0.0f;
                 }
             }
-            t.s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-            t.m = n;
+            run.s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
         }
     }
     // the largest logit's first place in its group, where it is the wave's (every lane's group read
     // again was a third of the part)
     float most = best;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, vf_lane_xor(most, o));
+    for (int o = 32; o > 0; o >>= 1) most = __builtin_fmaxf(most, es_lane_xor(most, o));
     uint64_t top = 0ull;
     if (best == most) {  // (not of a thread without vectors: NaN)
         for (int u = U - 1; u >= 0; --u) {
@@ -212,26 +193,51 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
                 if (v[j] == best) top = vf_pack(key_of(v[j]), lo + vi * VEC + j);
         }
     }
+    ExpSum t = run.close(c);
     const int i = nvec * VEC + tid;
     if (i < len) {
         const float x = Elem<T>::load1(row + i);
         top = vws_max64(top, vf_pack(key_of(x), lo + i));
-        if (prm.sums && x == x) t.merge(x * c, x > -kVfInf ? 1.0f : 0.0f);
+        if (prm.sums && x == x) t.merge(x, x > -kExpInf ? 1.0f : 0.0f, c);
     }
     top = wave_max_u64(top);
-    t.wave_merge();
+    t.wave_merge(c);
     if ((tid & 63) == 0) { red_top[wave] = top; red_m[wave] = t.m; red_s[wave] = t.s; }
     __syncthreads();
-    if (tid == 0) {
-        VfRec o;
-        VfSum s;
-        o.top = 0ull;
+    VfRec o{0ull, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kVfThreads / 64; ++w) {
-            o.top = vws_max64(o.top, red_top[w]);
-            s.merge(red_m[w], red_s[w]);
+    for (int w = 0; w < kVfThreads / 64; ++w) o.top = vws_max64(o.top, red_top[w]);
+    const float x_top = vf_value(o.top);
+    if (prm.sums && exp_far(x_top, c)) {
+        // far from zero: over y = fl(x / T), which the race and the masses take there (y spreads by its
+        // rounding); a second read of the part, from the caches
+        const float m = x_top / prm.T;
+        float s = 0.0f;
+        auto add = [&](float x) __attribute__((always_inline)) {
+            const float e = es_exp2((x / prm.T - m) * kExpLog2e);
+            s += e == e ? e : 0.0f;  // (NaN: x is, or x / T has no finite value)
+        };
+        for (int vi = tid; vi < nvec; vi += kVfThreads) {
+            float v[VEC];
+            vf_load<T>(row, vi, v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) add(v[j]);
         }
-        o.m2 = s.m;
+        if (i < len) add(Elem<T>::load1(row + i));
+        s = es_wave_sum(s);
+        if ((tid & 63) == 0) red_s[wave] = s;
+        __syncthreads();
+        if (tid == 0) {
+#pragma unroll
+            for (int w = 0; w < kVfThreads / 64; ++w) o.sum += red_s[w];
+            a.rec[(size_t)r * S + p] = o;
+        }
+        return;
+    }
+    if (tid == 0) {
+        ExpSum s;
+#pragma unroll
+        for (int w = 0; w < kVfThreads / 64; ++w) s.merge(red_m[w], red_s[w], c);
         o.sum = s.s;
         a.rec[(size_t)r * S + p] = o;
     }
@@ -746,10 +752,10 @@ __device__ __forceinline__ bool vf_gather(const VerifyArgs& a, const float* gmax
 // The maxima of a row's groups, joined into kVfPeaks.
 template <typename T>
 __device__ __forceinline__ void vf_join_peaks(const VerifyArgs& a, const float* gmax, VfCutShared& sh) {
-    float m = -kVfInf;
+    float m = -kExpInf;
     vf_each_group<T>(a, gmax, [&](float g, int, int) { m = __builtin_fmaxf(m, g); });
-    m = __builtin_fmaxf(m, vf_lane_xor(m, 1));
-    m = __builtin_fmaxf(m, vf_lane_xor(m, 2));
+    m = __builtin_fmaxf(m, es_lane_xor(m, 1));
+    m = __builtin_fmaxf(m, es_lane_xor(m, 2));
     static_assert(kVfCutThreads / kVfPeaks == 4, "a maximum for every four threads");
     if ((threadIdx.x & 3) == 0) sh.peaks[threadIdx.x / 4] = m;
     __syncthreads();
@@ -771,7 +777,7 @@ __device__ __forceinline__ float vf_peak(VfCutShared& sh, int n) {
             for (int i = 0; i < kVfPeaks / kWave; ++i) c += __popcll(wave_ballot(k[i] >= cand));
             if (c >= n) ans = cand;
         }
-        if (threadIdx.x == 0) sh.bound = ans >= 0x00800000u ? val_of(ans) : -kVfInf;  // (below: -inf or none)
+        if (threadIdx.x == 0) sh.bound = ans >= 0x00800000u ? val_of(ans) : -kExpInf;  // (below: -inf or none)
     }
     __syncthreads();
     return sh.bound;
@@ -781,24 +787,22 @@ struct VfRow {
     uint64_t top, cut;
     float m, sum;
     bool sure;  // greedy, or the maximum is not finite: the row's distribution is its argmax
+    bool far;   // exp_far of the maximum
 };
 
 // Row r's statistics from its parts, in every lane of the calling wave.
 __device__ __forceinline__ VfRow vf_join(const VerifyArgs& a, const VfParams& prm, int r) {
-    VfRec v{0ull, -kVfInf, 0.0f};
+    VfRec v{0ull, 0.0f, 0.0f};
     if (lane_id() < a.S) v = a.rec[(size_t)r * a.S + lane_id()];
-    VfSum t;
-    t.m = v.m2;
-    t.s = v.sum;
     VfRow o;
     o.top = wave_max_u64(v.top);
     o.cut = 0ull;
-    const float x = vf_value(o.top);
+    const float x = vf_value(o.top), part = vf_value(v.top), c = vf_c(prm);
     o.m = prm.greedy ? x : x / prm.T;
-    o.sure = prm.greedy || !(__builtin_fabsf(o.m) < kVfInf);
-    t.wave_merge();
-    // relative to x c - maximum, whose rounding leaves the largest element's own term off 1
-    o.sum = t.s * vf_exp2(-__builtin_fmaf(x, prm.greedy ? 0.0f : 0x1.715476p+0f / prm.T, -t.m));
+    o.sure = prm.greedy || !(__builtin_fabsf(o.m) < kExpInf);
+    o.far = exp_far(x, c);
+    const float e = es_exp2(o.far ? (part / prm.T - o.m) * kExpLog2e : (part - x) * c);
+    o.sum = es_wave_sum(v.sum > 0.0f ? v.sum * e : 0.0f);
     return o;
 }
 
@@ -887,7 +891,7 @@ __device__ __forceinline__ VfRule vf_rule(const VfParams& prm, const VfRow& w) {
     u.m = w.m;
     u.q32 = 1.0f - prm.top_p;
     u.k = prm.k;
-    u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kVfInf;
+    u.lp_min = prm.min_p > 0.0f ? log_det(prm.min_p < 1.0f ? prm.min_p : 1.0f) : -kExpInf;
     return u;
 }
 
@@ -904,7 +908,7 @@ __device__ __forceinline__ VfCut vf_solve_row(const T* row, int V, float Tt, VfC
 __device__ __forceinline__ void vf_write(const VerifyArgs& a, int r, const VfRow& w, const VfCut& o) {
     VfRec c;
     c.top = w.top;
-    c.m2 = w.m;
+    c.m = w.m;
     c.sum = (float)o.kept * 0x1p-44f;
     a.rec[(size_t)r * a.S] = c;
     a.cut[r] = o.cut;
@@ -952,14 +956,14 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
             o.cut = vf_block_max(last, sh);
             o.kept = 1ull << 44;
             done = true;
-        } else if (u.k > 0 || u.lp_min > -kVfInf) {
-            float t = -kVfInf;
+        } else if (u.k > 0 || u.lp_min > -kExpInf) {
+            float t = -kExpInf;
             if (u.k > 0 && u.k <= kVfPeakMost) t = below(vf_peak(sh, u.k));
-            if (u.lp_min > -kVfInf) {
+            if (u.lp_min > -kExpInf) {
                 const float y = u.m + u.lp_min;
                 t = __builtin_fmaxf(t, Tt * (y - (__builtin_fabsf(u.m) - u.lp_min) * 0x1p-20f) - tiny);
             }
-            const bool k_listed = u.k == 0 || t > -kVfInf;
+            const bool k_listed = u.k == 0 || t > -kExpInf;
             if (k_listed && vf_gather<T>(a, gmax, row, Tt, sh, t)) {
                 const int n = (int)sh.count;
                 o = n <= kVfSmall ? vf_solve_small(sh, u, n) : vf_solve(VfListIter{sh.list, n}, sh, u, (uint64_t)n);
@@ -968,11 +972,13 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a)
         } else {
             // top-p alone.  The first pass's sum is off by at most 2^-22 (2 |m| + 64) of itself: y and
             // y - m round to 2^-24 of |m| + 31 (beyond which a mass is 0), the exponent's fma and
-            // its constant likewise, the exponential and the sums by a few 2^-24
-            const double W = (double)w.sum * 0x1p44, eps = 0x1p-22 * (2.0 * (double)__builtin_fabsf(u.m) + 64.0);
+            // its constant likewise, the exponential and the sums by a few 2^-24.  A far row's is
+            // over the masses' own y.
+            const double W = (double)w.sum * 0x1p44, am = w.far ? 0.0 : (double)__builtin_fabsf(u.m);
+            const double eps = 0x1p-22 * (2.0 * am + 64.0);
             // the 100 or so logits above the 84th of 256 maxima
             const float t = below(vf_peak(sh, 84));
-            if (t > -kVfInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
+            if (t > -kExpInf && vf_gather<T>(a, gmax, row, Tt, sh, t) && sh.count <= (uint32_t)kVfSmall)
                 done = listed = vf_solve_top(sh, u, (int)sh.count, W * (1.0 - eps), W * (1.0 + eps), &o);
             if (!done) {
                 // for verify_mass_kernel, or (the launch has many such rows) here
@@ -1068,9 +1074,9 @@ __device__ __forceinline__ VfRow vf_row(const VerifyArgs& a, const VfParams& prm
     VfRow o;
     o.top = v.top;
     o.cut = a.cut[r];
-    o.m = v.m2;
+    o.m = v.m;
     o.sum = v.sum;
-    o.sure = !(__builtin_fabsf(v.m2) < kVfInf);
+    o.sure = !(__builtin_fabsf(v.m) < kExpInf);
     return o;
 }
 
@@ -1107,12 +1113,12 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     // Rows that decreasing bounds make another request's have its statistics, and its cut or none: what
     // this request would read of them need not have been written.
     const int32_t* owner = a.owner + first + b;
-    const bool mine = (lane > n || owner[lane] == b) && owner[n] == b;  // (n <= 64)
+    const int of = owner[min(lane, n)], of_last = owner[n];  // (n <= 64)
     for (int i = wave; i <= n; i += kVfThreads / 64) {
         const VfRow w = vf_row(a, prm, first + b + i);
         if (lane == 0) rows[i] = w;
     }
-    if (wave_ballot(!mine)) return misfit();  // (every wave alike)
+    if (wave_ballot(of != b || of_last != b)) return misfit();  // (every wave alike)
     __syncthreads();
     const T* x0 = static_cast<const T*>(a.x) + (size_t)(first + b) * a.xstride;
     const char* q0 = static_cast<const char*>(a.q) + (a.q ? (size_t)first * a.qstride * vf_esize(a.qdtype) : 0);
@@ -1152,10 +1158,12 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
         // The largest key so far, of the workgroup, is a bound: a key is w / E with E = -ln u >= 1 - u
         // >= 2^-24, so an element whose w (from the hardware's exp2, with its error on top) stays
         // below bound (1 - u) cannot win, and a logit below tl cannot whatever its uniform.
-        const float c = 0x1.715476p+0f / prm.T, x_top = vf_value(w.top), m2 = x_top * c;
-        const float eps = 1.0f + 0x1p-22f * (2.0f * __builtin_fabsf(w.m) + 64.0f), scale = (q ? inv : 1.0f) * eps;
-        const float y_cut = w.cut ? val_of((uint32_t)(w.cut >> 32)) : -kVfInf;
-        const float x_cut = w.cut ? prm.T * (y_cut - __builtin_fabsf(y_cut) * 0x1p-20f) - prm.T * 0x1p-120f : -kVfInf;
+        // (Far from zero fl(x_top c) says nothing of that: an infinite scale, nothing is left out.)
+        const float c = vf_c(prm), x_top = vf_value(w.top), m2 = x_top * c;
+        const float eps = 1.0f + 0x1p-22f * (2.0f * __builtin_fabsf(w.m) + 64.0f);
+        const float scale = exp_far(x_top, c) ? kExpInf : (q ? inv : 1.0f) * eps;
+        const float y_cut = w.cut ? val_of((uint32_t)(w.cut >> 32)) : -kExpInf;
+        const float x_cut = w.cut ? prm.T * (y_cut - __builtin_fabsf(y_cut) * 0x1p-20f) - prm.T * 0x1p-120f : -kExpInf;
         float bound = 0.0f;
         auto add = [&](int i, float x, float qi, float ui) {
             const float y = x / prm.T;
@@ -1166,11 +1174,11 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
             const float key = wt / (0.0f - log_det(ui));
             if (key >= 0.0f) {
                 best = vws_max64(best, vf_pack(f2u(key) + 1u, i));
-                if (key < kVfInf) bound = __builtin_fmaxf(bound, key * 0.9999f);
+                if (key < kExpInf) bound = __builtin_fmaxf(bound, key * 0.9999f);
             }
         };
         auto can_win = [&](float x, float qi, float ui) {
-            const float e = vf_exp2(__builtin_fmaf(x, c, -m2)) * scale;
+            const float e = es_exp2(__builtin_fmaf(x, c, -m2)) * scale;
             return !((q ? e - qi : e) < bound * (1.0f - ui)) || !(ui < 1.0f);  // (true for NaN)
         };
         // a cut row whose kept tokens are listed: they alone, by the first part
