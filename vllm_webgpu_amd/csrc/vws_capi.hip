@@ -1017,7 +1017,6 @@ int vws_verify_drafts(const vws_verify_args* a) {
     char* base = static_cast<char*>(a->workspace);
     k.rec = reinterpret_cast<VfRec*>(base + w.rec);
     k.gmax = reinterpret_cast<float*>(base + w.gmax);
-    k.owner = reinterpret_cast<int32_t*>(base + w.owner);
     k.cut = reinterpret_cast<uint64_t*>(base + w.cut);
     k.kept = reinterpret_cast<int32_t*>(base + w.kept);
     k.flat_n = reinterpret_cast<uint32_t*>(base + w.flat_n);

@@ -16,12 +16,12 @@ constexpr int kVfMaxDrafts = 64;     // VWS_MAX_DRAFTS: one lane each in the dec
 constexpr uint32_t kVfAcceptBase = 1u << 19;  // VWS_MAX_VOCAB: generated acceptance uniforms' tokens
 
 // A row's statistics.  One per part for rows that nothing cuts (sum: of the part's exponentials relative to
-// its own largest logit), or the row's own (part 0) once verify_cut_kernel has cut it (m: the
-// maximum of y, sum: the kept exponentials).
+// its own largest logit), or the row's own (part 0) once verify_cut_kernel has cut it (sum: of the kept
+// exponentials).
 struct VfRec {
-    uint64_t top;  // key of the largest logit << 32 | 0x7FFFFFFF - its lowest index; 0: all NaN
-    float m;
+    uint64_t top;   // key of the largest logit << 32 | 0x7FFFFFFF - its lowest index; 0: all NaN
     float sum;
+    int32_t owner;  // the request whose parameters cut the row
 };
 
 constexpr int kVfBins = 2048;      // bins of a row's masses
@@ -62,7 +62,6 @@ struct VerifyArgs {
     VfRec* rec;                  // [R, S]
     float* gmax;                 // [R, groups] maxima of groups of vectors, of rows that are cut; or null
     int groups;                  // of a row
-    int32_t* owner;              // [R] the request whose parameters cut the row
     uint64_t* cut;               // [R] kept: (key(y) << 32 | index) >= cut
     int32_t* kept;               // [R, 1 + kVfKept] of cut rows: how many are kept (-1: not listed), and they
     uint32_t* flat_n;            // rows whose masses verify_mass_kernel adds up; cleared by the statistics' launch
@@ -82,7 +81,7 @@ inline int vf_groups(int S, int part_len, int vec) {
 constexpr int kVfKept = 511;         // tokens of a cut row that the race takes from a list
 
 struct VfLayout {
-    size_t rec, gmax, owner, cut, kept, flat_n, flat, best, ctr, total;
+    size_t rec, gmax, cut, kept, flat_n, flat, best, ctr, total;
 };
 
 inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
@@ -90,7 +89,6 @@ inline VfLayout vf_layout(int R, int B, int S, int S2, int groups) {
     size_t off = align256(sizeof(CoopState));  // every workspace starts with the fixed region
     w.rec = off;   off = align256(off + sizeof(VfRec) * (size_t)R * S);
     w.gmax = off;  off = align256(off + sizeof(float) * (size_t)R * groups);
-    w.owner = off; off = align256(off + sizeof(int32_t) * (size_t)R);
     w.cut = off;   off = align256(off + sizeof(uint64_t) * (size_t)R);
     w.kept = off;  off = align256(off + sizeof(int32_t) * (size_t)R * (1 + kVfKept));
     w.flat_n = off; off = align256(off + sizeof(uint32_t));

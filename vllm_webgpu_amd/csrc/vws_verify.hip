@@ -65,7 +65,7 @@ __device__ __forceinline__ size_t vf_esize(int dtype) { return dtype == VWS_DTYP
 
 // The request of row r: the last whose first row (cu[b] + b) lies at or before it.  64 bounds at a
 // time, so two loads for up to 4096 requests; every lane of the calling wave returns it.  Bounds that
-// decrease can name a row twice: this is the one request that it is taken for, VerifyArgs::owner.
+// decrease can name a row twice: this is the one request that it is taken for, VfRec::owner.
 __device__ __forceinline__ int vf_request(const VerifyArgs& a, int r) {
     int lo = 0, n = a.B;
     while (n > 1) {
@@ -142,9 +142,8 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
         if (r < a.B) a.ctr[r] = 0u;  // (R >= B)
         if (r == 0) *a.flat_n = 0u;
     }
-    const int req = vf_request(a, r);
-    if (p == 0 && tid == 0) a.owner[r] = req;
-    const VfParams prm = vf_params(a, req);
+    const int owner = vf_request(a, r);
+    const VfParams prm = vf_params(a, owner);
     const float c = vf_c(prm);
     float* gmax = a.gmax + (size_t)r * a.groups + (size_t)p * (a.groups / S);
     ExpRun run(c);
@@ -204,7 +203,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     t.wave_merge(c);
     if ((tid & 63) == 0) { red_top[wave] = top; red_m[wave] = t.m; red_s[wave] = t.s; }
     __syncthreads();
-    VfRec o{0ull, 0.0f, 0.0f};
+    VfRec o{0ull, 0.0f, owner};
 #pragma unroll
     for (int w = 0; w < kVfThreads / 64; ++w) o.top = vws_max64(o.top, red_top[w]);
     const float x_top = vf_value(o.top);
@@ -786,15 +785,17 @@ __device__ __forceinline__ float vf_peak(VfCutShared& sh, int n) {
 struct VfRow {
     uint64_t top, cut;
     float m, sum;
+    int owner;  // VfRec::owner
     bool sure;  // greedy, or the maximum is not finite: the row's distribution is its argmax
     bool far;   // exp_far of the maximum
 };
 
 // Row r's statistics from its parts, in every lane of the calling wave.
 __device__ __forceinline__ VfRow vf_join(const VerifyArgs& a, const VfParams& prm, int r) {
-    VfRec v{0ull, 0.0f, 0.0f};
+    VfRec v{0ull, 0.0f, 0};
     if (lane_id() < a.S) v = a.rec[(size_t)r * a.S + lane_id()];
     VfRow o;
+    o.owner = (int)__builtin_amdgcn_readfirstlane((uint32_t)v.owner);
     o.top = wave_max_u64(v.top);
     o.cut = 0ull;
     const float x = vf_value(o.top), part = vf_value(v.top), c = vf_c(prm);
@@ -908,7 +909,7 @@ __device__ __forceinline__ VfCut vf_solve_row(const T* row, int V, float Tt, VfC
 __device__ __forceinline__ void vf_write(const VerifyArgs& a, int r, const VfRow& w, const VfCut& o) {
     VfRec c;
     c.top = w.top;
-    c.m = w.m;
+    c.owner = w.owner;
     c.sum = (float)o.kept * 0x1p-44f;
     a.rec[(size_t)r * a.S] = c;
     a.cut[r] = o.cut;
@@ -928,7 +929,7 @@ template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
     const int r = blockIdx.x;
-    const VfParams prm = vf_params(a, a.owner[r]);
+    const VfParams prm = vf_params(a, a.rec[(size_t)r * a.S].owner);
     if (!prm.cuts) return;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const float Tt = prm.T;
@@ -1038,7 +1039,7 @@ __global__ __launch_bounds__(kVfCutThreads) void verify_mass_kernel(VerifyArgs a
     if (at >= rows) return;
     VfFlat& f = a.flat[at];
     const int r = f.row;
-    const VfParams prm = vf_params(a, a.owner[r]);
+    const VfParams prm = vf_params(a, a.rec[(size_t)r * a.S].owner);
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const VfRow w = vf_join(a, prm, r);
     const VfRule u = vf_rule(prm, w);
@@ -1074,9 +1075,10 @@ __device__ __forceinline__ VfRow vf_row(const VerifyArgs& a, const VfParams& prm
     VfRow o;
     o.top = v.top;
     o.cut = a.cut[r];
-    o.m = v.m;
+    o.m = vf_value(v.top) / prm.T;
     o.sum = v.sum;
-    o.sure = !(__builtin_fabsf(v.m) < kExpInf);
+    o.owner = v.owner;
+    o.sure = !(__builtin_fabsf(o.m) < kExpInf);
     return o;
 }
 
@@ -1110,15 +1112,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
         if (tid == 0) a.accepted[b] = -1;
     };
     if (first < 0 || end < first || n > a.K || end > a.D) return misfit();
-    // Rows that decreasing bounds make another request's have its statistics, and its cut or none: what
-    // this request would read of them need not have been written.
-    const int32_t* owner = a.owner + first + b;
-    const int of = owner[min(lane, n)], of_last = owner[n];  // (n <= 64)
     for (int i = wave; i <= n; i += kVfThreads / 64) {
         const VfRow w = vf_row(a, prm, first + b + i);
         if (lane == 0) rows[i] = w;
     }
-    if (wave_ballot(of != b || of_last != b)) return misfit();  // (every wave alike)
     __syncthreads();
     const T* x0 = static_cast<const T*>(a.x) + (size_t)(first + b) * a.xstride;
     const char* q0 = static_cast<const char*>(a.q) + (a.q ? (size_t)first * a.qstride * vf_esize(a.qdtype) : 0);
@@ -1145,6 +1142,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
             }
         }
     }
+    // Rows that decreasing bounds make another request's have its statistics, and its cut or none: what
+    // this request would read of them from here on need not have been written.  (n <= 64; every wave alike)
+    if (wave_ballot(rows[min(lane, n)].owner != b || rows[n].owner != b)) return misfit();
     const uint64_t refused = wave_ballot(!ok && lane < n);
     const int acc = refused ? (int)__builtin_ctzll(refused) : n;
     const VfRow w = rows[acc];
