@@ -13,9 +13,9 @@ constexpr int kDsMaxK = 256;        // teacher entries of a row, one per thread 
 constexpr int kDsMaxParts = 64;     // parts of a row: one lane each in the join
 constexpr int kDsRowStats = 8;      // floats of a row's statistics (DistillStat)
 
-// What the backward needs of a row, in powers of two (z2 = x * log2(e) / T):
-// student elements outside the teacher's entries get e(z2 - ref) * coef, teacher entries
-// e(z2 - max) * inv_total - P (P: DistillArgs::entry_p), both times weight * upstream / T.
+// What the backward needs of a row, e(x) = exp2(x log2(e) / T): student elements outside the teacher's
+// entries get e(x - ref) * coef, teacher entries e(x - max) * inv_total - P (P: DistillArgs::entry_p), both
+// times weight * upstream / T.
 enum DistillStat { kDsRef = 0, kDsCoef = 1, kDsMax = 2, kDsInvTotal = 3, kDsLive = 4 };
 
 struct DistillArgs {
@@ -37,7 +37,7 @@ struct DistillArgs {
     float* loss;            // [N]
     float* stats;           // [N, kDsRowStats]
     float* entry_p;         // [N, K] probability of each id at its first entry, -1 elsewhere
-    uint64_t* rec;          // [N * S] parts' (max, sum), S > 1
+    uint64_t* rec;          // [N * S] parts' ExpSum, S > 1
     uint32_t* ctr;          // [N] parts arrived (left at zero), S > 1
 };
 

@@ -8,26 +8,24 @@
 //   bucket:      p = exp(l), r = 1 - sum p, s = sum of q outside the entries;
 //                                                   L = w (sum_k ... + r log(r / s))
 //                dL/dx_j = w / T (q_j - p_j) at the entries, w / T q_j (1 - r / s) elsewhere.
-// Exponentials are powers of two of z2 = x * log2(e) / T relative to a maximum; one fma and one
-// exp2 per logit.  s is the sum over the rest, never 1 - sum of the entries (which cancels when
+// Exponentials are powers of two of x * log2(e) / T relative to a maximum; one fma and one exp2 per logit
+// (vws_expsum.h).  Rows whose maximum is far from zero in those units (a mask's value, mostly) take
+// differences from it instead.  s is the sum over the rest, never 1 - sum of the entries (which cancels when
 // the student is sure), and the rest keeps its own maximum, so that log(s) and q_j / s stay finite
 // however far the rest lies below the entries: q_j (1 - r / s) = e_j (s - r) / Z_rest with e_j and
 // Z_rest relative to the rest's maximum.
 #include "vws_device.h"
 #include "vws_distill.h"
+#include "vws_expsum.h"
 #include "vws_sampler.h"
 
 namespace vws {
 
-constexpr float kDsInf = __builtin_inff();
 constexpr float kLn2 = 0x1.62e43p-1f;
 
-__device__ __forceinline__ float ds_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// 16 bytes at any element's address: rows of an odd vocabulary start unaligned.
+// Widened logits back to a row's words.
 template <typename T> struct DsVec;
 template <> struct DsVec<float> {
-    typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(4)));
     static constexpr uint32_t kNegInf = 0xFF800000u;
     static __device__ __forceinline__ void set_neg_inf(uint32_t (&w)[4], int j) { w[j] = kNegInf; }
     static __device__ __forceinline__ void pack(const float* v, uint32_t (&w)[4]) {
@@ -37,7 +35,6 @@ template <> struct DsVec<float> {
     static __device__ __forceinline__ float narrow(float v) { return v; }
 };
 template <> struct DsVec<uint16_t> {
-    typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2)));
     static constexpr uint32_t kNegInf = 0xFF80FF80u;
     static __device__ __forceinline__ void set_neg_inf(uint32_t (&w)[4], int j) {
         w[j >> 1] = (j & 1) ? (w[j >> 1] & 0xFFFFu) | 0xFF800000u : (w[j >> 1] & 0xFFFF0000u) | 0xFF80u;
@@ -49,7 +46,6 @@ template <> struct DsVec<uint16_t> {
     }
 };
 template <> struct DsVec<_Float16> {
-    typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2)));
     static constexpr uint32_t kNegInf = 0xFC00FC00u;
     static __device__ __forceinline__ void set_neg_inf(uint32_t (&w)[4], int j) {
         w[j >> 1] = (j & 1) ? (w[j >> 1] & 0xFFFFu) | 0xFC000000u : (w[j >> 1] & 0xFFFF0000u) | 0xFC00u;
@@ -66,55 +62,28 @@ template <> struct DsVec<_Float16> {
 // (vi: a 32-bit offset, at most 2 MB, on the row's pointer)
 template <typename T>
 __device__ __forceinline__ void ds_load(const T* row, int vi, uint32_t (&w)[4]) {
-    const auto u = *reinterpret_cast<const typename DsVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi);
+    const auto u = *reinterpret_cast<const typename RowVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi);
     w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
 }
 // The same for logits that are read once: they leave the caches to the gradients on their way out.
 template <typename T>
 __device__ __forceinline__ void ds_load_once(const T* row, int vi, uint32_t (&w)[4]) {
     const auto u = __builtin_nontemporal_load(
-        reinterpret_cast<const typename DsVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi));
+        reinterpret_cast<const typename RowVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi));
     w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
 }
 // (not temporal: what the forward has read stays in the last-level cache for the backward)
 template <typename T>
 __device__ __forceinline__ void ds_store(T* row, int vi, const uint32_t (&w)[4]) {
-    typename DsVec<T>::U4 u;
+    typename RowVec<T>::U4 u;
     u[0] = w[0]; u[1] = w[1]; u[2] = w[2]; u[3] = w[3];
-    __builtin_nontemporal_store(u, reinterpret_cast<typename DsVec<T>::U4*>(reinterpret_cast<char*>(row) + 16u * (uint32_t)vi));
+    __builtin_nontemporal_store(u, reinterpret_cast<typename RowVec<T>::U4*>(reinterpret_cast<char*>(row) + 16u * (uint32_t)vi));
 }
-
-__device__ __forceinline__ float ds_lane_xor(float v, int s) { return u2f(lane_xor(f2u(v), s)); }
-__device__ __forceinline__ float ds_wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = __builtin_fmaxf(v, ds_lane_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float ds_wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += ds_lane_xor(v, o);
-    return v;
-}
-
-// A running (maximum, sum of exp2(z2 - maximum)); the empty one is (-inf, 0).  NaN and +inf make
-// the sum NaN, as log-softmax has it.
-struct DsSum {
-    float m = -kDsInf, s = 0.0f;
-    __device__ __forceinline__ void merge(float om, float os) {
-        const float n = __builtin_fmaxf(m, om), ref = n == -kDsInf ? 0.0f : n;
-        s = s * ds_exp2(m - ref) + os * ds_exp2(om - ref);
-        m = n;
-    }
-    __device__ __forceinline__ void wave_merge() {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) merge(ds_lane_xor(m, o), ds_lane_xor(s, o));
-    }
-};
 
 // Adds U vectors (widened) to a thread's running sum: their maximum first, then one exponential
-// each and one for the rescaling.
+// each and one for the rescaling.  NaN and +inf make the sum NaN, as log-softmax has it.
 template <typename T, int U>
-__device__ __forceinline__ void ds_add(DsSum& t, const uint32_t (&w)[U][4], float c) {
+__device__ __forceinline__ void ds_add(ExpRun& t, const uint32_t (&w)[U][4], float c) {
     constexpr int VEC = Elem<T>::kVec;
     float v[U][VEC];
 #pragma unroll
@@ -124,18 +93,17 @@ __device__ __forceinline__ void ds_add(DsSum& t, const uint32_t (&w)[U][4], floa
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) g = __builtin_fmaxf(g, v[u][j]);
-    const float n = __builtin_fmaxf(t.m, g * c), ref = n == -kDsInf ? 0.0f : n;
-    float a[4] = {t.s * ds_exp2(t.m - ref), 0.0f, 0.0f, 0.0f};
+    float a[4] = {t.raise(g, c), 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) a[j & 3] += ds_exp2(__builtin_fmaf(v[u][j], c, -ref));
+        for (int j = 0; j < VEC; ++j) a[j & 3] += es_exp2(__builtin_fmaf(v[u][j], c, -t.ref));
     t.s = (a[0] + a[1]) + (a[2] + a[3]);
-    t.m = n;
 }
 
-__device__ __forceinline__ void ds_add1(DsSum& t, float z) {
-    t.merge(z, z == z && z < kDsInf ? (z == -kDsInf ? 0.0f : 1.0f) : __builtin_nanf(""));
+__device__ __forceinline__ void ds_add1(ExpRun& t, float x, float c) {
+    const float had = t.raise(x, c);
+    t.s = had + es_exp2(__builtin_fmaf(x, c, -t.ref));
 }
 
 // Bitmap of a part's elements that are teacher entries, from its first element on.
@@ -166,7 +134,7 @@ __device__ __forceinline__ void ds_drop(const uint32_t* bm, int vi, uint32_t (&w
 // A part's running sum: elements [0, len) of `row`, without those whose bit is set (BUCKET).  The next
 // four vectors' loads are issued before these are used; the first before `ready` (the bitmap).
 template <typename T, bool BUCKET, typename F>
-__device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const uint32_t* bm, F ready) {
+__device__ __forceinline__ ExpSum ds_stream(const T* row, int len, float c, const uint32_t* bm, F ready) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
     const int nvec = len / VEC, tid = threadIdx.x;
     uint32_t next[U][4];
@@ -176,7 +144,7 @@ __device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const
     };
     if (nvec > 0) fetch(tid);
     ready();
-    DsSum t;
+    ExpRun t(c);
     for (int b = tid; b < nvec; b += U * kDsThreads) {
         uint32_t w[U][4];
 #pragma unroll
@@ -197,8 +165,27 @@ __device__ __forceinline__ DsSum ds_stream(const T* row, int len, float c, const
         ds_add<T, U>(t, w, c);
     }
     const int i = nvec * VEC + tid;
-    if (i < len && !(BUCKET && ((bm[i >> 5] >> (i & 31)) & 1u))) ds_add1(t, Elem<T>::load1(row + i) * c);
-    return t;
+    if (i < len && !(BUCKET && ((bm[i >> 5] >> (i & 31)) & 1u))) ds_add1(t, Elem<T>::load1(row + i), c);
+    return t.close(c);
+}
+
+// This thread's share of the sum of a part whose maximum m is far from zero, over differences from it.
+template <typename T, bool BUCKET>
+__device__ __forceinline__ float ds_far_sum(const T* row, int len, float c, const uint32_t* bm, float m) {
+    constexpr int VEC = Elem<T>::kVec;
+    const int nvec = len / VEC, i = nvec * VEC + (int)threadIdx.x;
+    float s = 0.0f;
+    for (int vi = threadIdx.x; vi < nvec; vi += kDsThreads) {
+        uint32_t w[4];
+        ds_load<T>(row, vi, w);
+        if (BUCKET) ds_drop<T>(bm, vi, w);
+        float v[VEC];
+        Elem<T>::from_words(w[0], w[1], w[2], w[3], v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += es_exp2((v[j] - m) * c);
+    }
+    if (i < len && !(BUCKET && ((bm[i >> 5] >> (i & 31)) & 1u))) s += es_exp2((Elem<T>::load1(row + i) - m) * c);
+    return s;
 }
 
 // A row's teacher entry k, one for each of a workgroup's first K threads (id -1: none).
@@ -208,7 +195,7 @@ struct DsEntry {
 };
 __device__ __forceinline__ DsEntry ds_entry(const DistillArgs& a, int r) {
     const int k = threadIdx.x;
-    DsEntry e{-1, -kDsInf, 0.0f};
+    DsEntry e{-1, -kExpInf, 0.0f};
     if (k < a.K) {
         e.id = a.ids[(size_t)r * a.ids_stride + k];
         e.l = a.lp[(size_t)r * a.lp_stride + k];
@@ -260,50 +247,65 @@ struct DsRow {
     float p;                          // P of this thread's entry (-1: none)
 };
 
-// A row's loss and statistics, from each wave's merged sum over its rest (BUCKET) or all of it.  Every
-// thread of a workgroup of NW waves calls; `slot`: where this thread's entry was inserted, since
-// the last barrier or before.  Two barriers.
-template <typename T, bool BUCKET, int NW>
-__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, DsSum t, float w, DsEntry e, int slot,
+// Each wave's merged sum, and all of them (after a barrier).
+__device__ __forceinline__ void ds_put(DsShared& sh, const ExpSum& t) {
+    if ((threadIdx.x & 63) == 0) { sh.wm[threadIdx.x >> 6] = t.m; sh.ws[threadIdx.x >> 6] = t.s; }
+}
+template <int NW>
+__device__ __forceinline__ ExpSum ds_get(const DsShared& sh, float c) {
+    ExpSum t;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) t.m = __builtin_fmaxf(t.m, sh.wm[i]);
+    const float ref = t.m == -kExpInf ? 0.0f : t.m;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) t.s += sh.ws[i] * es_exp2((sh.wm[i] - ref) * c);
+    return t;
+}
+
+// The entries' ids and their maxima, for ds_finish after a barrier: of the student over its entries
+// (BUCKET), or of the teacher.
+template <bool BUCKET>
+__device__ __forceinline__ void ds_put_entries(const DistillArgs& a, const DsEntry& e, DsShared& sh) {
+    const int k = threadIdx.x, wave = k >> 6;
+    const float logp = e.l * a.inv_T;
+    // (a NaN makes the row NaN by way of the sums)
+    const float mine = e.id >= 0 ? (BUCKET ? e.x : (logp != logp ? kExpInf : logp)) : -kExpInf;
+    if (wave < kDsMaxK / 64) {
+        const float m = es_wave_max(mine);
+        if ((k & 63) == 0) sh.top[wave] = m;
+    }
+    if (k < a.K) sh.id[k] = e.id;
+}
+
+// A row's loss and statistics, from its sum over the rest (BUCKET) or all of it and what ds_put_entries left.
+// Every thread of the workgroup calls; `slot`: where this thread's entry was inserted, since the last
+// barrier or before.  One barrier.
+template <typename T, bool BUCKET>
+__device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const ExpSum& rest, float w, DsEntry e, int slot,
                                            const DsHash& hash, DsShared& sh) {
     constexpr int EW = kDsMaxK / 64;
     const int k = threadIdx.x, K = a.K, wave = k >> 6;
     const bool valid = e.id >= 0, lead = (k & 63) == 0;
-    // first the maxima: of the student over its entries, or of the teacher
-    const float z = e.x * a.c, logp = BUCKET ? e.l : e.l * a.inv_T;
-    // (a NaN makes the row NaN by way of the sums)
-    const float mine = valid ? (BUCKET ? z : (logp != logp ? kDsInf : logp)) : -kDsInf;
-    if (lead) { sh.wm[wave] = t.m; sh.ws[wave] = t.s; }
-    if (wave < EW) {
-        const float m = ds_wave_max(mine);
-        if (lead) sh.top[wave] = m;
-    }
-    if (k < K) sh.id[k] = e.id;
-    __syncthreads();
-    DsSum rest;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) rest.m = __builtin_fmaxf(rest.m, sh.wm[i]);
-    const float ref = rest.m == -kDsInf ? 0.0f : rest.m;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) rest.s += sh.ws[i] * ds_exp2(sh.wm[i] - ref);
-    float top = -kDsInf;
+    const float logp = BUCKET ? e.l : e.l * a.inv_T;
+    const float ref = rest.m == -kExpInf ? 0.0f : rest.m;
+    float top = -kExpInf;
 #pragma unroll
     for (int i = 0; i < EW; ++i) top = __builtin_fmaxf(top, sh.top[i]);
-    const float M = BUCKET ? __builtin_fmaxf(rest.m, top) : rest.m, mref = M == -kDsInf ? 0.0f : M;
+    const float M = BUCKET ? __builtin_fmaxf(rest.m, top) : rest.m, mref = M == -kExpInf ? 0.0f : M;
     // entries that share an id: the first takes their probability together
     const bool first = valid && hash.first[slot] == (uint32_t)k, several = first && hash.count[slot] > 1u;
-    // then the sums: p, p log p, p log2 q + log2(total), the student's at the entries, the entries
+    // then the sums: p, p log p, p T (log q + log(total)), the student's at the entries, the entries
     float p = 0.0f;
-    if (valid) p = BUCKET ? expf(logp) : (top > -kDsInf ? expf(logp - top) : 0.0f);
-    const float rel = __builtin_fmaf(e.x, a.c, -mref);
+    if (valid) p = BUCKET ? expf(logp) : (top > -kExpInf ? expf(logp - top) : 0.0f);
+    const float gap = e.x - mref;
     const bool on = valid && !(p <= 0.0f);
-    float v[5] = {p, on ? p * (BUCKET ? logp : logp - top) : 0.0f, on ? p * rel : 0.0f,
-                  BUCKET && first ? ds_exp2(rel) : 0.0f, valid ? 1.0f : 0.0f};
+    float v[5] = {p, on ? p * (BUCKET ? logp : logp - top) : 0.0f, on ? p * gap : 0.0f,
+                  BUCKET && first ? es_exp2(gap * a.c) : 0.0f, valid ? 1.0f : 0.0f};
     if (k < K) sh.p[k] = p;
     if (wave < EW) {
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-            v[i] = ds_wave_sum(v[i]);
+            v[i] = es_wave_sum(v[i]);
             if (lead) sh.sums[wave][i] = v[i];
         }
     }
@@ -322,7 +324,7 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, DsSum t,
     DsRow o;
     o.max = mref;
     o.ref = ref;
-    const float Z = BUCKET ? (rest.s != 0.0f ? rest.s * ds_exp2(ref - mref) : 0.0f) + v[3] : rest.s;
+    const float Z = BUCKET ? (rest.s != 0.0f ? rest.s * es_exp2((ref - mref) * a.c) : 0.0f) + v[3] : rest.s;
     const bool some = Z > 0.0f || Z != Z;  // (no finite logit: every log q is -inf)
     const float lz = some ? log2f(Z) : 0.0f;
     o.inv_total = some ? 1.0f / Z : 0.0f;
@@ -330,20 +332,20 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, DsSum t,
     if (BUCKET) {
         o.live = v[4] > 0.0f;
         const float sp = v[0], rr = 1.0f - sp;
-        L = v[1] - (v[2] - lz * sp) * kLn2;
+        L = v[1] - v[2] * a.inv_T + lz * sp * kLn2;
         // a rest without a finite logit is no event
         const bool have = rest.s > 0.0f || rest.s != rest.s;
         const float rem = have && !(rr < 0.0f) ? rr : 0.0f;
-        if (!(rem <= 0.0f)) L += rem * (logf(rem) - ((rest.m - mref) + log2f(rest.s) - lz) * kLn2);
+        if (!(rem <= 0.0f)) L += rem * (logf(rem) - (rest.m - mref) * a.inv_T - (log2f(rest.s) - lz) * kLn2);
         // the teacher's events add up to tot, 1 but where the rest is no event or sp exceeds 1:
         // an entry's gradient is tot q - p, the rest's tot q - rem q / s
         const float tot = sp + rem;
-        o.coef = have ? (tot * (rest.s * ds_exp2(ref - mref) * o.inv_total) - rem) / rest.s : 0.0f;
+        o.coef = have ? (tot * (rest.s * es_exp2((ref - mref) * a.c) * o.inv_total) - rem) / rest.s : 0.0f;
         o.inv_total *= tot;
     } else {
-        o.live = top > -kDsInf;
+        o.live = top > -kExpInf;
         const float inv = 1.0f / v[0];
-        L = (v[1] - v[2] * kLn2) * inv - logf(v[0]) + lz * kLn2;
+        L = (v[1] - v[2] * a.inv_T) * inv - logf(v[0]) + lz * kLn2;
         o.coef = o.inv_total;
         p *= inv;
     }
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo;
     DsEntry e = ds_entry(a, r);
-    DsSum t = ds_stream<T, BUCKET>(row + lo, len, a.c, bm, [&] {
+    ExpSum t = ds_stream<T, BUCKET>(row + lo, len, a.c, bm, [&] {
         hash.clear();
         if (BUCKET) {
             ds_clear_bits(bm, len);
@@ -399,36 +401,46 @@ __global__ __launch_bounds__(kDsThreads) void distill_forward_kernel(DistillArgs
         }
         __syncthreads();
     });
-    t.wave_merge();
+    t.wave_merge(a.c);
+    ds_put(sh, t);
+    __syncthreads();
+    t = ds_get<NW>(sh, a.c);
+    if (exp_far(t.m, a.c)) {  // (every thread alike: a second read of the part, from the caches)
+        const float mine = es_wave_sum(ds_far_sum<T, BUCKET>(row + lo, len, a.c, bm, t.m));
+        __syncthreads();
+        if ((tid & 63) == 0) sh.ws[tid >> 6] = mine;
+        __syncthreads();
+        t.s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) t.s += sh.ws[i];
+    }
     if (S > 1) {
         // the part that arrives last joins them, in their order
-        if ((tid & 63) == 0) { sh.wm[tid >> 6] = t.m; sh.ws[tid >> 6] = t.s; }
-        __syncthreads();
         if (tid == 0) {
-            DsSum s;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) s.merge(sh.wm[i], sh.ws[i]);
-            ag_store64(&a.rec[(size_t)r * S + p], ((uint64_t)f2u(s.m) << 32) | f2u(s.s));
+            ag_store64(&a.rec[(size_t)r * S + p], ((uint64_t)f2u(t.m) << 32) | f2u(t.s));
             stores_complete();
             last = ag_add32(&a.ctr[r], 1u) == (uint32_t)S - 1u ? 1u : 0u;
         }
         __syncthreads();
         if (!last) return;
         if (tid == 0) ag_store32(&a.ctr[r], 0u);
-        t = DsSum();
-        if (tid < S) {  // (S <= 64: the first wave holds them)
-            const uint64_t v = ag_load64(&a.rec[(size_t)r * S + tid]);
+        t = ExpSum();
+        const int part = tid & 63;
+        if (part < S) {  // (S <= 64: a lane each, in every wave)
+            const uint64_t v = ag_load64(&a.rec[(size_t)r * S + part]);
             t.m = u2f((uint32_t)(v >> 32));
             t.s = u2f((uint32_t)v);
         }
-        t.wave_merge();
+        t.wave_merge(a.c);
     }
     int slot = 0;
     if (e.id >= 0) {
         slot = hash.insert(e.id);
         e.x = Elem<T>::load1(row + e.id);
     }
-    const DsRow o = ds_finish<T, BUCKET, NW>(a, r, t, w, e, slot, hash, sh);
+    ds_put_entries<BUCKET>(a, e, sh);
+    __syncthreads();
+    const DsRow o = ds_finish<T, BUCKET>(a, r, t, w, e, slot, hash, sh);
     ds_save(a, r, o);
 }
 
@@ -461,31 +473,40 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
         const int id = a.ids[(size_t)r * a.ids_stride + tid];
         if (!(P < 0.0f) && id >= lo && id < lo + len) {
             at = id;
-            const float q = ds_exp2(__builtin_fmaf(Elem<T>::load1(row + id), a.c, -st[kDsMax])) * st[kDsInvTotal];
+            const float q = es_exp2((Elem<T>::load1(row + id) - st[kDsMax]) * a.c) * st[kDsInvTotal];
             fix = gs * (q - P);
         }
     }
     __syncthreads();
-    const float ref = st[kDsRef], coef = st[kDsCoef] * gs;
-    for (int b = tid; b < nvec; b += U * kDsThreads) {
-        uint32_t w[U][4];
+    const float m = st[kDsRef], ref = m * a.c, coef = st[kDsCoef] * gs;
+    auto stream = [&](auto value) __attribute__((always_inline)) {
+        for (int b = tid; b < nvec; b += U * kDsThreads) {
+            uint32_t w[U][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vi = b + u * kDsThreads;
-            ds_load<T>(row + lo, vi < nvec ? vi : b, w[u]);
+            for (int u = 0; u < U; ++u) {
+                const int vi = b + u * kDsThreads;
+                ds_load<T>(row + lo, vi < nvec ? vi : b, w[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int vi = b + u * kDsThreads;
+                float v[VEC];
+                Elem<T>::from_words(w[u][0], w[u][1], w[u][2], w[u][3], v);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = value(v[j]);
+                DsVec<T>::pack(v, w[u]);
+                if (vi < nvec) ds_store<T>(out + lo, vi, w[u]);
+            }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vi = b + u * kDsThreads;
-            float v[VEC];
-            Elem<T>::from_words(w[u][0], w[u][1], w[u][2], w[u][3], v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = ds_exp2(__builtin_fmaf(v[j], a.c, -ref)) * coef;
-            DsVec<T>::pack(v, w[u]);
-            if (vi < nvec) ds_store<T>(out + lo, vi, w[u]);
-        }
+        if (tail < len) out[lo + tail] = DsVec<T>::narrow(value(Elem<T>::load1(row + lo + tail)));
+    };
+    if (exp_far(m, a.c)) {
+        stream([&](float v) __attribute__((always_inline)) { return es_exp2((v - m) * a.c) * coef; });
+    } else {
+        // (ref is off m c by its rounding, and so is every power)
+        const float near = coef * es_exp2(-__builtin_fmaf(m, a.c, -ref));
+        stream([&](float v) __attribute__((always_inline)) { return es_exp2(__builtin_fmaf(v, a.c, -ref)) * near; });
     }
-    if (tail < len) out[lo + tail] = DsVec<T>::narrow(ds_exp2(__builtin_fmaf(Elem<T>::load1(row + lo + tail), a.c, -ref)) * coef);
     // the teacher's entries over what the stream wrote there, once that has arrived
     stores_complete();
     __syncthreads();
@@ -561,34 +582,64 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
             ds_set_bit(bm, V, e.id);
         }
         __syncthreads();
-        DsSum t;
-#pragma unroll
-        for (int q0 = 0; q0 < NV; q0 += U) {
-            uint32_t g[U][4];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int vi = fresh(tid) + (q0 + u) * kDsStepThreads;
-                if (BUCKET) ds_drop<T>(bm, min(vi, nvec - 1), w[q0 + u]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // (in place: what lies past the row is never written)
-                    w[q0 + u][k] = vi < nvec ? w[q0 + u][k] : DsVec<T>::kNegInf;
-                    asm volatile("" : "+v"(w[q0 + u][k]));
-                    g[u][k] = w[q0 + u][k];
-                }
-            }
-            ds_add<T, U>(t, g, a.c);
-            fence();
-        }
         const bool edge_entry = edge < V && ((bm[edge >> 5] >> (edge & 31)) & 1u);
-        if (edge < V && !(BUCKET && edge_entry)) ds_add1(t, xe * a.c);
-        t.wave_merge();
-        const DsRow o = ds_finish<T, BUCKET, NW>(a, r, t, wt, e, slot, hash, sh);
+        // Once, or twice: a row whose largest logit m is far from zero is first moved by it, in its type (x - m is
+        // exact where it counts, from m to 2 m or m / 2; what is rounded lies too far below).  Its entries, which may
+        // be as far from a masked rest, stay.
+        ExpSum rest;
+        float moved = 0.0f;
+        for (;;) {
+            ExpRun t(a.c);
+#pragma unroll
+            for (int q0 = 0; q0 < NV; q0 += U) {
+                uint32_t g[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int vi = fresh(tid) + (q0 + u) * kDsStepThreads;
+                    if (BUCKET) ds_drop<T>(bm, min(vi, nvec - 1), w[q0 + u]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        // (in place: what lies past the row is never written)
+                        w[q0 + u][k] = vi < nvec ? w[q0 + u][k] : DsVec<T>::kNegInf;
+                        asm volatile("" : "+v"(w[q0 + u][k]));
+                        g[u][k] = w[q0 + u][k];
+                    }
+                }
+                ds_add<T, U>(t, g, a.c);
+                fence();
+            }
+            if (edge < V && !(BUCKET && edge_entry)) ds_add1(t, xe, a.c);
+            ExpSum mine = t.close(a.c);
+            mine.wave_merge(a.c);
+            ds_put(sh, mine);
+            ds_put_entries<BUCKET>(a, e, sh);
+            __syncthreads();
+            rest = ds_get<NW>(sh, a.c);
+            if (!exp_far(rest.m, a.c)) break;
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                float v[VEC];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(w[q][k]));
+                Elem<T>::from_words(w[q][0], w[q][1], w[q][2], w[q][3], v);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] -= rest.m;
+                DsVec<T>::pack(v, w[q]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) asm volatile("" : "+v"(w[q][k]));
+                fence();
+            }
+            xe -= rest.m;
+            moved = rest.m;
+            __syncthreads();  // every wave has the sums of this time
+        }
+        rest.m += moved;  // (moved: of 0)
+        const DsRow o = ds_finish<T, BUCKET>(a, r, rest, wt, e, slot, hash, sh);
         const float gs = wt * (a.gout ? a.gout[r] : 1.0f) * a.inv_T;
         const bool on = o.live && gs != 0.0f;
-        const float ref = o.ref, coef = o.coef * gs;
+        const float here = o.ref - moved, ref = here * a.c, coef = o.coef * gs * es_exp2(-__builtin_fmaf(here, a.c, -ref));
         if (!(o.p < 0.0f)) {  // (the first of its id)
-            const float q = ds_exp2(__builtin_fmaf(e.x, a.c, -o.max)) * o.inv_total;
+            const float q = es_exp2((e.x - o.max) * a.c) * o.inv_total;
             hash.value[slot] = on ? gs * (q - o.p) : 0.0f;
         }
         r += gridDim.x;
@@ -600,7 +651,7 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
         hashes[parity ^ 1].clear();
         ds_clear_bits(bms + (parity ^ 1) * words, V);
         __syncthreads();
-        auto value = [&](float v) { return on ? ds_exp2(__builtin_fmaf(v, a.c, -ref)) * coef : 0.0f; };
+        auto value = [&](float v) { return on ? es_exp2(__builtin_fmaf(v, a.c, -ref)) * coef : 0.0f; };
 #pragma unroll
         for (int q = 0; q < NV; ++q) {
             const int vi = fresh(tid) + q * kDsStepThreads;
