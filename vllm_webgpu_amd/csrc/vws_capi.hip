@@ -509,20 +509,33 @@ int validate_verify(const vws_verify_args* a) {
 }
 
 template <typename T>
-int verify_launch(const VerifyArgs& k, bool cuts, bool top_p, hipStream_t s) {
+int verify_launch(VerifyArgs k, bool cuts, bool top_p, hipStream_t s) {
     const int K = VWS_KERNEL_VERIFY;
-    launch(K, verify_rows_kernel<T>, dim3((unsigned)k.R * (unsigned)k.S), dim3(kVfThreads), s, k);
-    if (int st = check_launch("vws_verify_drafts (rows)")) return st;
+    // f over n rows (or requests) in launches of at most kVfLaunchRows; more than that are one part each
+    auto each = [&](int n, const char* what, auto f) {
+        for (k.r0 = 0; k.r0 < n; k.r0 += kVfLaunchRows) {
+            f((unsigned)(n - k.r0 < kVfLaunchRows ? n - k.r0 : kVfLaunchRows));
+            if (int st = check_launch(what)) return st;
+        }
+        return (int)VWS_OK;
+    };
+    if (int st = each(k.R, "vws_verify_drafts (rows)", [&](unsigned n) {
+            launch(K, verify_rows_kernel<T>, dim3(n * (unsigned)k.S), dim3(kVfThreads), s, k);
+        }))
+        return st;
     if (cuts) {
-        launch(K, verify_cut_kernel<T>, dim3((unsigned)k.R), dim3(kVfCutThreads), s, k);
-        if (int st = check_launch("vws_verify_drafts (cuts)")) return st;
+        if (int st = each(k.R, "vws_verify_drafts (cuts)", [&](unsigned n) {
+                launch(K, verify_cut_kernel<T>, dim3(n), dim3(kVfCutThreads), s, k);
+            }))
+            return st;
         if (top_p) {
             launch(K, verify_mass_kernel<T>, dim3(kVfMassWgs), dim3(kVfCutThreads), s, k);
             if (int st = check_launch("vws_verify_drafts (masses)")) return st;
         }
     }
-    launch(K, verify_token_kernel<T>, dim3((unsigned)k.B * (unsigned)k.S2), dim3(kVfThreads), s, k);
-    return check_launch("vws_verify_drafts (tokens)");
+    return each(k.B, "vws_verify_drafts (tokens)", [&](unsigned n) {
+        launch(K, verify_token_kernel<T>, dim3(n * (unsigned)k.S2), dim3(kVfThreads), s, k);
+    });
 }
 
 enum DistillPart { kDistillForward = 1, kDistillBackward = 2 };

@@ -28,6 +28,10 @@ constexpr int kVfBins = 2048;      // bins of a row's masses
 constexpr int kVfFlat = 256;       // rows of a launch that verify_mass_kernel takes: a workgroup each, at least
 constexpr int kVfMassWgs = 256;    // its workgroups, one of 1024 threads for each compute unit
 
+// Rows or requests of a launch, at most: a workgroup of 1024 threads each stays below the 2^32 threads of
+// a grid, from where a launch runs some of its workgroups only and reports nothing.
+constexpr int kVfLaunchRows = 1 << 21;
+
 struct VfFlat {
     int32_t row;
     uint32_t ctr;                  // parts arrived
@@ -39,6 +43,7 @@ struct VerifyArgs {
     const void* x;               // [R, V] target logits, n_b + 1 rows per request
     int64_t xstride;
     int R, V, B, D, K;           // K: columns of drafts in the outputs
+    int r0;                      // first row (verify_token_kernel: request) of the launch
     const int32_t* drafts;       // [D]
     const int32_t* cu;           // [B + 1]
     const void* q;               // [D, V] draft probabilities or null

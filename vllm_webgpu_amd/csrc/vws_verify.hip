@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
     __shared__ uint64_t red_top[kVfThreads / 64];
     __shared__ float red_m[kVfThreads / 64], red_s[kVfThreads / 64];
-    const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, wave = tid >> 6;
+    const int S = a.S, at = blockIdx.x / S, r = a.r0 + at, p = blockIdx.x - at * S, tid = threadIdx.x, wave = tid >> 6;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
     const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
     row += lo;
@@ -928,7 +928,7 @@ __device__ __forceinline__ void vf_write(const VerifyArgs& a, int r, const VfRow
 template <typename T>
 __global__ __launch_bounds__(kVfCutThreads) void verify_cut_kernel(VerifyArgs a) {
     __shared__ VfCutShared sh;
-    const int r = blockIdx.x;
+    const int r = a.r0 + (int)blockIdx.x;
     const VfParams prm = vf_params(a, a.rec[(size_t)r * a.S].owner);
     if (!prm.cuts) return;
     const T* row = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
@@ -1100,7 +1100,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     __shared__ VfRow rows[kVfMaxDrafts + 1];
     __shared__ uint64_t red[kVfThreads / 64];
     __shared__ uint32_t last, shared_bound;
-    const int S2 = a.S2, b = blockIdx.x / S2, p = blockIdx.x - b * S2, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int S2 = a.S2, at = blockIdx.x / S2, b = a.r0 + at, p = blockIdx.x - at * S2, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const VfParams prm = vf_params(a, b);
     const int first = a.cu[b], end = a.cu[b + 1], n = (int)((uint32_t)end - (uint32_t)first), K1 = a.K + 1;
     auto misfit = [&] {  // bounds that do not fit: no token
