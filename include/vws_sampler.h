@@ -278,7 +278,9 @@ int vws_apply_penalties(float* logits, int32_t batch, int32_t vocab, int64_t row
  * q_i is 1 at d (a looked-up or greedy draft).  After the first refusal, at row a, one token is
  * drawn from max(p_a - q_a, 0); if none is refused, from the last row's p.  Both by vws_sample's
  * race with the request's uniforms (lowest index on equal keys; the most probable token if the
- * residual is empty).  The tokens so emitted are distributed as the target's own samples.
+ * residual is empty).  The tokens so emitted are distributed as the target's own samples, if their random
+ * numbers are not those that the drafts were drawn with: without drafts a request's token is vws_sample's
+ * under the same key, so sample drafts under other keys or offsets.
  * Requests with temperature < 1e-5 or NaN, and rows whose maximum is not finite, have their argmax
  * (lowest index) for sure.  A draft outside [0, vocab) is refused.  Nothing is read or written out
  * of bounds whatever cu_drafts holds: a request whose bounds do not fit (negative, decreasing, more

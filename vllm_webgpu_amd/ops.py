@@ -473,7 +473,9 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: t
     from ``max(p - q, 0)`` (None: p without the draft), after the last accepted draft from the last
     row's p.  The random numbers are ``accept_uniforms`` [D] and ``uniforms`` [B, V] float32 in
     (0, 1), or generated from ``rng_seeds`` / ``rng_offsets`` [B] int64 or one ``rng_key`` as for
-    ``sample`` (draft i's acceptance: token 2**19 + i of the request's key).
+    ``sample`` (draft i's acceptance: token 2**19 + i of the request's key).  They must not be the numbers that the
+    drafts were drawn with: give ``sample`` of the draft and this call different keys, or the same seeds
+    with different offsets.  (Without drafts the token is ``sample``'s under the same key.)
 
     Returns tokens [B, max_drafts + 1] (-1 past the drawn token), the number of accepted drafts [B]
     (-1 and no token for a request whose bounds do not fit) and the emitted tokens' log

@@ -8,7 +8,10 @@ and ``parse_output`` for the host's lists.  Unlike there, the logits are the tar
 request together, the row after its last draft included (the bonus token is drawn in the same call):
 ``metadata.num_draft_tokens[i] + 1`` consecutive rows for request ``i``.
 
-Temperature, top-k, top-p, min-p and seeded requests follow ``Sampler``.  Requests with penalties,
+Temperature, top-k, top-p, min-p and seeded requests follow ``Sampler``; the logits are those after a
+model's soft cap.  A seeded request with drafts is verified with keys of another domain than
+``Sampler``'s: its drafts may have been sampled from a stream of the same seed, and a token raced with
+the numbers that chose the refused draft would not be the target's.  Requests with penalties,
 logits processors or raw logprobs change the distribution from one draft to the next and are refused:
 sample them one by one.
 """
@@ -24,6 +27,7 @@ from .metadata import SamplingMetadata
 from .sampler import _SEED_HI, _SEED_LO, SeedStaging, draw_seeds
 
 PLACEHOLDER = -1
+_DOMAIN = 0x6A09E667F3BCC908  # of requests with drafts (the fraction of sqrt(2): any constant will do)
 
 
 @dataclass
@@ -69,7 +73,8 @@ class RejectionSampler:
         seeds = key = None
         if temperature is not None:
             if m.generators:
-                seeds = draw_seeds(B, m.generators, logits.device, self._seeds)
+                domain = torch.tensor([_DOMAIN if n else 0 for n in metadata.num_draft_tokens], dtype=torch.int64)
+                seeds = draw_seeds(B, m.generators, logits.device, self._seeds, domain)
             else:
                 key = int(torch.randint(_SEED_LO, _SEED_HI, (1,), dtype=torch.int64))
         r = ops.verify_drafts(logits, metadata.draft_token_ids, metadata.cu_num_draft_tokens, metadata.max_spec_len,

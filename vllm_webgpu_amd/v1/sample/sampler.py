@@ -99,14 +99,15 @@ class SeedStaging:
 
 
 def draw_seeds(B: int, generators: dict, device: torch.device,
-               staging: SeedStaging | None = None) -> torch.Tensor:
+               staging: SeedStaging | None = None, domain: torch.Tensor | None = None) -> torch.Tensor:
     """int64 ``[B]`` keys of the race's generated uniforms, one fresh draw per row and step: row
     ``i`` draws from ``generators[i]`` if present (a seeded request samples the same tokens
     again), the others from torch's default CPU generator.  ``KeyStream`` entries (the
     persistent batch's seeded requests) are computed together on the host; a ``torch.Generator``
     entry draws from its own stream.  One host-to-device copy; with ``staging`` (device
     tensors only) no allocation, and the returned tensor is the staging's device buffer, valid
-    until the next draw on it."""
+    until the next draw on it.  ``domain`` int64 ``[B]`` (on the host) is added to the keys by exclusive
+    or: draws of other domains share no numbers, though their streams have the same seeds."""
     use = staging is not None and device.type == "cuda"
     if use:
         keys, dev_keys = staging.acquire(B, device)
@@ -125,6 +126,8 @@ def draw_seeds(B: int, generators: dict, device: torch.device,
         if not isinstance(g, KeyStream):
             keys[i] = torch.randint(_SEED_LO, _SEED_HI, (1,), dtype=torch.int64,
                                     device=g.device, generator=g)[0].cpu()
+    if domain is not None:
+        keys ^= domain
     if use:
         dev_keys.copy_(keys, non_blocking=True)
         staging.copied()
