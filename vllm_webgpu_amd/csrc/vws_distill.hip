@@ -567,9 +567,13 @@ __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArg
     // A row of 128256 bf16 takes a workgroup some 13 us of sums and then some 15 of reading and writing.
     // Started together the workgroups would keep time, and the memory idle while all sum: they start
     // up to most of a row's time apart.  Against a common start, us: bf16 1600 x 128256 231 -> 216, 4096 x
-    // 487 -> 462, 3328 x 64000 219 -> 212, 1400 x 151936 249 -> 231; fp32 4000 x 32000 220 -> 213, but 2048 x
-    // 64000 226 -> 231 (twice the sleep for rows of 64000 bf16 would lose: 224).
-    for (int k = (int)((blockIdx.x >> 3) & 7u); k > 0; --k) __builtin_amdgcn_s_sleep(NV * 7 / 2);
+    // 487 -> 462, 3328 x 64000 219 -> 212; fp32 4000 x 32000 220 -> 213, but 2048 x
+    // 64000 226 -> 231 (twice the sleep for rows of 64000 bf16 would lose: 224).  38 vectors, with a sleep of 5, 64, 133
+    // units: bf16 1400 x 151936 232, 220, 219, 3000 x 442, 410, 404; f16 1500 x 140001 240, 246, 248, 2048 x 155000 329, 320, 312;
+    // fp32 2048 x 70000 259, 256, 263, 1500 x 77000 221, 217, 225.
+    constexpr int kApart = NV > 32 ? 64 : NV * 7 / 2;
+    static_assert(kApart <= 127, "the instruction takes seven bits");
+    for (int k = (int)((blockIdx.x >> 3) & 7u); k > 0; --k) __builtin_amdgcn_s_sleep(kApart);
     for (int parity = 0;; parity ^= 1) {
         const T* row = x + (size_t)r * a.xstride;
         T* out = grad + (size_t)r * a.gstride;
