@@ -621,7 +621,14 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     probabilities at temperature T) and the rest of the vocabulary is one more event, 1 - sum p
     against the student's probability of everything outside the entries.  Ids outside [0, V) are
     padding, entries that share an id add up.  ``row_weight`` (scalar or [N]) multiplies a row's
-    loss and gradient; rows of weight 0 are not read.  Rows without an entry have loss 0."""
+    loss and gradient; rows of weight 0 are not read.  Rows without an entry have loss 0.
+
+    Only ``logits`` get a gradient: a teacher's log-probabilities or weights that require one are refused
+    (detach them)."""
+    if torch.is_grad_enabled():
+        for name, t in (("teacher_logprobs", teacher_logprobs), ("row_weight", row_weight)):
+            if torch.is_tensor(t) and t.requires_grad:
+                raise ValueError(f"{name} would get no gradient: detach it")
     return _DistillLoss.apply(logits, teacher_ids, teacher_logprobs, row_weight, temperature, tail)
 
 
