@@ -23,3 +23,36 @@ def test_inputs_that_would_silently_get_no_gradient_are_refused(cuda):
     loss = ops.distill_loss(x, ids, lp.clone().requires_grad_(True).detach(), w)
     loss.sum().backward()
     assert x.grad is not None
+
+
+FAR = [-2 ** 63, 2 ** 63 - 1, 2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31 + 3, 2 ** 40]
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+def test_ids_past_32_bits_are_padding(cuda, tail):
+    """As any id outside the vocabulary, whatever their lower halves are."""
+    x, ids, lp = make(cuda, 5, 900, 12, "f32", seed=2)
+    wide, narrow = ids.long(), ids.clone()
+    wide[:, 3:9], narrow[:, 3:9] = torch.tensor(FAR, device=cuda), -1
+    want, want_grad = ops.distill_loss_and_grad(x, narrow, lp, tail=tail)
+    got, grad = ops.distill_loss_and_grad(x, wide, lp, tail=tail)
+    assert torch.equal(got, want) and torch.equal(grad, want_grad)
+    assert torch.equal(ops.distill_loss(x, wide, lp, tail=tail), ops.distill_loss(x, narrow, lp, tail=tail))
+
+
+def test_drafts_and_bounds_past_32_bits(cuda):
+    """Drafts there are refused, bounds there do not fit."""
+    V, n = 300, len(FAR)
+    x = torch.zeros((2 * n, V), device=cuda)
+    x[:, [0, 3, 5]] = 20.0                                   # the lower halves' tokens are likely
+    q = torch.full((n, V), 1e-6, device=cuda)
+    cu = torch.arange(n + 1)
+    r = ops.verify_drafts(x, torch.tensor(FAR), cu, 1, draft_probs=q, temperature=1.0, rng_key=3)
+    assert not r.num_accepted.any()
+    ok = ops.verify_drafts(x, torch.tensor([0, 3, 5, 5, 3, 0]), cu, 1, draft_probs=q, temperature=1.0, rng_key=3)
+    assert bool((ok.num_accepted == 1).all())
+    for far in FAR[:1] + FAR[2:4]:
+        bounds = cu.clone()
+        bounds[2] = far
+        r = ops.verify_drafts(x, torch.zeros(n, dtype=torch.int32), bounds, 1, temperature=1.0, rng_key=3)
+        assert r.num_accepted[1:3].tolist() == [-1, -1]

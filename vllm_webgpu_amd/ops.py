@@ -446,6 +446,13 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
 
 
+def _int32(t: torch.Tensor, device=None) -> torch.Tensor:
+    """``t`` as int32 on ``device``; what does not fit goes to its ends, where no token or bound lies."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=device, dtype=torch.int32)
+
+
 @dataclass
 class VerifyResult:
     tokens: torch.Tensor        # [B, max_drafts + 1] int32: accepted drafts, the drawn token, then -1
@@ -485,8 +492,7 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: t
         raise ValueError("logits must be [num_drafts + batch, V]")
     logits = _rows(logits)
     dev, (R, V) = logits.device, logits.shape
-    cu = cu_drafts.to(device=dev, dtype=torch.int32).contiguous()
-    drafts = draft_tokens.to(device=dev, dtype=torch.int32).contiguous()
+    cu, drafts = _int32(cu_drafts, dev).contiguous(), _int32(draft_tokens, dev).contiguous()
     if cu.dim() != 1 or cu.numel() < 1 or drafts.dim() != 1:
         raise ValueError("cu_drafts must be [batch + 1] and draft_tokens [num_drafts]")
     B, D, K = cu.numel() - 1, drafts.numel(), int(max_drafts)
@@ -561,7 +567,7 @@ def _distill_args(logits, teacher_ids, teacher_logprobs, row_weight, temperature
     if not 1 <= K <= _lib.MAX_TEACHER:
         raise ValueError(f"teacher entries per row must be in [1, {_lib.MAX_TEACHER}] (got {K})")
     if teacher_ids.dtype != torch.int32:
-        teacher_ids = teacher_ids.to(torch.int32)
+        teacher_ids = _int32(teacher_ids)
     if teacher_logprobs.dtype != torch.float32:
         teacher_logprobs = teacher_logprobs.float()
     logits, ids, lp = _rows(logits), _rows(teacher_ids), _rows(teacher_logprobs)
