@@ -23,16 +23,13 @@ __device__ __forceinline__ float u2f(uint32_t u) { return __uint_as_float(u); }
 // lane mask directly.
 __device__ __forceinline__ uint64_t wave_ballot(bool p) { return __builtin_amdgcn_ballot_w64(p); }
 
-// exp(d) for d in [-80, 80] (clamped above), 0 below -80 and for NaN.  Cody-Waite
-// reduction n = rint(d * log2 e), r = d - n * ln2 with a 16-bit head of ln2 (n * head is
-// exact) and an fp32 tail; exp(r) = 1 + r + r^2 Q(r) with Q of degree 4 fitted for this
-// project on [-ln2/2, ln2/2]; exact scaling by 2^n.  Max error 1 ulp (checked on every fp32).
-// Written without branches (special cases are selected at the end) so that it schedules freely
-// in straight-line code.
-__device__ __forceinline__ float exp_det(float d0) {
-    const float d = __builtin_fminf(__builtin_fmaxf(d0, -80.0f), 80.0f);
+// exp(d) / 2^n, n = rint(d * log2 e) (left in *ni as a float), for d in [-80, 80].  Cody-Waite
+// reduction r = d - n * ln2 with a 16-bit head of ln2 (n * head is exact) and an fp32 tail;
+// exp(r) = 1 + r + r^2 Q(r) with Q of degree 4 fitted for this project on [-ln2/2, ln2/2].
+__device__ __forceinline__ float exp_mantissa(float d, float* ni) {
     const float t = d * 0x1.715476p+0f;
     const float n = __builtin_rintf(t);
+    *ni = n;
     float r = __builtin_fmaf(-n, 0x1.62e4p-1f, d);
     r = __builtin_fmaf(-n, 0x1.7f7d1cp-20f, r);
     float p = __builtin_fmaf(0x1.6d7532p-10f, r, 0x1.120b66p-7f);
@@ -40,7 +37,16 @@ __device__ __forceinline__ float exp_det(float d0) {
     p = __builtin_fmaf(p, r, 0x1.5554dcp-3f);
     p = __builtin_fmaf(p, r, 0.5f);
     p = __builtin_fmaf(p, r, 1.0f);
-    p = __builtin_fmaf(p, r, 1.0f);
+    return __builtin_fmaf(p, r, 1.0f);
+}
+
+// exp(d) for d in [-80, 80] (clamped above), 0 below -80 and for NaN: exp_mantissa, exact scaling by
+// 2^n.  Max error 1 ulp (checked on every fp32).  Written without branches (special cases are
+// selected at the end) so that it schedules freely in straight-line code.
+__device__ __forceinline__ float exp_det(float d0) {
+    const float d = __builtin_fminf(__builtin_fmaxf(d0, -80.0f), 80.0f);
+    float n;
+    const float p = exp_mantissa(d, &n);
     const int ni = (int)n;
     const float v = p * u2f((uint32_t)(ni + 127) << 23);
     const float v1 = __builtin_fabsf(d) < 0x1p-30f ? 1.0f : v;

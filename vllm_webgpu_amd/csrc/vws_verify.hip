@@ -841,15 +841,8 @@ __device__ __forceinline__ uint64_t vf_masses(const T* row, int V, float Tt, VfC
             y = x / Tt;
         }
         const float d = y - u.m;  // (NaN where y overflows: no mass, as its exp_det is 0)
-        const float n = __builtin_rintf(d * 0x1.715476p+0f);
-        float e = __builtin_fmaf(-n, 0x1.62e4p-1f, d);
-        e = __builtin_fmaf(-n, 0x1.7f7d1cp-20f, e);
-        float p = __builtin_fmaf(0x1.6d7532p-10f, e, 0x1.120b66p-7f);
-        p = __builtin_fmaf(p, e, 0x1.5554b8p-5f);
-        p = __builtin_fmaf(p, e, 0x1.5554dcp-3f);
-        p = __builtin_fmaf(p, e, 0.5f);
-        p = __builtin_fmaf(p, e, 1.0f);
-        p = __builtin_fmaf(p, e, 1.0f);
+        float n;
+        const float p = exp_mantissa(d, &n);
         // 2^44 exp(d), 0 from where a mass is 0 (d < -31: below 2^-44)
         const float f = d >= -31.0f ? __builtin_ldexpf(p, (int)n + 44) : 0.0f;
         const float hf = __builtin_truncf(f * 0x1p-32f);
