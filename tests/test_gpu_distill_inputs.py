@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_distill import make
+from tests.test_gpu_distill import TOL, check, make
 from vllm_webgpu_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,17 @@ def test_drafts_and_bounds_past_32_bits(cuda):
         bounds[2] = far
         r = ops.verify_drafts(x, torch.zeros(n, dtype=torch.int32), bounds, 1, temperature=1.0, rng_key=3)
         assert r.num_accepted[1:3].tolist() == [-1, -1]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_teacher_whose_probabilities_exceed_one(cuda, dtype):
+    """Bucket: no rest is left, and the gradient is the stated loss's, w / T (q sum p - p)."""
+    x, ids, lp = make(cuda, 6, 3001, 20, dtype, seed=3)
+    lp = lp + torch.linspace(0.5, 1.5, 6, device=cuda).unsqueeze(1)
+    p = lp.double().exp()
+    assert bool((p.sum(1) > 1.05).all())
+    check(x, ids, lp, tail="bucket")
+    _, grad = ops.distill_loss_and_grad(x, ids, lp, tail="bucket")
+    want = torch.softmax(x.double(), 1) * p.sum(1, keepdim=True)
+    want.scatter_add_(1, ids.long(), -p)
+    assert ((grad.double() - want).abs() <= 4 * TOL + 2.0 ** -8 * want.abs() * (dtype == "bf16")).all()
