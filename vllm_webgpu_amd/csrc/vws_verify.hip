@@ -893,7 +893,10 @@ __device__ __forceinline__ VfRule vf_rule(const VfParams& prm, const VfRow& w) {
 template <typename T>
 __device__ __forceinline__ VfCut vf_solve_row(const T* row, int V, float Tt, VfCutShared& sh, const VfRule& u) {
     uint64_t n = 0ull;
-    vf_each<T>(row, V, [&](int, float x) { n += x == x ? 1u : 0u; });
+    vf_each<T>(row, V, [&](int, float x) {
+        const float y = vf_scaled(x, Tt);  // (NaN at T = inf where x is not finite)
+        n += y == y ? 1u : 0u;
+    });
     n = vf_block_sum(n, sh);
     return vf_solve(VfRowIter<T>{row, V, Tt}, sh, u, n);
 }
