@@ -281,8 +281,8 @@ int vws_apply_penalties(float* logits, int32_t batch, int32_t vocab, int64_t row
  * residual is empty).  The tokens so emitted are distributed as the target's own samples, if their random
  * numbers are not those that the drafts were drawn with: without drafts a request's token is vws_sample's
  * under the same key, so sample drafts under other keys or offsets.
- * Requests with temperature < 1e-5 or NaN, and rows whose maximum is not finite, have their argmax
- * (lowest index) for sure.  A draft outside [0, vocab) is refused.  Nothing is read or written out
+ * Requests with temperature < 1e-5 or NaN, and rows whose maximum over the temperature is not finite,
+ * have their argmax (lowest index) for sure.  A draft outside [0, vocab) is refused.  Nothing is read or written out
  * of bounds whatever cu_drafts holds: a request whose bounds do not fit (negative, decreasing, more
  * than max_drafts, past num_drafts) gets num_accepted -1 and no token, and so does one with a row that
  * the bounds give to another as well (a row is the last request's that starts at or before it). */
@@ -328,6 +328,8 @@ typedef struct vws_verify_args {
     void* stream;
 } vws_verify_args;
 
+/* Holds for every type and every set of cuts: some 2 KB and vocab / 4 bytes a row (at least 1 KB), and up
+ * to 4 MB. */
 size_t vws_verify_workspace_size(int32_t batch, int32_t num_drafts, int32_t vocab);
 int vws_verify_drafts(const vws_verify_args* args);
 
@@ -340,7 +342,8 @@ int vws_verify_drafts(const vws_verify_args* args);
  *   VWS_TAIL_BUCKET: p_k = exp(l_k), the rest r = max(0, 1 - sum_k p_k) one more event against the
  *     student's s = sum of q outside the entries (l: log-probabilities at temperature T);
  *     loss = w (sum_k p_k (log p_k - log q(id_k)) + r log(r / s));
- *     dloss/dx_j = w / T (q_j - p_j) at an entry, w / T q_j (1 - r / s) elsewhere.
+ *     dloss/dx_j = w / T (t q_j - p_j) at an entry, w / T q_j (t - r / s) elsewhere, t = r + sum_k p_k
+ *     (1, but where the entries' sum exceeds 1 or the rest is no event).
  * Ids outside [0, V) are padding; entries that share an id add up.  Rows whose weight is 0, or that
  * have no entry (renormalize: none above -inf), have loss and gradient 0, and rows of weight 0 are
  * not read.  A student logit of -inf at an entry of positive probability makes the loss +inf and

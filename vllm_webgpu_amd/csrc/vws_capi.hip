@@ -434,9 +434,9 @@ void split_row(int rows, int V, int wgs, int min_len, int most, int least, int* 
 
 // Workgroups (of 256 threads) that a launch's rows are split over, at most; parts of at least 4096
 // logits.  A pass that keeps a maximum and a sum pays for every part (its reduction, its record, the
-// join), and too few leave loads out: 276 rows x 128256 fp32, the whole verification, with
-// 512, 768, 1024, 1536: 57.1, 55.8, 56.8, 56.1 us; 512 x 151936 bf16, a loss: 31.7, 31.5, 36.7, 40, 42;
-// 48 x 262144 f16, loss and gradient: 25.1, 24.4, 26.2, 35.5, 45.
+// join), and too few leave loads out.  With 512, 768, 1024, 1536, 2048, us: 276 rows x 128256 fp32, the whole
+// verification, 57.0, 55.1, 55.4, 56.0, 55.2; 150 x 151936 bf16 with a top-k 35.8, 35.9, 36.2, 36.7, 39.4; 512 x
+// 151936 bf16, a loss, 29.6, 29.6, 33.7, 35.4, 35.2; 48 x 262144 f16, loss and gradient, 24.5, 24.7, 26.3, 29.9, 35.3.
 constexpr int kRowsWgs = 768;
 constexpr int kDistillWgs = 768;
 // The race reads one row a request.  Uncut rows are all read (64 x 128256 fp32 with 1024, 2048: 60.3,
@@ -588,12 +588,12 @@ int validate_distill(const vws_distill_args* a, int parts) {
 // in the last-level cache (256 MB) what they read first, so the one kernel is for calls beyond it
 // (long rows, of which a workgroup gets few and the last ones leave units idle: well beyond), whose
 // rows fill at least three quarters or so of its registers (16, 32 or 38 vectors of 16 bytes for each of 512
-// threads).  Measured, one kernel against two, us, bf16: 1024 x 128256 (263 MB) 143 and 145, 1200 x 165 and
-// 159, 1450 x (372 MB) 192 and 195, 2048 x 251 and 295, 4096 x 462 and 594, 300 x 68 and 47; 1200 x 151936
-// (365 MB) 209 and 192, 2048 x 310 and 354; 2300 x 64000 (294 MB) 153 and 156, 2100 x (269 MB) 149 and
-// 146, 1800 x 127 and 120, 4096 x 271 and 295.  By the registers' filling: 4096 x 53248 (13 vectors) 247 and
-// 247, 50264 250 and 240, 57344 252 and 263; 2048 x 102400 (25) 226 and 235; 2048 x 136000 (33.2) 313 and
-// 311; 4096 x 66000 (16.1 of 32) 401 and 315.
+// threads).  Measured, one kernel against two, us, bf16: 1024 x 128256 (263 MB) 145 and 146, 1200 x 167 and
+// 160, 1450 x (372 MB) 194 and 197, 2048 x 252 and 296, 4096 x 466 and 593, 300 x 81 and 48; 1200 x 151936
+// (365 MB) 188 and 194, 2048 x 291 and 354; 2300 x 64000 (294 MB) 154 and 158, 2100 x (269 MB) 151 and
+// 147, 1800 x 127 and 121, 4096 x 258 and 297.  By the registers' filling: 4096 x 53248 (13 vectors) 249 and
+// 248, 50264 251 and 243, 57344 255 and 265; 2048 x 102400 (25) 229 and 237; 2048 x 136000 (33.2) 278 and
+// 311; 4096 x 66000 (16.1 of 32) 400 and 317.
 template <typename T>
 auto distill_step(int rows, int V, bool bucket) -> void (*)(DistillArgs) {
     const size_t bytes = (size_t)rows * (size_t)V * sizeof(T);

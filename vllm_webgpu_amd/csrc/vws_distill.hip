@@ -7,12 +7,13 @@
 //                                                   dL/dx_j = w / T (q_j - p_j)
 //   bucket:      p = exp(l), r = 1 - sum p, s = sum of q outside the entries;
 //                                                   L = w (sum_k ... + r log(r / s))
-//                dL/dx_j = w / T (q_j - p_j) at the entries, w / T q_j (1 - r / s) elsewhere.
+//                dL/dx_j = w / T (t q_j - p_j) at the entries, w / T q_j (t - r / s) elsewhere, t = r + sum p
+//                (1, but where the entries' sum exceeds 1: r is 0 then, or the rest is no event).
 // Exponentials are powers of two of x * log2(e) / T relative to a maximum; one fma and one exp2 per logit
 // (vws_expsum.h).  Rows whose maximum is far from zero in those units (a mask's value, mostly) take
 // differences from it instead.  s is the sum over the rest, never 1 - sum of the entries (which cancels when
 // the student is sure), and the rest keeps its own maximum, so that log(s) and q_j / s stay finite
-// however far the rest lies below the entries: q_j (1 - r / s) = e_j (s - r) / Z_rest with e_j and
+// however far the rest lies below the entries: q_j (t - r / s) = e_j (t s - r) / Z_rest with e_j and
 // Z_rest relative to the rest's maximum.
 #include "vws_device.h"
 #include "vws_distill.h"
@@ -518,8 +519,8 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
 // time; as a row's gradients are written, the next row's logits and entries are loaded into the
 // registers they leave.  No barrier waits for memory: a vector that holds teacher entries (by the
 // bitmap) takes their gradients from the hash, so nothing is written twice.
-// Bound: HBM: 4096 x 128256 bf16 (1.05 GB read and as much written) 462 us, 4.5 TB/s of a copy's 5.07; forward and
-// backward kernels take 594.  What is left is each row's two reductions, in which its workgroup moves nothing but
+// Bound: HBM: 4096 x 128256 bf16 (1.05 GB read and as much written) 465 us, 4.5 TB/s of a copy's 5.07; forward and
+// backward kernels take 593.  What is left is each row's two reductions, in which its workgroup moves nothing but
 // the next row's loads.
 template <typename T, bool BUCKET, int NV>
 __global__ __launch_bounds__(kDsStepThreads) void distill_step_kernel(DistillArgs a) {

@@ -118,8 +118,9 @@ __device__ __forceinline__ float vf_value(uint64_t top) {
 // few logits that matter without a second read of the row.
 //
 // Bound: HBM.  The next iteration's loads are issued before this one's are used, and the first
-// before the request's parameters are known.  274 rows x 128256 fp32 (141 MB): 30.6 us, 4.6 TB/s of a copy's
-// 5.07; 745 x 262144 bf16 (391 MB), most of them cut: 87 us, 4.5 TB/s, and 19 MB of groups' maxima written; small batches are one latency chain (6 x 128256 bf16 5.6 us, 4 x 32000 fp32 4.6).
+// before the request's parameters are known.  274 rows x 128256 fp32 (141 MB): 31.2 us, 4.5 TB/s of a copy's
+// 5.07; 745 x 262144 bf16 (391 MB), most of them cut: 87 us, 4.5 TB/s, and 19 MB of groups' maxima written;
+// small batches are one latency chain (6 x 128256 bf16 5.8 us, 4 x 32000 fp32 4.8).
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec, U = kVfGroup;
@@ -253,7 +254,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 //   * top-p alone: the list of the logits above such a bound, if it holds the cut for any total
 //     within the error of the first pass's sum (a peaked row);
 //   * else the masses of all logits, summed in bins by the distance from the maximum;
-//     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).
+//     the bin that holds the cut goes into a list (two reads of the row, one exp_det per logit).  16-bit
+//     logits whose spacing is wider than a bin can overfill it with one value: 32 rows of 262144 bf16 with
+//     mean 0 or 10, T 1.3, top-p 0.5, 116 us, with mean 20 (1/8 apart) 589.
 //     verify_mass_kernel does that for the first kVfFlat such rows, all compute units at it
 //     however few the rows, and verify_cut_kernel itself for further ones (rows of 128256 bf16 in
 //     whole calls, with 64, 128, 256 rows taken: 80 such rows 128, 87, 87 us, 200 147, 154, 118, 320 217,
@@ -1088,8 +1091,8 @@ __device__ __forceinline__ bool vf_kept(const VfRow& w, float y, int i) {
 // A draw is argmax w / E, E = -ln u; as E >= 1 - u, a token whose w / (1 - u) is below the best so far needs
 // no logarithm.  Rows whose kept tokens are listed race those alone.
 // Bound: for uncut rows the reads (64 x 128256 fp32 logits, draft's probabilities and uniforms, 82 MB fetched:
-// 24 us, 4.1 TB/s of the 98 they hold); for listed ones the latency of decision and race (48 requests, top-k 50: 8.3 us, 22.6 reading
-// the row; one request 6.1); 256 mixed requests of 262144 bf16 44 us, Philox for the tokens near the best.
+// 24 us, 4.1 TB/s of the 98 they hold); for listed ones the latency of decision and race (48 requests, top-k 50: 9 us, 22.6 reading
+// the row; one request 5.8); 256 mixed requests of 262144 bf16 44 us, Philox for the tokens near the best.
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
     constexpr int VEC = Elem<T>::kVec;
