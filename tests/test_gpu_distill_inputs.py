@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_distill import TOL, check, make
+from tests import speculative_ref as R
+from tests.test_gpu_distill import TOL, check, close, make
 from vllm_webgpu_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +71,21 @@ def test_a_teacher_whose_probabilities_exceed_one(cuda, dtype):
     want = torch.softmax(x.double(), 1) * p.sum(1, keepdim=True)
     want.scatter_add_(1, ids.long(), -p)
     assert ((grad.double() - want).abs() <= 4 * TOL + 2.0 ** -8 * want.abs() * (dtype == "bf16")).all()
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_entries_that_the_student_masks_by_the_types_lowest_value(cuda, dtype, tail):
+    """Their loss is as large, and finite while it fits 32 bits; the gradient is -p."""
+    x, ids, lp = make(cuda, 4, 3001, 60, dtype, seed=4)
+    lp = lp - 0.7
+    lp[0] = -5.0                                             # many alike: unnormalised they add up to 60
+    x.scatter_(1, ids[:, ::2].long(), torch.finfo(x.dtype).min)
+    g = torch.ones(4, device=cuda)
+    z = x.double()
+    leaf = (z - z.amax(1, keepdim=True)).requires_grad_(True)
+    want = R.distill(leaf, ids, lp, None, 1.0, tail)
+    (want_grad,) = torch.autograd.grad(want, leaf, g.double())
+    assert dtype == "f16" or (want > 1e36).all()
+    loss, grad = ops.distill_loss_and_grad(x, ids, lp, tail=tail)
+    close(loss, grad, want.detach(), want_grad, None, g, 1.0, x.dtype)

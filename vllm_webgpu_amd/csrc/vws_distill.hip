@@ -295,12 +295,13 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const Ex
     const float M = BUCKET ? __builtin_fmaxf(rest.m, top) : rest.m, mref = M == -kExpInf ? 0.0f : M;
     // entries that share an id: the first takes their probability together
     const bool first = valid && hash.first[slot] == (uint32_t)k, several = first && hash.count[slot] > 1u;
-    // then the sums: p, p log p, p T (log q + log(total)), the student's at the entries, the entries
+    // then the sums: p, p log p, p T (log q + log(total)) (scaled, so that up to 256 entries of the type's
+    // lowest value do not overflow), the student's at the entries, the entries
     float p = 0.0f;
     if (valid) p = BUCKET ? expf(logp) : (top > -kExpInf ? expf(logp - top) : 0.0f);
     const float gap = e.x - mref;
     const bool on = valid && !(p <= 0.0f);
-    float v[5] = {p, on ? p * (BUCKET ? logp : logp - top) : 0.0f, on ? p * gap : 0.0f,
+    float v[5] = {p, on ? p * (BUCKET ? logp : logp - top) : 0.0f, on ? p * (gap * 0x1p-10f) : 0.0f,
                   BUCKET && first ? es_exp2(gap * a.c) : 0.0f, valid ? 1.0f : 0.0f};
     if (k < K) sh.p[k] = p;
     if (wave < EW) {
@@ -333,7 +334,7 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const Ex
     if (BUCKET) {
         o.live = v[4] > 0.0f;
         const float sp = v[0], rr = 1.0f - sp;
-        L = v[1] - v[2] * a.inv_T + lz * sp * kLn2;
+        L = v[1] - v[2] * a.inv_T * 0x1p10f + lz * sp * kLn2;
         // a rest without a finite logit is no event
         const bool have = rest.s > 0.0f || rest.s != rest.s;
         const float rem = have && !(rr < 0.0f) ? rr : 0.0f;
@@ -346,7 +347,7 @@ __device__ __forceinline__ DsRow ds_finish(const DistillArgs& a, int r, const Ex
     } else {
         o.live = top > -kExpInf;
         const float inv = 1.0f / v[0];
-        L = (v[1] - v[2] * a.inv_T) * inv - logf(v[0]) + lz * kLn2;
+        L = v[1] * inv - v[2] * inv * a.inv_T * 0x1p10f - logf(v[0]) + lz * kLn2;
         o.coef = o.inv_total;
         p *= inv;
     }
