@@ -60,13 +60,7 @@ template <> struct DsVec<_Float16> {
     }
 };
 
-// (vi: a 32-bit offset, at most 2 MB, on the row's pointer)
-template <typename T>
-__device__ __forceinline__ void ds_load(const T* row, int vi, uint32_t (&w)[4]) {
-    const auto u = *reinterpret_cast<const typename RowVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi);
-    w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
-}
-// The same for logits that are read once: they leave the caches to the gradients on their way out.
+// row_load for logits that are read once: they leave the caches to the gradients on their way out.
 template <typename T>
 __device__ __forceinline__ void ds_load_once(const T* row, int vi, uint32_t (&w)[4]) {
     const auto u = __builtin_nontemporal_load(
@@ -141,7 +135,7 @@ __device__ __forceinline__ ExpSum ds_stream(const T* row, int len, float c, cons
     uint32_t next[U][4];
     auto fetch = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) ds_load<T>(row, min(b + u * kDsThreads, nvec - 1), next[u]);
+        for (int u = 0; u < U; ++u) row_load<T>(row, min(b + u * kDsThreads, nvec - 1), next[u]);
     };
     if (nvec > 0) fetch(tid);
     ready();
@@ -178,7 +172,7 @@ __device__ __forceinline__ float ds_far_sum(const T* row, int len, float c, cons
     float s = 0.0f;
     for (int vi = threadIdx.x; vi < nvec; vi += kDsThreads) {
         uint32_t w[4];
-        ds_load<T>(row, vi, w);
+        row_load<T>(row, vi, w);
         if (BUCKET) ds_drop<T>(bm, vi, w);
         float v[VEC];
         Elem<T>::from_words(w[0], w[1], w[2], w[3], v);
@@ -487,7 +481,7 @@ __global__ __launch_bounds__(kDsThreads) void distill_backward_kernel(DistillArg
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int vi = b + u * kDsThreads;
-                ds_load<T>(row + lo, vi < nvec ? vi : b, w[u]);
+                row_load<T>(row + lo, vi < nvec ? vi : b, w[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {

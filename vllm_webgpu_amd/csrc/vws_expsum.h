@@ -78,4 +78,11 @@ struct ExpRun {
 template <typename T> struct RowVec { typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct RowVec<float> { typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(4))); };
 
+// Vector vi of a row (a 32-bit offset, at most 2 MB, on its pointer).
+template <typename T>
+__device__ __forceinline__ void row_load(const T* row, int vi, uint32_t (&w)[4]) {
+    const auto u = *reinterpret_cast<const typename RowVec<T>::U4*>(reinterpret_cast<const char*>(row) + 16u * (uint32_t)vi);
+    w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
+}
+
 }  // namespace vws

@@ -20,14 +20,9 @@
 namespace vws {
 
 template <typename T>
-__device__ __forceinline__ void vf_load_raw(const T* row, int vi, uint32_t (&w)[4]) {
-    const auto u = *reinterpret_cast<const typename RowVec<T>::U4*>(row + (size_t)vi * Elem<T>::kVec);
-    w[0] = u[0]; w[1] = u[1]; w[2] = u[2]; w[3] = u[3];
-}
-template <typename T>
 __device__ __forceinline__ void vf_load(const T* row, int vi, float (&v)[Elem<T>::kVec]) {
     uint32_t w[4];
-    vf_load_raw<T>(row, vi, w);
+    row_load<T>(row, vi, w);
     Elem<T>::from_words(w[0], w[1], w[2], w[3], v);
 }
 
@@ -135,7 +130,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int vi = b + u * kVfThreads;
-            if (nvec > 0) vf_load_raw<T>(row, vi < nvec ? vi : nvec - 1, next[u]);
+            if (nvec > 0) row_load<T>(row, vi < nvec ? vi : nvec - 1, next[u]);
         }
     };
     fetch(tid);
@@ -297,7 +292,7 @@ __device__ __forceinline__ void vf_vectors(const T* row, int V, FV fv, F f, int 
         uint32_t next[U][4];
         auto fetch = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) vf_load_raw<T>(row, min(b + u * kVfCutThreads, nvec - 1), next[u]);
+            for (int u = 0; u < U; ++u) row_load<T>(row, min(b + u * kVfCutThreads, nvec - 1), next[u]);
         };
         fetch(v0 + tid);
         for (int b = v0 + tid; b < nvec; b += U * kVfCutThreads) {
