@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define VWS_ABI_VERSION 9
+#define VWS_ABI_VERSION 10
 
 /* status codes */
 #define VWS_OK 0
@@ -389,6 +389,147 @@ int vws_distill_forward(const vws_distill_args* args);
 int vws_distill_backward(const vws_distill_args* args);
 int vws_distill_step(const vws_distill_args* args);
 
+/* vws_token_logprobs_*: log-probabilities of given tokens, with entropy, ranks and top alternatives (a
+ * prompt's, verified drafts', rollouts'), and the logits' gradient (no counterpart in the reference,
+ * which returns no log-probabilities).  Row n: logits x [V], z = x / T, token t;
+ *   logprob = z_t - log sum_j exp(z_j), entropy = -sum_j p_j log p_j, p = softmax(z),
+ *   rank = #{j : x_j >= x_t}, and the L largest x_j (the lower index first among equals; NaN never).
+ *   dx_j = (g_l (1{j = t} - p_j) - g_h p_j (log p_j + entropy)) / T of upstream gradients g_l and g_h.
+ * Rows whose token lies outside [0, V) are padding: not read, 0 in every output, -1 in the ids, gradient 0.
+ * Masked logits (-inf) have probability 0 and add nothing to the entropy; a NaN or +inf in a row, or no
+ * logit above -inf, makes its log-probabilities, entropy and gradient NaN.  Where a row has fewer than L
+ * logits that are numbers, the ids past them are -1 and their values NaN.
+ *
+ * The forward writes `saved` for the backward where it is not NULL; the backward reads it, the same inputs
+ * and the upstream gradients.  `grad` has the logits' type and must not overlap them. */
+typedef struct vws_token_logprobs_args {
+    uint32_t struct_size; /* sizeof(vws_token_logprobs_args): ABI guard */
+    int32_t rows;         /* N >= 1 */
+    int32_t vocab;        /* 1 <= V <= VWS_MAX_VOCAB */
+    int32_t dtype;        /* VWS_DTYPE_* of logits and grad */
+    const void* logits;   /* [N, V] */
+    int64_t logits_row_stride;
+    const int32_t* token_ids; /* [N] */
+    float temperature;    /* T >= 1e-5, finite */
+    int32_t num_logprobs; /* L: -1 (no ids, values or ranks), or 0 <= L <= min(VWS_MAX_LOGPROBS, V) */
+    float* logprobs;      /* [N] (forward) */
+    float* entropy;       /* [N] or NULL (forward) */
+    int32_t* logprob_ids; /* [N, L + 1]: the token, then the top L (L >= 0) */
+    float* logprob_vals;  /* [N, L + 1] */
+    int32_t* logprob_ranks; /* [N] */
+    void* saved;          /* vws_token_logprobs_saved_size() bytes, 16-byte aligned, or NULL (forward) */
+    size_t saved_bytes;
+    const float* grad_logprobs; /* [N] or NULL (0) (backward) */
+    const float* grad_entropy;  /* [N] or NULL (0) (backward) */
+    void* grad;           /* [N, V] (backward) */
+    int64_t grad_row_stride;
+    void* workspace;      /* vws_token_logprobs_workspace_size() bytes, clean (vws_workspace_init) (forward) */
+    size_t workspace_bytes;
+    void* stream;
+} vws_token_logprobs_args;
+
+size_t vws_token_logprobs_saved_size(int32_t rows);
+size_t vws_token_logprobs_workspace_size(int32_t rows, int32_t vocab, int32_t num_logprobs);
+int vws_token_logprobs_forward(const vws_token_logprobs_args* args);
+int vws_token_logprobs_backward(const vws_token_logprobs_args* args);
+
+/* The paged cache of one layer's keys and values (no counterpart in the reference, whose cache is one
+ * contiguous buffer a request).  Pages of P tokens (a power of two, 8 <= P <= 256): keys [pages, Hk, P, D],
+ * values [pages, Hk, D, P] (a head's dimension is contiguous over its tokens: the layout that the second
+ * matrix product of an attention reads), bfloat16 or float16, both 16-byte aligned.  A slot is page * P +
+ * place in the page. */
+#define VWS_MAX_TREE_NODES 256
+typedef struct vws_kv_cache {
+    void* k;              /* [pages, Hk, P, D] */
+    void* v;              /* [pages, Hk, D, P] */
+    int64_t k_page_stride; /* elements, a multiple of 8 */
+    int64_t v_page_stride;
+    int32_t num_pages;
+    int32_t page_size;    /* P */
+    int32_t kv_heads;     /* Hk */
+    int32_t head_dim;     /* D: 64, 96, 128, 192 or 256 */
+    int32_t dtype;        /* VWS_DTYPE_BF16 or VWS_DTYPE_F16 */
+} vws_kv_cache;
+
+/* Stores keys and values [T, Hk, D] of T tokens at `slots` (distinct; those outside [0, pages * P) are not
+ * stored), the keys rotated, and writes the rotated queries.  The first R of a head's D dimensions turn in
+ * pairs (i, i + R / 2), or (2i, 2i + 1) if `interleaved`, by the angle position * inv_freq[i] (taken in 64
+ * bits) and are scaled by rope_scale.  Without positions nothing is rotated. */
+typedef struct vws_append_kv_args {
+    uint32_t struct_size; /* sizeof(vws_append_kv_args): ABI guard */
+    int32_t tokens;       /* T >= 1 */
+    vws_kv_cache cache;
+    const void* k;        /* strides in elements; the last dimension is contiguous */
+    int64_t k_token_stride, k_head_stride;
+    const void* v;
+    int64_t v_token_stride, v_head_stride;
+    const int32_t* slots; /* [T] */
+    const int32_t* positions; /* [T] or NULL */
+    const float* inv_freq; /* [R / 2] */
+    int32_t rotary_dim;   /* R: a multiple of 16, at most D */
+    int32_t interleaved;
+    float rope_scale;     /* finite */
+    int32_t heads;        /* Hq, 0 without queries */
+    const void* q;        /* [T, Hq, D] */
+    int64_t q_token_stride, q_head_stride;
+    void* q_out;          /* [T, Hq, D]; may be q's own memory (same strides) */
+    int64_t q_out_token_stride, q_out_head_stride;
+    void* stream;
+} vws_append_kv_args;
+int vws_append_kv(const vws_append_kv_args* args);
+
+/* Moves each request's accepted keys and values up behind its context: of request b, the entries of path
+ * [B, width] (node numbers, strictly increasing from path[b, 0] = 0, padded with -1): entry j's node goes
+ * from position context_lens[b] + path[b, j] to context_lens[b] + j. */
+int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* block_table,
+                   int64_t block_table_row_stride, int32_t max_pages, const int32_t* context_lens,
+                   const int32_t* path, int64_t path_row_stride, int32_t path_width, void* stream);
+
+/* Attention of drafted tokens over a paged cache.  Request b has the nodes cu_nodes[b] .. cu_nodes[b + 1] - 1
+ * (rows of q and out), whose keys and values lie at its positions context_lens[b] and on; position i lies
+ * in page block_table[b, i / P].  Node i sees every position of the context, and of the request's nodes
+ * those whose bit is set in visible[row] (bit j % 32 of word j / 32), or without `visible` the nodes up to
+ * itself.  out = softmax(scale q k^T) v over what it sees, 0 where it sees nothing.  Hq is a multiple of
+ * Hk; query head h reads key head h / (Hq / Hk).  Positions past the block table, in pages outside
+ * [0, pages) and past the request's last node are not seen.  Requests whose bounds do not fit (decreasing,
+ * past T, more than max_nodes) and rows of no request are not written. */
+typedef struct vws_tree_attention_args {
+    uint32_t struct_size; /* sizeof(vws_tree_attention_args): ABI guard */
+    int32_t batch;        /* B >= 1 */
+    vws_kv_cache cache;
+    int32_t nodes;        /* T >= 1 */
+    int32_t max_nodes;    /* of a request: 1 .. VWS_MAX_TREE_NODES */
+    int32_t heads;        /* Hq */
+    const void* q;        /* [T, Hq, D]; strides in elements, the last dimension contiguous */
+    int64_t q_token_stride, q_head_stride;
+    void* out;            /* [T, Hq, D] */
+    int64_t out_token_stride, out_head_stride;
+    const int32_t* block_table; /* [B, max_pages] */
+    int64_t block_table_row_stride;
+    int32_t max_pages;
+    const int32_t* context_lens; /* [B] */
+    const int32_t* cu_nodes;     /* [B + 1] */
+    const uint32_t* visible;     /* [T, >= ceil(max_nodes / 32)] or NULL */
+    int64_t visible_row_stride;
+    float scale;          /* > 0, finite */
+    void* workspace;      /* vws_tree_attention_workspace_size() bytes, 256-byte aligned, clean where it */
+    size_t workspace_bytes; /* overlaps vws_sample_workspace_size(1, 1, 0) */
+    void* stream;
+} vws_tree_attention_args;
+size_t vws_tree_attention_workspace_size(int32_t batch, int32_t max_nodes, int32_t heads, int32_t kv_heads,
+                                         int32_t head_dim, int32_t page_size, int32_t max_pages);
+int vws_tree_attention(const vws_tree_attention_args* args);
+
+/* The walk down each request's tree.  sampled[row] is the token drawn from the target's logits at a node,
+ * tokens[row] the node's own (the root's is not read), parents[row] its parent's number in the request
+ * (less than its own; -1: none).  From node 0 on: the token sampled at the node is emitted, and the walk goes to
+ * the node's first child that holds it, or ends.  out_tokens [B, width] and path [B, width] (the visited
+ * nodes) are padded with -1, num_accepted counts the visited nodes but the root; a walk ends at `width`
+ * nodes.  Requests whose bounds do not fit, or without a node, have num_accepted -1. */
+int vws_accept_tree(int32_t batch, int32_t nodes, const int32_t* sampled, const int32_t* tokens,
+                    const int32_t* parents, const int32_t* cu_nodes, int32_t width, int32_t* out_tokens,
+                    int32_t* path, int32_t* num_accepted, void* stream);
+
 /* Test hook (no counterpart in the reference): the bound, in polls of a few dozen cycles each,
  * of a top-p row's wait for the chunks of its shared passes that other workgroups run (default
  * 2^20; process-wide, read by each vws_sample launch).  A row that stops waiting takes the
@@ -419,7 +560,10 @@ int32_t vws_set_single_pass(int32_t enabled);
 #define VWS_KERNEL_OTHER 5     /* workspace fill, self-test */
 #define VWS_KERNEL_VERIFY 6    /* the kernels of vws_verify_drafts */
 #define VWS_KERNEL_DISTILL 7   /* the kernels of vws_distill_* */
-#define VWS_KERNEL_KINDS 8
+#define VWS_KERNEL_SCORE 8     /* the kernels of vws_token_logprobs_* */
+#define VWS_KERNEL_CACHE 9     /* the kernels of vws_append_kv and vws_compact_kv */
+#define VWS_KERNEL_TREE 10     /* the kernels of vws_tree_attention and vws_accept_tree */
+#define VWS_KERNEL_KINDS 11
 int vws_profile_begin(int32_t max_launches);
 int vws_profile_end(double* ms, int32_t* count);
 

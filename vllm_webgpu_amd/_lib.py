@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(_HERE, "_vws.so")
 # the same kernels built with per-workgroup phase stamps (vws_trace_set; vllm_webgpu_amd/trace.py)
 TRACE_LIB_PATH = os.path.join(_HERE, "_vws_trace.so")
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 OK = 0
 ERR_INVALID_ARGUMENT = 1
 ERR_UNSUPPORTED_DTYPE = 2
@@ -44,6 +44,8 @@ TOPK_MAX = 256
 NOALLOC_SCRATCH_BYTES = 16 << 20
 MAX_DRAFTS = 64
 MAX_TEACHER = 256
+MAX_TREE_NODES = 256
+HEAD_DIMS = (64, 96, 128, 192, 256)
 TAIL_RENORMALIZE = 0
 TAIL_BUCKET = 1
 STATE_OUTPUT = 0
@@ -67,10 +69,14 @@ EXPORTED = (
     "vws_verify_workspace_size", "vws_verify_drafts",
     "vws_distill_saved_size", "vws_distill_workspace_size", "vws_distill_forward",
     "vws_distill_backward", "vws_distill_step",
+    "vws_token_logprobs_saved_size", "vws_token_logprobs_workspace_size", "vws_token_logprobs_forward",
+    "vws_token_logprobs_backward",
+    "vws_append_kv", "vws_compact_kv", "vws_tree_attention_workspace_size", "vws_tree_attention",
+    "vws_accept_tree",
 )
 
 KERNEL_KINDS = ("sample", "topk", "argmax", "softmax", "penalties", "other", "verify",
-                "distill")
+                "distill", "score", "cache", "tree")
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -128,6 +134,55 @@ class DistillArgs(ctypes.Structure):
         ("teacher_logprobs", _P), ("teacher_logprobs_row_stride", _I64), ("row_weight", _P),
         ("loss", _P), ("saved", _P), ("saved_bytes", _SZ), ("grad_output", _P),
         ("grad", _P), ("grad_row_stride", _I64),
+        ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of ``vws_kv_cache``."""
+
+    _fields_ = [
+        ("k", _P), ("v", _P), ("k_page_stride", _I64), ("v_page_stride", _I64), ("num_pages", _I32),
+        ("page_size", _I32), ("kv_heads", _I32), ("head_dim", _I32), ("dtype", _I32),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    """Mirror of ``vws_append_kv_args``."""
+
+    _fields_ = [
+        ("struct_size", _U32), ("tokens", _I32), ("cache", KvCache),
+        ("k", _P), ("k_token_stride", _I64), ("k_head_stride", _I64),
+        ("v", _P), ("v_token_stride", _I64), ("v_head_stride", _I64),
+        ("slots", _P), ("positions", _P), ("inv_freq", _P), ("rotary_dim", _I32), ("interleaved", _I32),
+        ("rope_scale", ctypes.c_float), ("heads", _I32),
+        ("q", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+        ("q_out", _P), ("q_out_token_stride", _I64), ("q_out_head_stride", _I64), ("stream", _P),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """Mirror of ``vws_tree_attention_args``."""
+
+    _fields_ = [
+        ("struct_size", _U32), ("batch", _I32), ("cache", KvCache), ("nodes", _I32), ("max_nodes", _I32),
+        ("heads", _I32), ("q", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+        ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+        ("block_table", _P), ("block_table_row_stride", _I64), ("max_pages", _I32),
+        ("context_lens", _P), ("cu_nodes", _P), ("visible", _P), ("visible_row_stride", _I64),
+        ("scale", ctypes.c_float), ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    """Mirror of ``vws_token_logprobs_args``."""
+
+    _fields_ = [
+        ("struct_size", _U32), ("rows", _I32), ("vocab", _I32), ("dtype", _I32),
+        ("logits", _P), ("logits_row_stride", _I64), ("token_ids", _P), ("temperature", ctypes.c_float),
+        ("num_logprobs", _I32), ("logprobs", _P), ("entropy", _P),
+        ("logprob_ids", _P), ("logprob_vals", _P), ("logprob_ranks", _P), ("saved", _P), ("saved_bytes", _SZ),
+        ("grad_logprobs", _P), ("grad_entropy", _P), ("grad", _P), ("grad_row_stride", _I64),
         ("workspace", _P), ("workspace_bytes", _SZ), ("stream", _P),
     ]
 
@@ -193,6 +248,23 @@ def _declare(L):
     for f in (L.vws_distill_forward, L.vws_distill_backward, L.vws_distill_step):
         f.restype = ctypes.c_int
         f.argtypes = [ctypes.POINTER(DistillArgs)]
+    L.vws_token_logprobs_saved_size.restype = _SZ
+    L.vws_token_logprobs_saved_size.argtypes = [_I32]
+    L.vws_token_logprobs_workspace_size.restype = _SZ
+    L.vws_token_logprobs_workspace_size.argtypes = [_I32, _I32, _I32]
+    for f in (L.vws_token_logprobs_forward, L.vws_token_logprobs_backward):
+        f.restype = ctypes.c_int
+        f.argtypes = [ctypes.POINTER(TokenLogprobsArgs)]
+    L.vws_append_kv.restype = ctypes.c_int
+    L.vws_append_kv.argtypes = [ctypes.POINTER(AppendArgs)]
+    L.vws_compact_kv.restype = ctypes.c_int
+    L.vws_compact_kv.argtypes = [ctypes.POINTER(KvCache), _I32, _P, _I64, _I32, _P, _P, _I64, _I32, _P]
+    L.vws_tree_attention_workspace_size.restype = _SZ
+    L.vws_tree_attention_workspace_size.argtypes = [_I32] * 7
+    L.vws_tree_attention.restype = ctypes.c_int
+    L.vws_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
+    L.vws_accept_tree.restype = ctypes.c_int
+    L.vws_accept_tree.argtypes = [_I32, _I32, _P, _P, _P, _P, _I32, _P, _P, _P, _P]
     L.vws_token_state_update.restype = ctypes.c_int
     L.vws_token_state_update.argtypes = [_P, _I64, _P, _I64, _I32, _I32, _P, _I32, _P, _I32, _P]
 

@@ -3,6 +3,7 @@
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -10,10 +11,13 @@
 #include <mutex>
 #include <string>
 
+#include "vws_cache.h"
 #include "vws_distill.h"
 #include "vws_internal.h"
 #include "vws_plain.h"
 #include "vws_sampler.h"
+#include "vws_score.h"
+#include "vws_tree.h"
 #include "vws_verify.h"
 
 namespace vws {
@@ -40,6 +44,13 @@ template <typename T> __global__ void verify_token_kernel(VerifyArgs);
 template <typename T, bool BUCKET> __global__ void distill_forward_kernel(DistillArgs);
 template <typename T> __global__ void distill_backward_kernel(DistillArgs);
 template <typename T, bool BUCKET, int NV> __global__ void distill_step_kernel(DistillArgs);
+template <typename T, bool ENT, bool TOP> __global__ void score_kernel(ScoreArgs);
+template <typename T> __global__ void score_backward_kernel(ScoreArgs);
+template <typename T> __global__ void append_kernel(AppendArgs);
+__global__ void compact_kernel(CompactArgs);
+template <typename T, int D, int MT, int WM> __global__ void tree_kernel(TreeArgs);
+template <typename T, int D> __global__ void tree_join_kernel(TreeArgs);
+__global__ void accept_kernel(AcceptArgs);
 }  // namespace vws
 
 using namespace vws;
@@ -675,6 +686,261 @@ int distill(const vws_distill_args* a, int parts) {
     return distill_launch<_Float16>(a, parts);
 }
 
+// As the distillation's forward; rows that list their largest logits are joined from fewer parts.
+constexpr int kScoreWgs = 768;
+void score_parts(int rows, int V, int L, int* S, int* len) {
+    split_row(rows, V, kScoreWgs, 4096, L > 0 ? kScMaxTopParts : kScMaxParts, 1, S, len);
+}
+
+int validate_score(const vws_token_logprobs_args* a, bool forward) {
+    if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
+    if (a->struct_size != sizeof(vws_token_logprobs_args))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(vws_token_logprobs_args));
+    if (int st = validate_rows(a->logits, a->dtype, a->rows, a->vocab, a->logits_row_stride)) return st;
+    if (a->rows > kVerifyMaxRows) return fail(VWS_ERR_LIMIT, "rows must be at most %d", kVerifyMaxRows);
+    if (!(a->temperature >= 1e-5f) || a->temperature == __builtin_inff())
+        return fail(VWS_ERR_INVALID_ARGUMENT, "temperature must be finite and >= 1e-5 (got %g)", (double)a->temperature);
+    if (!a->token_ids) return fail(VWS_ERR_INVALID_ARGUMENT, "token_ids is NULL");
+    if (a->saved || !forward) {
+        const size_t saved = vws_token_logprobs_saved_size(a->rows);
+        if (!a->saved || a->saved_bytes < saved)
+            return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "saved has %zu bytes, need %zu", a->saved ? a->saved_bytes : (size_t)0, saved);
+        if (reinterpret_cast<uintptr_t>(a->saved) & 15u) return fail(VWS_ERR_INVALID_ARGUMENT, "saved must be 16-byte aligned");
+    }
+    if (forward) {
+        if (!a->logprobs) return fail(VWS_ERR_INVALID_ARGUMENT, "logprobs is NULL");
+        if (a->num_logprobs < -1 || a->num_logprobs > VWS_MAX_LOGPROBS)
+            return fail(VWS_ERR_LIMIT, "num_logprobs must be in [-1, %d] (got %d)", VWS_MAX_LOGPROBS, a->num_logprobs);
+        if (a->num_logprobs > a->vocab) return fail(VWS_ERR_INVALID_ARGUMENT, "num_logprobs > vocab");
+        if (a->num_logprobs >= 0 && (!a->logprob_ids || !a->logprob_vals || !a->logprob_ranks))
+            return fail(VWS_ERR_INVALID_ARGUMENT, "logprob outputs are NULL while num_logprobs >= 0");
+        const size_t need = vws_token_logprobs_workspace_size(a->rows, a->vocab, a->num_logprobs);
+        if (!a->workspace || a->workspace_bytes < need)
+            return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace ? a->workspace_bytes : (size_t)0, need);
+        if (reinterpret_cast<uintptr_t>(a->workspace) & 255u) return fail(VWS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    } else {
+        if (!a->grad) return fail(VWS_ERR_INVALID_ARGUMENT, "grad is NULL");
+        if (a->grad_row_stride < a->vocab) return fail(VWS_ERR_INVALID_ARGUMENT, "grad_row_stride < vocab");
+        const size_t es = a->dtype == VWS_DTYPE_F32 ? 4 : 2;
+        const uintptr_t x0 = reinterpret_cast<uintptr_t>(a->logits), g0 = reinterpret_cast<uintptr_t>(a->grad);
+        const uintptr_t x1 = x0 + ((size_t)(a->rows - 1) * (size_t)a->logits_row_stride + (size_t)a->vocab) * es;
+        const uintptr_t g1 = g0 + ((size_t)(a->rows - 1) * (size_t)a->grad_row_stride + (size_t)a->vocab) * es;
+        if (x0 < g1 && g0 < x1) return fail(VWS_ERR_INVALID_ARGUMENT, "grad overlaps the logits");
+    }
+    return VWS_OK;
+}
+
+template <typename T>
+int score_rows(const vws_token_logprobs_args* a, bool forward, int r0, int rows) {
+    ScoreArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.x = static_cast<const T*>(a->logits) + (size_t)r0 * a->logits_row_stride;
+    k.xstride = a->logits_row_stride;
+    k.N = rows;
+    k.V = a->vocab;
+    k.ids = a->token_ids + r0;
+    k.c = (float)(1.4426950408889634 / (double)a->temperature);
+    k.inv_T = 1.0f / a->temperature;
+    k.stats = a->saved ? static_cast<float*>(a->saved) + (size_t)r0 * kScRowStats : nullptr;
+    const int K = VWS_KERNEL_SCORE;
+    hipStream_t s = (hipStream_t)a->stream;
+    const dim3 block(kScThreads);
+    if (forward) {
+        const int L = k.L = a->num_logprobs;
+        score_parts(rows, k.V, L, &k.S, &k.part_len);
+        k.logprobs = a->logprobs + r0;
+        k.entropy = a->entropy ? a->entropy + r0 : nullptr;
+        if (L >= 0) {
+            k.lp_ids = a->logprob_ids + (size_t)r0 * (size_t)(L + 1);
+            k.lp_vals = a->logprob_vals + (size_t)r0 * (size_t)(L + 1);
+            k.ranks = a->logprob_ranks + r0;
+        }
+        char* base = static_cast<char*>(a->workspace) + align256(sizeof(CoopState));
+        k.ctr = static_cast<CoopState*>(a->workspace)->topk_ctr;
+        k.rec = reinterpret_cast<ScoreRec*>(base);
+        k.list = reinterpret_cast<uint64_t*>(base + align256(sizeof(ScoreRec) * (size_t)rows * (size_t)k.S));
+        const dim3 grid((unsigned)rows * (unsigned)k.S);
+        if (k.entropy) {
+            if (L >= 0) launch(K, score_kernel<T, true, true>, grid, block, s, k);
+            else launch(K, score_kernel<T, true, false>, grid, block, s, k);
+        } else {
+            if (L >= 0) launch(K, score_kernel<T, false, true>, grid, block, s, k);
+            else launch(K, score_kernel<T, false, false>, grid, block, s, k);
+        }
+        return check_launch("vws_token_logprobs (forward)");
+    }
+    k.gl = a->grad_logprobs ? a->grad_logprobs + r0 : nullptr;
+    k.gh = a->grad_entropy ? a->grad_entropy + r0 : nullptr;
+    k.grad = static_cast<T*>(a->grad) + (size_t)r0 * a->grad_row_stride;
+    k.gstride = a->grad_row_stride;
+    split_row(rows, k.V, kGradWgs, 4096, 1 << 10, 1, &k.S, &k.part_len);
+    launch(K, score_backward_kernel<T>, dim3((unsigned)rows * (unsigned)k.S), block, s, k);
+    return check_launch("vws_token_logprobs (backward)");
+}
+
+template <typename T>
+int score_launch(const vws_token_logprobs_args* a, bool forward) {
+    for (int r0 = 0; r0 < a->rows; r0 += kTopkRows)
+        if (int st = score_rows<T>(a, forward, r0, a->rows - r0 < kTopkRows ? a->rows - r0 : kTopkRows)) return st;
+    return ok();
+}
+
+int score(const vws_token_logprobs_args* a, bool forward) {
+    if (int st = validate_score(a, forward)) return st;
+    if (a->dtype == VWS_DTYPE_F32) return score_launch<float>(a, forward);
+    if (a->dtype == VWS_DTYPE_BF16) return score_launch<uint16_t>(a, forward);
+    return score_launch<_Float16>(a, forward);
+}
+
+// Workgroups of a launch of 256 threads each: 2^32 threads and more run some of their workgroups only.
+constexpr int64_t kMaxWgs = (1 << 24) - 1;
+
+int validate_cache(const vws_kv_cache& c) {
+    if (!c.k || !c.v) return fail(VWS_ERR_INVALID_ARGUMENT, "cache: k or v is NULL");
+    if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15u)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "cache: k and v must be 16-byte aligned");
+    if (c.dtype != VWS_DTYPE_BF16 && c.dtype != VWS_DTYPE_F16)
+        return fail(VWS_ERR_UNSUPPORTED_DTYPE, "unsupported cache dtype %d", c.dtype);
+    if (c.page_size < kCacheMinPage || c.page_size > kCacheMaxPage || (c.page_size & (c.page_size - 1)))
+        return fail(VWS_ERR_LIMIT, "cache: page_size must be a power of two in [%d, %d] (got %d)", kCacheMinPage, kCacheMaxPage, c.page_size);
+    if (c.head_dim != 64 && c.head_dim != 96 && c.head_dim != 128 && c.head_dim != 192 && c.head_dim != 256)
+        return fail(VWS_ERR_LIMIT, "cache: head_dim must be 64, 96, 128, 192 or 256 (got %d)", c.head_dim);
+    if (c.kv_heads < 1 || c.kv_heads > 1024) return fail(VWS_ERR_LIMIT, "cache: kv_heads must be in [1, 1024] (got %d)", c.kv_heads);
+    if (c.num_pages < 1 || (int64_t)c.num_pages * c.page_size > 0x7FFFFFFF)
+        return fail(VWS_ERR_LIMIT, "cache: num_pages must be at least 1 and num_pages * page_size less than 2^31 (got %d pages)", c.num_pages);
+    const int64_t page = (int64_t)c.kv_heads * c.page_size * c.head_dim;
+    if (c.k_page_stride < page || c.v_page_stride < page || ((c.k_page_stride | c.v_page_stride) & 7))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "cache: page strides must be multiples of 8 and at least kv_heads * page_size * head_dim");
+    return VWS_OK;
+}
+
+CacheView cache_view(const vws_kv_cache& c) {
+    CacheView v;
+    v.k = static_cast<uint16_t*>(c.k);
+    v.v = static_cast<uint16_t*>(c.v);
+    v.kps = c.k_page_stride;
+    v.vps = c.v_page_stride;
+    v.pages = c.num_pages;
+    v.pshift = __builtin_ctz((unsigned)c.page_size);
+    v.heads = c.kv_heads;
+    v.D = c.head_dim;
+    return v;
+}
+
+// Tokens of a workgroup that rotates: one, until there are many more workgroups than the chip holds.
+int append_group(int T, int R) {
+    int g = 1;
+    while (g < 8 && T / (2 * g) >= 4096 && 2 * g * (R > 0 ? R : 1) <= kApThreads * 8) g *= 2;
+    return g;
+}
+
+int validate_append(const vws_append_kv_args* a) {
+    if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
+    if (a->struct_size != sizeof(vws_append_kv_args))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(vws_append_kv_args));
+    if (int st = validate_cache(a->cache)) return st;
+    if (a->tokens < 1) return fail(VWS_ERR_INVALID_ARGUMENT, "tokens must be >= 1 (got %d)", a->tokens);
+    if (!a->k || !a->v || !a->slots) return fail(VWS_ERR_INVALID_ARGUMENT, "k, v or slots is NULL");
+    if (a->positions) {
+        if (!a->inv_freq) return fail(VWS_ERR_INVALID_ARGUMENT, "inv_freq is required with positions");
+        if (a->rotary_dim < 16 || a->rotary_dim % 16 || a->rotary_dim > a->cache.head_dim)
+            return fail(VWS_ERR_LIMIT, "rotary_dim must be a multiple of 16 in [16, head_dim] (got %d)", a->rotary_dim);
+        if (!(__builtin_fabsf(a->rope_scale) < __builtin_inff()))
+            return fail(VWS_ERR_INVALID_ARGUMENT, "rope_scale must be finite");
+    }
+    if (a->heads < 0 || a->heads > (1 << 16)) return fail(VWS_ERR_LIMIT, "heads must be in [0, 65536] (got %d)", a->heads);
+    if (a->heads > 0 && (!a->q || !a->q_out)) return fail(VWS_ERR_INVALID_ARGUMENT, "q or q_out is NULL");
+    const int64_t wgs = (int64_t)a->tokens + ((int64_t)a->tokens + kApValueTokens - 1) / kApValueTokens * a->cache.kv_heads;
+    if (wgs > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many tokens (%d)", a->tokens);
+    return VWS_OK;
+}
+
+// How a launch divides its requests' rows and keys.  A workgroup takes up to 128 rows (64 of more than 128
+// dimensions); its four waves share rows first where there are many, keys otherwise.
+struct TreeShape {
+    int mt, wm;       // tiles of 16 rows a wave, waves along the rows
+    int blocks;       // workgroups along the rows
+    int splits, chunk;
+    int rows;         // blocks * 16 * mt * wm
+};
+constexpr int kTreeWgs = 1024;
+constexpr int kTreeMinKeys = 256;
+TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int page_size, int max_pages) {
+    TreeShape t;
+    const int need = max_nodes * (heads / kv_heads);
+    t.mt = need <= 16 || D > 128 ? 1 : 2;
+    t.wm = 1;
+    while (t.wm < 4 && need > 16 * t.mt * t.wm) t.wm *= 2;
+    const int tile = 16 * t.mt * t.wm, step = kTrKeys * (4 / t.wm);
+    t.blocks = (need + tile - 1) / tile;
+    t.rows = t.blocks * tile;
+    const int64_t most = std::min<int64_t>((int64_t)max_pages * page_size, kCacheMaxPosition);
+    const int64_t items = (int64_t)B * kv_heads * t.blocks;
+    int64_t s = std::min<int64_t>(std::min<int64_t>(kTreeWgs / items, most / kTreeMinKeys), kTrMaxSplits);
+    if (s < 1) s = 1;
+    const int64_t chunk = ((most + s - 1) / s + step - 1) / step * step;
+    t.chunk = (int)chunk;
+    t.splits = (int)((most + t.chunk - 1) / t.chunk);
+    return t;
+}
+
+int validate_tree(const vws_tree_attention_args* a) {
+    if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
+    if (a->struct_size != sizeof(vws_tree_attention_args))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(vws_tree_attention_args));
+    if (int st = validate_cache(a->cache)) return st;
+    if (a->batch < 1 || a->nodes < 1) return fail(VWS_ERR_INVALID_ARGUMENT, "batch and nodes must be >= 1 (got %d, %d)", a->batch, a->nodes);
+    if (a->max_nodes < 1 || a->max_nodes > VWS_MAX_TREE_NODES)
+        return fail(VWS_ERR_LIMIT, "max_nodes must be in [1, %d] (got %d)", VWS_MAX_TREE_NODES, a->max_nodes);
+    if (a->heads < 1 || a->heads % a->cache.kv_heads || a->heads / a->cache.kv_heads > 256)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "heads must be a multiple of kv_heads, at most 256 times as many (got %d of %d)", a->heads, a->cache.kv_heads);
+    if (!a->q || !a->out || !a->block_table || !a->context_lens || !a->cu_nodes)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "q, out, block_table, context_lens or cu_nodes is NULL");
+    if (a->max_pages < 1 || a->block_table_row_stride < a->max_pages)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "max_pages must be at least 1 and block_table_row_stride at least max_pages");
+    if (a->visible && a->visible_row_stride < (a->max_nodes + 31) / 32)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "visible_row_stride is less than max_nodes' words");
+    if (!(a->scale > 0.0f) || a->scale == __builtin_inff()) return fail(VWS_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+    const vws_kv_cache& c = a->cache;
+    const TreeShape t = tree_shape(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
+    const int64_t parts = (int64_t)a->batch * t.splits * c.kv_heads, joins = (int64_t)a->batch * c.kv_heads * ((t.rows + 3) / 4);
+    if ((parts + 7) * t.blocks > kMaxWgs || joins > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many requests (%d) for one launch", a->batch);
+    const size_t need = vws_tree_attention_workspace_size(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
+    if (!a->workspace || a->workspace_bytes < need)
+        return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace ? a->workspace_bytes : (size_t)0, need);
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 255u) return fail(VWS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    return VWS_OK;
+}
+
+template <typename T, int D>
+int tree_launch(const TreeArgs& k, const TreeShape& t, hipStream_t s) {
+    const int K = VWS_KERNEL_TREE;
+    const unsigned parts = (unsigned)(k.B * k.splits * k.c.heads);
+    const dim3 grid((parts + 7u) / 8u * 8u * (unsigned)t.blocks), block(kTrThreads);
+    constexpr int M = D > 128 ? 1 : 2;
+    if (t.wm == 4) launch(K, tree_kernel<T, D, M, 4>, grid, block, s, k);
+    else if (t.wm == 2) launch(K, tree_kernel<T, D, M, 2>, grid, block, s, k);
+    else if (t.mt == M) launch(K, tree_kernel<T, D, M, 1>, grid, block, s, k);
+    else launch(K, tree_kernel<T, D, 1, 1>, grid, block, s, k);
+    if (int st = check_launch("vws_tree_attention")) return st;
+    if (k.splits > 1) {
+        launch(K, tree_join_kernel<T, D>, dim3((unsigned)(k.B * k.c.heads) * (unsigned)((k.rows + 3) / 4)), block, s, k);
+        if (int st = check_launch("vws_tree_attention (join)")) return st;
+    }
+    return ok();
+}
+
+template <typename T>
+int tree_launch(const TreeArgs& k, const TreeShape& t, hipStream_t s) {
+    switch (k.c.D) {
+    case 64: return tree_launch<T, 64>(k, t, s);
+    case 96: return tree_launch<T, 96>(k, t, s);
+    case 128: return tree_launch<T, 128>(k, t, s);
+    case 192: return tree_launch<T, 192>(k, t, s);
+    default: return tree_launch<T, 256>(k, t, s);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -1066,6 +1332,152 @@ size_t vws_distill_workspace_size(int32_t rows, int32_t vocab) {
 int vws_distill_forward(const vws_distill_args* args) { return distill(args, kDistillForward); }
 int vws_distill_backward(const vws_distill_args* args) { return distill(args, kDistillBackward); }
 int vws_distill_step(const vws_distill_args* args) { return distill(args, kDistillForward | kDistillBackward); }
+
+size_t vws_token_logprobs_saved_size(int32_t rows) { return rows < 1 ? 0 : sizeof(float) * (size_t)rows * kScRowStats; }
+
+size_t vws_token_logprobs_workspace_size(int32_t rows, int32_t vocab, int32_t num_logprobs) {
+    if (rows < 1 || vocab < 1 || vocab > VWS_MAX_VOCAB || num_logprobs < -1 || num_logprobs > VWS_MAX_LOGPROBS) return 0;
+    // (of the launches of at most kTopkRows rows, the last may be split further than the others)
+    size_t most = 0;
+    for (const int n : {rows < kTopkRows ? rows : kTopkRows, rows % kTopkRows}) {
+        if (!n) continue;
+        int S, len;
+        score_parts(n, vocab, num_logprobs, &S, &len);
+        const size_t recs = (size_t)n * (size_t)S;
+        size_t b = align256(sizeof(ScoreRec) * recs);
+        if (S > 1 && num_logprobs > 0) b += align256(sizeof(uint64_t) * recs * (size_t)num_logprobs);
+        if (b > most) most = b;
+    }
+    return align256(sizeof(CoopState)) + most;
+}
+
+int vws_token_logprobs_forward(const vws_token_logprobs_args* args) { return score(args, true); }
+int vws_token_logprobs_backward(const vws_token_logprobs_args* args) { return score(args, false); }
+
+int vws_append_kv(const vws_append_kv_args* a) {
+    if (int st = validate_append(a)) return st;
+    AppendArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.c = cache_view(a->cache);
+    k.T = a->tokens;
+    k.k = static_cast<const uint16_t*>(a->k);
+    k.kts = a->k_token_stride;
+    k.khs = a->k_head_stride;
+    k.v = static_cast<const uint16_t*>(a->v);
+    k.vts = a->v_token_stride;
+    k.vhs = a->v_head_stride;
+    k.slots = a->slots;
+    k.positions = a->positions;
+    k.inv_freq = a->inv_freq;
+    k.R = a->positions ? a->rotary_dim : 0;
+    k.interleaved = a->interleaved != 0;
+    k.scale = a->rope_scale;
+    k.Hq = a->heads;
+    k.q = static_cast<const uint16_t*>(a->q);
+    k.qts = a->q_token_stride;
+    k.qhs = a->q_head_stride;
+    k.qo = static_cast<uint16_t*>(a->q_out);
+    k.qots = a->q_out_token_stride;
+    k.qohs = a->q_out_head_stride;
+    k.group = append_group(k.T, k.R);
+    k.wgs = (k.T + k.group - 1) / k.group;
+    const unsigned grid = (unsigned)k.wgs + (unsigned)((k.T + kApValueTokens - 1) / kApValueTokens) * (unsigned)k.c.heads;
+    hipStream_t s = (hipStream_t)a->stream;
+    if (a->cache.dtype == VWS_DTYPE_BF16) launch(VWS_KERNEL_CACHE, append_kernel<uint16_t>, dim3(grid), dim3(kApThreads), s, k);
+    else launch(VWS_KERNEL_CACHE, append_kernel<_Float16>, dim3(grid), dim3(kApThreads), s, k);
+    if (int st = check_launch("vws_append_kv")) return st;
+    return ok();
+}
+
+int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* block_table, int64_t block_table_row_stride,
+                   int32_t max_pages, const int32_t* context_lens, const int32_t* path, int64_t path_row_stride,
+                   int32_t path_width, void* stream) {
+    if (!cache) return fail(VWS_ERR_INVALID_ARGUMENT, "cache is NULL");
+    if (int st = validate_cache(*cache)) return st;
+    if (batch < 1) return fail(VWS_ERR_INVALID_ARGUMENT, "batch must be >= 1 (got %d)", batch);
+    if ((int64_t)batch * cache->kv_heads > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many requests (%d) for one launch", batch);
+    if (!block_table || !context_lens || !path) return fail(VWS_ERR_INVALID_ARGUMENT, "block_table, context_lens or path is NULL");
+    if (max_pages < 1 || block_table_row_stride < max_pages)
+        return fail(VWS_ERR_INVALID_ARGUMENT, "max_pages must be at least 1 and block_table_row_stride at least max_pages");
+    if (path_width < 1 || path_width > VWS_MAX_TREE_NODES)
+        return fail(VWS_ERR_LIMIT, "path_width must be in [1, %d] (got %d)", VWS_MAX_TREE_NODES, path_width);
+    if (path_row_stride < path_width) return fail(VWS_ERR_INVALID_ARGUMENT, "path_row_stride < path_width");
+    CompactArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.c = cache_view(*cache);
+    k.table = block_table;
+    k.table_stride = block_table_row_stride;
+    k.max_pages = max_pages;
+    k.context = context_lens;
+    k.path = path;
+    k.path_stride = path_row_stride;
+    k.width = path_width;
+    launch(VWS_KERNEL_CACHE, compact_kernel, dim3((unsigned)batch * (unsigned)k.c.heads), dim3(kApThreads), (hipStream_t)stream, k);
+    if (int st = check_launch("vws_compact_kv")) return st;
+    return ok();
+}
+
+size_t vws_tree_attention_workspace_size(int32_t batch, int32_t max_nodes, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                         int32_t page_size, int32_t max_pages) {
+    if (batch < 1 || max_nodes < 1 || max_nodes > VWS_MAX_TREE_NODES || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
+        page_size < 1 || max_pages < 1)
+        return 0;
+    const TreeShape t = tree_shape(batch, max_nodes, heads, kv_heads, head_dim, page_size, max_pages);
+    const size_t recs = t.splits > 1 ? (size_t)batch * (size_t)t.splits * (size_t)kv_heads * (size_t)t.rows : 0;
+    return align256(sizeof(CoopState)) + align256(sizeof(float) * recs * (size_t)head_dim) + align256(sizeof(float) * 2 * recs);
+}
+
+int vws_tree_attention(const vws_tree_attention_args* a) {
+    if (int st = validate_tree(a)) return st;
+    const vws_kv_cache& c = a->cache;
+    const TreeShape t = tree_shape(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
+    TreeArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.c = cache_view(c);
+    k.B = a->batch;
+    k.T = a->nodes;
+    k.max_nodes = a->max_nodes;
+    k.group = a->heads / c.kv_heads;
+    k.q = static_cast<const uint16_t*>(a->q);
+    k.qts = a->q_token_stride;
+    k.qhs = a->q_head_stride;
+    k.out = static_cast<uint16_t*>(a->out);
+    k.ots = a->out_token_stride;
+    k.ohs = a->out_head_stride;
+    k.table = a->block_table;
+    k.table_stride = a->block_table_row_stride;
+    k.max_pages = a->max_pages;
+    k.context = a->context_lens;
+    k.cu = a->cu_nodes;
+    k.visible = a->visible;
+    k.visible_stride = a->visible_row_stride;
+    k.words = (a->max_nodes + 31) / 32;
+    k.c2 = (float)(1.4426950408889634 * (double)a->scale);
+    k.splits = t.splits;
+    k.chunk = t.chunk;
+    k.blocks = t.blocks;
+    k.rows = t.rows;
+    char* base = static_cast<char*>(a->workspace) + align256(sizeof(CoopState));
+    const size_t recs = (size_t)k.B * (size_t)k.splits * (size_t)k.c.heads * (size_t)k.rows;
+    k.part = reinterpret_cast<float*>(base);
+    k.stat = reinterpret_cast<float*>(base + align256(sizeof(float) * recs * (size_t)c.head_dim));
+    hipStream_t s = (hipStream_t)a->stream;
+    return c.dtype == VWS_DTYPE_BF16 ? tree_launch<uint16_t>(k, t, s) : tree_launch<_Float16>(k, t, s);
+}
+
+int vws_accept_tree(int32_t batch, int32_t nodes, const int32_t* sampled, const int32_t* tokens, const int32_t* parents,
+                    const int32_t* cu_nodes, int32_t width, int32_t* out_tokens, int32_t* path, int32_t* num_accepted, void* stream) {
+    if (batch < 1 || batch > (1 << 24)) return fail(VWS_ERR_LIMIT, "batch must be in [1, 2^24] (got %d)", batch);
+    if (nodes < 0) return fail(VWS_ERR_INVALID_ARGUMENT, "nodes must be >= 0 (got %d)", nodes);
+    if (nodes > 0 && (!sampled || !tokens || !parents)) return fail(VWS_ERR_INVALID_ARGUMENT, "sampled, tokens or parents is NULL");
+    if (!cu_nodes || !out_tokens || !path || !num_accepted) return fail(VWS_ERR_INVALID_ARGUMENT, "cu_nodes or an output is NULL");
+    if (width < 1 || width > VWS_MAX_TREE_NODES)
+        return fail(VWS_ERR_LIMIT, "width must be in [1, %d] (got %d)", VWS_MAX_TREE_NODES, width);
+    const AcceptArgs k{batch, nodes, width, sampled, tokens, parents, cu_nodes, out_tokens, path, num_accepted};
+    launch(VWS_KERNEL_TREE, accept_kernel, dim3((unsigned)batch), dim3(kAcThreads), (hipStream_t)stream, k);
+    if (int st = check_launch("vws_accept_tree")) return st;
+    return ok();
+}
 
 int vws_math_selftest(int32_t fn, uint32_t key_lo, uint32_t key_hi, uint64_t* out2, void* stream) {
     if (fn < 0 || fn > 3) return fail(VWS_ERR_INVALID_ARGUMENT, "fn must be 0 (exp), 1 (log), 2 (soft cap) or 3 (f16 rounding)");

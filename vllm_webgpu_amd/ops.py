@@ -661,6 +661,328 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     return loss, out
 
 
+def _here(dev: torch.device, **tensors) -> None:
+    """Every tensor on ``dev``, which is the current device (whose stream the call takes)."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _check_device(t, name)
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev} (got {t.device})")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors' device must be the current one ({dev} against {torch.cuda.current_device()})")
+
+
+@dataclass
+class TokenLogprobs:
+    logprobs: torch.Tensor              # [N] float32, differentiable in the logits
+    entropy: torch.Tensor | None        # [N] float32, differentiable in the logits
+    logprob_ids: torch.Tensor | None    # [N, L + 1] int32: the token, then the L largest logits'
+    logprob_vals: torch.Tensor | None   # [N, L + 1] float32
+    logprob_ranks: torch.Tensor | None  # [N] int32: logits at least as large as the token's
+
+
+def _score_args(logits: torch.Tensor, ids: torch.Tensor, temperature: float):
+    return _lib.TokenLogprobsArgs(ctypes.sizeof(_lib.TokenLogprobsArgs), logits.shape[0], logits.shape[1],
+                                  _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
+                                  float(temperature))
+
+
+def _score_forward(logits, ids, L: int, entropy: bool, temperature: float, saved: torch.Tensor | None):
+    (N, V), dev = logits.shape, logits.device
+    # (memory of their own: views of one tensor would tie their gradients together)
+    logprobs = torch.empty(N, dtype=torch.float32, device=dev)
+    ent = torch.empty(N, dtype=torch.float32, device=dev) if entropy else None
+    lp_ids = lp_vals = ranks = None
+    if L >= 0:
+        lp_ids = torch.empty((N, L + 1), dtype=torch.int32, device=dev)
+        lp_vals = torch.empty((N, L + 1), dtype=torch.float32, device=dev)
+        ranks = torch.empty(N, dtype=torch.int32, device=dev)
+    if N:
+        lib, stream = _lib.lib(), _stream_ptr()
+        ws = _workspace(lib.vws_token_logprobs_workspace_size(N, V, L), dev.index, stream, _capturing(stream))
+        a = _score_args(logits, ids, temperature)
+        a.num_logprobs, a.logprobs, a.entropy = L, logprobs.data_ptr(), _ptr(ent)
+        a.logprob_ids, a.logprob_vals, a.logprob_ranks = _ptr(lp_ids), _ptr(lp_vals), _ptr(ranks)
+        if saved is not None:
+            a.saved, a.saved_bytes = saved.data_ptr(), 4 * saved.numel()
+        a.workspace, a.workspace_bytes, a.stream = ws.data_ptr(), ws.numel(), stream
+        _lib.check(lib.vws_token_logprobs_forward(ctypes.byref(a)))
+    return logprobs, ent, lp_ids, lp_vals, ranks
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, L, entropy, temperature):
+        ctx.set_materialize_grads(False)
+        saved = torch.empty(8 * logits.shape[0], dtype=torch.float32, device=logits.device)
+        out = _score_forward(logits, ids, L, entropy, temperature, saved)
+        ctx.save_for_backward(logits, ids, saved)
+        ctx.temperature = temperature
+        ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, *unused):
+        logits, ids, saved = ctx.saved_tensors
+        if g_logprobs is None and g_entropy is None:
+            return None, None, None, None, None
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if logits.shape[0]:
+            gl, gh = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy))
+            a = _score_args(logits, ids, ctx.temperature)
+            a.saved, a.saved_bytes = saved.data_ptr(), 4 * saved.numel()
+            a.grad_logprobs, a.grad_entropy = _ptr(gl), _ptr(gh)
+            a.grad, a.grad_row_stride, a.stream = grad.data_ptr(), grad.shape[1], _stream_ptr()
+            _lib.check(_lib.lib().vws_token_logprobs_backward(ctypes.byref(a)))
+        return grad, None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: int | None = None, entropy: bool = False,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """Log-probabilities of given tokens ``token_ids`` [N] under softmax(``logits`` / T), ``logits`` [N, V]
+    (float32, bfloat16 or float16): those of a prompt, of verified drafts or of a rollout.
+
+    ``num_logprobs`` (at most 64 and V): also, as ``sample`` returns them, ``logprob_ids`` and ``logprob_vals``
+    [N, L + 1] (the token, then the L largest logits, the lower index first among equals) and
+    ``logprob_ranks``.  ``entropy``: also -sum p log p.  ``logprobs`` and ``entropy`` are differentiable in ``logits``,
+    whose gradient has their type; the other outputs are not.
+
+    Tokens outside [0, V) pad a row: its logits are not read, its outputs are 0 (ids -1) and its gradient is 0.
+    Logits of -inf have probability 0; a NaN or +inf makes its row NaN."""
+    _check_device(logits, "logits")
+    _here(logits.device, token_ids=token_ids)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, V]")
+    if token_ids.shape != logits.shape[:1] or token_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"token_ids must be int32 or int64 [{logits.shape[0]}] (got {token_ids.dtype} {tuple(token_ids.shape)})")
+    L = -1 if num_logprobs is None else int(num_logprobs)
+    if num_logprobs is not None and not 0 <= L <= min(_lib.MAX_LOGPROBS, logits.shape[1]):
+        raise ValueError(f"num_logprobs must be in [0, {min(_lib.MAX_LOGPROBS, logits.shape[1])}] (got {num_logprobs})")
+    if not 1e-5 <= temperature < float("inf"):
+        raise ValueError(f"temperature must be finite and at least 1e-5 (got {temperature})")
+    logits, ids = _rows(logits), _int32(token_ids).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, L, bool(entropy), float(temperature)))
+    return TokenLogprobs(*_score_forward(logits, ids, L, bool(entropy), float(temperature), None))
+
+
+def _kv_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> _lib.KvCache:
+    if k_cache.dtype not in (torch.bfloat16, torch.float16) or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"k_cache and v_cache must both be bfloat16 or float16 (got {k_cache.dtype}, {v_cache.dtype})")
+    if k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("k_cache must be [pages, kv_heads, page, dim] and v_cache [pages, kv_heads, dim, page]")
+    pages, heads, page, dim = k_cache.shape
+    if v_cache.shape != (pages, heads, dim, page):
+        raise ValueError(f"v_cache must be [{pages}, {heads}, {dim}, {page}] (got {tuple(v_cache.shape)})")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.requires_grad:
+            raise ValueError(f"{name} would get no gradient: detach it")
+        if not t[:1].is_contiguous():
+            raise ValueError(f"{name} must have contiguous pages")
+    size = heads * page * dim
+    # (a single page's stride says nothing)
+    return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0) if pages > 1 else size,
+                        v_cache.stride(0) if pages > 1 else size, pages, page, heads, dim, _dtype_code(k_cache))
+
+
+def _head_rows(t: torch.Tensor, name: str, like: torch.Tensor, heads: int | None, dim: int) -> torch.Tensor:
+    """``t`` [tokens, heads, dim] of the cache's type, its last dimension contiguous."""
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must have the cache's type {like.dtype} (got {t.dtype})")
+    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {heads if heads is not None else 'heads'}, {dim}] (got {tuple(t.shape)})")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(f"{name} would get no gradient: detach it")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _out_rows(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(2) != 1:
+        raise ValueError(f"{name} must have the queries' shape, type and device, its last dimension contiguous")
+    if out.requires_grad:
+        raise ValueError(f"{name} would get no gradient: detach it")
+    T, H, D = out.shape
+    if (H > 1 and out.stride(1) < D) or (T > 1 and out.stride(0) < (H - 1) * out.stride(1) + D):
+        raise ValueError(f"{name} must not overlap itself")
+    return out
+
+
+def _spans(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of each overlaps."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+              q: torch.Tensor | None = None, positions: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+              rope_scale: float = 1.0, interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Appends keys and values [T, kv_heads, dim] of T tokens to a layer's paged cache at ``slots`` [T] (page *
+    page size + place in the page; distinct, those outside the cache are not stored), the position rotation
+    applied to the keys and to ``q`` [T, heads, dim] on the way.  Returns the rotated queries (in ``out``
+    if given, ``q`` itself among them), or None without ``q``.
+
+    The cache's pages are k_cache [pages, kv_heads, page, dim] and v_cache [pages, kv_heads, dim, page]
+    (bfloat16 or float16, contiguous pages; page a power of two from 8 to 256, dim 64, 96, 128, 192 or 256).
+    ``positions`` [T] and ``inv_freq`` [R / 2] float32 (R a multiple of 16): the first R of a head's dimensions turn in
+    pairs (i, i + R / 2), or (2i, 2i + 1) if ``interleaved``, by positions * inv_freq (in 64 bits), scaled by
+    ``rope_scale``; without them nothing is rotated."""
+    cache = _kv_cache(k_cache, v_cache)
+    _here(k_cache.device, k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, q=q, positions=positions, inv_freq=inv_freq)
+    T, D, dev = k.shape[0], cache.head_dim, k_cache.device
+    k, v = _head_rows(k, "k", k_cache, cache.kv_heads, D), _head_rows(v, "v", k_cache, cache.kv_heads, D)
+    if v.shape[0] != T or slots.shape != (T,):
+        raise ValueError(f"v and slots must be of {T} tokens (got {tuple(v.shape)} and {tuple(slots.shape)})")
+    slots = _int32(slots).contiguous()
+    R = 0
+    if positions is not None:
+        if inv_freq is None or inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+            raise ValueError("inv_freq must be float32 [R / 2] with positions")
+        R = 2 * inv_freq.numel()
+        if R < 16 or R % 16 or R > D:
+            raise ValueError(f"inv_freq must hold a multiple of 8 frequencies, at most {D // 2} (got {inv_freq.numel()})")
+        if positions.shape != (T,):
+            raise ValueError(f"positions must be [{T}] (got {tuple(positions.shape)})")
+        positions, inv_freq = _int32(positions).contiguous(), inv_freq.contiguous()
+    elif inv_freq is not None:
+        raise ValueError("positions are required with inv_freq")
+    a = _lib.AppendArgs(ctypes.sizeof(_lib.AppendArgs), T, cache, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                        v.stride(1), slots.data_ptr(), _ptr(positions), _ptr(inv_freq), R, 1 if interleaved else 0, float(rope_scale))
+    if q is None:
+        if out is not None:
+            raise ValueError("out is of the queries: q is required")
+    else:
+        q = _head_rows(q, "q", k_cache, None, D)
+        if q.shape[0] != T:
+            raise ValueError(f"q must be of {T} tokens (got {tuple(q.shape)})")
+        out = _out_rows(out, q, "out")
+        if not (out.data_ptr() == q.data_ptr() and out.stride() == q.stride()) and any(_spans(out, t) for t in (q, k, v)):
+            raise ValueError("out must not overlap the inputs, but be q's own memory")
+        a.heads, a.q, a.q_token_stride, a.q_head_stride = q.shape[1], q.data_ptr(), q.stride(0), q.stride(1)
+        a.q_out, a.q_out_token_stride, a.q_out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
+    if T:
+        a.stream = _stream_ptr()
+        _lib.check(_lib.lib().vws_append_kv(ctypes.byref(a)))
+    return out
+
+
+def _tables(block_table: torch.Tensor, context_lens: torch.Tensor):
+    if block_table.dim() != 2 or context_lens.shape != block_table.shape[:1] or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [batch, pages] and context_lens [batch] (got {tuple(block_table.shape)} and "
+                         f"{tuple(context_lens.shape)})")
+    return _rows(_int32(block_table)), _int32(context_lens).contiguous()
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   context_lens: torch.Tensor, cu_nodes: torch.Tensor, max_nodes: int, visible: torch.Tensor | None = None,
+                   scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens over a paged cache (see ``append_kv``), [T, heads, dim] like ``q``.
+
+    Request b has the nodes ``cu_nodes[b]:cu_nodes[b + 1]`` (rows of ``q``, at most ``max_nodes`` <= 256), whose keys
+    and values have been appended behind its context: node j's at position ``context_lens[b] + j``; position i
+    lies in page ``block_table[b, i // page]``.  A node sees its request's whole context, and of its nodes those
+    whose bit is set in its row of ``visible`` int32 [T, ceil(max_nodes / 32)] (``pack_allowed`` of a bool [T,
+    max_nodes]: its ancestors and itself, in a tree), or without it the nodes up to itself (a chain; one
+    node: plain decoding).  Rows that see nothing are 0.  heads is a multiple of kv_heads; ``scale`` is
+    dim ** -0.5 by default.  The table's width bounds the contexts that the call is laid out for: pass the columns that
+    are in use.  Rows of no request, and of requests whose bounds do not fit, are not written; give ``out`` to keep
+    what they hold.  Scores, sums and products are held in 32 bits; the weights of a softmax are rounded to the
+    cache's type before their product with the values."""
+    cache = _kv_cache(k_cache, v_cache)
+    _here(k_cache.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens,
+          cu_nodes=cu_nodes, visible=visible, out=out)
+    D, dev, N = cache.head_dim, k_cache.device, int(max_nodes)
+    q = _head_rows(q, "q", k_cache, None, D)
+    T, H = q.shape[:2]
+    if H < 1 or H % cache.kv_heads:
+        raise ValueError(f"q's heads must be a multiple of {cache.kv_heads} (got {H})")
+    if not 1 <= N <= _lib.MAX_TREE_NODES:
+        raise ValueError(f"max_nodes must be in [1, {_lib.MAX_TREE_NODES}] (got {max_nodes})")
+    table, context = _tables(block_table, context_lens)
+    B = table.shape[0]
+    if cu_nodes.shape != (B + 1,):
+        raise ValueError(f"cu_nodes must be [{B + 1}] (got {tuple(cu_nodes.shape)})")
+    cu = _int32(cu_nodes).contiguous()
+    if visible is not None:
+        if visible.dtype != torch.int32 or visible.dim() != 2 or visible.shape[0] != T or visible.shape[1] < (N + 31) // 32:
+            raise ValueError(f"visible must be int32 [{T}, {(N + 31) // 32}] (got {visible.dtype} {tuple(visible.shape)})")
+        visible = _rows(visible)
+    out = _out_rows(out, q, "out")
+    if _spans(out, q):
+        raise ValueError("out must not overlap q")
+    if T and B:
+        lib, stream = _lib.lib(), _stream_ptr()
+        ws = _workspace(lib.vws_tree_attention_workspace_size(B, N, H, cache.kv_heads, D, cache.page_size, table.shape[1]), dev.index,
+                        stream, _capturing(stream))
+        a = _lib.TreeAttentionArgs(
+            ctypes.sizeof(_lib.TreeAttentionArgs), B, cache, T, N, H, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
+            out.stride(0), out.stride(1), table.data_ptr(), _row_stride(table), table.shape[1], context.data_ptr(), cu.data_ptr(),
+            _ptr(visible), 0 if visible is None else _row_stride(visible), float(D ** -0.5 if scale is None else scale),
+            ws.data_ptr(), ws.numel(), stream)
+        _lib.check(lib.vws_tree_attention(ctypes.byref(a)))
+    return out
+
+
+@dataclass
+class TreeResult:
+    tokens: torch.Tensor        # [B, max_path] int32: the tokens sampled at the visited nodes, then -1
+    path: torch.Tensor          # [B, max_path] int32: the visited nodes' numbers in their request, then -1
+    num_accepted: torch.Tensor  # [B] int32: visited nodes but the root
+
+
+def accept_tree(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Tensor, max_path: int) -> TreeResult:
+    """Walks each request's tree of drafted tokens down as far as the target's own tokens lead.
+
+    Request b has the nodes ``cu_nodes[b]:cu_nodes[b + 1]`` (at most 256): ``sampled`` [T] is the token drawn from the
+    target's logits at each node, ``tokens`` [T] the node's own token, ``parents`` [T] its parent's number in
+    the request, less than its own (-1: the root, node 0, which holds the last token emitted before).  From the
+    root on, the token sampled at a node is emitted and the walk goes to the node's first child that holds that token,
+    or ends; so every emitted token was drawn from the target's distribution, whatever was drafted, if the nodes'
+    draws are independent (``sample`` over the rows of all nodes).  A walk ends at ``max_path`` <= 256 nodes at the
+    latest.  Requests without a node, or whose bounds do not fit, have num_accepted -1."""
+    _check_device(sampled, "sampled")
+    _here(sampled.device, tokens=tokens, parents=parents, cu_nodes=cu_nodes)
+    T, W, dev = sampled.numel(), int(max_path), sampled.device
+    for name, t in (("sampled", sampled), ("tokens", tokens), ("parents", parents)):
+        if t.shape != (T,) or t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be int32 or int64 [{T}] (got {t.dtype} {tuple(t.shape)})")
+    if cu_nodes.dim() != 1 or cu_nodes.numel() < 1:
+        raise ValueError("cu_nodes must be [batch + 1]")
+    if not 1 <= W <= _lib.MAX_TREE_NODES:
+        raise ValueError(f"max_path must be in [1, {_lib.MAX_TREE_NODES}] (got {max_path})")
+    sampled, tokens, parents, cu = (_int32(t).contiguous() for t in (sampled, tokens, parents, cu_nodes))
+    B = cu.numel() - 1
+    out = torch.empty((2, B, W), dtype=torch.int32, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    if B:
+        _lib.check(_lib.lib().vws_accept_tree(B, T, sampled.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu.data_ptr(), W,
+                                              out[0].data_ptr(), out[1].data_ptr(), accepted.data_ptr(), _stream_ptr()))
+    return TreeResult(out[0], out[1], accepted)
+
+
+def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+               path: torch.Tensor) -> None:
+    """Moves the accepted nodes' keys and values of a layer's paged cache (see ``append_kv``) up behind their
+    contexts, in place: entry j of ``path`` [B, width] (``accept_tree``'s: node numbers, increasing from the root's
+    0, then -1) goes from position ``context_lens[b] + path[b, j]`` to ``context_lens[b] + j``."""
+    cache = _kv_cache(k_cache, v_cache)
+    _here(k_cache.device, v_cache=v_cache, block_table=block_table, context_lens=context_lens, path=path)
+    table, context = _tables(block_table, context_lens)
+    B = table.shape[0]
+    if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= _lib.MAX_TREE_NODES:
+        raise ValueError(f"path must be [{B}, 1 .. {_lib.MAX_TREE_NODES}] (got {tuple(path.shape)})")
+    path = _rows(_int32(path))
+    if B:
+        _lib.check(_lib.lib().vws_compact_kv(ctypes.byref(cache), B, table.data_ptr(), _row_stride(table), table.shape[1],
+                                             context.data_ptr(), path.data_ptr(), _row_stride(path), path.shape[1], _stream_ptr()))
+
+
 def math_selftest(fn: int, key_lo: int, key_hi: int) -> tuple[int, int]:
     """Device hash of exp_det (fn=0), log_det (fn=1) or the soft cap's tanh (fn=2, cap 1) over
     an order-key range; synchronises."""
