@@ -48,7 +48,7 @@ template <typename T, bool ENT, bool TOP> __global__ void score_kernel(ScoreArgs
 template <typename T> __global__ void score_backward_kernel(ScoreArgs);
 template <typename T> __global__ void append_kernel(AppendArgs);
 __global__ void compact_kernel(CompactArgs);
-template <typename T, int D, int MT, int WM> __global__ void tree_kernel(TreeArgs);
+template <typename T, int D, int MT> __global__ void tree_kernel(TreeArgs);
 template <typename T, int D> __global__ void tree_join_kernel(TreeArgs);
 __global__ void accept_kernel(AcceptArgs);
 }  // namespace vws
@@ -855,25 +855,22 @@ int validate_append(const vws_append_kv_args* a) {
     return VWS_OK;
 }
 
-// How a launch divides its requests' rows and keys.  A workgroup takes up to 128 rows (64 of more than 128
-// dimensions); its four waves share rows first where there are many, keys otherwise.
+// How a launch divides its requests' rows and keys: workgroups of one or two tiles of 16 rows (one of more than
+// 128 dimensions), and parts of the keys where the rows alone do not fill the chip.
 struct TreeShape {
-    int mt, wm;       // tiles of 16 rows a wave, waves along the rows
-    int blocks;       // workgroups along the rows
+    int mt;            // tiles of 16 rows
+    int blocks;        // workgroups along the rows
     int splits, chunk;
-    int rows;         // blocks * 16 * mt * wm
+    int rows;          // blocks * 16 * mt
 };
-constexpr int kTreeWgs = 1024;
+constexpr int kTreeWgs = 512;
 constexpr int kTreeMinKeys = 256;
 TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int page_size, int max_pages) {
     TreeShape t;
-    const int need = max_nodes * (heads / kv_heads);
+    const int need = max_nodes * (heads / kv_heads), step = kTrKeys * kTrThreads / 64;
     t.mt = need <= 16 || D > 128 ? 1 : 2;
-    t.wm = 1;
-    while (t.wm < 4 && need > 16 * t.mt * t.wm) t.wm *= 2;
-    const int tile = 16 * t.mt * t.wm, step = kTrKeys * (4 / t.wm);
-    t.blocks = (need + tile - 1) / tile;
-    t.rows = t.blocks * tile;
+    t.blocks = (need + 16 * t.mt - 1) / (16 * t.mt);
+    t.rows = t.blocks * 16 * t.mt;
     const int64_t most = std::min<int64_t>((int64_t)max_pages * page_size, kCacheMaxPosition);
     const int64_t items = (int64_t)B * kv_heads * t.blocks;
     int64_t s = std::min<int64_t>(std::min<int64_t>(kTreeWgs / items, most / kTreeMinKeys), kTrMaxSplits);
@@ -917,11 +914,8 @@ int tree_launch(const TreeArgs& k, const TreeShape& t, hipStream_t s) {
     const int K = VWS_KERNEL_TREE;
     const unsigned parts = (unsigned)(k.B * k.splits * k.c.heads);
     const dim3 grid((parts + 7u) / 8u * 8u * (unsigned)t.blocks), block(kTrThreads);
-    constexpr int M = D > 128 ? 1 : 2;
-    if (t.wm == 4) launch(K, tree_kernel<T, D, M, 4>, grid, block, s, k);
-    else if (t.wm == 2) launch(K, tree_kernel<T, D, M, 2>, grid, block, s, k);
-    else if (t.mt == M) launch(K, tree_kernel<T, D, M, 1>, grid, block, s, k);
-    else launch(K, tree_kernel<T, D, 1, 1>, grid, block, s, k);
+    if (t.mt == 1) launch(K, tree_kernel<T, D, 1>, grid, block, s, k);
+    else launch(K, tree_kernel<T, D, (D > 128 ? 1 : 2)>, grid, block, s, k);
     if (int st = check_launch("vws_tree_attention")) return st;
     if (k.splits > 1) {
         launch(K, tree_join_kernel<T, D>, dim3((unsigned)(k.B * k.c.heads) * (unsigned)((k.rows + 3) / 4)), block, s, k);

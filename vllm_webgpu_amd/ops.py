@@ -661,16 +661,21 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     return loss, out
 
 
-def _here(dev: torch.device, **tensors) -> None:
-    """Every tensor on ``dev``, which is the current device (whose stream the call takes)."""
+def _device_of(idx: int, **tensors) -> None:
+    """Raises for the tensors that are not on device ``idx``, or if that is not the current one (whose stream a call
+    takes): callers compare the indices first."""
     for name, t in tensors.items():
-        if t is None:
-            continue
-        _check_device(t, name)
-        if t.device != dev:
-            raise ValueError(f"{name} must be on {dev} (got {t.device})")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors' device must be the current one ({dev} against {torch.cuda.current_device()})")
+        if t is not None:
+            _check_device(t, name)
+            if t.get_device() != idx:
+                raise ValueError(f"{name} must be on cuda:{idx} (got {t.device})")
+    if idx != torch.cuda.current_device():
+        raise ValueError(f"the tensors' device must be the current one (cuda:{idx} against cuda:{torch.cuda.current_device()})")
+
+
+def _ints(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as contiguous int32 on its device; what does not fit goes to its ends."""
+    return t if t.dtype is torch.int32 and t.is_contiguous() else _int32(t).contiguous()
 
 
 @dataclass
@@ -682,31 +687,22 @@ class TokenLogprobs:
     logprob_ranks: torch.Tensor | None  # [N] int32: logits at least as large as the token's
 
 
-def _score_args(logits: torch.Tensor, ids: torch.Tensor, temperature: float):
-    return _lib.TokenLogprobsArgs(ctypes.sizeof(_lib.TokenLogprobsArgs), logits.shape[0], logits.shape[1],
-                                  _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
-                                  float(temperature))
-
-
 def _score_forward(logits, ids, L: int, entropy: bool, temperature: float, saved: torch.Tensor | None):
     (N, V), dev = logits.shape, logits.device
     # (memory of their own: views of one tensor would tie their gradients together)
     logprobs = torch.empty(N, dtype=torch.float32, device=dev)
-    ent = torch.empty(N, dtype=torch.float32, device=dev) if entropy else None
+    ent = torch.empty_like(logprobs) if entropy else None
     lp_ids = lp_vals = ranks = None
     if L >= 0:
-        lp_ids = torch.empty((N, L + 1), dtype=torch.int32, device=dev)
-        lp_vals = torch.empty((N, L + 1), dtype=torch.float32, device=dev)
-        ranks = torch.empty(N, dtype=torch.int32, device=dev)
+        lp_ids, lp_vals, ranks = ids.new_empty((N, L + 1)), logprobs.new_empty((N, L + 1)), torch.empty_like(ids)
     if N:
-        lib, stream = _lib.lib(), _stream_ptr()
-        ws = _workspace(lib.vws_token_logprobs_workspace_size(N, V, L), dev.index, stream, _capturing(stream))
-        a = _score_args(logits, ids, temperature)
-        a.num_logprobs, a.logprobs, a.entropy = L, logprobs.data_ptr(), _ptr(ent)
-        a.logprob_ids, a.logprob_vals, a.logprob_ranks = _ptr(lp_ids), _ptr(lp_vals), _ptr(ranks)
-        if saved is not None:
-            a.saved, a.saved_bytes = saved.data_ptr(), 4 * saved.numel()
-        a.workspace, a.workspace_bytes, a.stream = ws.data_ptr(), ws.numel(), stream
+        lib, idx = _lib.lib(), dev.index
+        stream = torch._C._cuda_getCurrentRawStream(idx)
+        ws = _workspace(lib.vws_token_logprobs_workspace_size(N, V, L), idx, stream, _capturing(stream))
+        a = _lib.TokenLogprobsArgs(
+            ctypes.sizeof(_lib.TokenLogprobsArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
+            temperature, L, logprobs.data_ptr(), _ptr(ent), _ptr(lp_ids), _ptr(lp_vals), _ptr(ranks), _ptr(saved),
+            0 if saved is None else 4 * saved.numel(), None, None, None, 0, ws.data_ptr(), ws.numel(), stream)
         _lib.check(lib.vws_token_logprobs_forward(ctypes.byref(a)))
     return logprobs, ent, lp_ids, lp_vals, ranks
 
@@ -731,10 +727,11 @@ class _TokenLogprobs(torch.autograd.Function):
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if logits.shape[0]:
             gl, gh = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy))
-            a = _score_args(logits, ids, ctx.temperature)
-            a.saved, a.saved_bytes = saved.data_ptr(), 4 * saved.numel()
-            a.grad_logprobs, a.grad_entropy = _ptr(gl), _ptr(gh)
-            a.grad, a.grad_row_stride, a.stream = grad.data_ptr(), grad.shape[1], _stream_ptr()
+            N, V = logits.shape
+            a = _lib.TokenLogprobsArgs(
+                ctypes.sizeof(_lib.TokenLogprobsArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
+                ctx.temperature, -1, None, None, None, None, None, saved.data_ptr(), 4 * saved.numel(), _ptr(gl), _ptr(gh),
+                grad.data_ptr(), V, None, 0, _stream_ptr())
             _lib.check(_lib.lib().vws_token_logprobs_backward(ctypes.byref(a)))
         return grad, None, None, None, None
 
@@ -751,8 +748,9 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
 
     Tokens outside [0, V) pad a row: its logits are not read, its outputs are 0 (ids -1) and its gradient is 0.
     Logits of -inf have probability 0; a NaN or +inf makes its row NaN."""
-    _check_device(logits, "logits")
-    _here(logits.device, token_ids=token_ids)
+    idx = logits.get_device()
+    if idx < 0 or token_ids.get_device() != idx or idx != torch.cuda.current_device():
+        _device_of(idx, logits=logits, token_ids=token_ids)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, V]")
     if token_ids.shape != logits.shape[:1] or token_ids.dtype not in (torch.int32, torch.int64):
@@ -762,45 +760,47 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
         raise ValueError(f"num_logprobs must be in [0, {min(_lib.MAX_LOGPROBS, logits.shape[1])}] (got {num_logprobs})")
     if not 1e-5 <= temperature < float("inf"):
         raise ValueError(f"temperature must be finite and at least 1e-5 (got {temperature})")
-    logits, ids = _rows(logits), _int32(token_ids).contiguous()
+    logits, ids = _rows(logits), _ints(token_ids)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, L, bool(entropy), float(temperature)))
     return TokenLogprobs(*_score_forward(logits, ids, L, bool(entropy), float(temperature), None))
 
 
 def _kv_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> _lib.KvCache:
-    if k_cache.dtype not in (torch.bfloat16, torch.float16) or v_cache.dtype != k_cache.dtype:
+    if k_cache.dtype not in (torch.bfloat16, torch.float16) or v_cache.dtype is not k_cache.dtype:
         raise TypeError(f"k_cache and v_cache must both be bfloat16 or float16 (got {k_cache.dtype}, {v_cache.dtype})")
     if k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("k_cache must be [pages, kv_heads, page, dim] and v_cache [pages, kv_heads, dim, page]")
     pages, heads, page, dim = k_cache.shape
     if v_cache.shape != (pages, heads, dim, page):
         raise ValueError(f"v_cache must be [{pages}, {heads}, {dim}, {page}] (got {tuple(v_cache.shape)})")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.requires_grad:
-            raise ValueError(f"{name} would get no gradient: detach it")
-        if not t[:1].is_contiguous():
-            raise ValueError(f"{name} must have contiguous pages")
-    size = heads * page * dim
-    # (a single page's stride says nothing)
-    return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0) if pages > 1 else size,
-                        v_cache.stride(0) if pages > 1 else size, pages, page, heads, dim, _dtype_code(k_cache))
+    ks, vs, size = k_cache.stride(), v_cache.stride(), heads * page * dim
+    if ks[1:] != (page * dim, dim, 1) or vs[1:] != (page * dim, page, 1):
+        # (a stride of a single head or token says nothing)
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if pages and not t[:1].is_contiguous():
+                raise ValueError(f"{name} must have contiguous pages")
+    if k_cache.requires_grad or v_cache.requires_grad:
+        raise ValueError("k_cache and v_cache would get no gradient: detach them")
+    # (nor does a single page's)
+    return _lib.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0] if pages > 1 else size, vs[0] if pages > 1 else size, pages,
+                        page, heads, dim, _dtype_code(k_cache))
 
 
 def _head_rows(t: torch.Tensor, name: str, like: torch.Tensor, heads: int | None, dim: int) -> torch.Tensor:
     """``t`` [tokens, heads, dim] of the cache's type, its last dimension contiguous."""
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise TypeError(f"{name} must have the cache's type {like.dtype} (got {t.dtype})")
     if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads if heads is not None else 'heads'}, {dim}] (got {tuple(t.shape)})")
-    if torch.is_grad_enabled() and t.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} would get no gradient: detach it")
     return t if t.stride(2) == 1 else t.contiguous()
 
 
 def _out_rows(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(2) != 1:
         raise ValueError(f"{name} must have the queries' shape, type and device, its last dimension contiguous")
     if out.requires_grad:
@@ -833,13 +833,16 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     ``positions`` [T] and ``inv_freq`` [R / 2] float32 (R a multiple of 16): the first R of a head's dimensions turn in
     pairs (i, i + R / 2), or (2i, 2i + 1) if ``interleaved``, by positions * inv_freq (in 64 bits), scaled by
     ``rope_scale``; without them nothing is rotated."""
-    cache = _kv_cache(k_cache, v_cache)
-    _here(k_cache.device, k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, q=q, positions=positions, inv_freq=inv_freq)
-    T, D, dev = k.shape[0], cache.head_dim, k_cache.device
-    k, v = _head_rows(k, "k", k_cache, cache.kv_heads, D), _head_rows(v, "v", k_cache, cache.kv_heads, D)
+    cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
+    if idx < 0 or any(t is not None and t.get_device() != idx for t in (k, v, v_cache, slots, q, positions, inv_freq)) \
+            or idx != torch.cuda.current_device():
+        _device_of(idx, k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots, q=q, positions=positions, inv_freq=inv_freq)
+    Hk, _, D = k_cache.shape[1:]
+    k, v = _head_rows(k, "k", k_cache, Hk, D), _head_rows(v, "v", k_cache, Hk, D)
+    T = k.shape[0]
     if v.shape[0] != T or slots.shape != (T,):
         raise ValueError(f"v and slots must be of {T} tokens (got {tuple(v.shape)} and {tuple(slots.shape)})")
-    slots = _int32(slots).contiguous()
+    slots = _ints(slots)
     R = 0
     if positions is not None:
         if inv_freq is None or inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
@@ -849,11 +852,11 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             raise ValueError(f"inv_freq must hold a multiple of 8 frequencies, at most {D // 2} (got {inv_freq.numel()})")
         if positions.shape != (T,):
             raise ValueError(f"positions must be [{T}] (got {tuple(positions.shape)})")
-        positions, inv_freq = _int32(positions).contiguous(), inv_freq.contiguous()
+        positions, inv_freq = _ints(positions), inv_freq.contiguous()
     elif inv_freq is not None:
         raise ValueError("positions are required with inv_freq")
-    a = _lib.AppendArgs(ctypes.sizeof(_lib.AppendArgs), T, cache, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                        v.stride(1), slots.data_ptr(), _ptr(positions), _ptr(inv_freq), R, 1 if interleaved else 0, float(rope_scale))
+    ks, vs, qs, os = k.stride(), v.stride(), (0, 0), (0, 0)
+    heads = 0
     if q is None:
         if out is not None:
             raise ValueError("out is of the queries: q is required")
@@ -861,13 +864,15 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         q = _head_rows(q, "q", k_cache, None, D)
         if q.shape[0] != T:
             raise ValueError(f"q must be of {T} tokens (got {tuple(q.shape)})")
-        out = _out_rows(out, q, "out")
-        if not (out.data_ptr() == q.data_ptr() and out.stride() == q.stride()) and any(_spans(out, t) for t in (q, k, v)):
+        given, out = out is not None, _out_rows(out, q, "out")
+        heads, qs, os = q.shape[1], q.stride(), out.stride()
+        if given and not (out.data_ptr() == q.data_ptr() and os == qs) and any(_spans(out, t) for t in (q, k, v)):
             raise ValueError("out must not overlap the inputs, but be q's own memory")
-        a.heads, a.q, a.q_token_stride, a.q_head_stride = q.shape[1], q.data_ptr(), q.stride(0), q.stride(1)
-        a.q_out, a.q_out_token_stride, a.q_out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
     if T:
-        a.stream = _stream_ptr()
+        a = _lib.AppendArgs(
+            ctypes.sizeof(_lib.AppendArgs), T, cache, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], slots.data_ptr(),
+            _ptr(positions), _ptr(inv_freq), R, 1 if interleaved else 0, rope_scale, heads, _ptr(q), qs[0], qs[1], _ptr(out), os[0],
+            os[1], torch._C._cuda_getCurrentRawStream(idx))
         _lib.check(_lib.lib().vws_append_kv(ctypes.byref(a)))
     return out
 
@@ -876,7 +881,7 @@ def _tables(block_table: torch.Tensor, context_lens: torch.Tensor):
     if block_table.dim() != 2 or context_lens.shape != block_table.shape[:1] or block_table.shape[1] < 1:
         raise ValueError(f"block_table must be [batch, pages] and context_lens [batch] (got {tuple(block_table.shape)} and "
                          f"{tuple(context_lens.shape)})")
-    return _rows(_int32(block_table)), _int32(context_lens).contiguous()
+    return _rows(block_table if block_table.dtype is torch.int32 else _int32(block_table)), _ints(context_lens)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -894,37 +899,38 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     are in use.  Rows of no request, and of requests whose bounds do not fit, are not written; give ``out`` to keep
     what they hold.  Scores, sums and products are held in 32 bits; the weights of a softmax are rounded to the
     cache's type before their product with the values."""
-    cache = _kv_cache(k_cache, v_cache)
-    _here(k_cache.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens,
-          cu_nodes=cu_nodes, visible=visible, out=out)
-    D, dev, N = cache.head_dim, k_cache.device, int(max_nodes)
+    cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
+    if idx < 0 or any(t is not None and t.get_device() != idx for t in (q, v_cache, block_table, context_lens, cu_nodes, visible, out)) \
+            or idx != torch.cuda.current_device():
+        _device_of(idx, k_cache=k_cache, q=q, v_cache=v_cache, block_table=block_table, context_lens=context_lens, cu_nodes=cu_nodes,
+                   visible=visible, out=out)
+    (_, Hk, page, D), N = k_cache.shape, int(max_nodes)
     q = _head_rows(q, "q", k_cache, None, D)
-    T, H = q.shape[:2]
-    if H < 1 or H % cache.kv_heads:
-        raise ValueError(f"q's heads must be a multiple of {cache.kv_heads} (got {H})")
+    T, H, _ = q.shape
+    if H < 1 or H % Hk:
+        raise ValueError(f"q's heads must be a multiple of {Hk} (got {H})")
     if not 1 <= N <= _lib.MAX_TREE_NODES:
         raise ValueError(f"max_nodes must be in [1, {_lib.MAX_TREE_NODES}] (got {max_nodes})")
     table, context = _tables(block_table, context_lens)
     B = table.shape[0]
     if cu_nodes.shape != (B + 1,):
         raise ValueError(f"cu_nodes must be [{B + 1}] (got {tuple(cu_nodes.shape)})")
-    cu = _int32(cu_nodes).contiguous()
+    cu = _ints(cu_nodes)
     if visible is not None:
         if visible.dtype != torch.int32 or visible.dim() != 2 or visible.shape[0] != T or visible.shape[1] < (N + 31) // 32:
             raise ValueError(f"visible must be int32 [{T}, {(N + 31) // 32}] (got {visible.dtype} {tuple(visible.shape)})")
         visible = _rows(visible)
-    out = _out_rows(out, q, "out")
-    if _spans(out, q):
+    given, out = out is not None, _out_rows(out, q, "out")
+    if given and _spans(out, q):
         raise ValueError("out must not overlap q")
     if T and B:
-        lib, stream = _lib.lib(), _stream_ptr()
-        ws = _workspace(lib.vws_tree_attention_workspace_size(B, N, H, cache.kv_heads, D, cache.page_size, table.shape[1]), dev.index,
-                        stream, _capturing(stream))
+        lib, stream, W = _lib.lib(), torch._C._cuda_getCurrentRawStream(idx), table.shape[1]
+        ws = _workspace(lib.vws_tree_attention_workspace_size(B, N, H, Hk, D, page, W), idx, stream, _capturing(stream))
+        qs, os = q.stride(), out.stride()
         a = _lib.TreeAttentionArgs(
-            ctypes.sizeof(_lib.TreeAttentionArgs), B, cache, T, N, H, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-            out.stride(0), out.stride(1), table.data_ptr(), _row_stride(table), table.shape[1], context.data_ptr(), cu.data_ptr(),
-            _ptr(visible), 0 if visible is None else _row_stride(visible), float(D ** -0.5 if scale is None else scale),
-            ws.data_ptr(), ws.numel(), stream)
+            ctypes.sizeof(_lib.TreeAttentionArgs), B, cache, T, N, H, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+            table.data_ptr(), _row_stride(table), W, context.data_ptr(), cu.data_ptr(), _ptr(visible),
+            0 if visible is None else _row_stride(visible), D ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), stream)
         _lib.check(lib.vws_tree_attention(ctypes.byref(a)))
     return out
 
@@ -946,9 +952,10 @@ def accept_tree(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
     or ends; so every emitted token was drawn from the target's distribution, whatever was drafted, if the nodes'
     draws are independent (``sample`` over the rows of all nodes).  A walk ends at ``max_path`` <= 256 nodes at the
     latest.  Requests without a node, or whose bounds do not fit, have num_accepted -1."""
-    _check_device(sampled, "sampled")
-    _here(sampled.device, tokens=tokens, parents=parents, cu_nodes=cu_nodes)
-    T, W, dev = sampled.numel(), int(max_path), sampled.device
+    idx = sampled.get_device()
+    if idx < 0 or any(t.get_device() != idx for t in (tokens, parents, cu_nodes)) or idx != torch.cuda.current_device():
+        _device_of(idx, sampled=sampled, tokens=tokens, parents=parents, cu_nodes=cu_nodes)
+    T, W = sampled.numel(), int(max_path)
     for name, t in (("sampled", sampled), ("tokens", tokens), ("parents", parents)):
         if t.shape != (T,) or t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be int32 or int64 [{T}] (got {t.dtype} {tuple(t.shape)})")
@@ -956,14 +963,15 @@ def accept_tree(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
         raise ValueError("cu_nodes must be [batch + 1]")
     if not 1 <= W <= _lib.MAX_TREE_NODES:
         raise ValueError(f"max_path must be in [1, {_lib.MAX_TREE_NODES}] (got {max_path})")
-    sampled, tokens, parents, cu = (_int32(t).contiguous() for t in (sampled, tokens, parents, cu_nodes))
+    sampled, tokens, parents, cu = _ints(sampled), _ints(tokens), _ints(parents), _ints(cu_nodes)
     B = cu.numel() - 1
-    out = torch.empty((2, B, W), dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    out, path = cu.new_empty((2, B, W)).unbind()
+    accepted = cu.new_empty(B)
     if B:
         _lib.check(_lib.lib().vws_accept_tree(B, T, sampled.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu.data_ptr(), W,
-                                              out[0].data_ptr(), out[1].data_ptr(), accepted.data_ptr(), _stream_ptr()))
-    return TreeResult(out[0], out[1], accepted)
+                                              out.data_ptr(), path.data_ptr(), accepted.data_ptr(),
+                                              torch._C._cuda_getCurrentRawStream(idx)))
+    return TreeResult(out, path, accepted)
 
 
 def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
@@ -971,16 +979,18 @@ def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     """Moves the accepted nodes' keys and values of a layer's paged cache (see ``append_kv``) up behind their
     contexts, in place: entry j of ``path`` [B, width] (``accept_tree``'s: node numbers, increasing from the root's
     0, then -1) goes from position ``context_lens[b] + path[b, j]`` to ``context_lens[b] + j``."""
-    cache = _kv_cache(k_cache, v_cache)
-    _here(k_cache.device, v_cache=v_cache, block_table=block_table, context_lens=context_lens, path=path)
+    cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
+    if idx < 0 or any(t.get_device() != idx for t in (v_cache, block_table, context_lens, path)) or idx != torch.cuda.current_device():
+        _device_of(idx, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens, path=path)
     table, context = _tables(block_table, context_lens)
     B = table.shape[0]
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= _lib.MAX_TREE_NODES:
         raise ValueError(f"path must be [{B}, 1 .. {_lib.MAX_TREE_NODES}] (got {tuple(path.shape)})")
-    path = _rows(_int32(path))
+    path = _rows(path if path.dtype is torch.int32 else _int32(path))
     if B:
         _lib.check(_lib.lib().vws_compact_kv(ctypes.byref(cache), B, table.data_ptr(), _row_stride(table), table.shape[1],
-                                             context.data_ptr(), path.data_ptr(), _row_stride(path), path.shape[1], _stream_ptr()))
+                                             context.data_ptr(), path.data_ptr(), _row_stride(path), path.shape[1],
+                                             torch._C._cuda_getCurrentRawStream(idx)))
 
 
 def math_selftest(fn: int, key_lo: int, key_hi: int) -> tuple[int, int]:
