@@ -36,6 +36,7 @@ struct TreeArgs {
     int chunk;                // keys of a part: a multiple of every wave's step
     int blocks;               // workgroups that a part's rows need, at most
     int rows;                 // rows of a part's record (splits > 1)
+    int longest_first;        // requests are served by their length (B <= kTrThreads)
     float* part;              // [B, splits, heads, rows, D] products, then
     float* stat;              // [B, splits, heads, rows, 2] references and sums
 };

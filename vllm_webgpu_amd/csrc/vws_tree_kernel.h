@@ -99,8 +99,8 @@ __device__ __forceinline__ uint32_t tr_seen(const TreeArgs& a, const TrBounds& o
 constexpr int tr_acc(int D, int MT) { return MT * (D / 4 + 2); }
 // Bytes of a step's keys, and of its values, that a wave keeps in LDS.
 constexpr int tr_tile(int D) { return 2 * kTrKeys * D; }
-constexpr int tr_lds(int D, int MT) {
-    const int ring = kTrThreads / 64 * 2 * tr_tile(D), merge = kTrThreads / 128 * 64 * 4 * tr_acc(D, MT);
+constexpr int tr_lds(int D, int MT, int waves) {
+    const int ring = waves * 2 * tr_tile(D), merge = waves / 2 * 64 * 4 * tr_acc(D, MT);
     return ring > merge ? ring : merge;
 }
 
@@ -117,21 +117,32 @@ __device__ __forceinline__ void tr_arrived() {
 // Until what a wave has read from LDS is in its registers, and may be overwritten there.
 __device__ __forceinline__ void tr_read() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The workgroup's waves meet; what each has in flight stays so.
+__device__ __forceinline__ void tr_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // Where a tile keeps 16-byte chunk c of key row i (0 .. 15), and chunk c of dimension row i of its values: lanes
 // that read together lie in different banks.
 template <int D>
 __device__ __forceinline__ int tr_key_place(int c, int i) { return c ^ (i & (D % 128 == 0 ? 15 : D % 64 == 0 ? 7 : 3)); }
 __device__ __forceinline__ int tr_value_place(int c, int i) { return c ^ ((i >> 1 & 2) | ((i >> 1 ^ i >> 3) & 1)); }
 
-// MT tiles of 16 rows, from m0 on; the workgroup's four waves take the keys in turn, 32 at a time, each through LDS
-// of its own (no wave waits for another), and join what they have in LDS.
-template <typename T, int D, int MT>
+// MT tiles of 16 rows for each of WM waves, from m0 on.  The workgroup's waves make WAVES / WM lanes, which take the
+// keys in turn, 32 at a time, each through LDS of its own, and join what they have there.  A lane of one wave waits for
+// no other; the waves of a wider one share its tiles, WM of them in turn, and meet once a step.
+template <typename T, int D, int MT, int WAVES, int WM>
 __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, int b, int h, int split, int m0, char* lds) {
-    constexpr int WK = kTrThreads / 64, KS = D / 32, DT = D / 16, kAcc = tr_acc(D, MT), kStep = WK * kTrKeys;
+    constexpr int WK = WAVES / WM, KS = D / 32, DT = D / 16, kAcc = tr_acc(D, MT), kStep = WK * kTrKeys;
     constexpr int kTile = tr_tile(D), kLoads = D / 16;  // loads of a tile
+    constexpr int kMine = 2 * kLoads / WM;              // ... of a step's two that a wave makes
+    static_assert(2 * kLoads % WM == 0, "");
     typedef TrElem<T> E;
-    const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / WM, wm = wave % WM;
     const int i16 = lane & 15, g = lane >> 4, rows = o.n * a.group;
+    m0 += wm * MT * 16;
     const int k0 = split * a.chunk, k1 = min(o.len, k0 + a.chunk), first = k0 + wk * kTrKeys;
     const int pm = (1 << a.c.pshift) - 1;
     const uint16_t* const kh = a.c.k + (((int64_t)h << a.c.pshift) * D);
@@ -151,7 +162,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
         for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = TrF4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    char* const ring = lds + wk * 2 * kTile;
+    char* const ring = lds + wk * WM * 2 * kTile;
     // the pages of a step's four eights of keys (entries past the request's last are not read), 0 for those that do not exist, and
     // the keys that lie in pages that do
     struct Pages { int p[4]; uint32_t live; };
@@ -167,45 +178,46 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
         }
         return s;
     };
-    auto fetch_k = [&](const Pages& s, int kb) __attribute__((always_inline)) {
+    // Loads [first, last) of a step's keys, then of its values, to the tiles at `to`
+    auto fetch = [&](const Pages& s, int kb, char* to, int first, int last) __attribute__((always_inline)) {
         const uint16_t* at[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) at[e] = kh + (int64_t)s.p[e] * a.c.kps + ((kb + 8 * e) & pm) * D;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int n = 64 * j + lane, key = n / (D / 8), c = n - key * (D / 8), i = (key >> 3) * 4 + (key & 3);
-            const uint16_t* base = at[(64 * j) / D];
-            // (of 96 dimensions a load may span two eights)
-            if ((64 * j) / D != (64 * j + 63) / D) base = key >= 8 * ((64 * j) / D + 1) ? at[(64 * j + 63) / D] : base;
-            tr_fetch(ring + 1024 * j, base + (key & 7) * D + 8 * tr_key_place<D>(c, i));
-        }
-    };
-    auto fetch_v = [&](const Pages& s, int kb) __attribute__((always_inline)) {
         const int r = lane >> 2, e = tr_value_place(lane & 3, r);  // this lane's dimension and eight
         const int p01 = e & 1 ? s.p[1] : s.p[0], p23 = e & 1 ? s.p[3] : s.p[2];
-        const uint16_t* p = vh + (int64_t)(e & 2 ? p23 : p01) * a.c.vps + ((r << a.c.pshift) + ((kb + 8 * e) & pm));
+        const uint16_t* const p = vh + (int64_t)(e & 2 ? p23 : p01) * a.c.vps + ((r << a.c.pshift) + ((kb + 8 * e) & pm));
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) tr_fetch(ring + kTile + 1024 * j, p + ((16 * j) << a.c.pshift));
+        for (int j = 0; j < 2 * kLoads; ++j) {
+            if (j < first || j >= last) continue;
+            if (j < kLoads) {
+                const int n = 64 * j + lane, key = n / (D / 8), c = n - key * (D / 8), i = (key >> 3) * 4 + (key & 3);
+                const uint16_t* base = at[(64 * j) / D];
+                // (of 96 dimensions a load may span two eights)
+                if ((64 * j) / D != (64 * j + 63) / D) base = key >= 8 * ((64 * j) / D + 1) ? at[(64 * j + 63) / D] : base;
+                tr_fetch(to + 1024 * j, base + (key & 7) * D + 8 * tr_key_place<D>(c, i));
+            } else {
+                tr_fetch(to + 1024 * j, p + ((16 * (j - kLoads)) << a.c.pshift));
+            }
+        }
     };
-    auto key_of_tile = [&](int t, int s) __attribute__((always_inline)) {
+    auto key_of_tile = [&](const char* tile, int t, int s) __attribute__((always_inline)) {
         const int key = 8 * (i16 >> 2) + 4 * t + (i16 & 3);
-        return *reinterpret_cast<const TrU4*>(ring + key * (2 * D) + 16 * tr_key_place<D>(4 * s + g, i16));
+        return *reinterpret_cast<const TrU4*>(tile + key * (2 * D) + 16 * tr_key_place<D>(4 * s + g, i16));
     };
-    auto value_of_tile = [&](int dt) __attribute__((always_inline)) {
-        return *reinterpret_cast<const TrU4*>(ring + kTile + (16 * dt + i16) * 64 + 16 * tr_value_place(g, i16));
+    auto value_of_tile = [&](const char* tile, int dt) __attribute__((always_inline)) {
+        return *reinterpret_cast<const TrU4*>(tile + kTile + (16 * dt + i16) * 64 + 16 * tr_value_place(g, i16));
     };
 
-    // one step, of keys kb and on; the tiles take the next one's as soon as the products have read them
-    auto step = [&](int kb, uint32_t live, const Pages& next_pages) __attribute__((always_inline)) {
-        const int next = kb + kStep;
-        const bool more = next < k1, edge = kb + kTrKeys > o.context || live != ~0u;
-        tr_arrived<kLoads>();  // (but for the values)
+    // one step, of keys kb and on, whose tiles lie at `tile`: keys_read once the first product has read the keys,
+    // values_here before the second one reads the values
+    auto step = [&](int kb, uint32_t live, const char* tile, auto keys_read, auto values_here) __attribute__((always_inline)) {
+        const bool edge = kb + kTrKeys > o.context || live != ~0u;
         TrF4 s[MT][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const TrU4 f = key_of_tile(t, k);
+                const TrU4 f = key_of_tile(tile, t, k);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][t] = E::mma(f, q[mt][k], k ? s[mt][t] : TrF4{0.0f, 0.0f, 0.0f, 0.0f});
             }
@@ -224,8 +236,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 }
             }
         }
-        tr_read();
-        if (more) fetch_k(next_pages, next);
+        keys_read();
         bool raise = false;
         float top[MT];
 #pragma unroll
@@ -259,12 +270,11 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[mt][j] = E::pack(e[2 * j], e[2 * j + 1]);
         }
-        if (more) tr_arrived<kLoads>();  // (but for the next keys)
-        else tr_arrived<0>();
+        values_here();
         if (!edge) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const TrU4 f = value_of_tile(dt);
+                const TrU4 f = value_of_tile(tile, dt);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = E::mma(f, p[mt], acc[mt][dt]);
             }
@@ -277,7 +287,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
             for (int w = 0; w < 4; ++w) keep[w] = (tr_bit(have, 2 * w) & 0xFFFFu) | (tr_bit(have, 2 * w + 1) << 16);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                TrU4 f = value_of_tile(dt);
+                TrU4 f = value_of_tile(tile, dt);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const uint32_t x = f[w] & keep[w], bad = tr_odd<E>(x);
@@ -294,7 +304,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                     const uint32_t mine = g == (e >> 3) && ((live >> e) & 1u) ? 0xFFFFu << (16 * (e & 1)) : 0u;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        TrU4 f = value_of_tile(dt);
+                        TrU4 f = value_of_tile(tile, dt);
 #pragma unroll
                         for (int w = 0; w < 4; ++w) f[w] &= w == ((e & 7) >> 1) ? mine & tr_odd<E>(f[w]) : 0u;
 #pragma unroll
@@ -309,13 +319,9 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
             }
         }
         tr_read();
-        if (more) fetch_v(next_pages, next);
     };
 
-    int kb = first;
-    if (kb < k1) {
-        const Pages now = pages_at(kb);
-        fetch_k(now, kb);
+    auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int m = m0 + mt * 16 + i16, node = m / a.group;
@@ -326,17 +332,69 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 q[mt][s] = m < rows ? *reinterpret_cast<const TrU4a2*>(p + 32 * s) : z;
             }
         }
-        fetch_v(now, kb);
-        // (queries are waited for here, not by way of everything in flight in every step)
+    };
+    // (queries are waited for once, not by way of everything in flight in every step)
+    auto q_here = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[mt][s]));
-        uint32_t live = now.live;
-        for (; kb < k1; kb += kStep) {
-            const Pages next = pages_at(kb + kStep);
-            step(kb, live, next);
-            live = next.live;
+    };
+    if (WM == 1) {
+        // a step's tiles take the next one's keys and values as soon as the products have read them
+        if (first < k1) {
+            const Pages now = pages_at(first);
+            fetch(now, first, ring, 0, kLoads);
+            load_q();
+            fetch(now, first, ring, kLoads, 2 * kLoads);
+            q_here();
+            uint32_t live = now.live;
+            for (int kb = first; kb < k1; kb += kStep) {
+                const Pages next = pages_at(kb + kStep);
+                const bool more = kb + kStep < k1;
+                tr_arrived<kLoads>();  // (but for the values)
+                step(kb, live, ring,
+                     [&]() __attribute__((always_inline)) {
+                         tr_read();
+                         if (more) fetch(next, kb + kStep, ring, 0, kLoads);
+                     },
+                     [&]() __attribute__((always_inline)) {
+                         if (more) tr_arrived<kLoads>();  // (but for the next keys)
+                         else tr_arrived<0>();
+                     });
+                if (more) fetch(next, kb + kStep, ring, kLoads, 2 * kLoads);
+                live = next.live;
+            }
+        }
+    } else {
+        // the tiles of WM - 1 steps are on their way or being read; past the last key they are the last page's, not used
+        const int steps = (k1 - k0 + kStep - 1) / kStep;
+        const bool idle = m0 >= rows;
+        uint32_t live[WM];
+        load_q();
+#pragma unroll
+        for (int i = 0; i < WM - 1; ++i) {
+            const Pages s = pages_at(first + i * kStep);
+            fetch(s, first + i * kStep, ring + i * 2 * kTile, wm * kMine, (wm + 1) * kMine);
+            live[i] = s.live;
+        }
+        q_here();
+        for (int i0 = 0; i0 < steps; i0 += WM) {
+#pragma unroll
+            for (int u = 0; u < WM; ++u) {
+                if (i0 + u >= steps) break;
+                const int kb = first + (i0 + u) * kStep;
+                tr_arrived<(WM - 2) * kMine>();
+                tr_meet();  // (this step's tiles are whole, and the last one's have been read)
+                {
+                    constexpr int kAhead = WM - 1;
+                    const int v = (u + kAhead) % WM;
+                    const Pages s = pages_at(kb + kAhead * kStep);
+                    fetch(s, kb + kAhead * kStep, ring + v * 2 * kTile, wm * kMine, (wm + 1) * kMine);
+                    live[v] = s.live;
+                }
+                if (kb < k1 && !idle) step(kb, live[u], ring + u * 2 * kTile, []() {}, []() {});
+            }
         }
     }
     tr_arrived<0>();  // (what lands in LDS lands before it is used for something else)
@@ -351,7 +409,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     auto give = [&](int half) __attribute__((always_inline)) {
         __syncthreads();
         if (wk >= half && wk < 2 * half) {
-            float* to = merge + (wk - half) * kAcc * 64 + lane;
+            float* to = merge + ((wk - half) * WM + wm) * kAcc * 64 + lane;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 to[(2 * mt) * 64] = ref[mt];
@@ -364,7 +422,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
         }
         __syncthreads();
         if (wk < half) {
-            const float* from = merge + wk * kAcc * 64 + lane;
+            const float* from = merge + (wk * WM + wm) * kAcc * 64 + lane;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const float other = from[(2 * mt) * 64], m = __builtin_fmaxf(ref[mt], other), z = m == -kTrInf ? 0.0f : m;
@@ -379,8 +437,8 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
             }
         }
     };
-    static_assert(WK == 4, "two halvings");
-    give(2);
+    if (WK > 4) give(4);
+    if (WK > 2) give(2);
     give(1);
     if (wk > 0) return;
 #pragma unroll
@@ -412,66 +470,110 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     }
 }
 
-// A workgroup's rows: up to MT tiles, as many as its request has there.
-template <typename T, int D, int MT>
-__global__ __launch_bounds__(kTrThreads, 2) void tree_kernel(TreeArgs a) {
-    __shared__ __align__(1024) char lds[tr_lds(D, MT)];
+// A workgroup's rows: up to 16 MT of four waves (two workgroups a compute unit), or up to 64 MT of eight, which share
+// them as its request has them.
+template <typename T, int D, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void tree_kernel(TreeArgs a) {
+    constexpr int kThreads = 64 * WAVES, kRows = 16 * MT * (WAVES > 4 ? 4 : 1);
+    __shared__ __align__(1024) char lds[tr_lds(D, MT, WAVES)];
     // workgroups of the same keys lie eight apart, on one chiplet
     const int per = 8 * a.blocks, item = (blockIdx.x / per) * 8 + (blockIdx.x & 7), mb = (blockIdx.x % per) >> 3;
-    const int bs = item / a.c.heads, h = item - bs * a.c.heads, b = bs / a.splits, split = bs - b * a.splits;
+    const int bs = item / a.c.heads, h = item - bs * a.c.heads, split = bs % a.splits;
+    int b = bs / a.splits;
     if (b >= a.B) return;
     TrBounds o;
+    if (a.longest_first) {
+        // the workgroups that start last would leave most of the chip idle if theirs were the longest requests
+        int* const lens = reinterpret_cast<int*>(lds);
+        const int t = threadIdx.x;
+        int mine = -1;
+        if (t < a.B) mine = tr_bounds(a, t, &o) ? o.len : 0;
+        lens[t] = mine;
+        __syncthreads();
+        int before = 0;
+        for (int i = 0; i < a.B; ++i) before += lens[i] > mine || (lens[i] == mine && i < t) ? 1 : 0;
+        if (t < a.B && before == b) lens[kThreads] = t;
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(lens[kThreads]);
+        __syncthreads();
+    }
     if (!tr_bounds(a, b, &o)) return;
-    const int rows = o.n * a.group, m0 = mb * MT * 16;
-    if (m0 >= rows || (split * a.chunk >= o.len && split > 0)) return;
-    if (MT == 1 || rows - m0 <= 16) tree_rows<T, D, 1>(a, o, b, h, split, m0, lds);
-    else tree_rows<T, D, MT>(a, o, b, h, split, m0, lds);
+    const int m0 = mb * kRows, rows = o.n * a.group - m0;
+    if (rows <= 0 || (split * a.chunk >= o.len && split > 0)) return;
+    if constexpr (WAVES > 4) {
+        if (rows > 2 * 16 * MT) tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds);
+        else if (rows > 16 * MT) tree_rows<T, D, MT, WAVES, 2>(a, o, b, h, split, m0, lds);
+        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds);
+    } else {
+        if (MT == 1 || rows <= 16) tree_rows<T, D, 1, WAVES, 1>(a, o, b, h, split, m0, lds);
+        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds);
+    }
 }
 
-// Joins the parts of a request's rows, a wave each.
+// Joins the parts of a request's rows, 16 bytes of a part's row a lane: D / 4 lanes a row, as many rows of a
+// request's key head as a workgroup has room for.
 template <typename T, int D>
 __global__ __launch_bounds__(kTrThreads) void tree_join_kernel(TreeArgs a) {
     typedef TrElem<T> E;
-    constexpr int N = (D + 63) / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quads = (a.rows + 3) / 4;
-    const int bh = blockIdx.x / quads, m = (blockIdx.x - bh * quads) * 4 + wave, b = bh / a.c.heads, h = bh - b * a.c.heads;
+    constexpr int kLanes = D / 4, kRows = kTrThreads / kLanes;
+    const int tid = threadIdx.x, groups = (a.max_nodes * a.group + kRows - 1) / kRows;
+    const int bh = blockIdx.x / groups, b = bh / a.c.heads, h = bh - b * a.c.heads;
+    const int m = (blockIdx.x - bh * groups) * kRows + tid / kLanes, d = 4 * (tid % kLanes);
     TrBounds o;
-    if (!tr_bounds(a, b, &o) || m >= o.n * a.group) return;
+    if (tid >= kRows * kLanes || !tr_bounds(a, b, &o) || m >= o.n * a.group) return;
     const int parts = max(1, (o.len + a.chunk - 1) / a.chunk);
-    const int64_t first = ((int64_t)b * a.splits * a.c.heads + h) * a.rows + m, pitch = (int64_t)a.c.heads * a.rows;
-    float top = -kTrInf;
-    for (int i = lane; i < parts; i += 64) top = __builtin_fmaxf(top, a.stat[2 * (first + i * pitch)]);
+    const int64_t pitch = (int64_t)a.c.heads * a.rows, first = (int64_t)b * a.splits * pitch + (int64_t)h * a.rows + m;
+    // a running reference, eight parts' loads in flight
+    constexpr int U = 8;
+    float top = -kTrInf, total = 0.0f;
+    TrF4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < parts; i0 += U) {
+        TrF4 x[U];
+        float r[U], s[U];
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) top = __builtin_fmaxf(top, tr_xor(top, s));
-    const float z = top == -kTrInf ? 0.0f : top;
-    float total = 0.0f, v[N];
+        for (int u = 0; u < U; ++u) {
+            const int64_t rec = first + min(i0 + u, parts - 1) * pitch;
+            r[u] = a.stat[2 * rec];
+            s[u] = a.stat[2 * rec + 1];
+            x[u] = *reinterpret_cast<const TrF4*>(a.part + rec * D + d);
+        }
+        float m1 = top;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = 0.0f;
-    for (int i = 0; i < parts; ++i) {
-        const int64_t rec = first + i * pitch;
-        const float f = tr_exp2(a.stat[2 * rec] - z);
-        total += a.stat[2 * rec + 1] * f;
+        for (int u = 0; u < U; ++u) m1 = __builtin_fmaxf(m1, i0 + u < parts ? r[u] : -kTrInf);
+        const float z = m1 == -kTrInf ? 0.0f : m1, f = tr_exp2(top - z);
+        top = m1;
+        total *= f;
+        v *= f;
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (lane + 64 * j < D) v[j] += a.part[rec * D + lane + 64 * j] * f;
+        for (int u = 0; u < U; ++u) {
+            const float w = i0 + u < parts ? tr_exp2(r[u] - z) : 0.0f;
+            if (w != 0.0f) {
+                total += s[u] * w;
+                v += x[u] * w;
+            }
+        }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const int node = m / a.group;
-    uint16_t* p = a.out + (int64_t)(o.t0 + node) * a.ots + (int64_t)(h * a.group + m - node * a.group) * a.ohs;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        if (lane + 64 * j < D) p[lane + 64 * j] = (uint16_t)E::pack(v[j] * inv, 0.0f);
+    typedef uint32_t U2 __attribute__((ext_vector_type(2), aligned(2)));
+    U2 w;
+    w[0] = E::pack(v[0] * inv, v[1] * inv);
+    w[1] = E::pack(v[2] * inv, v[3] * inv);
+    *reinterpret_cast<U2*>(a.out + (int64_t)(o.t0 + node) * a.ots + (int64_t)(h * a.group + m - node * a.group) * a.ohs + d) = w;
 }
 
-#define VWS_TREE(T, D)                                       \
-    template __global__ void tree_kernel<T, D, 1>(TreeArgs);  \
+#define VWS_TREE(T, D)                                         \
+    template __global__ void tree_kernel<T, D, 1, 4>(TreeArgs); \
     template __global__ void tree_join_kernel<T, D>(TreeArgs);
-// (past 128 dimensions two tiles do not fit the registers)
-#define VWS_TREES(T)                                          \
-    VWS_TREE(T, 64) VWS_TREE(T, 96) VWS_TREE(T, 128)          \
-    VWS_TREE(T, 192) VWS_TREE(T, 256)                         \
-    template __global__ void tree_kernel<T, 64, 2>(TreeArgs); \
-    template __global__ void tree_kernel<T, 96, 2>(TreeArgs); \
-    template __global__ void tree_kernel<T, 128, 2>(TreeArgs);
+// (past 128 dimensions neither two tiles fit the registers nor eight waves' tiles the LDS)
+#define VWS_TREES(T)                                              \
+    VWS_TREE(T, 64) VWS_TREE(T, 96) VWS_TREE(T, 128)              \
+    VWS_TREE(T, 192) VWS_TREE(T, 256)                             \
+    template __global__ void tree_kernel<T, 64, 2, 4>(TreeArgs);  \
+    template __global__ void tree_kernel<T, 96, 2, 4>(TreeArgs);  \
+    template __global__ void tree_kernel<T, 128, 2, 4>(TreeArgs); \
+    template __global__ void tree_kernel<T, 64, 2, 8>(TreeArgs);  \
+    template __global__ void tree_kernel<T, 96, 2, 8>(TreeArgs);  \
+    template __global__ void tree_kernel<T, 128, 2, 8>(TreeArgs);
 
 }  // namespace vws
