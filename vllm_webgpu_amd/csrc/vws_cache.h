@@ -10,7 +10,8 @@ namespace vws {
 constexpr int kCacheMinPage = 8, kCacheMaxPage = 256;
 constexpr int kCacheMaxPosition = 0x7FFF0000;  // of a request: what a step's arithmetic adds fits 32 bits
 constexpr int kApThreads = 256;    // threads of a workgroup, all three kernels
-constexpr int kApValueTokens = 64;  // tokens of a workgroup that stores values
+constexpr int kApValueTokens = 32;  // tokens of a workgroup that stores values (at most 64)
+constexpr int kApGroup = 4;         // ... that rotates, at most
 
 // One layer's cache (vws_kv_cache): 16-bit elements whatever their type.
 struct CacheView {

@@ -45,83 +45,120 @@ __device__ __forceinline__ bool cache_slot(const CacheView& c, int slot, int* pa
     return slot >= 0 && *page < c.pages;
 }
 
-// Queries and keys of `group` tokens: cosines and sines once for a token, then 16 bytes of each half of a pair (or
-// of four pairs) at a time.
+// Queries and keys of `group` tokens.  A head is `units` of 16 bytes or 32: pairs of vectors that turn together (or
+// vectors of four pairs), then vectors that do not turn; a thread has one unit of several heads, and loads four of them
+// before it turns any, the first four before the cosines and sines are there.
 template <typename T>
 __device__ __forceinline__ void append_rotate(const AppendArgs& a, float* cs) {
+    constexpr int U = 4;
     const int t0 = blockIdx.x * a.group, n = min(a.group, a.T - t0), half = a.R >> 1, tid = threadIdx.x;
     const CacheView& c = a.c;
+    const int turned = a.interleaved ? a.R >> 3 : half >> 3, units = turned + ((c.D - a.R) >> 3), heads = a.Hq + c.heads;
+    const int first = tid / units, u = tid - first * units, step = kApThreads / units;
+    const bool turns = u < turned, wide = turns && !a.interleaved;
+    const int d = turns ? u * 8 : a.R + (u - turned) * 8;  // the unit's first element
+    // this thread's (token, head), which advances by `step` heads
+    int t = 0, h = first;
+    auto wrap = [&]() __attribute__((always_inline)) {
+        while (h >= heads && t < n) {
+            h -= heads;
+            ++t;
+        }
+    };
+    wrap();
+    bool live = first < step && t < n;  // (the last few threads may have no unit)
+    CacheVec x[U], z[U];
+    uint16_t* to[U];
+    int at[U];  // token, or -1
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            at[i] = -1;
+            if (live) {
+                const uint16_t* from;
+                bool store = true;
+                if (h < a.Hq) {
+                    from = a.q + (int64_t)(t0 + t) * a.qts + (int64_t)h * a.qhs + d;
+                    to[i] = a.qo + (int64_t)(t0 + t) * a.qots + (int64_t)h * a.qohs + d;
+                } else {
+                    int page = 0, off = 0;
+                    store = cache_slot(c, a.slots[t0 + t], &page, &off);
+                    from = a.k + (int64_t)(t0 + t) * a.kts + (int64_t)(h - a.Hq) * a.khs + d;
+                    to[i] = c.k + (int64_t)page * c.kps + ((int64_t)((h - a.Hq) << c.pshift) + off) * c.D + d;
+                }
+                if (store) {
+                    at[i] = t;
+                    x[i] = cache_load(from);
+                    if (wide) z[i] = cache_load(from + half);
+                }
+                h += step;
+                wrap();
+                live = t < n;
+            }
+        }
+    };
+    load();
     for (int i = tid; i < n * half; i += kApThreads) {
-        const int t = i / half, f = i - t * half;
-        double turns = (double)a.positions[t0 + t] * (double)a.inv_freq[f] * 0.15915494309189533577;
-        turns -= __builtin_rint(turns);
+        const int k = i / half, f = i - k * half;
+        double turn = (double)a.positions[t0 + k] * (double)a.inv_freq[f] * 0.15915494309189533577;
+        turn -= __builtin_rint(turn);
         float s, co;
-        sincospif(2.0f * (float)turns, &s, &co);
+        sincospif(2.0f * (float)turn, &s, &co);
         cs[2 * i] = co * a.scale;
         cs[2 * i + 1] = s * a.scale;
     }
     if (half) __syncthreads();
-    // a head's units: pairs of vectors (or vectors) that turn, then vectors that do not
-    const int turned = a.interleaved ? a.R >> 3 : half >> 3, units = turned + ((c.D - a.R) >> 3), heads = a.Hq + c.heads;
-    const int total = n * heads * units;
-    for (int i = tid; i < total; i += kApThreads) {
-        const int hu = i / units, u = i - hu * units, t = hu / heads, h = hu - t * heads;
-        const uint16_t* from;
-        uint16_t* to;
-        if (h < a.Hq) {
-            from = a.q + (int64_t)(t0 + t) * a.qts + (int64_t)h * a.qhs;
-            to = a.qo + (int64_t)(t0 + t) * a.qots + (int64_t)h * a.qohs;
-        } else {
-            int page, off;
-            if (!cache_slot(c, a.slots[t0 + t], &page, &off)) continue;
-            from = a.k + (int64_t)(t0 + t) * a.kts + (int64_t)(h - a.Hq) * a.khs;
-            to = c.k + (int64_t)page * c.kps + ((int64_t)((h - a.Hq) << c.pshift) + off) * c.D;
-        }
-        if (u >= turned) {
-            const int d = a.R + (u - turned) * 8;
-            cache_store(to + d, cache_load(from + d));
-            continue;
-        }
-        float x[8], y[8];
-        if (a.interleaved) {
-            const float* p = cs + 2 * (t * half + u * 4);
-            const CacheVec w = cache_load(from + u * 8);
-            Elem<T>::from_words(w.w[0], w.w[1], w.w[2], w.w[3], x);
+    for (;;) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                y[2 * j] = x[2 * j] * p[2 * j] - x[2 * j + 1] * p[2 * j + 1];
-                y[2 * j + 1] = x[2 * j + 1] * p[2 * j] + x[2 * j] * p[2 * j + 1];
+        for (int i = 0; i < U; ++i) {
+            if (at[i] < 0) continue;
+            if (!turns) {
+                cache_store(to[i], x[i]);
+                continue;
             }
-            cache_store(to + u * 8, cache_pack8<T>(y));
-        } else {
-            const float* p = cs + 2 * (t * half + u * 8);
-            const CacheVec w0 = cache_load(from + u * 8), w1 = cache_load(from + half + u * 8);
-            float z[8], r[8];
-            Elem<T>::from_words(w0.w[0], w0.w[1], w0.w[2], w0.w[3], x);
-            Elem<T>::from_words(w1.w[0], w1.w[1], w1.w[2], w1.w[3], z);
+            float v[8], y[8];
+            Elem<T>::from_words(x[i].w[0], x[i].w[1], x[i].w[2], x[i].w[3], v);
+            if (!wide) {
+                const float* p = cs + 2 * (at[i] * half + u * 4);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                y[j] = x[j] * p[2 * j] - z[j] * p[2 * j + 1];
-                r[j] = z[j] * p[2 * j] + x[j] * p[2 * j + 1];
+                for (int j = 0; j < 4; ++j) {
+                    y[2 * j] = v[2 * j] * p[2 * j] - v[2 * j + 1] * p[2 * j + 1];
+                    y[2 * j + 1] = v[2 * j + 1] * p[2 * j] + v[2 * j] * p[2 * j + 1];
+                }
+                cache_store(to[i], cache_pack8<T>(y));
+            } else {
+                const float* p = cs + 2 * (at[i] * half + u * 8);
+                float w[8], r[8];
+                Elem<T>::from_words(z[i].w[0], z[i].w[1], z[i].w[2], z[i].w[3], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = v[j] * p[2 * j] - w[j] * p[2 * j + 1];
+                    r[j] = w[j] * p[2 * j] + v[j] * p[2 * j + 1];
+                }
+                cache_store(to[i], cache_pack8<T>(y));
+                cache_store(to[i] + half, cache_pack8<T>(r));
             }
-            cache_store(to + u * 8, cache_pack8<T>(y));
-            cache_store(to + half + u * 8, cache_pack8<T>(r));
         }
+        if (!live) break;
+        load();
     }
 }
 
 // Values of one head: a page keeps a dimension's tokens together, so a tile of tokens is turned in LDS.  Eight
-// tokens whose slots fill an aligned eighth of a page (a run's inside) leave as one 16-byte store for
-// each dimension; a token is looked up where its eight would begin, which another tile may hold.
+// tokens whose slots fill an aligned eighth of a page (a run's inside) leave as one 16-byte store for each
+// dimension, the eights of one dimension side by side; other tokens element by element.  A token is looked up where its
+// eight would begin, which another tile may hold.
 struct AppendValues {
     int32_t slot[kApValueTokens + 14];  // from 7 tokens before the tile to 7 behind it; -1: none
-    uint16_t x[(kApValueTokens + 7) * (256 + 2)];
+    int32_t eight[kApValueTokens], one[kApValueTokens];  // tokens that begin an eight, tokens of none
+    uint32_t eights, ones;
 };
-__device__ __forceinline__ void append_values(const AppendArgs& a, AppendValues& sh) {
+__device__ __forceinline__ void append_values(const AppendArgs& a, AppendValues& sh, uint16_t* x) {
     const CacheView& c = a.c;
     const int b = blockIdx.x - a.wgs, tile = b / c.heads, h = b - tile * c.heads, t0 = tile * kApValueTokens, tid = threadIdx.x;
     const int n = min(kApValueTokens, a.T - t0), have = min(kApValueTokens + 7, a.T - t0), D = c.D, pitch = D + 2, vecs = D >> 3;
     const int most = c.pages << c.pshift;  // (at most 2^31 - 1: the launcher's check)
+    if (tid < 2) (tid ? sh.ones : sh.eights) = 0u;
     for (int i = tid; i < kApValueTokens + 14; i += kApThreads) {
         const int t = t0 - 7 + i;
         const int s = t >= 0 && t < a.T ? a.slots[t] : -1;
@@ -130,53 +167,62 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, AppendValues&
     for (int i = tid; i < have * vecs; i += kApThreads) {
         const int t = i / vecs, d = (i - t * vecs) * 8;
         const CacheVec w = cache_load(a.v + (int64_t)(t0 + t) * a.vts + (int64_t)h * a.vhs + d);
-        uint32_t* to = reinterpret_cast<uint32_t*>(sh.x + t * pitch + d);
+        uint32_t* to = reinterpret_cast<uint32_t*>(x + t * pitch + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = w.w[j];
     }
     __syncthreads();
-    // whether eight slots in a row begin at the tile's token i (from -7 on)
-    auto eight = [&](int i) {
-        if (i < -7 || i + 7 >= kApValueTokens + 7) return false;
-        const int s = sh.slot[i + 7];
-        if (s < 0 || (s & 7)) return false;
+    if (tid < n && sh.slot[tid + 7] >= 0) {
+        // whether the eight slots from where this token's eight begins (7 tokens before the tile at the earliest) follow
+        // each other
+        const int begin = tid + 7 - (sh.slot[tid + 7] & 7), s0 = sh.slot[tid + 7] & ~7;
+        bool whole = true;
 #pragma unroll
-        for (int j = 1; j < 8; ++j)
-            if (sh.slot[i + 7 + j] != s + j) return false;
-        return true;
-    };
+        for (int j = 0; j < 8; ++j) whole &= sh.slot[begin + j] == s0 + j;
+        if (!whole) sh.one[atomicAdd(&sh.ones, 1u)] = tid;
+    }
+    __syncthreads();
+    // (in order, so that neighbours are stored together)
+    if (tid < 64) {
+        const int s = tid < n ? sh.slot[tid + 7] : -1;
+        bool begins = s >= 0 && (s & 7) == 0;
+        if (begins) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) begins &= sh.slot[tid + 7 + j] == s + j;
+        }
+        const uint64_t all = wave_ballot(begins);
+        if (begins) sh.eight[lane_prefix(all)] = tid;
+        if (tid == 0) sh.eights = (uint32_t)__builtin_popcountll(all);
+    }
+    __syncthreads();
     auto at = [&](int s, int d) {
         return c.v + (int64_t)(s >> c.pshift) * c.vps + ((int64_t)(h * D + d) << c.pshift) + (s & ((1 << c.pshift) - 1));
     };
-    const int wave = tid >> 6, lane = tid & 63;
-    for (int i = wave; i < n; i += kApThreads / 64) {
-        const int s = sh.slot[i + 7];
-        if (s < 0) continue;
-        const int first = i - (s & 7);
-        if (eight(first)) {
-            if (first != i) continue;  // (its eight's first token stores it)
-            for (int d = lane; d < D; d += 64) {
-                CacheVec v;
+    const int eights = (int)sh.eights, ones = (int)sh.ones;
+    constexpr int kSide = kApValueTokens / 8;
+    for (int i = tid; i < kSide * D; i += kApThreads) {
+        const int e = i % kSide, d = i / kSide;
+        if (e >= eights) continue;
+        const int t = sh.eight[e];
+        CacheVec v;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v.w[j] = (uint32_t)sh.x[(i + 2 * j) * pitch + d] | ((uint32_t)sh.x[(i + 2 * j + 1) * pitch + d] << 16);
-                cache_store(at(s, d), v);
-            }
-        } else {
-            for (int d = lane; d < D; d += 64) *at(s, d) = sh.x[i * pitch + d];
-        }
+        for (int j = 0; j < 4; ++j) v.w[j] = (uint32_t)x[(t + 2 * j) * pitch + d] | ((uint32_t)x[(t + 2 * j + 1) * pitch + d] << 16);
+        cache_store(at(sh.slot[t + 7], d), v);
+    }
+    const int wave = tid >> 6, lane = tid & 63;
+    for (int i = wave; i < ones; i += kApThreads / 64) {
+        const int t = sh.one[i];
+        for (int d = lane; d < D; d += 64) *at(sh.slot[t + 7], d) = x[t * pitch + d];
     }
 }
 
 // Keys rotated, queries rotated, values turned: one launch, the rotating workgroups first.
 template <typename T>
 __global__ __launch_bounds__(kApThreads) void append_kernel(AppendArgs a) {
-    __shared__ union {
-        float cs[kApThreads * 8];
-        AppendValues v;
-    } sh;
-    if ((int)blockIdx.x < a.wgs) append_rotate<T>(a, sh.cs);
-    else append_values(a, sh.v);
+    extern __shared__ __align__(16) char append_lds[];
+    __shared__ AppendValues sh;
+    if ((int)blockIdx.x < a.wgs) append_rotate<T>(a, reinterpret_cast<float*>(append_lds));
+    else append_values(a, sh, reinterpret_cast<uint16_t*>(append_lds));
 }
 
 // A request's position; false where it lies in no page (what it leaves then is no place).

@@ -827,12 +827,8 @@ CacheView cache_view(const vws_kv_cache& c) {
     return v;
 }
 
-// Tokens of a workgroup that rotates: one, until there are many more workgroups than the chip holds.
-int append_group(int T, int R) {
-    int g = 1;
-    while (g < 8 && T / (2 * g) >= 4096 && 2 * g * (R > 0 ? R : 1) <= kApThreads * 8) g *= 2;
-    return g;
-}
+// Tokens of a workgroup that rotates: one, until there are more workgroups than the chip holds.
+int append_group(int T) { return T >= 8192 ? kApGroup : T >= 4096 ? 2 : 1; }
 
 int validate_append(const vws_append_kv_args* a) {
     if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
@@ -1386,12 +1382,14 @@ int vws_append_kv(const vws_append_kv_args* a) {
     k.qo = static_cast<uint16_t*>(a->q_out);
     k.qots = a->q_out_token_stride;
     k.qohs = a->q_out_head_stride;
-    k.group = append_group(k.T, k.R);
+    k.group = append_group(k.T);
     k.wgs = (k.T + k.group - 1) / k.group;
     const unsigned grid = (unsigned)k.wgs + (unsigned)((k.T + kApValueTokens - 1) / kApValueTokens) * (unsigned)k.c.heads;
     hipStream_t s = (hipStream_t)a->stream;
-    if (a->cache.dtype == VWS_DTYPE_BF16) launch(VWS_KERNEL_CACHE, append_kernel<uint16_t>, dim3(grid), dim3(kApThreads), s, k);
-    else launch(VWS_KERNEL_CACHE, append_kernel<_Float16>, dim3(grid), dim3(kApThreads), s, k);
+    const unsigned turns = (unsigned)(k.group * k.R) * sizeof(float), values = (kApValueTokens + 7) * (unsigned)(k.c.D + 2) * 2u;
+    const unsigned lds = turns > values ? turns : values;
+    if (a->cache.dtype == VWS_DTYPE_BF16) launch_lds(VWS_KERNEL_CACHE, append_kernel<uint16_t>, dim3(grid), dim3(kApThreads), lds, s, k);
+    else launch_lds(VWS_KERNEL_CACHE, append_kernel<_Float16>, dim3(grid), dim3(kApThreads), lds, s, k);
     if (int st = check_launch("vws_append_kv")) return st;
     return ok();
 }

@@ -177,16 +177,23 @@ __device__ __attribute__((noinline)) void sc_ties(const T* row, int len, int lo,
     __syncthreads();
 }
 
-// The L largest of sh.cand (sh.cands of them), in order, to sh.top; none: 0.  After a barrier; ends with one.
+// The L largest of sh.cand (sh.cands of them), in order, to sh.top; none: 0.  After a barrier; ends with one.  A
+// candidate's place is the number of larger ones, counted by eight neighbouring threads.
 __device__ __forceinline__ void sc_sort(ScShared& sh, int L) {
-    const int tid = threadIdx.x, n = (int)sh.cands;
+    constexpr int kSide = 8;
+    const int tid = threadIdx.x, side = tid % kSide, n = (int)sh.cands;
     if (tid < L) sh.top[tid] = 0u;
     __syncthreads();
-    for (int i = tid; i < n; i += kScThreads) {
-        const uint64_t k = sh.cand[i];
-        int at = 0;
-        for (int j = 0; j < n; ++j) at += sh.cand[j] > k ? 1 : 0;
-        if (at < L && k) sh.top[at] = k;
+    for (int i0 = 0; i0 < n; i0 += kScThreads / kSide) {
+        const int i = i0 + tid / kSide;
+        const uint64_t k = i < n ? sh.cand[i] : 0u;
+        uint32_t at = 0u;
+#pragma unroll 4
+        for (int j = side; j < n; j += kSide) at += sh.cand[j] > k ? 1u : 0u;
+        at += lane_xor(at, 1);
+        at += lane_xor(at, 2);
+        at += lane_xor(at, 4);
+        if (side == 0 && at < (uint32_t)L && k) sh.top[at] = k;
     }
     __syncthreads();
 }
@@ -196,14 +203,26 @@ template <typename T>
 __device__ __forceinline__ void sc_top(const T* row, int len, int lo, int L, int per, float own, ScShared& sh) {
     constexpr int VEC = Elem<T>::kVec, U = 4;
     const int tid = threadIdx.x, nvec = len / VEC;
-    // (the threads' maxima lie where the candidates will: gmax[kScSlots] has been folded into `own`)
+    // The L-th largest of the threads' maxima, or, where L is small, the largest of the waves' own L-th largest: as good a
+    // bound, without looking at every thread's (L = 32: some 130 candidates in place of 32).
     __shared__ float tops[kScThreads];
-    tops[tid] = own;
     if (tid == 0) sh.groups = sh.cands = 0u;
-    __syncthreads();
-    {
+    if (L <= 32) {
+        const uint32_t key = wave_mth_largest64_count(key_of(own), L);
+        if ((tid & 63) == 0) tops[tid >> 6] = val_of(key);
+        __syncthreads();
+        if (tid == 0) {
+            float t = tops[0];
+#pragma unroll
+            for (int i = 1; i < kScThreads / 64; ++i) t = __builtin_fmaxf(t, tops[i]);
+            sh.t = t;
+        }
+    } else {
+        tops[tid] = own;
+        __syncthreads();
         int at = 0;
         const float4* q = reinterpret_cast<const float4*>(tops);
+#pragma unroll 4
         for (int j = 0; j < kScThreads / 4; ++j) {
             const float4 v = q[j];
             at += v.x > own || (v.x == own && 4 * j < tid) ? 1 : 0;
@@ -260,6 +279,16 @@ __global__ __launch_bounds__(kScThreads) void score_kernel(ScoreArgs a) {
     __shared__ ScShared sh;
     __shared__ uint32_t last;
     const int S = a.S, r = blockIdx.x / S, p = blockIdx.x - r * S, tid = threadIdx.x, L = a.L;
+    const T* whole = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
+    const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
+    const T* row = whole + lo;
+    uint32_t next[U][4];
+    auto fetch = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) row_load<T>(row, min(b + u * kScThreads, nvec - 1), next[u]);
+    };
+    // (rows that are split are few: they need not wait for their token, which pads a row at the cost of these loads)
+    if (S > 1 && nvec > 0) fetch(tid);
     const int token = a.ids[r];
     if (token < 0 || token >= a.V) {  // padding: not read
         if (p == 0) {
@@ -276,9 +305,6 @@ __global__ __launch_bounds__(kScThreads) void score_kernel(ScoreArgs a) {
         }
         return;
     }
-    const T* whole = static_cast<const T*>(a.x) + (size_t)r * a.xstride;
-    const int lo = p * a.part_len, len = min(a.V, lo + a.part_len) - lo, nvec = len / VEC;
-    const T* row = whole + lo;
     const float c = a.c, xt = Elem<T>::load1(whole + token);
     const int batches = (nvec + U * kScThreads - 1) / (U * kScThreads), per = max(1, (batches + kScSlots - 1) / kScSlots);
 
@@ -286,11 +312,6 @@ __global__ __launch_bounds__(kScThreads) void score_kernel(ScoreArgs a) {
     ExpRun run(c);
     float wsum = 0.0f, own = -kExpInf;
     uint32_t rank = 0u;
-    uint32_t next[U][4];
-    auto fetch = [&](int b) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) row_load<T>(row, min(b + u * kScThreads, nvec - 1), next[u]);
-    };
     auto add = [&](float g, const auto& v) __attribute__((always_inline)) {
         constexpr int n = sizeof(v) / sizeof(float);
         const float was = run.ref, had = run.s, kept = run.raise(g, c);
@@ -305,7 +326,7 @@ __global__ __launch_bounds__(kScThreads) void score_kernel(ScoreArgs a) {
         run.s = (s[0] + s[1]) + (s[2] + s[3]);
         if (ENT) wsum = (w[0] + w[1]) + (w[2] + w[3]);
     };
-    if (nvec > 0) fetch(tid);
+    if (S == 1 && nvec > 0) fetch(tid);
     if (TOP) {
 #pragma unroll
         for (int s = 0; s <= kScSlots; ++s) sh.gmax[s * kScThreads + tid] = -kExpInf;
@@ -422,8 +443,17 @@ __global__ __launch_bounds__(kScThreads) void score_kernel(ScoreArgs a) {
         if (TOP) {
             VWS_BUTTERFLY(rank, lane_xor, sc_plus);
             if (L > 0) {
-                for (int i = tid; i < S * L; i += kScThreads) sh.cand[i] = ag_load64(&a.list[(size_t)r * S * L + i]);
-                if (tid == 0) sh.cands = (uint32_t)(S * L);
+                // every part's first ceil(L / S) reach the least of those parts' last: L together
+                const uint64_t* list = a.list + (size_t)r * S * L;
+                const int deep = (L + S - 1) / S;
+                const uint32_t least = part < S ? (uint32_t)(ag_load64(list + (size_t)part * L + deep - 1) >> 32) : ~0u;
+                const uint32_t t = wave_min_u32(least);
+                if (tid == 0) sh.cands = 0u;
+                __syncthreads();
+                for (int i = tid; i < S * L; i += kScThreads) {
+                    const uint64_t k = ag_load64(list + i);
+                    if (k && (uint32_t)(k >> 32) >= t) sh.cand[atomicAdd(&sh.cands, 1u)] = k;
+                }
                 __syncthreads();
                 sc_sort(sh, L);
             }

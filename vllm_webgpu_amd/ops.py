@@ -749,7 +749,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
     Tokens outside [0, V) pad a row: its logits are not read, its outputs are 0 (ids -1) and its gradient is 0.
     Logits of -inf have probability 0; a NaN or +inf makes its row NaN."""
     idx = logits.get_device()
-    if idx < 0 or token_ids.get_device() != idx or idx != torch.cuda.current_device():
+    if not 0 <= idx == token_ids.get_device() == torch.cuda.current_device():
         _device_of(idx, logits=logits, token_ids=token_ids)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, V]")
@@ -834,8 +834,9 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     pairs (i, i + R / 2), or (2i, 2i + 1) if ``interleaved``, by positions * inv_freq (in 64 bits), scaled by
     ``rope_scale``; without them nothing is rotated."""
     cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
-    if idx < 0 or any(t is not None and t.get_device() != idx for t in (k, v, v_cache, slots, q, positions, inv_freq)) \
-            or idx != torch.cuda.current_device():
+    if not (0 <= idx == k.get_device() == v.get_device() == v_cache.get_device() == slots.get_device() == torch.cuda.current_device()
+            and (q is None or q.get_device() == idx) and (positions is None or positions.get_device() == idx)
+            and (inv_freq is None or inv_freq.get_device() == idx)):
         _device_of(idx, k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots, q=q, positions=positions, inv_freq=inv_freq)
     Hk, _, D = k_cache.shape[1:]
     k, v = _head_rows(k, "k", k_cache, Hk, D), _head_rows(v, "v", k_cache, Hk, D)
@@ -900,10 +901,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     what they hold.  Scores, sums and products are held in 32 bits; the weights of a softmax are rounded to the
     cache's type before their product with the values."""
     cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
-    if idx < 0 or any(t is not None and t.get_device() != idx for t in (q, v_cache, block_table, context_lens, cu_nodes, visible, out)) \
-            or idx != torch.cuda.current_device():
+    if not (0 <= idx == q.get_device() == v_cache.get_device() == block_table.get_device() == context_lens.get_device()
+            == cu_nodes.get_device() == torch.cuda.current_device() and (visible is None or visible.get_device() == idx)):
         _device_of(idx, k_cache=k_cache, q=q, v_cache=v_cache, block_table=block_table, context_lens=context_lens, cu_nodes=cu_nodes,
-                   visible=visible, out=out)
+                   visible=visible)
     (_, Hk, page, D), N = k_cache.shape, int(max_nodes)
     q = _head_rows(q, "q", k_cache, None, D)
     T, H, _ = q.shape
@@ -953,7 +954,7 @@ def accept_tree(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
     draws are independent (``sample`` over the rows of all nodes).  A walk ends at ``max_path`` <= 256 nodes at the
     latest.  Requests without a node, or whose bounds do not fit, have num_accepted -1."""
     idx = sampled.get_device()
-    if idx < 0 or any(t.get_device() != idx for t in (tokens, parents, cu_nodes)) or idx != torch.cuda.current_device():
+    if not 0 <= idx == tokens.get_device() == parents.get_device() == cu_nodes.get_device() == torch.cuda.current_device():
         _device_of(idx, sampled=sampled, tokens=tokens, parents=parents, cu_nodes=cu_nodes)
     T, W = sampled.numel(), int(max_path)
     for name, t in (("sampled", sampled), ("tokens", tokens), ("parents", parents)):
@@ -980,7 +981,8 @@ def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     contexts, in place: entry j of ``path`` [B, width] (``accept_tree``'s: node numbers, increasing from the root's
     0, then -1) goes from position ``context_lens[b] + path[b, j]`` to ``context_lens[b] + j``."""
     cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
-    if idx < 0 or any(t.get_device() != idx for t in (v_cache, block_table, context_lens, path)) or idx != torch.cuda.current_device():
+    if not (0 <= idx == v_cache.get_device() == block_table.get_device() == context_lens.get_device() == path.get_device()
+            == torch.cuda.current_device()):
         _device_of(idx, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens, path=path)
     table, context = _tables(block_table, context_lens)
     B = table.shape[0]
