@@ -49,6 +49,15 @@ class SpecDecodeMetadata:
         return cls(flat.to(device), counts, cu.to(device), max(counts, default=0))
 
 
+def refuse_processors(m: SamplingMetadata) -> None:
+    """Raises for what changes the target's distribution from one drafted token to the next."""
+    if not m.no_penalties:
+        raise NotImplementedError("drafts of requests with penalties are not verified")
+    if (m.allowed_token_ids_mask is not None or m.allowed_words is not None or m.bad_words_token_ids or m.min_tokens
+            or (m.logit_bias and any(m.logit_bias))):
+        raise NotImplementedError("drafts of requests with logits processors are not verified")
+
+
 class RejectionSampler:
     def __init__(self) -> None:
         self._seeds = SeedStaging()
@@ -61,11 +70,7 @@ class RejectionSampler:
         """``draft_probs`` ``[num_tokens, V]``: what the drafts were drawn from; None: looked-up or
         greedy drafts."""
         m = sampling_metadata
-        if not m.no_penalties:
-            raise NotImplementedError("drafts of requests with penalties are not verified")
-        if (m.allowed_token_ids_mask is not None or m.allowed_words is not None or m.bad_words_token_ids or m.min_tokens
-                or (m.logit_bias and any(m.logit_bias))):
-            raise NotImplementedError("drafts of requests with logits processors are not verified")
+        refuse_processors(m)
         if m.max_num_logprobs is not None:
             raise NotImplementedError("raw logprobs are not computed for drafts")
         B = len(metadata.num_draft_tokens)

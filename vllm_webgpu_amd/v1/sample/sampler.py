@@ -275,3 +275,12 @@ class Sampler:
         if m.max_num_logprobs is not None:
             lp = LogprobsTensors(res.logprob_ids, res.logprob_vals, res.logprob_ranks)
         return SamplerOutput(sampled_token_ids=res.sampled.unsqueeze(-1), logprobs_tensors=lp)
+
+    def gather_logprobs(self, logits: torch.Tensor, num_logprobs: int, token_ids: torch.Tensor) -> LogprobsTensors:
+        """Raw logprobs of given tokens ``token_ids`` [N] (a prompt's next tokens, say) with the ``num_logprobs`` most
+        likely ones of each row, from ``logits`` [N, V] (vLLM-v1's method of that name takes log-softmaxed rows; here
+        one launch reads the logits).  Rows whose token is outside the vocabulary are padding."""
+        if self.logit_softcap is not None:
+            raise NotImplementedError("logprobs of given tokens are of logits after the soft cap: cap them first")
+        r = ops.token_logprobs(logits, token_ids, num_logprobs)
+        return LogprobsTensors(r.logprob_ids, r.logprob_vals, r.logprob_ranks)
