@@ -207,6 +207,36 @@ def test_graphs_beside_each_other(cuda):
     assert torch.equal(r.logprobs, a.logprobs) and not r.logprobs.requires_grad
 
 
+def test_gradients_twice_and_not_of_gradients(cuda):
+    """A retained graph gives its gradient again; with create_graph the gradient is the same and has none of its own; saved
+    tensors that went through host memory, and logits changed in between."""
+    x, ids = make(cuda, 7, 900, "f32", seed=10)
+    x.requires_grad_()
+    g = torch.linspace(-1, 1, 7, device=cuda)
+    r = ops.token_logprobs(x, ids, 2, True)
+    a, = torch.autograd.grad([r.logprobs, r.entropy], [x], [g, g], retain_graph=True)
+    b, = torch.autograd.grad([r.logprobs, r.entropy], [x], [g, g], retain_graph=True)
+    c, = torch.autograd.grad([r.logprobs, r.entropy], [x], [g, g], create_graph=True)
+    assert torch.equal(a, b) and torch.equal(a, c) and a.data_ptr() != b.data_ptr()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(c.sum(), x)
+    with torch.autograd.graph.save_on_cpu():
+        r = ops.token_logprobs(x, ids, 2, True)
+    d, = torch.autograd.grad([r.logprobs, r.entropy], [x], [g, g])
+    assert torch.equal(a, d)
+    e, = torch.autograd.grad((ops.token_logprobs(x, ids).logprobs.double() * g.double()).sum(), x)   # (an upstream of 64 bits)
+    f, = torch.autograd.grad(ops.token_logprobs(x, ids).logprobs, x, g)
+    assert torch.equal(e, f)
+    with torch.no_grad():
+        r = ops.token_logprobs(x, ids)
+    y = x * 1.0
+    r = ops.token_logprobs(y, ids)
+    with torch.no_grad():
+        y += 1.0
+    with pytest.raises(RuntimeError):
+        r.logprobs.sum().backward()
+
+
 def test_overlapping_rows_are_copied(cuda):
     x, ids = make(cuda, 1, 3000, "f32", seed=9)
     wide, want = x.expand(5, 3000), x.repeat(5, 1)

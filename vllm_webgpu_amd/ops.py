@@ -707,33 +707,52 @@ def _score_forward(logits, ids, L: int, entropy: bool, temperature: float, saved
     return logprobs, ent, lp_ids, lp_vals, ranks
 
 
+def _score_backward(ctx, g_logprobs, g_entropy):
+    logits, ids, saved = ctx.saved_tensors
+    grad = logits.new_empty(logits.shape)
+    if logits.shape[0]:
+        # (the forward's arguments: what is left to do here runs on a thread that autograd has just woken, which is slow)
+        a = _lib.TokenLogprobsArgs.from_buffer_copy(ctx.args)
+        if logits.data_ptr() != a.logits or ids.data_ptr() != a.token_ids or saved.data_ptr() != a.saved:  # (saved elsewhere)
+            a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
+            a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr()
+        if g_logprobs is not None:
+            if g_logprobs.dtype is not torch.float32 or not g_logprobs.is_contiguous():
+                g_logprobs = g_logprobs.to(torch.float32).contiguous()
+            a.grad_logprobs = g_logprobs.data_ptr()
+        if g_entropy is not None:
+            if g_entropy.dtype is not torch.float32 or not g_entropy.is_contiguous():
+                g_entropy = g_entropy.to(torch.float32).contiguous()
+            a.grad_entropy = g_entropy.data_ptr()
+        a.grad, a.stream = grad.data_ptr(), _stream_ptr()
+        _lib.check(_lib.lib().vws_token_logprobs_backward(ctypes.byref(a)))
+    return grad, None, None, None, None
+
+
+_score_backward_once = torch.autograd.function.once_differentiable(_score_backward)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, L, entropy, temperature):
         ctx.set_materialize_grads(False)
-        saved = torch.empty(8 * logits.shape[0], dtype=torch.float32, device=logits.device)
+        (N, V), saved = logits.shape, logits.new_empty(8 * logits.shape[0], dtype=torch.float32)
         out = _score_forward(logits, ids, L, entropy, temperature, saved)
         ctx.save_for_backward(logits, ids, saved)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
+        if N:
+            ctx.args = _lib.TokenLogprobsArgs(
+                ctypes.sizeof(_lib.TokenLogprobsArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
+                temperature, -1, None, None, None, None, None, saved.data_ptr(), 4 * saved.numel(), None, None, None, V)
+        if L >= 0:
+            ctx.mark_non_differentiable(*out[2:])
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprobs, g_entropy, *unused):
-        logits, ids, saved = ctx.saved_tensors
         if g_logprobs is None and g_entropy is None:
             return None, None, None, None, None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if logits.shape[0]:
-            gl, gh = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy))
-            N, V = logits.shape
-            a = _lib.TokenLogprobsArgs(
-                ctypes.sizeof(_lib.TokenLogprobsArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
-                ctx.temperature, -1, None, None, None, None, None, saved.data_ptr(), 4 * saved.numel(), _ptr(gl), _ptr(gh),
-                grad.data_ptr(), V, None, 0, _stream_ptr())
-            _lib.check(_lib.lib().vws_token_logprobs_backward(ctypes.byref(a)))
-        return grad, None, None, None, None
+        # (gradients of gradients, which there are none of, are asked for with gradients on)
+        return (_score_backward_once if torch.is_grad_enabled() else _score_backward)(ctx, g_logprobs, g_entropy)
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: int | None = None, entropy: bool = False,
