@@ -48,7 +48,7 @@ template <typename T, bool ENT, bool TOP> __global__ void score_kernel(ScoreArgs
 template <typename T> __global__ void score_backward_kernel(ScoreArgs);
 template <typename T> __global__ void append_kernel(AppendArgs);
 __global__ void compact_kernel(CompactArgs);
-template <typename T, int D, int MT, int WAVES> __global__ void tree_kernel(TreeArgs);
+template <typename T, int D, int MT, int WAVES, int WIDE> __global__ void tree_kernel(TreeArgs);
 template <typename T, int D> __global__ void tree_join_kernel(TreeArgs);
 __global__ void accept_kernel(AcceptArgs);
 }  // namespace vws
@@ -851,11 +851,11 @@ int validate_append(const vws_append_kv_args* a) {
     return VWS_OK;
 }
 
-// How a launch divides its requests' rows and keys: workgroups of 16, 32 or 128 rows (16 past 128 dimensions), and
-// parts of the keys where the rows alone do not fill the chip.
+// How a launch divides its requests' rows and keys: workgroups of 16, 32 or 128 rows (16 or 128 past 128 dimensions),
+// and parts of the keys where the rows alone do not fill the chip.
 struct TreeShape {
     int block_rows;
-    int slots;         // workgroups that are resident at once: two a compute unit, one of 128 rows
+    int slots;         // workgroups that are resident at once: two a compute unit, one of 128 rows or past 128 dimensions
     int blocks;        // workgroups along the rows
     int splits, chunk;
     int rows;          // of all of a request's workgroups
@@ -866,11 +866,13 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     const int need = max_nodes * (heads / kv_heads), step = kTrKeys * kTrThreads / 64;
     const int64_t most = std::min<int64_t>((int64_t)max_pages * page_size, kCacheMaxPosition);
     // More than 32 rows: workgroups of 128 read the keys once (64 trees of up to 32 nodes, four heads each, over 8192
-    // tokens: 280 us, of 32 rows 376), but where those of 32 are all resident at once anyway (one tree of 12 nodes over
-    // 1900: 19.8 us and 16.0).
-    const int64_t narrow = (int64_t)B * kv_heads * ((need + 31) / 32) * ((most + kTreeMinKeys - 1) / kTreeMinKeys);
-    t.block_rows = need <= 16 || D > 128 ? 16 : need <= 32 || narrow <= 512 ? 32 : 128;
-    t.slots = t.block_rows > 32 ? 256 : 512;
+    // tokens: 261 us, of 32 rows 376; eight heads each of 256 dimensions: 472, of 16 rows 919), but where those of 32 are all
+    // resident at once anyway (one tree of 12 nodes over 1900: 19.8 us and 16.0).
+    const int few = D > 128 ? 16 : 32;  // rows of a workgroup whose waves share none
+    const int64_t narrow = (int64_t)B * kv_heads * ((need + few - 1) / few) * ((most + kTreeMinKeys - 1) / kTreeMinKeys);
+    const bool wide = need > 32 && narrow > 512;
+    t.block_rows = wide ? 128 : need <= 16 ? 16 : few;
+    t.slots = wide || D > 128 ? 256 : 512;
     t.blocks = (need + t.block_rows - 1) / t.block_rows;
     t.rows = t.blocks * t.block_rows;
     // Parts: one workgroup for each slot, since every part costs its start, its end and its record (64 requests over
@@ -878,7 +880,7 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     // workgroups of 128 rows leave most requests undivided, a long one would be the launch: two a slot then (20 ragged
     // requests of up to 8192: 216 us, 137).
     const int64_t items = (int64_t)B * kv_heads * t.blocks;
-    const int64_t wgs = t.block_rows > 32 && items * 8 > t.slots ? 2 * t.slots : t.slots;
+    const int64_t wgs = wide && items * 8 > t.slots ? 2 * t.slots : t.slots;
     int64_t s = std::min<int64_t>(std::min<int64_t>(wgs / items, most / kTreeMinKeys), kTrMaxSplits);
     if (s < 1) s = 1;
     const int64_t chunk = ((most + s - 1) / s + step - 1) / step * step;
@@ -920,10 +922,10 @@ int tree_launch(const TreeArgs& k, const TreeShape& t, hipStream_t s) {
     const int K = VWS_KERNEL_TREE;
     const unsigned parts = (unsigned)(k.B * k.splits * k.c.heads);
     const dim3 grid((parts + 7u) / 8u * 8u * (unsigned)t.blocks), block(kTrThreads);
-    constexpr int M = D > 128 ? 1 : 2, W = D > 128 ? 4 : 8;
-    if (t.block_rows == 16) launch(K, tree_kernel<T, D, 1, 4>, grid, block, s, k);
-    else if (t.block_rows == 32) launch(K, tree_kernel<T, D, M, 4>, grid, block, s, k);
-    else launch(K, tree_kernel<T, D, M, W>, grid, dim3(64 * W), s, k);
+    if (t.block_rows == 16) launch(K, tree_kernel<T, D, 1, 4, 1>, grid, block, s, k);
+    else if constexpr (D > 128) launch(K, tree_kernel<T, D, 1, 8, 8>, grid, dim3(512), s, k);
+    else if (t.block_rows == 32) launch(K, tree_kernel<T, D, 2, 4, 1>, grid, block, s, k);
+    else launch(K, tree_kernel<T, D, 2, 8, 4>, grid, dim3(512), s, k);
     if (int st = check_launch("vws_tree_attention")) return st;
     if (k.splits > 1) {
         constexpr int kJoin = kTrThreads / (D / 4);  // rows of a workgroup

@@ -12,6 +12,8 @@
 // relative precision there, and sums are in 32): nearly every step then neither exchanges nor rescales.
 #pragma once
 
+#include <type_traits>
+
 #include "vws_device.h"
 #include "vws_tree.h"
 
@@ -99,8 +101,11 @@ __device__ __forceinline__ uint32_t tr_seen(const TreeArgs& a, const TrBounds& o
 constexpr int tr_acc(int D, int MT) { return MT * (D / 4 + 2); }
 // Bytes of a step's keys, and of its values, that a wave keeps in LDS.
 constexpr int tr_tile(int D) { return 2 * kTrKeys * D; }
+// Steps that a workgroup keeps in LDS (128 KB of 128 or 256 dimensions), and of those each lane.
+constexpr int tr_steps(int D, int waves) { return D > 128 ? 4 : waves; }
+constexpr int tr_deep(int D, int waves, int WM) { return tr_steps(D, waves) * WM / waves; }
 constexpr int tr_lds(int D, int MT, int waves) {
-    const int ring = waves * 2 * tr_tile(D), merge = waves / 2 * 64 * 4 * tr_acc(D, MT);
+    const int ring = tr_steps(D, waves) * 2 * tr_tile(D), merge = waves / 2 * 64 * 4 * tr_acc(D, MT);
     return ring > merge ? ring : merge;
 }
 
@@ -132,13 +137,14 @@ __device__ __forceinline__ int tr_value_place(int c, int i) { return c ^ ((i >> 
 
 // MT tiles of 16 rows for each of WM waves, from m0 on.  The workgroup's waves make WAVES / WM lanes, which take the
 // keys in turn, 32 at a time, each through LDS of its own, and join what they have there.  A lane of one wave waits for
-// no other; the waves of a wider one share its tiles, WM of them in turn, and meet once a step.
+// no other; the waves of a wider one share its tiles, and meet once a step.
 template <typename T, int D, int MT, int WAVES, int WM>
 __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, int b, int h, int split, int m0, char* lds) {
     constexpr int WK = WAVES / WM, KS = D / 32, DT = D / 16, kAcc = tr_acc(D, MT), kStep = WK * kTrKeys;
     constexpr int kTile = tr_tile(D), kLoads = D / 16;  // loads of a tile
     constexpr int kMine = 2 * kLoads / WM;              // ... of a step's two that a wave makes
-    static_assert(2 * kLoads % WM == 0, "");
+    constexpr int kDeep = tr_deep(D, WAVES, WM);        // steps of a lane's LDS
+    static_assert(2 * kLoads % WM == 0, "every wave makes as many");
     typedef TrElem<T> E;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / WM, wm = wave % WM;
     const int i16 = lane & 15, g = lane >> 4, rows = o.n * a.group;
@@ -162,7 +168,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
         for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = TrF4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    char* const ring = lds + wk * WM * 2 * kTile;
+    char* const ring = lds + wk * kDeep * 2 * kTile;
     // the pages of a step's four eights of keys (entries past the request's last are not read), 0 for those that do not exist, and
     // the keys that lie in pages that do
     struct Pages { int p[4]; uint32_t live; };
@@ -178,28 +184,44 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
         }
         return s;
     };
-    // Loads [first, last) of a step's keys, then of its values, to the tiles at `to`
-    auto fetch = [&](const Pages& s, int kb, char* to, int first, int last) __attribute__((always_inline)) {
-        const uint16_t* at[4];
+    // A wave's share (part of WM: every WM-th load) of a step's keys (what & 1) and of its values (what & 2), to the tiles
+    // at `to`
+    auto fetch = [&](const Pages& s, int kb, char* to, int part, auto what) __attribute__((always_inline)) {
+        constexpr int kWhat = decltype(what)::value;
+        if (kWhat & 1) {
+            const uint16_t* at[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) at[e] = kh + (int64_t)s.p[e] * a.c.kps + ((kb + 8 * e) & pm) * D;
-        const int r = lane >> 2, e = tr_value_place(lane & 3, r);  // this lane's dimension and eight
-        const int p01 = e & 1 ? s.p[1] : s.p[0], p23 = e & 1 ? s.p[3] : s.p[2];
-        const uint16_t* const p = vh + (int64_t)(e & 2 ? p23 : p01) * a.c.vps + ((r << a.c.pshift) + ((kb + 8 * e) & pm));
+            for (int e = 0; e < 4; ++e) at[e] = kh + (int64_t)s.p[e] * a.c.kps + ((kb + 8 * e) & pm) * D;
 #pragma unroll
-        for (int j = 0; j < 2 * kLoads; ++j) {
-            if (j < first || j >= last) continue;
-            if (j < kLoads) {
-                const int n = 64 * j + lane, key = n / (D / 8), c = n - key * (D / 8), i = (key >> 3) * 4 + (key & 3);
-                const uint16_t* base = at[(64 * j) / D];
-                // (of 96 dimensions a load may span two eights)
-                if ((64 * j) / D != (64 * j + 63) / D) base = key >= 8 * ((64 * j) / D + 1) ? at[(64 * j + 63) / D] : base;
-                tr_fetch(to + 1024 * j, base + (key & 7) * D + 8 * tr_key_place<D>(c, i));
-            } else {
-                tr_fetch(to + 1024 * j, p + ((16 * (j - kLoads)) << a.c.pshift));
+            for (int i = 0; i < (kLoads + WM - 1) / WM; ++i) {
+                // (a load's first and last eight differ for 96 dimensions only)
+                const int j = i * WM + part, e0 = (64 * j) / D, e1 = (64 * j + 63) / D;
+                if (kLoads % WM && j >= kLoads) continue;
+                const int n = 64 * j + lane, key = n / (D / 8), c = n - key * (D / 8), row = (key >> 3) * 4 + (key & 3);
+                const uint16_t* base = e0 & 2 ? (e0 & 1 ? at[3] : at[2]) : (e0 & 1 ? at[1] : at[0]);
+                if (D % 64) {
+                    const uint16_t* last = e1 & 2 ? (e1 & 1 ? at[3] : at[2]) : (e1 & 1 ? at[1] : at[0]);
+                    base = key >= 8 * (e0 + 1) ? last : base;
+                }
+                tr_fetch(to + 1024 * j, base + (key & 7) * D + 8 * tr_key_place<D>(c, row));
+            }
+        }
+        if (kWhat & 2) {
+            const int r = lane >> 2, e = tr_value_place(lane & 3, r);  // this lane's dimension and eight
+            const int p01 = e & 1 ? s.p[1] : s.p[0], p23 = e & 1 ? s.p[3] : s.p[2];
+            const uint16_t* const p = vh + (int64_t)(e & 2 ? p23 : p01) * a.c.vps + ((r << a.c.pshift) + ((kb + 8 * e) & pm));
+#pragma unroll
+            for (int i = 0; i < (kLoads + WM - 1) / WM; ++i) {
+                // (of 96 dimensions half of four waves make one load of keys more, the others one of values)
+                const int j = i * WM + (kLoads % WM ? (part + WM / 2) % WM : part);
+                if (kLoads % WM && j >= kLoads) continue;
+                tr_fetch(to + kTile + 1024 * j, p + ((16 * j) << a.c.pshift));
             }
         }
     };
+    typedef std::integral_constant<int, 1> Keys;
+    typedef std::integral_constant<int, 2> Values;
+    typedef std::integral_constant<int, 3> Both;
     auto key_of_tile = [&](const char* tile, int t, int s) __attribute__((always_inline)) {
         const int key = 8 * (i16 >> 2) + 4 * t + (i16 & 3);
         return *reinterpret_cast<const TrU4*>(tile + key * (2 * D) + 16 * tr_key_place<D>(4 * s + g, i16));
@@ -340,13 +362,13 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 #pragma unroll
             for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[mt][s]));
     };
-    if (WM == 1) {
+    if constexpr (WM == 1) {
         // a step's tiles take the next one's keys and values as soon as the products have read them
         if (first < k1) {
             const Pages now = pages_at(first);
-            fetch(now, first, ring, 0, kLoads);
+            fetch(now, first, ring, 0, Keys());
             load_q();
-            fetch(now, first, ring, kLoads, 2 * kLoads);
+            fetch(now, first, ring, 0, Values());
             q_here();
             uint32_t live = now.live;
             for (int kb = first; kb < k1; kb += kStep) {
@@ -356,45 +378,43 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 step(kb, live, ring,
                      [&]() __attribute__((always_inline)) {
                          tr_read();
-                         if (more) fetch(next, kb + kStep, ring, 0, kLoads);
+                         if (more) fetch(next, kb + kStep, ring, 0, Keys());
                      },
                      [&]() __attribute__((always_inline)) {
                          if (more) tr_arrived<kLoads>();  // (but for the next keys)
                          else tr_arrived<0>();
                      });
-                if (more) fetch(next, kb + kStep, ring, kLoads, 2 * kLoads);
+                if (more) fetch(next, kb + kStep, ring, 0, Values());
                 live = next.live;
             }
         }
     } else {
-        // the tiles of WM - 1 steps are on their way or being read; past the last key they are the last page's, not used
+        // the tiles of kDeep - 1 steps are on their way; past the last key they are the last page's, not used
+        constexpr int kAhead = kDeep - 1;
+        static_assert(kAhead > 0, "");
         const int steps = (k1 - k0 + kStep - 1) / kStep;
         const bool idle = m0 >= rows;
-        uint32_t live[WM];
+        uint32_t live[kAhead];
         load_q();
 #pragma unroll
-        for (int i = 0; i < WM - 1; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
             const Pages s = pages_at(first + i * kStep);
-            fetch(s, first + i * kStep, ring + i * 2 * kTile, wm * kMine, (wm + 1) * kMine);
+            fetch(s, first + i * kStep, ring + i * 2 * kTile, wm, Both());
             live[i] = s.live;
         }
         q_here();
-        for (int i0 = 0; i0 < steps; i0 += WM) {
+        char *tile = ring, *free = ring + kAhead * 2 * kTile;
+        for (int i = 0, kb = first; i < steps; ++i, kb += kStep) {
+            tr_arrived<(kAhead - 1) * kMine>();
+            tr_meet();  // (this step's tiles are whole, and the last one's have been read)
+            const Pages s = pages_at(kb + kAhead * kStep);
+            fetch(s, kb + kAhead * kStep, free, wm, Both());
+            if (kb < k1 && !idle) step(kb, live[0], tile, []() {}, []() {});
 #pragma unroll
-            for (int u = 0; u < WM; ++u) {
-                if (i0 + u >= steps) break;
-                const int kb = first + (i0 + u) * kStep;
-                tr_arrived<(WM - 2) * kMine>();
-                tr_meet();  // (this step's tiles are whole, and the last one's have been read)
-                {
-                    constexpr int kAhead = WM - 1;
-                    const int v = (u + kAhead) % WM;
-                    const Pages s = pages_at(kb + kAhead * kStep);
-                    fetch(s, kb + kAhead * kStep, ring + v * 2 * kTile, wm * kMine, (wm + 1) * kMine);
-                    live[v] = s.live;
-                }
-                if (kb < k1 && !idle) step(kb, live[u], ring + u * 2 * kTile, []() {}, []() {});
-            }
+            for (int j = 0; j + 1 < kAhead; ++j) live[j] = live[j + 1];
+            live[kAhead - 1] = s.live;
+            free = tile;
+            tile = tile == ring + kAhead * 2 * kTile ? ring : tile + 2 * kTile;
         }
     }
     tr_arrived<0>();  // (what lands in LDS lands before it is used for something else)
@@ -439,7 +459,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     };
     if (WK > 4) give(4);
     if (WK > 2) give(2);
-    give(1);
+    if (WK > 1) give(1);
     if (wk > 0) return;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -470,11 +490,10 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     }
 }
 
-// A workgroup's rows: up to 16 MT of four waves (two workgroups a compute unit), or up to 64 MT of eight, which share
-// them as its request has them.
-template <typename T, int D, int MT, int WAVES>
+// A workgroup's rows: up to 16 MT for each of WIDE groups of its waves, which share them as its request has them.
+template <typename T, int D, int MT, int WAVES, int WIDE>
 __global__ __launch_bounds__(64 * WAVES, 2) void tree_kernel(TreeArgs a) {
-    constexpr int kThreads = 64 * WAVES, kRows = 16 * MT * (WAVES > 4 ? 4 : 1);
+    constexpr int kThreads = 64 * WAVES, kRows = 16 * MT * WIDE;
     __shared__ __align__(1024) char lds[tr_lds(D, MT, WAVES)];
     // workgroups of the same keys lie eight apart, on one chiplet
     const int per = 8 * a.blocks, item = (blockIdx.x / per) * 8 + (blockIdx.x & 7), mb = (blockIdx.x % per) >> 3;
@@ -500,7 +519,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void tree_kernel(TreeArgs a) {
     if (!tr_bounds(a, b, &o)) return;
     const int m0 = mb * kRows, rows = o.n * a.group - m0;
     if (rows <= 0 || (split * a.chunk >= o.len && split > 0)) return;
-    if constexpr (WAVES > 4) {
+    if constexpr (WIDE == 8) {
+        if (rows > 4 * 16 * MT) tree_rows<T, D, MT, WAVES, 8>(a, o, b, h, split, m0, lds);
+        else tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds);
+    } else if constexpr (WIDE == 4) {
         if (rows > 2 * 16 * MT) tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds);
         else if (rows > 16 * MT) tree_rows<T, D, MT, WAVES, 2>(a, o, b, h, split, m0, lds);
         else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds);
@@ -562,18 +584,19 @@ __global__ __launch_bounds__(kTrThreads) void tree_join_kernel(TreeArgs a) {
     *reinterpret_cast<U2*>(a.out + (int64_t)(o.t0 + node) * a.ots + (int64_t)(h * a.group + m - node * a.group) * a.ohs + d) = w;
 }
 
-#define VWS_TREE(T, D)                                         \
-    template __global__ void tree_kernel<T, D, 1, 4>(TreeArgs); \
+#define VWS_TREE(T, D)                                            \
+    template __global__ void tree_kernel<T, D, 1, 4, 1>(TreeArgs); \
     template __global__ void tree_join_kernel<T, D>(TreeArgs);
-// (past 128 dimensions neither two tiles fit the registers nor eight waves' tiles the LDS)
-#define VWS_TREES(T)                                              \
-    VWS_TREE(T, 64) VWS_TREE(T, 96) VWS_TREE(T, 128)              \
-    VWS_TREE(T, 192) VWS_TREE(T, 256)                             \
-    template __global__ void tree_kernel<T, 64, 2, 4>(TreeArgs);  \
-    template __global__ void tree_kernel<T, 96, 2, 4>(TreeArgs);  \
-    template __global__ void tree_kernel<T, 128, 2, 4>(TreeArgs); \
-    template __global__ void tree_kernel<T, 64, 2, 8>(TreeArgs);  \
-    template __global__ void tree_kernel<T, 96, 2, 8>(TreeArgs);  \
-    template __global__ void tree_kernel<T, 128, 2, 8>(TreeArgs);
+#define VWS_TREE_128(T, D)                                           \
+    VWS_TREE(T, D)                                                    \
+    template __global__ void tree_kernel<T, D, 2, 4, 1>(TreeArgs);    \
+    template __global__ void tree_kernel<T, D, 2, 8, 4>(TreeArgs);
+// (past 128 dimensions two tiles do not fit the registers, nor eight steps the LDS)
+#define VWS_TREE_256(T, D)                                           \
+    VWS_TREE(T, D)                                                    \
+    template __global__ void tree_kernel<T, D, 1, 8, 8>(TreeArgs);
+#define VWS_TREES(T)                                                     \
+    VWS_TREE_128(T, 64) VWS_TREE_128(T, 96) VWS_TREE_128(T, 128)          \
+    VWS_TREE_256(T, 192) VWS_TREE_256(T, 256)
 
 }  // namespace vws
