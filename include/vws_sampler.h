@@ -395,13 +395,14 @@ int vws_distill_step(const vws_distill_args* args);
  *   logprob = z_t - log sum_j exp(z_j), entropy = -sum_j p_j log p_j, p = softmax(z),
  *   rank = #{j : x_j >= x_t}, and the L largest x_j (the lower index first among equals; NaN never).
  *   dx_j = (g_l (1{j = t} - p_j) - g_h p_j (log p_j + entropy)) / T of upstream gradients g_l and g_h.
- * Rows whose token lies outside [0, V) are padding: not read, 0 in every output, -1 in the ids, gradient 0.
+ * Rows whose token lies outside [0, V) are padding: their logits count for nothing, 0 in every output, -1 in
+ * the ids, gradient 0.
  * Masked logits (-inf) have probability 0 and add nothing to the entropy; a NaN or +inf in a row, or no
  * logit above -inf, makes its log-probabilities, entropy and gradient NaN.  Where a row has fewer than L
  * logits that are numbers, the ids past them are -1 and their values NaN.
  *
  * The forward writes `saved` for the backward where it is not NULL; the backward reads it, the same inputs
- * and the upstream gradients.  `grad` has the logits' type and must not overlap them. */
+ * and the upstream gradients (that of the entropy needs a forward that wrote the entropy).  `grad` has the logits' type and must not overlap them. */
 typedef struct vws_token_logprobs_args {
     uint32_t struct_size; /* sizeof(vws_token_logprobs_args): ABI guard */
     int32_t rows;         /* N >= 1 */
@@ -436,8 +437,8 @@ int vws_token_logprobs_backward(const vws_token_logprobs_args* args);
 /* The paged cache of one layer's keys and values (no counterpart in the reference, whose cache is one
  * contiguous buffer a request).  Pages of P tokens (a power of two, 8 <= P <= 256): keys [pages, Hk, P, D],
  * values [pages, Hk, D, P] (a head's dimension is contiguous over its tokens: the layout that the second
- * matrix product of an attention reads), bfloat16 or float16, both 16-byte aligned.  A slot is page * P +
- * place in the page. */
+ * matrix product of an attention reads), bfloat16 or float16, both 16-byte aligned, without a common
+ * element.  A slot is page * P + place in the page. */
 #define VWS_MAX_TREE_NODES 256
 typedef struct vws_kv_cache {
     void* k;              /* [pages, Hk, P, D] */

@@ -156,3 +156,25 @@ def test_workspace_sizes():
     assert L.vws_tree_attention_workspace_size(2000, 16, 32, 8, 128, 16, 4) == fixed       # (nothing to join)
     for bad in ((0, 1, 8, 8, 64, 16, 1), (1, 0, 8, 8, 64, 16, 1), (1, 257, 8, 8, 64, 16, 1), (1, 1, 8, 3, 64, 16, 1), (1, 1, 8, 8, 64, 16, 0)):
         assert L.vws_tree_attention_workspace_size(*bad) == 0
+
+
+def test_keys_and_values_share_no_element():
+    L = _lib.lib()
+    page = 2 * 16 * 64
+    for v, ks, vs in ((0, page, page), (2 * 8, page, page), (9 * 2 * page, page, page), (page, 2 * page, 2 * page), (2 * page, 2 * page, 3 * page),
+                      (-2 * page + 16, 3 * page, 3 * page)):
+        c = cache(k=1 << 30, v=(1 << 30) + v, k_page_stride=ks, v_page_stride=vs)
+        for status in (L.vws_append_kv(ctypes.byref(append_args(c))), L.vws_tree_attention(ctypes.byref(tree_args(L, c))),
+                       L.vws_compact_kv(ctypes.byref(c), 1, FAKE, 4, 4, FAKE, FAKE, 3, 3, None)):
+            assert status == _lib.ERR_INVALID_ARGUMENT and b"overlap" in L.vws_last_error()
+
+
+def test_slots_past_a_requests_pages():
+    """Nodes behind the pages that a request holds have no slot."""
+    c = PagedKVCache(1, 10, 1, 64, page_size=16, device="cpu")
+    c.reserve("a", 20)
+    c.reserve("b", 40)
+    tree = DraftTree.make([[-1, 0, 1], [-1, 0, 1]], torch.device("cpu"))
+    t = c.block_table(["a", "b"])
+    slots = c.slots(t, torch.tensor([31, 46]), tree).tolist()
+    assert slots == [int(t[0, 1]) * 16 + 15, -1, -1, int(t[1, 2]) * 16 + 14, int(t[1, 2]) * 16 + 15, -1]

@@ -814,6 +814,17 @@ int validate_cache(const vws_kv_cache& c) {
     return VWS_OK;
 }
 
+// Keys and values share no element (their pages may lie between each other).
+int validate_apart(const vws_kv_cache& c) {
+    const int64_t page = (int64_t)c.kv_heads * c.page_size * c.head_dim;
+    const uint16_t *k = static_cast<const uint16_t*>(c.k), *v = static_cast<const uint16_t*>(c.v);
+    const int64_t gap = v >= k ? v - k : k - v, step = v >= k ? c.k_page_stride : c.v_page_stride;
+    const int64_t first = (c.num_pages - 1) * step + page;  // elements of the one that comes first
+    if (gap < first && (c.k_page_stride != c.v_page_stride || gap % step < page || step - gap % step < page))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "cache: k and v overlap");
+    return VWS_OK;
+}
+
 CacheView cache_view(const vws_kv_cache& c) {
     CacheView v;
     v.k = static_cast<uint16_t*>(c.k);
@@ -848,7 +859,7 @@ int validate_append(const vws_append_kv_args* a) {
     if (a->heads > 0 && (!a->q || !a->q_out)) return fail(VWS_ERR_INVALID_ARGUMENT, "q or q_out is NULL");
     const int64_t wgs = (int64_t)a->tokens + ((int64_t)a->tokens + kApValueTokens - 1) / kApValueTokens * a->cache.kv_heads;
     if (wgs > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many tokens (%d)", a->tokens);
-    return VWS_OK;
+    return validate_apart(a->cache);
 }
 
 // How a launch divides its requests' rows and keys: workgroups of 16, 32 or 128 rows (16 or 128 past 128 dimensions),
@@ -871,7 +882,7 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     const int few = D > 128 ? 16 : 32;  // rows of a workgroup whose waves share none
     const int64_t narrow = (int64_t)B * kv_heads * ((need + few - 1) / few) * ((most + kTreeMinKeys - 1) / kTreeMinKeys);
     const bool wide = need > 32 && narrow > 512;
-    t.block_rows = wide ? 128 : need <= 16 ? 16 : few;
+    t.block_rows = wide ? kTrWideRows : need <= 16 ? 16 : few;
     t.slots = wide || D > 128 ? 256 : 512;
     t.blocks = (need + t.block_rows - 1) / t.block_rows;
     t.rows = t.blocks * t.block_rows;
@@ -909,12 +920,12 @@ int validate_tree(const vws_tree_attention_args* a) {
     const vws_kv_cache& c = a->cache;
     const TreeShape t = tree_shape(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
     const int64_t parts = (int64_t)a->batch * t.splits * c.kv_heads, joins = (int64_t)a->batch * c.kv_heads * ((t.rows + 3) / 4);
-    if ((parts + 7) * t.blocks > kMaxWgs || joins > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many requests (%d) for one launch", a->batch);
+    if ((parts + 7) * t.blocks > kMaxWgs / 2 || joins > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many requests (%d) for one launch", a->batch);
     const size_t need = vws_tree_attention_workspace_size(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
     if (!a->workspace || a->workspace_bytes < need)
         return fail(VWS_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", a->workspace ? a->workspace_bytes : (size_t)0, need);
     if (reinterpret_cast<uintptr_t>(a->workspace) & 255u) return fail(VWS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
-    return VWS_OK;
+    return validate_apart(c);
 }
 
 template <typename T, int D>
@@ -923,9 +934,9 @@ int tree_launch(const TreeArgs& k, const TreeShape& t, hipStream_t s) {
     const unsigned parts = (unsigned)(k.B * k.splits * k.c.heads);
     const dim3 grid((parts + 7u) / 8u * 8u * (unsigned)t.blocks), block(kTrThreads);
     if (t.block_rows == 16) launch(K, tree_kernel<T, D, 1, 4, 1>, grid, block, s, k);
-    else if constexpr (D > 128) launch(K, tree_kernel<T, D, 1, 8, 8>, grid, dim3(512), s, k);
+    else if constexpr (D > 128) launch(K, tree_kernel<T, D, 1, 8, 8>, grid, dim3(kTrWideThreads), s, k);
     else if (t.block_rows == 32) launch(K, tree_kernel<T, D, 2, 4, 1>, grid, block, s, k);
-    else launch(K, tree_kernel<T, D, 2, 8, 4>, grid, dim3(512), s, k);
+    else launch(K, tree_kernel<T, D, 2, 8, 4>, grid, dim3(kTrWideThreads), s, k);
     if (int st = check_launch("vws_tree_attention")) return st;
     if (k.splits > 1) {
         constexpr int kJoin = kTrThreads / (D / 4);  // rows of a workgroup
@@ -1409,6 +1420,7 @@ int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* bloc
     if (path_width < 1 || path_width > VWS_MAX_TREE_NODES)
         return fail(VWS_ERR_LIMIT, "path_width must be in [1, %d] (got %d)", VWS_MAX_TREE_NODES, path_width);
     if (path_row_stride < path_width) return fail(VWS_ERR_INVALID_ARGUMENT, "path_row_stride < path_width");
+    if (int st = validate_apart(*cache)) return st;
     CompactArgs k;
     std::memset(&k, 0, sizeof(k));
     k.c = cache_view(*cache);
@@ -1426,8 +1438,8 @@ int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* bloc
 
 size_t vws_tree_attention_workspace_size(int32_t batch, int32_t max_nodes, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                          int32_t page_size, int32_t max_pages) {
-    if (batch < 1 || max_nodes < 1 || max_nodes > VWS_MAX_TREE_NODES || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
-        page_size < 1 || max_pages < 1)
+    if (batch < 1 || max_nodes < 1 || max_nodes > VWS_MAX_TREE_NODES || heads < 1 || kv_heads < 1 || heads % kv_heads || heads / kv_heads > 256 ||
+        kv_heads > 1024 || head_dim < 1 || head_dim > 256 || page_size < 1 || max_pages < 1)
         return 0;
     const TreeShape t = tree_shape(batch, max_nodes, heads, kv_heads, head_dim, page_size, max_pages);
     const size_t recs = t.splits > 1 ? (size_t)batch * (size_t)t.splits * (size_t)kv_heads * (size_t)t.rows : 0;

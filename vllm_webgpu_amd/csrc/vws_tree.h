@@ -10,6 +10,7 @@
 namespace vws {
 
 constexpr int kTrThreads = 256;   // four waves
+constexpr int kTrWideThreads = 512, kTrWideRows = 128;  // eight, which share their keys
 constexpr int kTrKeys = 32;       // keys of a wave's step
 constexpr int kTrMaxSplits = 256;
 constexpr int kAcThreads = 64;    // one wave a request

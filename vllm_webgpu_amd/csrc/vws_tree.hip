@@ -10,7 +10,7 @@ __global__ __launch_bounds__(kAcThreads) void accept_kernel(AcceptArgs a) {
     constexpr int N = kAcMaxNodes / kAcThreads;
     __shared__ int32_t sampled[kAcMaxNodes];
     const int b = blockIdx.x, lane = threadIdx.x;
-    const int t0 = a.cu[b], end = a.cu[b + 1], n = end - t0;
+    const int t0 = a.cu[b], end = a.cu[b + 1], n = (int)((uint32_t)end - (uint32_t)t0);
     int32_t* out = a.out + (int64_t)b * a.width;
     int32_t* path = a.path + (int64_t)b * a.width;
     const bool fits = t0 >= 0 && end > t0 && end <= a.T && n <= kAcMaxNodes;

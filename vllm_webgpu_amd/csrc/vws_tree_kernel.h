@@ -68,7 +68,7 @@ struct TrBounds { int t0, n, context, len; };
 __device__ __forceinline__ bool tr_bounds(const TreeArgs& a, int b, TrBounds* o) {
     o->t0 = a.cu[b];
     const int end = a.cu[b + 1];
-    o->n = end - o->t0;
+    o->n = (int)((uint32_t)end - (uint32_t)o->t0);
     if (o->t0 < 0 || end > a.T || end <= o->t0 || o->n > a.max_nodes) return false;
     const int most = (int)min((int64_t)a.max_pages << a.c.pshift, (int64_t)kCacheMaxPosition);
     o->context = min(max(a.context[b], 0), most);
@@ -483,7 +483,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<TrF4*>(p + 16 * dt) = acc[mt][dt];
             if (g == 0) {
-                a.stat[2 * rec] = ref[mt];
+                a.stat[2 * rec] = sum[mt] == sum[mt] ? ref[mt] : sum[mt];  // (a NaN without a reference counts in the join)
                 a.stat[2 * rec + 1] = sum[mt];
             }
         }

@@ -713,7 +713,9 @@ def _score_backward(ctx, g_logprobs, g_entropy):
     if logits.shape[0]:
         # (the forward's arguments: what is left to do here runs on a thread that autograd has just woken, which is slow)
         a = _lib.TokenLogprobsArgs.from_buffer_copy(ctx.args)
-        if logits.data_ptr() != a.logits or ids.data_ptr() != a.token_ids or saved.data_ptr() != a.saved:  # (saved elsewhere)
+        if (logits.data_ptr() != a.logits or logits.stride() != ctx.strides or ids.data_ptr() != a.token_ids
+                or saved.data_ptr() != a.saved):  # (saved elsewhere)
+            logits, ids, saved = _rows(logits), ids.contiguous(), saved.contiguous()
             a.logits, a.logits_row_stride = logits.data_ptr(), _row_stride(logits)
             a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr()
         if g_logprobs is not None:
@@ -740,6 +742,7 @@ class _TokenLogprobs(torch.autograd.Function):
         out = _score_forward(logits, ids, L, entropy, temperature, saved)
         ctx.save_for_backward(logits, ids, saved)
         if N:
+            ctx.strides = logits.stride()
             ctx.args = _lib.TokenLogprobsArgs(
                 ctypes.sizeof(_lib.TokenLogprobsArgs), N, V, _dtype_code(logits), logits.data_ptr(), _row_stride(logits), ids.data_ptr(),
                 temperature, -1, None, None, None, None, None, saved.data_ptr(), 4 * saved.numel(), None, None, None, V)
@@ -765,7 +768,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
     ``logprob_ranks``.  ``entropy``: also -sum p log p.  ``logprobs`` and ``entropy`` are differentiable in ``logits``,
     whose gradient has their type; the other outputs are not.
 
-    Tokens outside [0, V) pad a row: its logits are not read, its outputs are 0 (ids -1) and its gradient is 0.
+    Tokens outside [0, V) pad a row: its logits count for nothing, its outputs are 0 (ids -1) and its gradient is 0.
     Logits of -inf have probability 0; a NaN or +inf makes its row NaN."""
     idx = logits.get_device()
     if not 0 <= idx == token_ids.get_device() == torch.cuda.current_device():
@@ -825,18 +828,30 @@ def _out_rows(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.
     if out.requires_grad:
         raise ValueError(f"{name} would get no gradient: detach it")
     T, H, D = out.shape
-    if (H > 1 and out.stride(1) < D) or (T > 1 and out.stride(0) < (H - 1) * out.stride(1) + D):
+    a, b = out.stride(0), out.stride(1)  # (tokens inside a head or heads inside a token)
+    if T and H and not ((H == 1 or b >= D) and (T == 1 or a >= (H - 1) * b + D)) and not (
+            (T == 1 or a >= D) and (H == 1 or b >= (T - 1) * a + D)):
         raise ValueError(f"{name} must not overlap itself")
     return out
 
 
-def _spans(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from the first to the last element of each overlaps."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors [tokens, heads, dim] share memory (parts of the same rows, as of one projection, lie side by
+    side and do not; otherwise what lies from the first to the last element of each counts)."""
+    if not a.numel() or not b.numel():
+        return False
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+    def span(t, dims):  # elements from the first to the last
+        return 1 + sum((t.shape[i] - 1) * t.stride(i) for i in dims)
+
+    size, a0, b0 = a.element_size(), a.data_ptr(), b.data_ptr()
+    if a0 >= b0 + size * span(b, range(b.dim())) or b0 >= a0 + size * span(a, range(a.dim())):
+        return False
+    pitch, inner = a.stride(0), range(1, a.dim())
+    if a.dim() != b.dim() or b.stride(0) != pitch or a.shape[0] < 2 or b.shape[0] < 2 or (b0 - a0) % size:
+        return True
+    gap = (b0 - a0) // size % pitch if pitch else 0
+    return gap < span(a, inner) or pitch - gap < span(b, inner)
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
@@ -886,8 +901,10 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             raise ValueError(f"q must be of {T} tokens (got {tuple(q.shape)})")
         given, out = out is not None, _out_rows(out, q, "out")
         heads, qs, os = q.shape[1], q.stride(), out.stride()
-        if given and not (out.data_ptr() == q.data_ptr() and os == qs) and any(_spans(out, t) for t in (q, k, v)):
-            raise ValueError("out must not overlap the inputs, but be q's own memory")
+        if given:
+            others = (k, v, k_cache, v_cache) if out.data_ptr() == q.data_ptr() and os == qs else (q, k, v, k_cache, v_cache)
+            if any(_meet(out, t) for t in others):
+                raise ValueError("out must not overlap the inputs, but be q's own memory")
     if T:
         a = _lib.AppendArgs(
             ctypes.sizeof(_lib.AppendArgs), T, cache, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], slots.data_ptr(),
@@ -941,8 +958,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError(f"visible must be int32 [{T}, {(N + 31) // 32}] (got {visible.dtype} {tuple(visible.shape)})")
         visible = _rows(visible)
     given, out = out is not None, _out_rows(out, q, "out")
-    if given and _spans(out, q):
-        raise ValueError("out must not overlap q")
+    if given and (_meet(out, q) or _meet(out, k_cache) or _meet(out, v_cache)):
+        raise ValueError("out must not overlap q or the cache")
     if T and B:
         lib, stream, W = _lib.lib(), torch._C._cuda_getCurrentRawStream(idx), table.shape[1]
         ws = _workspace(lib.vws_tree_attention_workspace_size(B, N, H, Hk, D, page, W), idx, stream, _capturing(stream))

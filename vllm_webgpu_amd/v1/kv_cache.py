@@ -44,9 +44,12 @@ class PagedKVCache:
         return torch.tensor([p + [-1] * (width - len(p)) for p in pages], dtype=torch.int32).view(len(pages), width).to(self.k[0].device)
 
     def slots(self, block_table: torch.Tensor, context_lens: torch.Tensor, tree: DraftTree) -> torch.Tensor:
-        """int32 [T]: where the nodes' keys and values go, behind their contexts."""
+        """int32 [T]: where the nodes' keys and values go, behind their contexts; -1 (nowhere) past a request's pages."""
         at = context_lens.long()[tree.requests] + tree.numbers
-        return (block_table[tree.requests, at // self.page_size] * self.page_size + at % self.page_size).int()
+        i = at // self.page_size
+        held = (i >= 0) & (i < block_table.shape[1])
+        page = block_table[tree.requests, i.clamp(0, block_table.shape[1] - 1)]
+        return torch.where(held & (page >= 0), page * self.page_size + at % self.page_size, -1).int()
 
     # ---- a layer's step, on the device
 
