@@ -838,8 +838,10 @@ CacheView cache_view(const vws_kv_cache& c) {
     return v;
 }
 
-// Tokens of a workgroup that rotates: one, until there are more workgroups than the chip holds.
-int append_group(int T) { return T >= 8192 ? kApGroup : T >= 4096 ? 2 : 1; }
+// Tokens of a workgroup that rotates: one, until there are more workgroups than the chip holds (16384, 4096 and 2048
+// tokens of 32 + 4 heads: one a workgroup 84.8, 20.1 and 13.2 us, four 74.4, 17.3 and 11.9; 701 tokens of 32 + 8: 12.1
+// and 12.5).
+int append_group(int T) { return T >= 2048 ? kApGroup : 1; }
 
 int validate_append(const vws_append_kv_args* a) {
     if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
@@ -871,6 +873,8 @@ struct TreeShape {
     int splits, chunk;
     int rows;          // of all of a request's workgroups
 };
+constexpr int kTreeUnits = 256;     // compute units
+// A part's keys, at least (one tree of 12 nodes over 1900: 15.7 us, with 512 18.3; over 8000: 22.8, with 128 24.2).
 constexpr int kTreeMinKeys = 256;
 TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int page_size, int max_pages) {
     TreeShape t;
@@ -881,17 +885,18 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     // resident at once anyway (one tree of 12 nodes over 1900: 19.8 us and 16.0).
     const int few = D > 128 ? 16 : 32;  // rows of a workgroup whose waves share none
     const int64_t narrow = (int64_t)B * kv_heads * ((need + few - 1) / few) * ((most + kTreeMinKeys - 1) / kTreeMinKeys);
-    const bool wide = need > 32 && narrow > 512;
+    const bool wide = need > 32 && narrow > 2 * kTreeUnits;
     t.block_rows = wide ? kTrWideRows : need <= 16 ? 16 : few;
-    t.slots = wide || D > 128 ? 256 : 512;
+    t.slots = wide || D > 128 ? kTreeUnits : 2 * kTreeUnits;
     t.blocks = (need + t.block_rows - 1) / t.block_rows;
     t.rows = t.blocks * t.block_rows;
-    // Parts: one workgroup for each slot, since every part costs its start, its end and its record (64 requests over
-    // 4096 tokens, 8 nodes, one and two a slot: 191 us, 216; three of 8 nodes x 8 heads over 131000: 290, 305).  But where
-    // workgroups of 128 rows leave most requests undivided, a long one would be the launch: two a slot then (20 ragged
-    // requests of up to 8192: 216 us, 137).
+    // Parts: one workgroup a compute unit, since every part costs its start, its end and its record (one tree of 12 nodes
+    // over 8000: 19.6 us, two a unit 23.1; one node over 64000: 57.8, 64.5; three of 8 nodes x 8 heads over 131000: 290,
+    // 305).  But where that leaves most requests undivided, a long one would be the launch: two a unit then (20 ragged
+    // requests of up to 32 nodes over 8192: 216 us, two a unit 137; 12 of 8 over 30000: 225, 193).  Not for few rows past
+    // 128 dimensions, where a unit holds one at a time (30 of 4 nodes over 8192: 171, 190).
     const int64_t items = (int64_t)B * kv_heads * t.blocks;
-    const int64_t wgs = wide && items * 8 > t.slots ? 2 * t.slots : t.slots;
+    const int64_t wgs = items * 8 > kTreeUnits && (wide || D <= 128) ? 2 * kTreeUnits : kTreeUnits;
     int64_t s = std::min<int64_t>(std::min<int64_t>(wgs / items, most / kTreeMinKeys), kTrMaxSplits);
     if (s < 1) s = 1;
     const int64_t chunk = ((most + s - 1) / s + step - 1) / step * step;

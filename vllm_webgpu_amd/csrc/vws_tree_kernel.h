@@ -104,6 +104,8 @@ constexpr int tr_tile(int D) { return 2 * kTrKeys * D; }
 // Steps that a workgroup keeps in LDS (128 KB of 128 or 256 dimensions), and of those each lane.
 constexpr int tr_steps(int D, int waves) { return D > 128 ? 4 : waves; }
 constexpr int tr_deep(int D, int waves, int WM) { return tr_steps(D, waves) * WM / waves; }
+// Waves of a SIMD: two, of one workgroup or two; of four waves past 128 dimensions the LDS holds one workgroup.
+constexpr int tr_waves(int D, int waves) { return D > 128 && waves == 4 ? 1 : 2; }
 constexpr int tr_lds(int D, int MT, int waves) {
     const int ring = tr_steps(D, waves) * 2 * tr_tile(D), merge = waves / 2 * 64 * 4 * tr_acc(D, MT);
     return ring > merge ? ring : merge;
@@ -127,6 +129,13 @@ __device__ __forceinline__ void tr_meet() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// Of 256 dimensions, operands are read four at a time: read ahead without a bound they do not fit the registers (79
+// spilled of eight waves; a tree of 16 nodes, 64 requests, 493 us and 444).
+template <int D>
+__device__ __forceinline__ void tr_narrow(int i) {
+    if (D > 192 && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
 }
 
 // Where a tile keeps 16-byte chunk c of key row i (0 .. 15), and chunk c of dimension row i of its values: lanes
@@ -242,6 +251,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 const TrU4 f = key_of_tile(tile, t, k);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][t] = E::mma(f, q[mt][k], k ? s[mt][t] : TrF4{0.0f, 0.0f, 0.0f, 0.0f});
+                tr_narrow<D>(k);
             }
         }
         uint32_t seen[MT];
@@ -299,6 +309,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 const TrU4 f = value_of_tile(tile, dt);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = E::mma(f, p[mt], acc[mt][dt]);
+                tr_narrow<D>(dt);
             }
         } else {
             // values of keys that no row sees are nothing's; others that are not finite stay out of the common product
@@ -318,6 +329,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = E::mma(f, p[mt], acc[mt][dt]);
+                tr_narrow<D>(dt);
             }
             if (wave_ballot(odd != 0u)) {
                 // a product for each key that has such values, added for the rows that see it
@@ -492,7 +504,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 
 // A workgroup's rows: up to 16 MT for each of WIDE groups of its waves, which share them as its request has them.
 template <typename T, int D, int MT, int WAVES, int WIDE>
-__global__ __launch_bounds__(64 * WAVES, 2) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * WAVES, tr_waves(D, WAVES)) void tree_kernel(TreeArgs a) {
     constexpr int kThreads = 64 * WAVES, kRows = 16 * MT * WIDE;
     __shared__ __align__(1024) char lds[tr_lds(D, MT, WAVES)];
     // workgroups of the same keys lie eight apart, on one chiplet
