@@ -455,7 +455,8 @@ typedef struct vws_kv_cache {
 /* Stores keys and values [T, Hk, D] of T tokens at `slots` (distinct; those outside [0, pages * P) are not
  * stored), the keys rotated, and writes the rotated queries.  The first R of a head's D dimensions turn in
  * pairs (i, i + R / 2), or (2i, 2i + 1) if `interleaved`, by the angle position * inv_freq[i] (taken in 64
- * bits) and are scaled by rope_scale.  Without positions nothing is rotated. */
+ * bits) and are scaled by rope_scale.  Without positions nothing is rotated.  Inputs overlap neither the cache
+ * nor q_out (but q, whose own memory it may be). */
 typedef struct vws_append_kv_args {
     uint32_t struct_size; /* sizeof(vws_append_kv_args): ABI guard */
     int32_t tokens;       /* T >= 1 */
@@ -526,7 +527,7 @@ int vws_tree_attention(const vws_tree_attention_args* args);
  * (less than its own; -1: none).  From node 0 on: the token sampled at the node is emitted, and the walk goes to
  * the node's first child that holds it, or ends.  out_tokens [B, width] and path [B, width] (the visited
  * nodes) are padded with -1, num_accepted counts the visited nodes but the root; a walk ends at `width`
- * nodes.  Requests whose bounds do not fit, or without a node, have num_accepted -1. */
+ * nodes.  Requests whose bounds do not fit, without a node or with more than VWS_MAX_TREE_NODES have num_accepted -1. */
 int vws_accept_tree(int32_t batch, int32_t nodes, const int32_t* sampled, const int32_t* tokens,
                     const int32_t* parents, const int32_t* cu_nodes, int32_t width, int32_t* out_tokens,
                     int32_t* path, int32_t* num_accepted, void* stream);

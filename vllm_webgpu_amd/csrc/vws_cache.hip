@@ -45,9 +45,12 @@ __device__ __forceinline__ bool cache_slot(const CacheView& c, int slot, int* pa
     return slot >= 0 && *page < c.pages;
 }
 
+// What bounds both writes is HBM: 16384 tokens of 32 + 4 heads take 74 us, 4.5 TB/s read and written (a copy's 4.9), 4096 17
+// us; 701 tokens of trees 8.2 us, of which the chain slot, load, store is most, and the call 12.
+
 // Queries and keys of `group` tokens.  A head is `units` of 16 bytes or 32: pairs of vectors that turn together (or
 // vectors of four pairs), then vectors that do not turn; a thread has one unit of several heads, and loads four of them
-// before it turns any, the first four before the cosines and sines are there.
+// before it turns any, the first four before the cosines and sines are there (one at a time: 16384 tokens 100 us, 74).
 template <typename T>
 __device__ __forceinline__ void append_rotate(const AppendArgs& a, float* cs) {
     constexpr int U = 4;
@@ -145,7 +148,7 @@ __device__ __forceinline__ void append_rotate(const AppendArgs& a, float* cs) {
 }
 
 // Values of one head: a page keeps a dimension's tokens together, so a tile of tokens is turned in LDS.  Eight
-// tokens whose slots fill an aligned eighth of a page (a run's inside) leave as one 16-byte store for each
+// tokens whose slots fill an aligned eight of a page (a run's inside) leave as one 16-byte store for each
 // dimension, the eights of one dimension side by side; other tokens element by element.  A token is looked up where its
 // eight would begin, which another tile may hold.
 struct AppendValues {
@@ -234,7 +237,8 @@ __device__ __forceinline__ bool cache_position(const CompactArgs& a, int b, int 
     return *page >= 0 && *page < a.c.pages;
 }
 
-// One head of one request.  Entry j's node never lies before position j, so entries are taken in order, some at
+// One head of one request: a chain of table, load and store, 4.9 us for one request and 7.8 for 200 of 4 heads (700 moves of
+// 2 KB; the call's host work is as long).  Entry j's node never lies before position j, so entries are taken in order, some at
 // a time: all read before any is written.
 constexpr int kCpEntries = 16;
 __global__ __launch_bounds__(kApThreads) void compact_kernel(CompactArgs a) {

@@ -686,7 +686,8 @@ int distill(const vws_distill_args* a, int parts) {
     return distill_launch<_Float16>(a, parts);
 }
 
-// As the distillation's forward; rows that list their largest logits are joined from fewer parts.
+// As the distillation's forward (100 x 151936 bf16 with 20 alternatives: 384 workgroups 24.2 us, 768 23.2, 1536 32.1);
+// rows that list their largest logits are joined from fewer parts (one of 262144 fp32: at most 8 13.6 us, 16 13.1).
 constexpr int kScoreWgs = 768;
 void score_parts(int rows, int V, int L, int* S, int* len) {
     split_row(rows, V, kScoreWgs, 4096, L > 0 ? kScMaxTopParts : kScMaxParts, 1, S, len);

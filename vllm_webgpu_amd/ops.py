@@ -822,7 +822,7 @@ def _head_rows(t: torch.Tensor, name: str, like: torch.Tensor, heads: int | None
 
 def _out_rows(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return like.new_empty(like.shape)
+        return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(2) != 1:
         raise ValueError(f"{name} must have the queries' shape, type and device, its last dimension contiguous")
     if out.requires_grad:
