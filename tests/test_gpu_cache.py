@@ -197,3 +197,21 @@ def test_no_tokens(cuda):
     e = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=cuda)
     out = ops.append_kv(e, e, kc, vc, torch.empty(0, device=cuda).int(), q=e)
     assert out.shape == (0, 2, 64) and torch.equal(kc, k0)
+
+
+@pytest.mark.parametrize("T,interleaved", [(2051, True), (2047, False), (4098, False)])
+def test_append_of_several_tokens_a_workgroup(cuda, T, interleaved):
+    """Queries turned in place, the last workgroup's tokens fewer, every third head's stride apart."""
+    wide = torch.randn((T, 9, 72), device=cuda, generator=torch.Generator(device=cuda).manual_seed(T)).bfloat16()
+    q, k, v = wide[:, :4, :64], wide[:, 4:6, :64], wide[:, 6:8, 8:]
+    kc, vc = R.make_cache(cuda, T // 16 + 2, 2, 16, 64, "bf16")
+    slots, pos = torch.arange(T, device=cuda).flip(0).int(), torch.arange(T, device=cuda).int() * 37
+    f = freqs(cuda, 48)
+    want, off = R.rotate(q, pos, f, interleaved=interleaved)
+    wk, wv, koff = R.append(k, v, kc, vc, slots.cpu(), positions=pos, inv_freq=f, interleaved=interleaved)
+    rest = wide[:, 8].clone()
+    out = ops.append_kv(k, v, kc, vc, slots, q=q, positions=pos, inv_freq=f, interleaved=interleaved, out=q)
+    assert out.data_ptr() == wide.data_ptr() and torch.equal(wide[:, 8], rest)
+    check(q, want, off, "bf16")
+    check(kc, wk, koff, "bf16")
+    assert torch.equal(vc.double(), wv)

@@ -14,7 +14,7 @@
 // maximum reaches it hold any: a handful of groups is read again.
 //
 // HBM bounds both: 1999 x 151936 bf16 with entropy and 20 alternatives 135 us (4.5 TB/s of
-// logits, 5.9 with the groups' lines), 4096 x 128256 bf16, a fifth of
+// logits, 5.9 with the groups' lines; without alternatives 115), 4096 x 128256 bf16, a fifth of
 // the rows padding, forward 150 (5.6 TB/s, reads alone) and backward 345 (5.5 TB/s read and written, some of the reads from the
 // last-level cache).  Few rows are split over workgroups: 7 x 50257 fp32 with 5 alternatives 10.9 us, a part's read, its list and the join one after another.
 #include "vws_device.h"
@@ -209,7 +209,8 @@ __device__ __forceinline__ void sc_top(const T* row, int len, int lo, int L, int
     constexpr int VEC = Elem<T>::kVec, U = 4;
     const int tid = threadIdx.x, nvec = len / VEC;
     // The L-th largest of the threads' maxima, or, where L is small, the largest of the waves' own L-th largest: as good a
-    // bound, without looking at every thread's (L = 32: some 130 candidates in place of 32).
+    // bound, without looking at every thread's (L = 32: some 130 candidates in place of 32; L = 20, 1999 x 151936: 135 us, 141
+    // with the threads' own).
     __shared__ float tops[kScThreads];
     if (tid == 0) sh.groups = sh.cands = 0u;
     if (L <= 32) {
