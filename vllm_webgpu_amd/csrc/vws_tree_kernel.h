@@ -10,9 +10,12 @@
 // Keys and values pass through LDS, by loads that go there directly: whole lines of a page, each lane's 16 bytes
 // at a place where the products' reads find them in different banks (64 trees of up to 32 nodes over 8192 tokens took
 // 1001 us from memory straight to the operands' lanes, whose loads touch sixteen rows each; 398 by way of LDS).
-// The running reference of a row is raised only when some score exceeds it by 2^8 (sums are in 32 bits; P is rounded to
-// the cache's type, by at most 2^-9 (bf16) or 2^-12 of itself wherever it lies): nearly every step then neither
-// exchanges nor rescales.  P in 16 bits is what the matrix instructions take; sums are of the unrounded exponentials.
+// The running reference of a row is raised only when some score exceeds it by more than 2^kRaise: nearly every step then
+// neither exchanges nor rescales.  Sums are in 32 bits, of the unrounded exponentials; P is rounded to the cache's type,
+// which is what the matrix instructions take, by at most 2^-8 (bf16) or 2^-11 of itself.  f16 has steps of 2^-24 below
+// 2^-14: there the reference lies 2^kLift below the largest score, so that weights down to 2^-25 of the largest are rounded as
+// any others, and 2^20 smaller ones lose less than 2^-16 in all (a first token of value 0, 17.5 nats above 131071 others in one
+// part: the result is off by 0.03 %, with the reference at the largest score by 50; the time is the same).
 //
 // What bounds it is the cache's one read: 64 requests over 8192 tokens, 128 dimensions, take 246 us with one node each (4.9
 // TB/s, a copy's rate), 249 with 8 and 262 with up to 32 (4.7); three over 131000 292 (5.5 TB/s, reads alone).  From 64
@@ -33,7 +36,6 @@ typedef uint32_t TrU4 __attribute__((ext_vector_type(4)));
 typedef TrU4 TrU4a2 __attribute__((aligned(2)));
 
 constexpr float kTrInf = __builtin_inff();
-constexpr float kTrRaise = 8.0f;
 
 __device__ __forceinline__ float tr_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float tr_xor(float v, int s) { return u2f(lane_xor(f2u(v), s)); }
@@ -48,6 +50,8 @@ template <> struct TrElem<uint16_t> {
         return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)hi) << 16);
     }
     static constexpr uint32_t kExp = 0x7F80u;  // the exponent's bits: all set where a value is not finite
+    // powers of two: that a score may exceed its reference, and that the largest exceeds it at least
+    static constexpr float kRaise = 8.0f, kLift = 0.0f;
 };
 template <> struct TrElem<_Float16> {
     typedef _Float16 V8 __attribute__((ext_vector_type(8)));
@@ -58,6 +62,7 @@ template <> struct TrElem<_Float16> {
         return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
     }
     static constexpr uint32_t kExp = 0x7C00u;
+    static constexpr float kRaise = 15.0f, kLift = 11.0f;  // (2^16 is infinite)
 };
 
 // All ones in the halves of a word that are not finite (E's exponents; without compares, whose masks would take
@@ -287,13 +292,13 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 #pragma unroll
             for (int j = 1; j < 4; ++j) m = __builtin_fmaxf(m, __builtin_fmaxf(s[mt][0][j], s[mt][1][j]));
             top[mt] = m * a.c2;
-            raise |= top[mt] > ref[mt] + kTrRaise;
+            raise |= top[mt] > ref[mt] + E::kRaise;
         }
         if (wave_ballot(raise)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 float m = __builtin_fmaxf(top[mt], tr_xor(top[mt], 16));
-                m = __builtin_fmaxf(ref[mt], __builtin_fmaxf(m, tr_xor(m, 32)));
+                m = __builtin_fmaxf(ref[mt], __builtin_fmaxf(m, tr_xor(m, 32)) - E::kLift);
                 const float w = m == -kTrInf ? 1.0f : tr_exp2(ref[mt] - m);
                 ref[mt] = m;
                 sum[mt] *= w;
