@@ -59,3 +59,60 @@ def test_a_first_token_that_takes_the_weight(cuda, B, nodes, heads, dim, gap):
         bound = 2.0 ** -11 * want + want * (2.0 ** -11 + 2.5 * off + n * 2.0 ** -24 / 4 + 2.0 ** -19) + 2.0 ** -36 * v[:at + 1].sum(0)
         got = out[node::nodes]
         assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("B,nodes,heads,dim,n", [(1, 1, 1, 64, 128), (1, 5, 4, 128, 4096), (300, 64, 2, 128, 512), (300, 40, 1, 256, 512),
+                                                 (3, 9, 2, 192, 8192)])
+@pytest.mark.parametrize("size,dtype", [(300.0, "f16"), (3000.0, "f16"), (5000.0, "f16"), (20000.0, "f16"), (60000.0, "f16"), (3e5, "bf16"),
+                                        (1e8, "bf16"), (1e15, "bf16")])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_far_from_zero(cuda, B, nodes, heads, dim, n, size, dtype, sign):
+    """Equal scores of 1e6 to 1e31, where neighbouring 32-bit numbers lie up to many powers of two apart, have equal weights; keys
+    with scores of half of that have none, or all of it where those are negative."""
+    args = shared(cuda, B, nodes, heads, 1, dim, 16, n, dtype)
+    g = torch.Generator(device=cuda).manual_seed(n + dim)
+    args["q"][:] = size
+    args["v_cache"][:] = torch.randn(args["v_cache"].shape, generator=g, device=cuda)
+    half = torch.rand((n // 16, 1, 16, 1), generator=g, device=cuda) < 0.5
+    half[0, 0, 0], half[0, 0, 1] = True, False
+    args["k_cache"][:] = torch.where(half, sign * size / 2, sign * size)
+    out = ops.tree_attention(**args).double()
+    v = args["v_cache"][:, 0].transpose(1, 2).reshape(n, dim).double()
+    most = (half.flatten() == (sign < 0)).unsqueeze(1)
+    for node in {0, nodes // 2, nodes - 1}:
+        end = n - nodes + node + 1
+        w = most[:end].double() / most[:end].sum()
+        want, near = (w * v[:end]).sum(0), (w * v[:end].abs()).sum(0)
+        eps = R.half_step(R.DTYPES[dtype])
+        bound = eps * want.abs() + near * (eps + n * 2.0 ** -24 / 4 + 2.0 ** -19)   # (equal weights, rounded; sums; the result)
+        got = out[node::nodes]
+        assert bool(((got - want).abs() <= bound).all()), (node, got[0, 0, :3], want[:3])
+
+
+@pytest.mark.parametrize("B,nodes,heads,dim,n", [(1, 1, 1, 64, 512), (1, 5, 4, 128, 4096), (300, 64, 2, 128, 512), (300, 40, 1, 256, 512),
+                                                 (3, 9, 2, 192, 8192)])
+@pytest.mark.parametrize("size,dtype", [(8000.0, "f16"), (60000.0, "f16"), (3e4, "bf16"), (1e9, "bf16"), (1e15, "bf16")])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("at", [0.1, 0.5, 1.0])
+def test_scores_far_from_zero_beside_others(cuda, B, nodes, heads, dim, n, size, dtype, sign, at):
+    """Some keys' scores are far above or below the others', which are zero, before and behind them: the larger ones take all weight."""
+    args = shared(cuda, B, nodes, heads, 1, dim, 16, n, dtype)
+    g = torch.Generator(device=cuda).manual_seed(n + dim)
+    args["q"][:] = size
+    args["v_cache"][:] = torch.randn(args["v_cache"].shape, generator=g, device=cuda)
+    end = n - nodes + 1 if at == 1.0 else int(at * n)      # (the last ones are what the first node sees last)
+    far = torch.zeros(n, dtype=torch.bool, device=cuda)
+    far[end - 7:end] = True
+    far[40:60] |= at == 0.5
+    args["k_cache"].view(n // 16, 16, dim)[far.view(n // 16, 16)] = sign * size
+    out = ops.tree_attention(**args).double()
+    v = args["v_cache"][:, 0].transpose(1, 2).reshape(n, dim).double()
+    most = (far == (sign > 0)).unsqueeze(1)
+    for node in {0, nodes // 2, nodes - 1}:
+        end = n - nodes + node + 1
+        w = most[:end].double() / most[:end].sum()
+        want, near = (w * v[:end]).sum(0), (w * v[:end].abs()).sum(0)
+        eps = R.half_step(R.DTYPES[dtype])
+        bound = eps * want.abs() + near * (eps + n * 2.0 ** -24 / 4 + 2.0 ** -19)
+        got = out[node::nodes]
+        assert bool(((got - want).abs() <= bound).all()), (node, got[0, 0, :3], want[:3])

@@ -1478,6 +1478,7 @@ int vws_tree_attention(const vws_tree_attention_args* a) {
     k.visible_stride = a->visible_row_stride;
     k.words = (a->max_nodes + 31) / 32;
     k.c2 = (float)(1.4426950408889634 * (double)a->scale);
+    k.back = 1.0f / k.c2;
     k.splits = t.splits;
     k.chunk = t.chunk;
     k.blocks = t.blocks;

@@ -33,6 +33,7 @@ struct TreeArgs {
     int64_t visible_stride;
     int words;                // of a row that may be read
     float c2;                 // scale * log2(e)
+    float back;               // 1 / c2
     int splits;               // parts of the longest request's keys
     int chunk;                // keys of a part: a multiple of every wave's step
     int blocks;               // workgroups that a part's rows need, at most

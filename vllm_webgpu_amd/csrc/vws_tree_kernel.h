@@ -36,6 +36,13 @@ typedef uint32_t TrU4 __attribute__((ext_vector_type(4)));
 typedef TrU4 TrU4a2 __attribute__((aligned(2)));
 
 constexpr float kTrInf = __builtin_inff();
+// Scores (times log2 e) past this are far from zero: a 32-bit number's step is then no longer small beside 1, and a score less
+// its rounded reference may be any power of two.  The reference of a row that holds one lies in LDS, two such steps lower, so that the
+// largest weight is no less than kLift says, and its scores are taken less that reference in every step and end at
+// kMost: keys whose scores differ by less than their rounding may weigh the same there.  It is part of raising a
+// reference, without a branch (0.2 to 0.6 % of 64 requests' time, 2 % of a single tree's; with a branch around it 0.5 to 1 and 5).
+constexpr float kTrFar = 0x1p22f;
+__device__ __forceinline__ bool tr_far(float x) { return __builtin_fabsf(x) > kTrFar && __builtin_fabsf(x) < kTrInf; }
 
 __device__ __forceinline__ float tr_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float tr_xor(float v, int s) { return u2f(lane_xor(f2u(v), s)); }
@@ -50,8 +57,8 @@ template <> struct TrElem<uint16_t> {
         return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)hi) << 16);
     }
     static constexpr uint32_t kExp = 0x7F80u;  // the exponent's bits: all set where a value is not finite
-    // powers of two: that a score may exceed its reference, and that the largest exceeds it at least
-    static constexpr float kRaise = 8.0f, kLift = 0.0f;
+    // powers of two: that a score may exceed its reference, that the largest exceeds it at least, and at most far from zero
+    static constexpr float kRaise = 8.0f, kLift = 0.0f, kMost = 64.0f;
 };
 template <> struct TrElem<_Float16> {
     typedef _Float16 V8 __attribute__((ext_vector_type(8)));
@@ -62,7 +69,7 @@ template <> struct TrElem<_Float16> {
         return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
     }
     static constexpr uint32_t kExp = 0x7C00u;
-    static constexpr float kRaise = 15.0f, kLift = 11.0f;  // (2^16 is infinite)
+    static constexpr float kRaise = 15.0f, kLift = 11.0f, kMost = 15.0f;  // (2^16 is infinite)
 };
 
 // All ones in the halves of a word that are not finite (E's exponents; without compares, whose masks would take
@@ -161,9 +168,10 @@ __device__ __forceinline__ int tr_value_place(int c, int i) { return c ^ ((i >> 
 // (Two tiles of rows a wave read each operand once for both; four spill.)
 // MT tiles of 16 rows for each of WM waves, from m0 on.  The workgroup's waves make WAVES / WM lanes, which take the
 // keys in turn, 32 at a time, each through LDS of its own, and join what they have there.  A lane of one wave waits for
-// no other; the waves of a wider one share its tiles, and meet once a step.
+// no other; the waves of a wider one share its tiles, and meet once a step.  `far`: the references of rows far from zero, 16 MT
+// of each wave.
 template <typename T, int D, int MT, int WAVES, int WM>
-__device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, int b, int h, int split, int m0, char* lds) {
+__device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, int b, int h, int split, int m0, char* lds, float* far) {
     constexpr int WK = WAVES / WM, KS = D / 32, DT = D / 16, kAcc = tr_acc(D, MT), kStep = WK * kTrKeys;
     constexpr int kTile = tr_tile(D), kLoads = D / 16;  // loads of a tile
     constexpr int kMine = 2 * kLoads / WM;              // ... of a step's two that a wave makes
@@ -193,6 +201,13 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     }
 
     char* const ring = lds + wk * kDeep * 2 * kTile;
+    auto far_ref = [&](int mt) __attribute__((always_inline)) -> float& {
+        int i = i16;
+        asm volatile("" : "+v"(i));  // (the address is rarely needed: not kept in a register)
+        return far[(wave * MT + mt) * 16 + i];
+    };
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) far_ref(mt) = -kTrInf;
     // the pages of a step's four eights of keys (entries past the request's last are not read), 0 for those that do not exist, and
     // the keys that lie in pages that do
     struct Pages { int p[4]; uint32_t live; };
@@ -298,9 +313,19 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 float m = __builtin_fmaxf(top[mt], tr_xor(top[mt], 16));
-                m = __builtin_fmaxf(ref[mt], __builtin_fmaxf(m, tr_xor(m, 32)) - E::kLift);
-                const float w = m == -kTrInf ? 1.0f : tr_exp2(ref[mt] - m);
-                ref[mt] = m;
+                m = __builtin_fmaxf(m, tr_xor(m, 32));
+                const float was = ref[mt] == -kTrInf ? far_ref(mt) : ref[mt];
+                m = __builtin_fmaxf(was, tr_far(m) ? m - E::kLift - __builtin_fabsf(m) * 0x1p-22f : m - E::kLift);
+                const float w = m == -kTrInf ? 1.0f : tr_exp2(was - m);
+                // (without a reference in its register a row comes here in every step)
+                const bool off = tr_far(m);
+                ref[mt] = off ? -kTrInf : m;
+                far_ref(mt) = off ? m : -kTrInf;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = s[mt][j >> 2][j & 3], y = __builtin_fmaf(x, a.c2, -m);
+                    s[mt][j >> 2][j & 3] = off ? (y > E::kMost ? E::kMost : y) * a.back : x;
+                }
                 sum[mt] *= w;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= w;
@@ -449,6 +474,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TrBounds& o, 
     for (int mt = 0; mt < MT; ++mt) {
         sum[mt] += tr_xor(sum[mt], 16);
         sum[mt] += tr_xor(sum[mt], 32);
+        if (ref[mt] == -kTrInf) ref[mt] = far_ref(mt);
     }
 
     // the waves, joined by halves, where their tiles were
@@ -522,6 +548,7 @@ template <typename T, int D, int MT, int WAVES, int WIDE>
 __global__ __launch_bounds__(64 * WAVES, tr_waves(D, WAVES)) void tree_kernel(TreeArgs a) {
     constexpr int kThreads = 64 * WAVES, kRows = 16 * MT * WIDE;
     __shared__ __align__(1024) char lds[tr_lds(D, MT, WAVES)];
+    __shared__ float far[16 * MT * WAVES];
     // workgroups of the same keys lie eight apart, on one chiplet
     const int per = 8 * a.blocks, item = (blockIdx.x / per) * 8 + (blockIdx.x & 7), mb = (blockIdx.x % per) >> 3;
     const int bs = item / a.c.heads, h = item - bs * a.c.heads, split = bs % a.splits;
@@ -547,15 +574,15 @@ __global__ __launch_bounds__(64 * WAVES, tr_waves(D, WAVES)) void tree_kernel(Tr
     const int m0 = mb * kRows, rows = o.n * a.group - m0;
     if (rows <= 0 || (split * a.chunk >= o.len && split > 0)) return;
     if constexpr (WIDE == 8) {
-        if (rows > 4 * 16 * MT) tree_rows<T, D, MT, WAVES, 8>(a, o, b, h, split, m0, lds);
-        else tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds);
+        if (rows > 4 * 16 * MT) tree_rows<T, D, MT, WAVES, 8>(a, o, b, h, split, m0, lds, far);
+        else tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds, far);
     } else if constexpr (WIDE == 4) {
-        if (rows > 2 * 16 * MT) tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds);
-        else if (rows > 16 * MT) tree_rows<T, D, MT, WAVES, 2>(a, o, b, h, split, m0, lds);
-        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds);
+        if (rows > 2 * 16 * MT) tree_rows<T, D, MT, WAVES, 4>(a, o, b, h, split, m0, lds, far);
+        else if (rows > 16 * MT) tree_rows<T, D, MT, WAVES, 2>(a, o, b, h, split, m0, lds, far);
+        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds, far);
     } else {
-        if (MT == 1 || rows <= 16) tree_rows<T, D, 1, WAVES, 1>(a, o, b, h, split, m0, lds);
-        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds);
+        if (MT == 1 || rows <= 16) tree_rows<T, D, 1, WAVES, 1>(a, o, b, h, split, m0, lds, far);
+        else tree_rows<T, D, MT, WAVES, 1>(a, o, b, h, split, m0, lds, far);
     }
 }
 
