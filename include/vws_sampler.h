@@ -482,7 +482,8 @@ int vws_append_kv(const vws_append_kv_args* args);
 
 /* Moves each request's accepted keys and values up behind its context: of request b, the entries of path
  * [B, width] (node numbers, strictly increasing from path[b, 0] = 0, padded with -1): entry j's node goes
- * from position context_lens[b] + path[b, j] to context_lens[b] + j. */
+ * from position context_lens[b] + path[b, j] to context_lens[b] + j.  Entries whose positions lie in no page, and
+ * those of a negative context, move nothing. */
 int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* block_table,
                    int64_t block_table_row_stride, int32_t max_pages, const int32_t* context_lens,
                    const int32_t* path, int64_t path_row_stride, int32_t path_width, void* stream);
@@ -493,7 +494,7 @@ int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* bloc
  * those whose bit is set in visible[row] (bit j % 32 of word j / 32), or without `visible` the nodes up to
  * itself.  out = softmax(scale q k^T) v over what it sees, 0 where it sees nothing.  Hq is a multiple of
  * Hk; query head h reads key head h / (Hq / Hk).  Positions past the block table, in pages outside
- * [0, pages) and past the request's last node are not seen.  Requests whose bounds do not fit (decreasing,
+ * [0, pages) and past the request's last node are not seen; a negative context is 0.  Requests whose bounds do not fit (decreasing,
  * past T, more than max_nodes) and rows of no request are not written. */
 typedef struct vws_tree_attention_args {
     uint32_t struct_size; /* sizeof(vws_tree_attention_args): ABI guard */
