@@ -116,3 +116,21 @@ def test_scores_far_from_zero_beside_others(cuda, B, nodes, heads, dim, n, size,
         bound = eps * want.abs() + near * (eps + n * 2.0 ** -24 / 4 + 2.0 ** -19)
         got = out[node::nodes]
         assert bool(((got - want).abs() <= bound).all()), (node, got[0, 0, :3], want[:3])
+
+
+@pytest.mark.parametrize("B,nodes,heads,dim,columns", [(1, 3, 4, 64, 200), (1, 40, 4, 128, 2400), (1, 20, 2, 256, 400), (1, 3, 4, 64, 8),
+                                                       (600, 1, 1, 128, 24)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_no_numbers_count_whatever_their_weight(cuda, B, nodes, heads, dim, columns, bad):
+    """A seen value that is not finite makes the result so, though its key stands 300 nats below the others, with the keys divided
+    or not."""
+    n, at = columns * 16, columns * 5
+    args = shared(cuda, B, nodes, heads, 1, dim, 16, n, "bf16")
+    assert parts(args) == (columns >= 200)
+    args["q"][:] = 1.0
+    args["k_cache"][at // 16, 0, at % 16] = 300.0 / dim ** 0.5
+    args["v_cache"][:] = 1.0
+    args["v_cache"][0, 0, 7, 5] = bad
+    out = ops.tree_attention(**args)
+    fine = torch.isfinite(out)
+    assert not bool(fine[..., 7].any()) and bool(fine[..., :7].all()) and bool(fine[..., 8:].all())

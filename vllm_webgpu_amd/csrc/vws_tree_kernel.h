@@ -622,11 +622,12 @@ __global__ __launch_bounds__(kTrThreads) void tree_join_kernel(TreeArgs a) {
         v *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float w = i0 + u < parts ? tr_exp2(r[u] - z) : 0.0f;
-            if (w != 0.0f) {
-                total += s[u] * w;
-                v += x[u] * w;
-            }
+            // (of weight 0 too: a value that is no number counts whatever its weight)
+            const bool in = i0 + u < parts;
+            const float w = in ? tr_exp2(r[u] - z) : 0.0f;
+            total += (in ? s[u] : 0.0f) * w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += (in ? x[u][j] : 0.0f) * w;
         }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
