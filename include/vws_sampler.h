@@ -398,7 +398,7 @@ int vws_distill_step(const vws_distill_args* args);
  * Rows whose token lies outside [0, V) are padding: their logits count for nothing, 0 in every output, -1 in
  * the ids, gradient 0.
  * Masked logits (-inf) have probability 0 and add nothing to the entropy; a NaN or +inf in a row, or no
- * logit above -inf, makes its log-probabilities, entropy and gradient NaN.  Where a row has fewer than L
+ * logit above -inf, makes its log-probabilities, entropy and gradient (for upstreams of 0 too) NaN.  Where a row has fewer than L
  * logits that are numbers, the ids past them are -1 and their values NaN.
  *
  * The forward writes `saved` for the backward where it is not NULL; the backward reads it, the same inputs

@@ -507,7 +507,8 @@ __global__ __launch_bounds__(kScThreads) void score_backward_kernel(ScoreArgs a)
     out += lo;
     const float* st = a.stats + (size_t)r * kScRowStats;
     const float gl = (a.gl ? a.gl[r] : 0.0f) * a.inv_T, gh = (a.gh ? a.gh[r] : 0.0f) * a.inv_T;
-    if (st[kScLive] == 0.0f || (gl == 0.0f && gh == 0.0f)) {
+    // (a row that is not a number has no total, and a gradient of NaN whatever its upstream)
+    if (st[kScLive] == 0.0f || (gl == 0.0f && gh == 0.0f && st[kScLog2Total] == st[kScLog2Total])) {
         const uint32_t zero[4] = {0u, 0u, 0u, 0u};
         for (int vi = tid; vi < nvec; vi += kScThreads) sc_store<T>(out, vi, zero);
         if (tail < len) out[tail] = sc_narrow<T>(0.0f);

@@ -769,7 +769,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
     whose gradient has their type; the other outputs are not.
 
     Tokens outside [0, V) pad a row: its logits count for nothing, its outputs are 0 (ids -1) and its gradient is 0.
-    Logits of -inf have probability 0; a NaN or +inf makes its row NaN."""
+    Logits of -inf have probability 0; a NaN or +inf, or no logit above -inf, makes its row NaN, the gradient too whatever
+    reaches it."""
     idx = logits.get_device()
     if not 0 <= idx == token_ids.get_device() == torch.cuda.current_device():
         _device_of(idx, logits=logits, token_ids=token_ids)
