@@ -4,10 +4,52 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+from tests import tree_ref as R
 from vllm_webgpu_amd import ops
 
 pytestmark = pytest.mark.gpu
+
+
+def operands(dev):
+    """Arguments of a step of one request of three tokens, whose own keys lie at positions 5 to 7."""
+    kc, vc = R.make_cache(dev, 2, 2, 16, 64, "bf16")
+    q, k, v = (torch.randn((3, h, 64), device=dev).bfloat16() for h in (4, 2, 2))
+    at = lambda *x: torch.tensor(x, device=dev).int()  # noqa: E731
+    append = dict(k=k, v=v, k_cache=kc, v_cache=vc, slots=at(5, 6, 7), q=q, positions=at(5, 6, 7), inv_freq=torch.ones(32, device=dev))
+    tree = dict(q=q, k_cache=kc, v_cache=vc, block_table=at(0, 1).view(1, 2), context_lens=at(5), cu_nodes=at(0, 3), max_nodes=3)
+    return append, tree
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_derivatives_are_refused(cuda, grad):
+    """Tangents would be lost: the calls raise, with gradients on and off, and take tensors without one as before."""
+    append, tree = operands(cuda)
+    x, ids = torch.randn((3, 50), device=cuda), torch.tensor([1, 2, 3], device=cuda)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for leaf in (x, x.clone().requires_grad_()):
+            with pytest.raises((ValueError, RuntimeError)):
+                ops.token_logprobs(dual(leaf), ids)
+        for name in ("q", "k", "v", "k_cache", "v_cache", "inv_freq"):
+            with pytest.raises(ValueError):
+                ops.append_kv(**{**append, name: dual(append[name])})
+        for name in ("q", "k_cache", "v_cache"):
+            with pytest.raises(ValueError):
+                ops.tree_attention(**{**tree, name: dual(tree[name])})
+        for name in ("k_cache", "v_cache"):
+            with pytest.raises(ValueError):
+                ops.compact_kv(**{**{n: tree[n] for n in ("k_cache", "v_cache", "block_table", "context_lens")}, name: dual(tree[name])},
+                               path=torch.zeros((1, 1), device=cuda).int())
+        for call, args in ((ops.append_kv, append), (ops.tree_attention, tree)):
+            out = torch.empty_like(args["q"])
+            with pytest.raises(ValueError):
+                call(**args, out=dual(out))
+            assert call(**args, out=out) is out
+        assert ops.token_logprobs(x, ids).logprobs.shape == (3,)
 
 
 @pytest.mark.parametrize("V", [100, 30000])

@@ -16,6 +16,7 @@ import threading
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -678,6 +679,14 @@ def _ints(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype is torch.int32 and t.is_contiguous() else _int32(t).contiguous()
 
 
+def _refuse_tangents(**tensors) -> None:
+    """Raises for tensors that carry a forward-mode derivative, which there is none of here (callers look first whether any
+    may: ``forward_ad._current_level`` is at least 0 then)."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} would lose its forward-mode derivative: detach it")
+
+
 @dataclass
 class TokenLogprobs:
     logprobs: torch.Tensor              # [N] float32, differentiable in the logits
@@ -766,7 +775,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
     ``num_logprobs`` (at most 64 and V): also, as ``sample`` returns them, ``logprob_ids`` and ``logprob_vals``
     [N, L + 1] (the token, then the L largest logits, the lower index first among equals) and
     ``logprob_ranks``.  ``entropy``: also -sum p log p.  ``logprobs`` and ``entropy`` are differentiable in ``logits``,
-    whose gradient has their type; the other outputs are not.
+    whose gradient has their type (backward only: forward-mode derivatives are refused); the other outputs are not.
 
     Tokens outside [0, V) pad a row: its logits count for nothing, its outputs are 0 (ids -1) and its gradient is 0.
     Logits of -inf have probability 0; a NaN or +inf, or no logit above -inf, makes its row NaN, the gradient too whatever
@@ -783,6 +792,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
         raise ValueError(f"num_logprobs must be in [0, {min(_lib.MAX_LOGPROBS, logits.shape[1])}] (got {num_logprobs})")
     if not 1e-5 <= temperature < float("inf"):
         raise ValueError(f"temperature must be finite and at least 1e-5 (got {temperature})")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits=logits)
     logits, ids = _rows(logits), _ints(token_ids)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, L, bool(entropy), float(temperature)))
@@ -873,6 +884,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             and (q is None or q.get_device() == idx) and (positions is None or positions.get_device() == idx)
             and (inv_freq is None or inv_freq.get_device() == idx)):
         _device_of(idx, k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots, q=q, positions=positions, inv_freq=inv_freq)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q, inv_freq=inv_freq, out=out)
     Hk, _, D = k_cache.shape[1:]
     k, v = _head_rows(k, "k", k_cache, Hk, D), _head_rows(v, "v", k_cache, Hk, D)
     T = k.shape[0]
@@ -942,6 +955,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             == cu_nodes.get_device() == torch.cuda.current_device() and (visible is None or visible.get_device() == idx)):
         _device_of(idx, k_cache=k_cache, q=q, v_cache=v_cache, block_table=block_table, context_lens=context_lens, cu_nodes=cu_nodes,
                    visible=visible)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     (_, Hk, page, D), N = k_cache.shape, int(max_nodes)
     q = _head_rows(q, "q", k_cache, None, D)
     T, H, _ = q.shape
@@ -1021,6 +1036,8 @@ def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     if not (0 <= idx == v_cache.get_device() == block_table.get_device() == context_lens.get_device() == path.get_device()
             == torch.cuda.current_device()):
         _device_of(idx, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens, path=path)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(k_cache=k_cache, v_cache=v_cache)
     table, context = _tables(block_table, context_lens)
     B = table.shape[0]
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= _lib.MAX_TREE_NODES:
