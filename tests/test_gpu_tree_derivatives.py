@@ -52,6 +52,16 @@ def test_forward_derivatives_are_refused(cuda, grad):
         assert ops.token_logprobs(x, ids).logprobs.shape == (3,)
 
 
+def test_frequencies_that_require_a_gradient_are_refused(cuda):
+    append, _ = operands(cuda)
+    f = append["inv_freq"].clone().requires_grad_()
+    with pytest.raises(ValueError):
+        ops.append_kv(**{**append, "inv_freq": f})
+    want = ops.append_kv(**append)
+    with torch.no_grad():
+        assert torch.equal(ops.append_kv(**{**append, "inv_freq": f}), want)
+
+
 @pytest.mark.parametrize("V", [100, 30000])
 @pytest.mark.parametrize("gl,gh", [(0.0, 0.0), (1.5, 0.0), (0.0, -0.5), (1.0, 2.0), (0.0, None), (None, 0.0), (None, 1.0)])
 def test_gradients_of_rows_that_are_not_numbers(cuda, V, gl, gh):

@@ -896,6 +896,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if positions is not None:
         if inv_freq is None or inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
             raise ValueError("inv_freq must be float32 [R / 2] with positions")
+        if inv_freq.requires_grad and torch.is_grad_enabled():
+            raise ValueError("inv_freq would get no gradient: detach it")
         R = 2 * inv_freq.numel()
         if R < 16 or R % 16 or R > D:
             raise ValueError(f"inv_freq must hold a multiple of 8 frequencies, at most {D // 2} (got {inv_freq.numel()})")
