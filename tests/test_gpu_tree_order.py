@@ -126,3 +126,11 @@ def test_contexts_past_the_table(cuda, nodes, heads, kv_heads, dim, columns, wan
             bound = 2.0 ** -8 * o.abs() + (w @ v.abs()) * (2.0 ** -8 + 2.5 * score + see.shape[2] * 2.0 ** -24 / 4 + 2.0 ** -19)
             got = out[b * nodes:(b + 1) * nodes, mine]
             assert bool(((got - o).abs() <= bound).all()), (contexts[b], float(((got - o).abs() / bound).max()))
+
+
+def test_a_cache_without_heads_is_refused(cuda):
+    args, _, _ = arguments(cuda, [20], [4], 4, 2, 64, 16, "bf16")
+    none = dict(k_cache=args["k_cache"][:, :0], v_cache=args["v_cache"][:, :0])
+    for heads in (0, 4):
+        with pytest.raises(ValueError):
+            ops.tree_attention(**{**args, **none, "q": args["q"][:, :heads]})

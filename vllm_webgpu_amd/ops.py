@@ -962,8 +962,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     (_, Hk, page, D), N = k_cache.shape, int(max_nodes)
     q = _head_rows(q, "q", k_cache, None, D)
     T, H, _ = q.shape
-    if H < 1 or H % Hk:
-        raise ValueError(f"q's heads must be a multiple of {Hk} (got {H})")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"q's heads must be a multiple of the cache's {Hk}, at least one (got {H})")
     if not 1 <= N <= _lib.MAX_TREE_NODES:
         raise ValueError(f"max_nodes must be in [1, {_lib.MAX_TREE_NODES}] (got {max_nodes})")
     table, context = _tables(block_table, context_lens)
