@@ -514,7 +514,7 @@ typedef struct vws_tree_attention_args {
     const int32_t* cu_nodes;     /* [B + 1] */
     const uint32_t* visible;     /* [T, >= ceil(max_nodes / 32)] or NULL */
     int64_t visible_row_stride;
-    float scale;          /* > 0, finite */
+    float scale;          /* > 0; finite, also times log2(e) */
     void* workspace;      /* vws_tree_attention_workspace_size() bytes, 256-byte aligned, clean where it */
     size_t workspace_bytes; /* overlaps vws_sample_workspace_size(1, 1, 0) */
     void* stream;

@@ -906,6 +906,8 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     return t;
 }
 
+float tree_c2(float scale) { return (float)(1.4426950408889634 * (double)scale); }
+
 int validate_tree(const vws_tree_attention_args* a) {
     if (!a) return fail(VWS_ERR_INVALID_ARGUMENT, "args is NULL");
     if (a->struct_size != sizeof(vws_tree_attention_args))
@@ -922,7 +924,8 @@ int validate_tree(const vws_tree_attention_args* a) {
         return fail(VWS_ERR_INVALID_ARGUMENT, "max_pages must be at least 1 and block_table_row_stride at least max_pages");
     if (a->visible && a->visible_row_stride < (a->max_nodes + 31) / 32)
         return fail(VWS_ERR_INVALID_ARGUMENT, "visible_row_stride is less than max_nodes' words");
-    if (!(a->scale > 0.0f) || a->scale == __builtin_inff()) return fail(VWS_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+    if (!(a->scale > 0.0f) || !(tree_c2(a->scale) < __builtin_inff()))
+        return fail(VWS_ERR_INVALID_ARGUMENT, "scale must be > 0, and finite times log2 e");
     const vws_kv_cache& c = a->cache;
     const TreeShape t = tree_shape(a->batch, a->max_nodes, a->heads, c.kv_heads, c.head_dim, c.page_size, a->max_pages);
     const int64_t parts = (int64_t)a->batch * t.splits * c.kv_heads, joins = (int64_t)a->batch * c.kv_heads * ((t.rows + 3) / 4);
@@ -1477,7 +1480,7 @@ int vws_tree_attention(const vws_tree_attention_args* a) {
     k.visible = a->visible;
     k.visible_stride = a->visible_row_stride;
     k.words = (a->max_nodes + 31) / 32;
-    k.c2 = (float)(1.4426950408889634 * (double)a->scale);
+    k.c2 = tree_c2(a->scale);
     k.back = 1.0f / k.c2;
     k.splits = t.splits;
     k.chunk = t.chunk;
