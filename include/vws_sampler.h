@@ -455,8 +455,8 @@ typedef struct vws_kv_cache {
 /* Stores keys and values [T, Hk, D] of T tokens at `slots` (distinct; those outside [0, pages * P) are not
  * stored), the keys rotated, and writes the rotated queries.  The first R of a head's D dimensions turn in
  * pairs (i, i + R / 2), or (2i, 2i + 1) if `interleaved`, by the angle position * inv_freq[i] (taken in 64
- * bits) and are scaled by rope_scale.  Without positions nothing is rotated.  Inputs overlap neither the cache
- * nor q_out (but q, whose own memory it may be). */
+ * bits) and are scaled by rope_scale.  Without positions nothing is rotated.  Inputs that overlap the cache
+ * (from its first element to its last) or q_out (but q, whose own memory it may be) are refused. */
 typedef struct vws_append_kv_args {
     uint32_t struct_size; /* sizeof(vws_append_kv_args): ABI guard */
     int32_t tokens;       /* T >= 1 */
@@ -495,7 +495,7 @@ int vws_compact_kv(const vws_kv_cache* cache, int32_t batch, const int32_t* bloc
  * itself.  out = softmax(scale q k^T) v over what it sees, 0 where it sees nothing.  Hq is a multiple of
  * Hk; query head h reads key head h / (Hq / Hk).  Positions past the block table, in pages outside
  * [0, pages) and past the request's last node are not seen; a negative context is 0.  Requests whose bounds do not fit (decreasing,
- * past T, more than max_nodes) and rows of no request are not written. */
+ * past T, more than max_nodes) and rows of no request are not written.  `out` overlaps neither q nor the cache. */
 typedef struct vws_tree_attention_args {
     uint32_t struct_size; /* sizeof(vws_tree_attention_args): ABI guard */
     int32_t batch;        /* B >= 1 */

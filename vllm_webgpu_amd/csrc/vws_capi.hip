@@ -826,6 +826,32 @@ int validate_apart(const vws_kv_cache& c) {
     return VWS_OK;
 }
 
+// Rows [T, H, D] of 16-bit elements, or with H = 1 any T x D of them.
+struct Rows16 {
+    const void* p;
+    int64_t T, ts, H, hs, D;
+    // elements from the lowest to the highest of a token, and of all
+    int64_t inner() const { return (H - 1) * (hs < 0 ? -hs : hs) + D; }
+    int64_t lo() const { return (int64_t)(reinterpret_cast<uintptr_t>(p) >> 1) + (ts < 0 ? (T - 1) * ts : 0) + (hs < 0 ? (H - 1) * hs : 0); }
+    int64_t all() const { return (T - 1) * (ts < 0 ? -ts : ts) + inner(); }
+};
+// Whether two share memory: parts of the same rows or of the same heads, as of one projection, lie side by side and do not;
+// otherwise what lies from the first to the last element of each counts.
+bool rows_meet(const Rows16& a, const Rows16& b) {
+    const int64_t a0 = a.lo(), b0 = b.lo();
+    if (a0 >= b0 + b.all() || b0 >= a0 + a.all()) return false;
+    if ((reinterpret_cast<uintptr_t>(a.p) ^ reinterpret_cast<uintptr_t>(b.p)) & 1u) return true;
+    const auto apart = [&](int64_t period, int64_t len_a, int64_t len_b) {
+        const int64_t gap = ((b0 - a0) % period + period) % period;
+        return gap >= len_a && period - gap >= len_b;
+    };
+    // (a single token's or head's stride says nothing)
+    const int64_t ts = a.T > 1 ? a.ts : b.ts, hs = a.H > 1 ? a.hs : b.hs;
+    const bool rows = ts > 0 && (a.T > 1 || b.T > 1) && (b.T == 1 || b.ts == ts);
+    const bool heads = hs > 0 && (a.H > 1 || b.H > 1) && (b.H == 1 || b.hs == hs) && (a.T == 1 || a.ts % hs == 0) && (b.T == 1 || b.ts % hs == 0);
+    return !(rows && apart(ts, a.inner(), b.inner())) && !(heads && apart(hs, a.D, b.D));
+}
+
 CacheView cache_view(const vws_kv_cache& c) {
     CacheView v;
     v.k = static_cast<uint16_t*>(c.k);
@@ -862,7 +888,23 @@ int validate_append(const vws_append_kv_args* a) {
     if (a->heads > 0 && (!a->q || !a->q_out)) return fail(VWS_ERR_INVALID_ARGUMENT, "q or q_out is NULL");
     const int64_t wgs = (int64_t)a->tokens + ((int64_t)a->tokens + kApValueTokens - 1) / kApValueTokens * a->cache.kv_heads;
     if (wgs > kMaxWgs) return fail(VWS_ERR_LIMIT, "too many tokens (%d)", a->tokens);
-    return validate_apart(a->cache);
+    if (int st = validate_apart(a->cache)) return st;
+    // what is written (the cache, the turned queries) against what is read
+    const vws_kv_cache& c = a->cache;
+    const int64_t T = a->tokens, D = c.head_dim, page = (int64_t)c.kv_heads * c.page_size * D;
+    const Rows16 read[] = {{a->k, T, a->k_token_stride, c.kv_heads, a->k_head_stride, D}, {a->v, T, a->v_token_stride, c.kv_heads, a->v_head_stride, D},
+                           {a->slots, 1, 0, 1, 0, 2 * T}, {a->positions, 1, 0, 1, 0, 2 * T}, {a->inv_freq, 1, 0, 1, 0, a->rotary_dim},
+                           {a->q, T, a->q_token_stride, a->heads, a->q_head_stride, D}};
+    const Rows16 keys{c.k, 1, 0, 1, 0, (c.num_pages - 1) * c.k_page_stride + page}, values{c.v, 1, 0, 1, 0, (c.num_pages - 1) * c.v_page_stride + page};
+    const Rows16 out{a->q_out, T, a->q_out_token_stride, a->heads, a->q_out_head_stride, D};
+    const bool queries = a->heads > 0, in_place = a->q_out == a->q && a->q_out_token_stride == a->q_token_stride && a->q_out_head_stride == a->q_head_stride;
+    if (queries && (rows_meet(out, keys) || rows_meet(out, values))) return fail(VWS_ERR_INVALID_ARGUMENT, "q_out and the cache overlap");
+    for (const Rows16& r : read) {
+        if (((&r == &read[3] || &r == &read[4]) && !a->positions) || (&r == &read[5] && !queries)) continue;
+        if (rows_meet(r, keys) || rows_meet(r, values)) return fail(VWS_ERR_INVALID_ARGUMENT, "an input and the cache overlap");
+        if (queries && !(&r == &read[5] && in_place) && rows_meet(r, out)) return fail(VWS_ERR_INVALID_ARGUMENT, "an input and q_out overlap");
+    }
+    return VWS_OK;
 }
 
 // How a launch divides its requests' rows and keys: workgroups of 16, 32 or 128 rows (16 or 128 past 128 dimensions),

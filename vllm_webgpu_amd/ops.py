@@ -872,7 +872,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     """Appends keys and values [T, kv_heads, dim] of T tokens to a layer's paged cache at ``slots`` [T] (page *
     page size + place in the page; distinct, those outside the cache are not stored), the position rotation
     applied to the keys and to ``q`` [T, heads, dim] on the way.  Returns the rotated queries (in ``out``
-    if given, ``q`` itself among them), or None without ``q``.
+    if given, ``q`` itself among them), or None without ``q``.  Inputs in the cache's own memory are refused.
 
     The cache's pages are k_cache [pages, kv_heads, page, dim] and v_cache [pages, kv_heads, dim, page]
     (bfloat16 or float16, contiguous pages; page a power of two from 8 to 256, dim 64, 96, 128, 192 or 256).
