@@ -848,8 +848,8 @@ def _out_rows(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.
 
 
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors [tokens, heads, dim] share memory (parts of the same rows, as of one projection, lie side by
-    side and do not; otherwise what lies from the first to the last element of each counts)."""
+    """Whether two tensors [tokens, heads, dim] share memory (parts of the same rows or of the same heads, as of one projection,
+    lie side by side and do not; otherwise what lies from the first to the last element of each counts)."""
     if not a.numel() or not b.numel():
         return False
 
@@ -859,11 +859,20 @@ def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     size, a0, b0 = a.element_size(), a.data_ptr(), b.data_ptr()
     if a0 >= b0 + size * span(b, range(b.dim())) or b0 >= a0 + size * span(a, range(a.dim())):
         return False
-    pitch, inner = a.stride(0), range(1, a.dim())
-    if a.dim() != b.dim() or b.stride(0) != pitch or a.shape[0] < 2 or b.shape[0] < 2 or (b0 - a0) % size:
+    if a.dim() != b.dim() or (b0 - a0) % size:
         return True
-    gap = (b0 - a0) // size % pitch if pitch else 0
-    return gap < span(a, inner) or pitch - gap < span(b, inner)
+
+    def apart(period, length_a, length_b):
+        gap = (b0 - a0) // size % period
+        return gap >= length_a and period - gap >= length_b
+
+    # (a single token's or head's stride says nothing)
+    (T, H, D), (U, I, E) = a.shape, b.shape
+    ts, hs, inner = a.stride(0) if T > 1 else b.stride(0), a.stride(1) if H > 1 else b.stride(1), range(1, 3)
+    if ts and (T > 1 or U > 1) and (U == 1 or b.stride(0) == ts) and apart(ts, span(a, inner), span(b, inner)):
+        return False
+    return not (hs and (H > 1 or I > 1) and (I == 1 or b.stride(1) == hs) and (T == 1 or a.stride(0) % hs == 0)
+                and (U == 1 or b.stride(0) % hs == 0) and apart(hs, D, E))
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
