@@ -93,15 +93,19 @@ class TreeSampler:
         if logits.dim() != 2 or logits.shape[0] != T or token_ids.shape != (T,):
             raise ValueError(f"logits must be [{T}, V] and token_ids [{T}] (got {tuple(logits.shape)} and {tuple(token_ids.shape)})")
 
-        def rows(t):
+        def rows(name):
+            t = getattr(m, name)
+            if t is not None and t.shape != (B,):  # (a device would index past its end)
+                raise ValueError(f"{name} must be [{B}], one for each tree (got {tuple(t.shape)})")
             return None if t is None else t[tree.requests]
 
         kw: dict = {}
         if not m.all_greedy and m.temperature is not None:
-            kw = dict(temperature=rows(m.temperature), top_k=rows(m.top_k), top_p=rows(m.top_p), min_p=rows(m.min_p))
+            kw = {name: rows(name) for name in ("temperature", "top_k", "top_p", "min_p")}
             if m.generators:
                 domain = torch.full((B,), _DOMAIN, dtype=torch.int64)
-                kw.update(rng_seeds=rows(draw_seeds(B, m.generators, logits.device, self._seeds, domain)), rng_offsets=tree.numbers)
+                seeds = draw_seeds(B, m.generators, logits.device, self._seeds, domain)
+                kw.update(rng_seeds=seeds[tree.requests], rng_offsets=tree.numbers)
             else:
                 kw["rng_key"] = int(torch.randint(_SEED_LO, _SEED_HI, (1,), dtype=torch.int64))
         sampled = ops.sample(logits, **kw).sampled
