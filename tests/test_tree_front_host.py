@@ -4,6 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from vllm_webgpu_amd.v1.kv_cache import PagedKVCache
 from vllm_webgpu_amd.v1.sample.metadata import SamplingMetadata
 from vllm_webgpu_amd.v1.sample.tree_sampler import DraftTree, TreeSampler
 
@@ -22,3 +23,15 @@ def test_settings_of_another_count_of_requests(name, count):
         m.min_p = torch.ones(count)
     with pytest.raises(ValueError, match=name):
         TreeSampler()(tree, torch.zeros(6, dtype=torch.int32), torch.zeros((6, 20)), m)
+
+
+@pytest.mark.parametrize("tables,contexts", [(2, 3), (3, 2), (4, 3), (3, 4), (2, 2)])
+def test_tables_and_contexts_of_another_count_of_requests(tables, contexts):
+    c = PagedKVCache(1, 10, 1, 64, page_size=16, device="cpu")
+    for i in range(4):
+        c.reserve(str(i), 20)
+    tree = DraftTree.make([[-1, 0], [-1], [-1, 0, 0]], CPU)
+    table = c.block_table([str(i) for i in range(4)])
+    with pytest.raises(ValueError):
+        c.slots(table[:tables], torch.zeros(contexts, dtype=torch.int32), tree)
+    assert c.slots(table[:3], torch.zeros(3, dtype=torch.int32), tree).shape == (6,)

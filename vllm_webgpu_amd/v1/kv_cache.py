@@ -45,6 +45,10 @@ class PagedKVCache:
 
     def slots(self, block_table: torch.Tensor, context_lens: torch.Tensor, tree: DraftTree) -> torch.Tensor:
         """int32 [T]: where the nodes' keys and values go, behind their contexts; -1 (nowhere) past a request's pages."""
+        B = len(tree.num_nodes)
+        if block_table.dim() != 2 or block_table.shape[0] != B or context_lens.shape != (B,):  # (a device would index past its end)
+            raise ValueError(f"block_table must be [{B}, pages] and context_lens [{B}], one row for each tree (got {tuple(block_table.shape)} "
+                             f"and {tuple(context_lens.shape)})")
         at = context_lens.long()[tree.requests] + tree.numbers
         i = at // self.page_size
         held = (i >= 0) & (i < block_table.shape[1])
