@@ -674,9 +674,17 @@ def _device_of(idx: int, **tensors) -> None:
         raise ValueError(f"the tensors' device must be the current one (cuda:{idx} against cuda:{torch.cuda.current_device()})")
 
 
-def _ints(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as contiguous int32 on its device; what does not fit goes to its ends."""
-    return t if t.dtype is torch.int32 and t.is_contiguous() else _int32(t).contiguous()
+def _ints(t: torch.Tensor, name: str) -> torch.Tensor:
+    """``t``, of an integer type, as contiguous int32 on its device; what does not fit goes to its ends."""
+    return t if t.dtype is torch.int32 and t.is_contiguous() else _int_rows(t, name).contiguous()
+
+
+def _int_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype is torch.int32:
+        return t
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool:  # (not to be cut to whole numbers)
+        raise ValueError(f"{name} must be of an integer type (got {t.dtype})")
+    return _int32(t)
 
 
 def _refuse_tangents(**tensors) -> None:
@@ -794,7 +802,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, num_logprobs: 
         raise ValueError(f"temperature must be finite and at least 1e-5 (got {temperature})")
     if forward_ad._current_level >= 0:
         _refuse_tangents(logits=logits)
-    logits, ids = _rows(logits), _ints(token_ids)
+    logits, ids = _rows(logits), _ints(token_ids, "token_ids")
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, L, bool(entropy), float(temperature)))
     return TokenLogprobs(*_score_forward(logits, ids, L, bool(entropy), float(temperature), None))
@@ -900,7 +908,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     T = k.shape[0]
     if v.shape[0] != T or slots.shape != (T,):
         raise ValueError(f"v and slots must be of {T} tokens (got {tuple(v.shape)} and {tuple(slots.shape)})")
-    slots = _ints(slots)
+    slots = _ints(slots, "slots")
     R = 0
     if positions is not None:
         if inv_freq is None or inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
@@ -912,7 +920,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             raise ValueError(f"inv_freq must hold a multiple of 8 frequencies, at most {D // 2} (got {inv_freq.numel()})")
         if positions.shape != (T,):
             raise ValueError(f"positions must be [{T}] (got {tuple(positions.shape)})")
-        positions, inv_freq = _ints(positions), inv_freq.contiguous()
+        positions, inv_freq = _ints(positions, "positions"), inv_freq.contiguous()
     elif inv_freq is not None:
         raise ValueError("positions are required with inv_freq")
     ks, vs, qs, os = k.stride(), v.stride(), (0, 0), (0, 0)
@@ -943,7 +951,7 @@ def _tables(block_table: torch.Tensor, context_lens: torch.Tensor):
     if block_table.dim() != 2 or context_lens.shape != block_table.shape[:1] or block_table.shape[1] < 1:
         raise ValueError(f"block_table must be [batch, pages] and context_lens [batch] (got {tuple(block_table.shape)} and "
                          f"{tuple(context_lens.shape)})")
-    return _rows(block_table if block_table.dtype is torch.int32 else _int32(block_table)), _ints(context_lens)
+    return _rows(_int_rows(block_table, "block_table")), _ints(context_lens, "context_lens")
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -979,7 +987,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     B = table.shape[0]
     if cu_nodes.shape != (B + 1,):
         raise ValueError(f"cu_nodes must be [{B + 1}] (got {tuple(cu_nodes.shape)})")
-    cu = _ints(cu_nodes)
+    cu = _ints(cu_nodes, "cu_nodes")
     if visible is not None:
         if visible.dtype != torch.int32 or visible.dim() != 2 or visible.shape[0] != T or visible.shape[1] < (N + 31) // 32:
             raise ValueError(f"visible must be int32 [{T}, {(N + 31) // 32}] (got {visible.dtype} {tuple(visible.shape)})")
@@ -1027,7 +1035,8 @@ def accept_tree(sampled: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
         raise ValueError("cu_nodes must be [batch + 1]")
     if not 1 <= W <= _lib.MAX_TREE_NODES:
         raise ValueError(f"max_path must be in [1, {_lib.MAX_TREE_NODES}] (got {max_path})")
-    sampled, tokens, parents, cu = _ints(sampled), _ints(tokens), _ints(parents), _ints(cu_nodes)
+    sampled, tokens, parents = _ints(sampled, "sampled"), _ints(tokens, "tokens"), _ints(parents, "parents")
+    cu = _ints(cu_nodes, "cu_nodes")
     B = cu.numel() - 1
     out, path = cu.new_empty((2, B, W)).unbind()
     accepted = cu.new_empty(B)
@@ -1053,7 +1062,7 @@ def compact_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     B = table.shape[0]
     if path.dim() != 2 or path.shape[0] != B or not 1 <= path.shape[1] <= _lib.MAX_TREE_NODES:
         raise ValueError(f"path must be [{B}, 1 .. {_lib.MAX_TREE_NODES}] (got {tuple(path.shape)})")
-    path = _rows(path if path.dtype is torch.int32 else _int32(path))
+    path = _rows(_int_rows(path, "path"))
     if B:
         _lib.check(_lib.lib().vws_compact_kv(ctypes.byref(cache), B, table.data_ptr(), _row_stride(table), table.shape[1],
                                              context.data_ptr(), path.data_ptr(), _row_stride(path), path.shape[1],
