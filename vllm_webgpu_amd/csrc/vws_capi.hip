@@ -917,15 +917,15 @@ struct TreeShape {
     int rows;          // of all of a request's workgroups
 };
 constexpr int kTreeUnits = 256;     // compute units
-// A part's keys, at least (one tree of 12 nodes over 1900: 15.7 us, with 512 18.3; over 8000: 22.8, with 128 24.2).
+// A part's keys, at least (one tree of 12 nodes over 1900: 15.8 us, with 512 18.9, with 128 14.7; over 8000: 18.7, 19.8, 21.8).
 constexpr int kTreeMinKeys = 256;
 TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int page_size, int max_pages) {
     TreeShape t;
     const int need = max_nodes * (heads / kv_heads), step = kTrKeys * kTrThreads / 64;
     const int64_t most = std::min<int64_t>((int64_t)max_pages * page_size, kCacheMaxPosition);
     // More than 32 rows: workgroups of 128 read the keys once (64 trees of up to 32 nodes, four heads each, over 8192
-    // tokens: 261 us, of 32 rows 376; eight heads each of 256 dimensions: 472, of 16 rows 919), but where those of 32 are all
-    // resident at once anyway (one tree of 12 nodes over 1900: 19.8 us and 16.0).
+    // tokens: 258 us, of 32 rows 375; eight heads each of 256 dimensions: 482, of 16 rows 1045), but where those of 32 are all
+    // resident at once anyway (one tree of 12 nodes over 1900: 18.6 us and 15.8).
     const int few = D > 128 ? 16 : 32;  // rows of a workgroup whose waves share none
     const int64_t narrow = (int64_t)B * kv_heads * ((need + few - 1) / few) * ((most + kTreeMinKeys - 1) / kTreeMinKeys);
     const bool wide = need > 32 && narrow > 2 * kTreeUnits;
@@ -934,10 +934,12 @@ TreeShape tree_shape(int B, int max_nodes, int heads, int kv_heads, int D, int p
     t.blocks = (need + t.block_rows - 1) / t.block_rows;
     t.rows = t.blocks * t.block_rows;
     // Parts: one workgroup a compute unit, since every part costs its start, its end and its record (one tree of 12 nodes
-    // over 8000: 19.6 us, two a unit 23.1; one node over 64000: 57.8, 64.5; three of 8 nodes x 8 heads over 131000: 290,
-    // 305).  But where that leaves most requests undivided, a long one would be the launch: two a unit then (20 ragged
-    // requests of up to 32 nodes over 8192: 216 us, two a unit 137; 12 of 8 over 30000: 225, 193).  Not for few rows past
-    // 128 dimensions, where a unit holds one at a time (30 of 4 nodes over 8192: 171, 190).
+    // over 8000: 18.7 us, two a unit 21.8; one node over 64000: 57.4, 59.2; three of 8 nodes x 8 heads over 131000: 293,
+    // 309).  But where that leaves most requests undivided, a long one would be the launch: two a unit then (20 ragged
+    // requests of up to 32 nodes over 8192: 193 us, two a unit 124; 12 of 8 over 30000: 233, 186).  Not for few rows past
+    // 128 dimensions, where a unit holds one at a time (30 of 4 nodes over 8192: 237, 247).  Parts are cut from the table's
+    // width, so a table much wider than a few requests' lengths leaves most of them empty (one tree of 12 nodes over 1900, in a
+    // table of 131072 tokens: 39 us).
     const int64_t items = (int64_t)B * kv_heads * t.blocks;
     const int64_t wgs = items * 8 > kTreeUnits && (wide || D <= 128) ? 2 * kTreeUnits : kTreeUnits;
     int64_t s = std::min<int64_t>(std::min<int64_t>(wgs / items, most / kTreeMinKeys), kTrMaxSplits);
@@ -1528,6 +1530,8 @@ int vws_tree_attention(const vws_tree_attention_args* a) {
     k.chunk = t.chunk;
     k.blocks = t.blocks;
     k.rows = t.rows;
+    // (one thread a request finds its place, so up to 256: 64 ragged trees of up to 32 nodes over 8192 258 us, as they come 327;
+    // 256 over 2048 348 and 325, 256 of one node 222 and 218; 20 in parts 124 and 108)
     k.longest_first = k.B > 1 && k.B <= kTrThreads && (int64_t)k.B * k.splits * k.c.heads * k.blocks > t.slots;
     char* base = static_cast<char*>(a->workspace) + align256(sizeof(CoopState));
     const size_t recs = (size_t)k.B * (size_t)k.splits * (size_t)k.c.heads * (size_t)k.rows;

@@ -14,7 +14,7 @@
 // maximum reaches it hold any: a handful of groups is read again.
 //
 // HBM bounds both: 1999 x 151936 bf16 with entropy and 20 alternatives 135 us (4.5 TB/s of
-// logits, 5.9 with the groups' lines; without alternatives 115), 4096 x 128256 bf16, a fifth of
+// logits, 5.9 with the groups' lines; without alternatives 109), 4096 x 128256 bf16, a fifth of
 // the rows padding, forward 150 (5.6 TB/s, reads alone) and backward 345 (5.5 TB/s read and written, some of the reads from the
 // last-level cache).  Few rows are split over workgroups: 7 x 50257 fp32 with 5 alternatives 10.9 us, a part's read, its list and the join one after another.
 #include "vws_device.h"
@@ -92,7 +92,7 @@ struct ScShared {
     float m[kScThreads / 64], s[kScThreads / 64], w[kScThreads / 64];
     uint32_t n[kScThreads / 64];
     float t;               // threshold of the listed logits
-    uint32_t groups, cands, found;
+    uint32_t groups, cands;
     uint16_t group[kScGroups];
     uint64_t top[kScMaxTop];
     union {

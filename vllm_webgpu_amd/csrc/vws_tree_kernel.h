@@ -17,9 +17,9 @@
 // any others, and 2^20 smaller ones lose less than 2^-16 in all (a first token of value 0, 17.5 nats above 131071 others in one
 // part: the result is off by 0.03 %, with the reference at the largest score by 50; the time is the same).
 //
-// What bounds it is the cache's one read: 64 requests over 8192 tokens, 128 dimensions, take 246 us with one node each (4.9
-// TB/s, a copy's rate), 249 with 8 and 262 with up to 32 (4.7); three over 131000 292 (5.5 TB/s, reads alone).  From 64
-// nodes of four heads on it is the arithmetic: 256 rows, 64 requests over 4096 tokens, 439 us, 0.6 PFLOP/s, with an
+// What bounds it is the cache's one read: 64 requests over 8192 tokens, 128 dimensions, take 241 us with one node each (5.2
+// TB/s), 243 with 8 and 259 with up to 32 (4.9); three over 131000 293 (5.5 TB/s, reads alone).  From 64
+// nodes of four heads on it is the arithmetic: 256 rows, 64 requests over 4096 tokens, 448 us, 0.6 PFLOP/s, with an
 // exponential, two fmas and a rounding for every 512 of the products' operations.  One small request (12 nodes over 1900) takes
 // 12 us and 4 for the join, of which 8.7 are a step's own latency (one key): launch, bounds, table, tile, products, joins.
 #pragma once
@@ -587,7 +587,9 @@ __global__ __launch_bounds__(64 * WAVES, tr_waves(D, WAVES)) void tree_kernel(Tr
 }
 
 // Joins the parts of a request's rows, 16 bytes of a part's row a lane: D / 4 lanes a row, as many rows of a
-// request's key head as a workgroup has room for.  Latency: 4.0 us for 5 parts of 48 rows, 6.5 for 10 of 64; a launch of its own, since the parts of 128 rows are too much for the workgroup that would come last.
+// request's key head as a workgroup has room for.  Latency: 4.0 us for 5 parts of 48 rows, 5.8 for 10 of 64.  A launch of its own: the
+// parts of 128 rows are too much for the workgroup that would come last; those of 32 and fewer, where it is a quarter of the
+// time, would not be, and take it too.
 template <typename T, int D>
 __global__ __launch_bounds__(kTrThreads) void tree_join_kernel(TreeArgs a) {
     typedef TrElem<T> E;

@@ -966,9 +966,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     max_nodes]: its ancestors and itself, in a tree), or without it the nodes up to itself (a chain; one
     node: plain decoding).  Rows that see nothing are 0.  heads is a multiple of kv_heads; ``scale`` is
     dim ** -0.5 by default.  The table's width bounds the contexts that the call is laid out for: pass the columns that
-    are in use.  Rows of no request, and of requests whose bounds do not fit, are not written; give ``out`` to keep
-    what they hold.  Scores, sums and products are held in 32 bits; the weights of a softmax are rounded to the
-    cache's type before their product with the values."""
+    are in use (few requests in a table many times their length take two to three times as long).  Rows of no
+    request, and of requests whose bounds do not fit, are not written; give ``out`` to keep what they hold.  Scores,
+    sums and products are held in 32 bits; the weights of a softmax are rounded to the cache's type before their
+    product with the values."""
     cache, idx = _kv_cache(k_cache, v_cache), k_cache.get_device()
     if not (0 <= idx == q.get_device() == v_cache.get_device() == block_table.get_device() == context_lens.get_device()
             == cu_nodes.get_device() == torch.cuda.current_device() and (visible is None or visible.get_device() == idx)):
